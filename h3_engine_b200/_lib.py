@@ -62,6 +62,21 @@ SIGNATURES: dict[str, tuple] = {
     "h3b_peer_buffer_close": (_i32, [_c_void_p]),
     "h3b_peer_buffer_destroy": (_i32, [_c_void_p]),
     "h3b_amax_exchange": (_i32, [_c_void_p, _c_void_p, _i32, _i32, _i64, _i64, _c_void_p]),
+    "h3b_mxfp4_quantize": (_i32, [_c_void_p, _i32, _i64, _i64, _i64, _c_void_p, _c_void_p,
+                                  _c_void_p]),
+    "h3b_mxfp4_dequantize": (_i32, [_c_void_p, _c_void_p, _i64, _i64, _c_void_p, _i32, _i64,
+                                    _c_void_p]),
+    "h3b_mxfp4_gemm": (_i32, [_c_void_p, _c_void_p, _i64, _c_void_p, _c_void_p, _i64, _i64,
+                              _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _i32, _i64,
+                              _c_void_p]),
+    "h3b_mxfp4_linear_ws": (_i64, [_i64, _i64, _i64]),
+    "h3b_mxfp4_linear": (_i32, [_c_void_p, _i32, _i64, _i64, _c_void_p, _c_void_p, _i64, _i64,
+                                _c_void_p, _i32, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                                _i64, _c_void_p]),
+    "h3b_mxfp4_ffn_ws": (_i64, [_i64, _i64, _i64]),
+    "h3b_mxfp4_ffn": (_i32, [_c_void_p, _i32, _i64, _i64, _c_void_p, _c_void_p, _c_void_p,
+                             _c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _i64, _c_void_p,
+                             _i64, _c_void_p]),
 }
 
 _lock = threading.Lock()

@@ -1,0 +1,244 @@
+// Host side of the MXFP4 entry points (declared in include/h3b.h): argument
+// checks, TMA descriptors, kernel choice and launch.
+#pragma once
+
+#include "gemm_mxfp4.cuh"
+#include "quant_mx.cuh"
+
+namespace h3b {
+
+// Opt in a kernel's dynamic shared memory once per device (the attribute
+// belongs to the device's context).
+struct SmemAttr {
+  std::atomic<bool> done[64];
+  int set(const void* fn, int bytes) {
+    int dev = 0;
+    if (cudaGetDevice(&dev) != cudaSuccess) return H3B_ERR_CUDA;
+    if (dev < 64 && done[dev].load(std::memory_order_acquire)) return H3B_OK;
+    if (cudaFuncSetAttribute(fn, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes) !=
+        cudaSuccess)
+      return H3B_ERR_CUDA;
+    if (dev < 64) done[dev].store(true, std::memory_order_release);
+    return H3B_OK;
+  }
+};
+
+// 2-D tensor of 16-bit values, box box_cols x box_rows, 128-byte swizzle.
+static int make_tmap_16_sw128(CUtensorMap* map, const void* base, int dtype, uint64_t rows,
+                              uint64_t cols, uint64_t pitch_elems, uint32_t box_cols,
+                              uint32_t box_rows) {
+  auto fn = encode_fn();
+  if (!fn) return H3B_ERR_UNSUPPORTED;
+  cuuint64_t dims[2] = {cols, rows};
+  cuuint64_t strides[1] = {pitch_elems * 2};
+  cuuint32_t box[2] = {box_cols, box_rows};
+  cuuint32_t estr[2] = {1, 1};
+  CUresult r = fn(map, dtype == H3B_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                           : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+                  2, const_cast<void*>(base), dims, strides, box, estr,
+                  CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B,
+                  CU_TENSOR_MAP_L2_PROMOTION_NONE, CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  return r == CUDA_SUCCESS ? H3B_OK : H3B_ERR_INVALID_ARG;
+}
+
+static inline int dt_bytes(int dtype) { return dtype == H3B_DT_F32 ? 4 : 2; }
+static inline bool dt_any(int d) { return d == H3B_DT_BF16 || d == H3B_DT_F16 || d == H3B_DT_F32; }
+static inline bool dt_16(int d) { return d == H3B_DT_BF16 || d == H3B_DT_F16; }
+
+constexpr int64_t kMxMaxDim = (int64_t)INT32_MAX - 512;
+
+template <typename T>
+static void mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
+                               int64_t Mpad, cudaStream_t st) {
+  int64_t blocks = (Mpad + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
+  blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
+  mx::k_mxfp4_quantize<T, 4><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
+      static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
+      Mpad);
+}
+
+template <typename T>
+static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
+                                 int64_t ldo, cudaStream_t st) {
+  int64_t blocks = (M + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
+  blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
+  mx::k_mxfp4_dequantize<T><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
+      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
+      static_cast<T*>(out), ldo);
+}
+
+// Operands of both MXFP4 GEMM forms: shapes and alignment.
+static int mx_gemm_args(mxgemm::Args& a, const void* A, const void* sfA, int64_t M, const void* B,
+                        const void* sfB, int64_t N, int64_t K) {
+  if (!A || !sfA || !B || !sfB) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(A) || !aligned16(sfA) || !aligned16(B) || !aligned16(sfB))
+    return H3B_ERR_ALIGNMENT;
+  int rc = check_sm100();
+  if (rc != H3B_OK) return rc;
+  memset(&a, 0, sizeof(a));
+  rc = make_tmap_u8_sw128(&a.tmap_a, A, (uint64_t)M, (uint64_t)(K / 2), (uint64_t)(K / 2),
+                          mxgemm::KB_BYTES, mxgemm::BM);
+  if (rc != H3B_OK) return rc;
+  rc = make_tmap_u8_sw128(&a.tmap_b, B, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)(K / 2),
+                          mxgemm::KB_BYTES, mxgemm::BN);
+  if (rc != H3B_OK) return rc;
+  a.sfa = static_cast<const uint8_t*>(sfA);
+  a.sfb = static_cast<const uint8_t*>(sfB);
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.sf_tiles_k = (int)mx::sf_tiles(K);
+  a.n_tiles = (int)((N + mxgemm::BN - 1) / mxgemm::BN);
+  const int64_t tiles = (int64_t)a.n_tiles * ((M + mxgemm::BM - 1) / mxgemm::BM);
+  if (tiles > INT32_MAX) return H3B_ERR_INVALID_ARG;
+  a.num_tiles = (int)tiles;
+  return H3B_OK;
+}
+
+template <typename T, int EPI>
+static int mx_gemm_launch(const mxgemm::Args& a, cudaStream_t st) {
+  static SmemAttr attr;
+  const int rc = attr.set(reinterpret_cast<const void*>(&mxgemm::k_gemm_mxfp4<T, EPI>),
+                          mxgemm::SMEM_BYTES);
+  if (rc != H3B_OK) return rc;
+  const int grid = std::min(a.num_tiles, num_sms());
+  mxgemm::k_gemm_mxfp4<T, EPI><<<grid, mxgemm::THREADS, mxgemm::SMEM_BYTES, st>>>(a);
+  return launched(cudaGetLastError());
+}
+
+// Bytes of an activation's codes and blocked scales in a workspace, each part
+// rounded up to 256 bytes.
+static inline int64_t mx_code_bytes(int64_t rows, int64_t k) {
+  return (rows * (k / 2) + 255) / 256 * 256;
+}
+static inline int64_t mx_operand_bytes(int64_t rows, int64_t k) {
+  return mx_code_bytes(rows, k) + (rows + 127) / 128 * mx::sf_tiles(k) * mxgemm::SF_ATOM;
+}
+
+// Checks of everything but the operands of a product D = act(A B^T + bias) + residual.
+static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* bias, int act,
+                        const void* residual, int64_t ldr, const void* D, int64_t ldd) {
+  if (!dt_16(dtype) || M < 0 || N <= 0 || K <= 0 || K % mx::BLOCK || N % 8) return H3B_ERR_INVALID_ARG;
+  if (act != H3B_ACT_NONE && act != H3B_ACT_GELU_TANH) return H3B_ERR_INVALID_ARG;
+  if (M > kMxMaxDim || N > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
+  if (ldd < N || (residual && ldr < N)) return H3B_ERR_INVALID_ARG;
+  if (M == 0) return H3B_OK;
+  if (!D) return H3B_ERR_INVALID_ARG;
+  if (ldd % 8 || (residual && ldr % 8) || !aligned16(D) || (bias && !aligned16(bias)) ||
+      (residual && !aligned16(residual)))
+    return H3B_ERR_ALIGNMENT;
+  return H3B_OK;
+}
+
+static int mx_gemm_out(const void* A, const void* sfA, int64_t M, const void* B, const void* sfB,
+                       int64_t N, int64_t K, const void* bias, int act, const void* residual,
+                       int64_t ldr, void* D, int dtype, int64_t ldd, cudaStream_t st) {
+  mxgemm::Args a;
+  int rc = mx_gemm_args(a, A, sfA, M, B, sfB, N, K);
+  if (rc != H3B_OK) return rc;
+  rc = make_tmap_16_sw128(&a.tmap_d, D, dtype, (uint64_t)M, (uint64_t)N, (uint64_t)ldd,
+                          mxgemm::OUT_COLS, 32);
+  if (rc != H3B_OK) return rc;
+  a.bias = bias;
+  a.residual = residual;
+  a.ldr = residual ? ldr : 0;
+  a.act = act;
+  return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(a, st)
+                             : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(a, st);
+}
+
+}  // namespace h3b
+
+extern "C" {
+
+int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
+                       void* sf, void* stream) {
+  if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldx < K) return H3B_ERR_INVALID_ARG;
+  if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
+  if (M == 0) return H3B_OK;
+  if (!x || !q || !sf) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(x) || !aligned16(q) || (ldx * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
+  const int64_t Mpad = (M + 127) / 128 * 128;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == H3B_DT_BF16) mx_quantize_launch<__nv_bfloat16>(x, M, K, ldx, q, sf, Mpad, st);
+  else if (dtype == H3B_DT_F16) mx_quantize_launch<__half>(x, M, K, ldx, q, sf, Mpad, st);
+  else mx_quantize_launch<float>(x, M, K, ldx, q, sf, Mpad, st);
+  return launched(cudaGetLastError());
+}
+
+int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, void* out, int dtype,
+                         int64_t ldo, void* stream) {
+  if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldo < K) return H3B_ERR_INVALID_ARG;
+  if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
+  if (M == 0) return H3B_OK;
+  if (!q || !sf || !out) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(out) || (ldo * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (dtype == H3B_DT_BF16) mx_dequantize_launch<__nv_bfloat16>(q, sf, M, K, out, ldo, st);
+  else if (dtype == H3B_DT_F16) mx_dequantize_launch<__half>(q, sf, M, K, out, ldo, st);
+  else mx_dequantize_launch<float>(q, sf, M, K, out, ldo, st);
+  return launched(cudaGetLastError());
+}
+
+int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, const void* sfB,
+                   int64_t N, int64_t K, const void* bias, int act, const void* residual,
+                   int64_t ldr, void* D, int dtype, int64_t ldd, void* stream) {
+  const int rc = mx_out_check(dtype, M, N, K, bias, act, residual, ldr, D, ldd);
+  if (rc != H3B_OK || M == 0) return rc;
+  return mx_gemm_out(A, sfA, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int64_t h3b_mxfp4_linear_ws(int64_t M, int64_t N, int64_t K) {
+  if (M < 0 || N <= 0 || K <= 0 || M > kMxMaxDim || K > kMxMaxDim) return 0;
+  return mx_operand_bytes(M, K);
+}
+
+int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const void* B,
+                     const void* sfB, int64_t N, int64_t K, const void* bias, int act,
+                     const void* residual, int64_t ldr, void* D, int64_t ldd, void* ws,
+                     int64_t ws_bytes, void* stream) {
+  int rc = mx_out_check(dtype, M, N, K, bias, act, residual, ldr, D, ldd);
+  if (rc != H3B_OK || M == 0) return rc;
+  if (!ws || ws_bytes < h3b_mxfp4_linear_ws(M, N, K)) return H3B_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return H3B_ERR_ALIGNMENT;
+  uint8_t* q = static_cast<uint8_t*>(ws);
+  uint8_t* sf = q + mx_code_bytes(M, K);
+  rc = h3b_mxfp4_quantize(x, dtype, M, K, ldx, q, sf, stream);
+  if (rc != H3B_OK) return rc;
+  return mx_gemm_out(q, sf, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
+                     static_cast<cudaStream_t>(stream));
+}
+
+int64_t h3b_mxfp4_ffn_ws(int64_t M, int64_t N, int64_t F) {
+  if (M < 0 || N <= 0 || F <= 0 || M > kMxMaxDim || N > kMxMaxDim || F > kMxMaxDim) return 0;
+  return mx_operand_bytes(M, N) + mx_operand_bytes(M, F);
+}
+
+int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* Bu,
+                  const void* sfBu, const void* Bd, const void* sfBd, int64_t N, int64_t F,
+                  const void* residual, int64_t ldr, void* D, int64_t ldd, void* ws,
+                  int64_t ws_bytes, void* stream) {
+  if (F <= 0 || F % 128 || F > kMxMaxDim / 2 || N % mx::BLOCK) return H3B_ERR_INVALID_ARG;
+  int rc = mx_out_check(dtype, M, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D, ldd);
+  if (rc != H3B_OK || M == 0) return rc;
+  if (!ws || ws_bytes < h3b_mxfp4_ffn_ws(M, N, F)) return H3B_ERR_INVALID_ARG;
+  if (reinterpret_cast<uintptr_t>(ws) & 255u) return H3B_ERR_ALIGNMENT;
+  uint8_t* q = static_cast<uint8_t*>(ws);
+  uint8_t* sf = q + mx_code_bytes(M, N);
+  uint8_t* qh = q + mx_operand_bytes(M, N);
+  uint8_t* sfh = qh + mx_code_bytes(M, F);
+  rc = h3b_mxfp4_quantize(x, dtype, M, N, ldx, q, sf, stream);
+  if (rc != H3B_OK) return rc;
+  mxgemm::Args a;
+  rc = mx_gemm_args(a, q, sf, M, Bu, sfBu, 2 * F, N);
+  if (rc != H3B_OK) return rc;
+  a.q_out = qh;
+  a.sf_out = sfh;
+  rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(a, static_cast<cudaStream_t>(stream));
+  if (rc != H3B_OK) return rc;
+  return mx_gemm_out(qh, sfh, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D, dtype,
+                     ldd, static_cast<cudaStream_t>(stream));
+}
+
+}  // extern "C"

@@ -1,0 +1,106 @@
+"""MXFP4 linears beside the NVFP4 ones of ``nvfp4.py``: E2M1 codes with one
+power-of-two (E8M0) scale per 32 values of K and no tensor-wide scale.
+
+Without a tensor-wide scale an activation is quantized in one pass, and the
+gated feed-forward's up projection writes its hidden activation as MXFP4 from
+its own epilogue.  Activations and results are bf16 or fp16, products
+accumulate in fp32.  As for NVFP4 there is no CPU path: without a CUDA device
+and the built library every entry point raises.
+"""
+from __future__ import annotations
+
+import torch
+from torch import nn
+
+from . import ops
+from .nvfp4 import _block_linears, _set_child
+
+MXFP4_BLOCK = ops.MX_BLOCK
+
+_ACTS = {None: ops.ACT_NONE, "gelu": ops.ACT_GELU_TANH}
+
+
+class MXFP4Weight:
+    """A quantized ``nn.Linear`` weight ``[out_features, in_features]``:
+    ``qdata`` u8 ``[N, K/2]`` (low nibble = even K) and ``scale`` the flat
+    blocked E8M0 bytes the GEMM reads."""
+
+    __slots__ = ("qdata", "scale", "out_features", "in_features")
+
+    def __init__(self, weight: torch.Tensor):
+        self.out_features, self.in_features = weight.shape
+        if self.out_features % 8:
+            raise ValueError(f"out_features = {self.out_features} must be a multiple of 8")
+        self.qdata, self.scale = ops.mxfp4_quantize(weight.detach())
+
+    @classmethod
+    def from_packed(cls, qdata: torch.Tensor, scale: torch.Tensor, out_features: int,
+                    in_features: int) -> "MXFP4Weight":
+        """From stored codes and blocked scales (checked when they are used)."""
+        w = cls.__new__(cls)
+        w.qdata, w.scale = qdata, scale
+        w.out_features, w.in_features = out_features, in_features
+        return w
+
+    def dequantize(self, dtype: torch.dtype = torch.bfloat16) -> torch.Tensor:
+        return ops.mxfp4_dequantize(self.qdata, self.scale, self.out_features, self.in_features,
+                                    dtype=dtype)
+
+    def nbytes(self) -> int:
+        return self.qdata.numel() + self.scale.numel()
+
+
+def mxfp4_linear(w: MXFP4Weight, x: torch.Tensor, *, bias: torch.Tensor | None = None,
+                 act: str | None = None, residual: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(Q(x) @ w.T + bias) + residual`` in x's type (bf16 or fp16);
+    ``act`` is None or "gelu" (tanh form)."""
+    if act not in _ACTS:
+        raise ValueError(f"unknown activation {act!r}")
+    return ops.mxfp4_linear(x, w.qdata, w.scale, w.out_features, w.in_features, bias=bias,
+                            act=_ACTS[act], residual=residual, out=out)
+
+
+def gated_up_weight(weight: torch.Tensor) -> MXFP4Weight:
+    """The fused [value | gate] up projection ``[2F, K]`` (the reference's chunk
+    order) as the weight ``gated_ffn`` takes: rows in ``ops.swiglu_rows``
+    order."""
+    return MXFP4Weight(weight[ops.swiglu_rows(weight.shape[0] // 2).to(weight.device)])
+
+
+def gated_ffn(up: MXFP4Weight, down: MXFP4Weight, x: torch.Tensor, *,
+              residual: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """``Q(v * silu(g)) @ down.T + residual`` with ``[v | g] = Q(x) @ up.T``
+    (``up`` from ``gated_up_weight``), in x's type."""
+    f = up.out_features // 2
+    if down.in_features != f or down.out_features != up.in_features or up.out_features % 2:
+        raise ValueError(f"up [{up.out_features}, {up.in_features}] and down "
+                         f"[{down.out_features}, {down.in_features}] do not form a feed-forward")
+    return ops.mxfp4_ffn(x, up.qdata, up.scale, down.qdata, down.scale, up.in_features, f,
+                         residual=residual, out=out)
+
+
+class MXFP4Linear(nn.Module):
+    """An MXFP4 linear, with or without bias."""
+
+    def __init__(self, linear: nn.Linear):
+        super().__init__()
+        self.weight_mxfp4 = MXFP4Weight(linear.weight.data)
+        self.in_features, self.out_features = linear.in_features, linear.out_features
+        self.bias = None if linear.bias is None else nn.Parameter(linear.bias.data,
+                                                                  requires_grad=False)
+
+    def forward(self, x: torch.Tensor) -> torch.Tensor:
+        return mxfp4_linear(self.weight_mxfp4, x, bias=self.bias)
+
+
+@torch.no_grad()
+def quantize_blocks(model) -> dict:
+    """Swap the six block linears of every transformer block for MXFP4 ones, as
+    ``nvfp4.quantize_blocks`` does for NVFP4."""
+    slots = [(parent, name) for block in model.transformer_blocks
+             for parent, name, _ in _block_linears(block)]
+    for parent, name in slots:
+        _set_child(parent, name, MXFP4Linear(parent._modules[name]))
+    return {"linears_quantized": len(slots)}

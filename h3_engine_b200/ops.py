@@ -365,3 +365,205 @@ def ada_modulate(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
     o2 = out.view(rows, C)
     _H3B.ada_modulate(x2, x2.stride(0), sc, sh, i2, n, rows, C, o2, o2.stride(0))
     return out
+
+
+# ---------------------------------------------------------------- MXFP4
+MX_BLOCK = 32
+_16BIT = (torch.bfloat16, torch.float16)
+
+
+def mxfp4_sf_bytes(rows: int, k: int) -> int:
+    """Bytes of the blocked E8M0 scales of ``rows`` x ``k`` values (rows padded
+    to 128, scale columns to 4)."""
+    return pad_m(rows) // 128 * (-(-k // 128)) * 512
+
+
+def _mx_rows(t: torch.Tensor) -> torch.Tensor:
+    """A [rows, K] view with a contiguous last dim and 16-byte aligned rows (a
+    copy only when the layout needs one)."""
+    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
+    size = t2.element_size()
+    if t2.stride(1) != 1 or t2.stride(0) * size % 16 or t2.storage_offset() * size % 16 \
+            or t2.stride(0) < t2.shape[1]:
+        t2 = t2.clone(memory_format=torch.contiguous_format)
+    return t2
+
+
+def _mx_operand(q: torch.Tensor, sf: torch.Tensor, rows: int, k: int, what: str) -> None:
+    if q.dtype != torch.uint8 or sf.dtype != torch.uint8:
+        raise TypeError(f"{what}: codes and scales must be uint8")
+    if k <= 0 or k % MX_BLOCK:
+        raise ValueError(f"{what}: K = {k} must be a positive multiple of {MX_BLOCK}")
+    if not (q.is_contiguous() and sf.is_contiguous()):
+        raise ValueError(f"{what}: codes and scales must be contiguous")
+    if q.numel() < rows * (k // 2) or sf.numel() < mxfp4_sf_bytes(rows, k):
+        raise ValueError(f"{what}: codes or scales too small for {rows} x {k} values")
+
+
+def _mx_out(out: torch.Tensor | None, m: int, n: int, dtype: torch.dtype, dev,
+            lead: torch.Size) -> tuple[torch.Tensor, torch.Tensor, int]:
+    """(the tensor to return, the [m, n] view the kernel writes, its row stride)."""
+    if out is None:
+        out = torch.empty(*lead, n, dtype=dtype, device=dev)
+        return out, out, n
+    if out.dtype != dtype or out.shape != (*lead, n):
+        raise ValueError(f"out must be {dtype} {(*lead, n)}")
+    o2 = out if out.dim() == 2 else out.view(m, n)
+    size = o2.element_size()
+    if m and (o2.stride(1) != 1 or o2.stride(0) * size % 16 or o2.stride(0) < n
+              or o2.storage_offset() * size % 16):
+        raise ValueError("out must have contiguous, 16-byte aligned rows")
+    torch.autograd.graph.increment_version(out)
+    return out, o2, o2.stride(0)
+
+
+def _mx_residual(residual: torch.Tensor | None, m: int, n: int, dtype: torch.dtype):
+    if residual is None:
+        return None, 0
+    if residual.dtype != dtype or residual.numel() != m * n or residual.shape[-1] != n:
+        raise ValueError(f"residual must be {dtype} with {m} rows of {n}")
+    r2 = _mx_rows(residual)
+    return r2, r2.stride(0)
+
+
+def _mx_bias(bias: torch.Tensor | None, n: int, dtype: torch.dtype) -> torch.Tensor | None:
+    if bias is None:
+        return None
+    if bias.dtype != dtype or bias.shape != (n,):
+        raise ValueError(f"bias must be {dtype} [{n}]")
+    if bias.stride(0) != 1 or bias.storage_offset() % 8:
+        bias = bias.clone(memory_format=torch.contiguous_format)
+    return bias
+
+
+def _mx_act(act: int) -> None:
+    if act not in (ACT_NONE, ACT_GELU_TANH):
+        raise ValueError("the MXFP4 products take ACT_NONE or ACT_GELU_TANH")
+
+
+def mxfp4_quantize(x: torch.Tensor, *, q_out: torch.Tensor | None = None,
+                   sf_out: torch.Tensor | None = None):
+    """bf16, fp16 or fp32 ``[..., K]`` -> (codes u8 ``[M, K/2]``, blocked E8M0
+    scales u8, flat): MXFP4, one power-of-two scale per 32 values and no
+    tensor-wide scale, so no amax pass.  ``K % 32 == 0``.  A block holding an
+    infinity or a NaN becomes NaN as a whole."""
+    dev = _need_cuda(x, q_out, sf_out)
+    if x.dtype not in torch_ops.DTYPES:
+        raise TypeError(f"mxfp4_quantize takes bf16, fp16 or fp32, not {x.dtype}")
+    K = x.shape[-1]
+    if K <= 0 or K % MX_BLOCK:
+        raise ValueError(f"K = {K} must be a positive multiple of {MX_BLOCK}")
+    x2 = _mx_rows(x)
+    M = x2.shape[0]
+    if q_out is None:
+        q_out = torch.empty(M, K // 2, dtype=torch.uint8, device=dev)
+    else:
+        torch.autograd.graph.increment_version(q_out)
+    if sf_out is None:
+        sf_out = torch.empty(mxfp4_sf_bytes(M, K), dtype=torch.uint8, device=dev)
+    else:
+        torch.autograd.graph.increment_version(sf_out)
+    _mx_operand(q_out, sf_out, M, K, "mxfp4_quantize")
+    if M:
+        _H3B.mxfp4_quantize(x2, M, K, x2.stride(0), q_out, sf_out)
+    return q_out, sf_out
+
+
+def mxfp4_dequantize(q: torch.Tensor, sf: torch.Tensor, M: int, K: int, *,
+                     dtype: torch.dtype = torch.bfloat16,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """``[M, K]`` values of MXFP4 codes and blocked scales (exact in bf16 and
+    fp32, rounded in fp16)."""
+    dev = _need_cuda(q, sf, out)
+    if dtype not in torch_ops.DTYPES:
+        raise TypeError(f"mxfp4_dequantize gives bf16, fp16 or fp32, not {dtype}")
+    _mx_operand(q, sf, M, K, "mxfp4_dequantize")
+    out, o2, ldo = _mx_out(out, M, K, dtype, dev, (M,))
+    if M:
+        _H3B.mxfp4_dequantize(q, sf, M, K, o2, ldo)
+    return out
+
+
+def mxfp4_gemm(qa: torch.Tensor, sfa: torch.Tensor, M: int, qb: torch.Tensor, sfb: torch.Tensor,
+               N: int, K: int, *, bias: torch.Tensor | None = None, act: int = ACT_NONE,
+               residual: torch.Tensor | None = None, dtype: torch.dtype = torch.bfloat16,
+               out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(deq(qa) @ deq(qb)^T + bias) + residual`` in bf16 or fp16
+    ``[M, N]``, accumulated in fp32, both operands MXFP4 (``mxfp4_quantize``).
+    ``K % 32 == 0``, ``N % 8 == 0``."""
+    dev = _need_cuda(qa, sfa, qb, sfb, bias, residual, out)
+    if dtype not in _16BIT:
+        raise TypeError(f"mxfp4_gemm gives bf16 or fp16, not {dtype}")
+    if N <= 0 or N % 8:
+        raise ValueError(f"N = {N} must be a positive multiple of 8")
+    _mx_act(act)
+    _mx_operand(qa, sfa, M, K, "mxfp4_gemm: A")
+    _mx_operand(qb, sfb, N, K, "mxfp4_gemm: B")
+    bias = _mx_bias(bias, N, dtype)
+    residual, ldr = _mx_residual(residual, M, N, dtype)
+    out, o2, ldd = _mx_out(out, M, N, dtype, dev, (M,))
+    if M:
+        _H3B.mxfp4_gemm(qa, sfa, M, qb, sfb, N, K, bias, act, residual, ldr, o2, ldd)
+    return out
+
+
+def _mx_input(x: torch.Tensor, K: int) -> torch.Tensor:
+    if x.dtype not in _16BIT:
+        raise TypeError(f"MXFP4 products take bf16 or fp16 activations, not {x.dtype}")
+    if x.shape[-1] != K:
+        raise ValueError(f"activation width {x.shape[-1]} != in_features {K}")
+    return _mx_rows(x)
+
+
+def mxfp4_linear(x: torch.Tensor, qb: torch.Tensor, sfb: torch.Tensor, N: int, K: int, *,
+                 bias: torch.Tensor | None = None, act: int = ACT_NONE,
+                 residual: torch.Tensor | None = None,
+                 out: torch.Tensor | None = None) -> torch.Tensor:
+    """``act(Q(x) @ deq(qb)^T + bias) + residual`` in x's type for ``x``
+    ``[..., K]`` bf16 or fp16: quantization and product in one call, from one
+    token to whole sequences."""
+    dev = _need_cuda(x, qb, sfb, bias, residual, out)
+    if N <= 0 or N % 8:
+        raise ValueError(f"N = {N} must be a positive multiple of 8")
+    _mx_act(act)
+    _mx_operand(qb, sfb, N, K, "mxfp4_linear: weight")
+    x2 = _mx_input(x, K)
+    M = x2.shape[0]
+    bias = _mx_bias(bias, N, x.dtype)
+    residual, ldr = _mx_residual(residual, M, N, x.dtype)
+    out, o2, ldd = _mx_out(out, M, N, x.dtype, dev, x.shape[:-1])
+    if M:
+        ws = torch.empty(_mx_operand_bytes(M, K), dtype=torch.uint8, device=dev)
+        _H3B.mxfp4_linear(x2, M, x2.stride(0), qb, sfb, N, K, bias, act, residual, ldr, o2, ldd,
+                          ws)
+    return out
+
+
+def _mx_operand_bytes(rows: int, k: int) -> int:
+    """Workspace of one quantized activation (h3b_mxfp4_linear_ws): its codes,
+    rounded up to 256 bytes, and its blocked scales."""
+    return -(-rows * (k // 2) // 256) * 256 + mxfp4_sf_bytes(rows, k)
+
+
+def mxfp4_ffn(x: torch.Tensor, qu: torch.Tensor, sfu: torch.Tensor, qd: torch.Tensor,
+              sfd: torch.Tensor, N: int, F: int, *, residual: torch.Tensor | None = None,
+              out: torch.Tensor | None = None) -> torch.Tensor:
+    """The gated feed-forward ``Q(v * silu(g)) @ deq(qd)^T + residual`` with
+    ``[v | g] = Q(x) @ deq(qu)^T`` for ``x`` ``[..., N]`` bf16 or fp16: ``qu``
+    the up projection's 2F rows in ``swiglu_rows`` order, ``qd`` ``[N, F]``.
+    The hidden activation is quantized in the up projection's epilogue.
+    ``N % 32 == 0``, ``F % 128 == 0``."""
+    dev = _need_cuda(x, qu, sfu, qd, sfd, residual, out)
+    if F <= 0 or F % 128:
+        raise ValueError(f"feed-forward width {F} must be a positive multiple of 128")
+    _mx_operand(qu, sfu, 2 * F, N, "mxfp4_ffn: up projection")
+    _mx_operand(qd, sfd, N, F, "mxfp4_ffn: down projection")
+    x2 = _mx_input(x, N)
+    M = x2.shape[0]
+    residual, ldr = _mx_residual(residual, M, N, x.dtype)
+    out, o2, ldd = _mx_out(out, M, N, x.dtype, dev, x.shape[:-1])
+    if M:
+        ws = torch.empty(_mx_operand_bytes(M, N) + _mx_operand_bytes(M, F), dtype=torch.uint8,
+                         device=dev)
+        _H3B.mxfp4_ffn(x2, M, x2.stride(0), qu, sfu, qd, sfd, N, F, residual, ldr, o2, ldd, ws)
+    return out

@@ -186,3 +186,73 @@ def amax_exchange(amax: torch.Tensor, slot_table: torch.Tensor, rank: int, world
     """amax[0] = max over the ranks of each rank's amax[0], through peer
     memory (h3b_amax_exchange); slot_table: int64 [world] device pointers."""
     _run(amax, "h3b_amax_exchange", _p(amax), _p(slot_table), rank, world, epoch, limit_us)
+
+
+# ---------------------------------------------------------------- MXFP4 and windowed attention
+# These operators serve single tokens too, where the dispatch costs as much as
+# the kernel, so they are registered with the lighter ``torch.library.Library``
+# interface (same schema rules: mutated outputs declared, CUDA only, fake
+# implementations).  Their wrappers in ops.py bump the version counter of an
+# output that the caller passed in.
+_LIGHT = torch.library.Library("h3b", "FRAGMENT")
+DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+
+
+def _light(schema: str):
+    def wrap(fn):
+        name = schema.split("(", 1)[0]
+        _LIGHT.define(schema)
+        _LIGHT.impl(name, fn, "CUDA")
+        torch.library.register_fake(f"h3b::{name}", _no_output, lib=_LIGHT)
+        return fn
+    return wrap
+
+
+def _call(t: torch.Tensor, name: str, *args) -> None:
+    """As ``_run``, entering the device guard only when it changes anything."""
+    dev = t.device.index
+    fn = getattr(_lib.lib(), name)
+    if dev == torch.cuda.current_device():
+        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    else:
+        with torch.cuda.device(dev):
+            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
+    if st:
+        _lib.check(st, name)
+
+
+@_light("mxfp4_quantize(Tensor x, int rows, int cols, int ldx, Tensor(a!) q, Tensor(b!) sf) -> ()")
+def mxfp4_quantize(x, rows, cols, ldx, q, sf):
+    """E2M1 codes and blocked E8M0 scales of a [rows, cols] view (h3b_mxfp4_quantize)."""
+    _call(q, "h3b_mxfp4_quantize", _p(x), DTYPES[x.dtype], rows, cols, ldx, _p(q), _p(sf))
+
+
+@_light("mxfp4_dequantize(Tensor q, Tensor sf, int rows, int cols, Tensor(a!) out, int ldo) -> ()")
+def mxfp4_dequantize(q, sf, rows, cols, out, ldo):
+    """Codes times scales in out's type (h3b_mxfp4_dequantize)."""
+    _call(out, "h3b_mxfp4_dequantize", _p(q), _p(sf), rows, cols, _p(out), DTYPES[out.dtype], ldo)
+
+
+@_light("mxfp4_gemm(Tensor qa, Tensor sfa, int m, Tensor qb, Tensor sfb, int n, int k, "
+        "Tensor? bias, int act, Tensor? residual, int ldr, Tensor(a!) out, int ldd) -> ()")
+def mxfp4_gemm(qa, sfa, m, qb, sfb, n, k, bias, act, residual, ldr, out, ldd):
+    """Block-scaled MXFP4 GEMM with the fused epilogue (h3b_mxfp4_gemm)."""
+    _call(out, "h3b_mxfp4_gemm", _p(qa), _p(sfa), m, _p(qb), _p(sfb), n, k, _p(bias), act,
+          _p(residual), ldr, _p(out), DTYPES[out.dtype], ldd)
+
+
+@_light("mxfp4_linear(Tensor x, int m, int ldx, Tensor qb, Tensor sfb, int n, int k, "
+        "Tensor? bias, int act, Tensor? residual, int ldr, Tensor(a!) out, int ldd, "
+        "Tensor(b!) ws) -> ()")
+def mxfp4_linear(x, m, ldx, qb, sfb, n, k, bias, act, residual, ldr, out, ldd, ws):
+    """act(Q(x) W^T + bias) + residual (h3b_mxfp4_linear)."""
+    _call(out, "h3b_mxfp4_linear", _p(x), DTYPES[x.dtype], m, ldx, _p(qb), _p(sfb), n, k, _p(bias),
+          act, _p(residual), ldr, _p(out), ldd, _p(ws), ws.numel())
+
+
+@_light("mxfp4_ffn(Tensor x, int m, int ldx, Tensor qu, Tensor sfu, Tensor qd, Tensor sfd, int n, "
+        "int f, Tensor? residual, int ldr, Tensor(a!) out, int ldd, Tensor(b!) ws) -> ()")
+def mxfp4_ffn(x, m, ldx, qu, sfu, qd, sfd, n, f, residual, ldr, out, ldd, ws):
+    """Q(v * silu(g)) Wd^T + residual, [v | g] = Q(x) Wu^T (h3b_mxfp4_ffn)."""
+    _call(out, "h3b_mxfp4_ffn", _p(x), DTYPES[x.dtype], m, ldx, _p(qu), _p(sfu), _p(qd), _p(sfd),
+          n, f, _p(residual), ldr, _p(out), ldd, _p(ws), ws.numel())

@@ -45,6 +45,9 @@ enum { H3B_SF_ROWMAJOR = 0,  /* e4m3 [rows, K/16], row-major                    
 /* GEMM epilogue activations. */
 enum { H3B_ACT_NONE = 0, H3B_ACT_GELU_TANH = 1, H3B_ACT_SWIGLU = 2 };
 
+/* Element types of the MXFP4 and windowed-attention entry points. */
+enum { H3B_DT_BF16 = 0, H3B_DT_F16 = 1, H3B_DT_F32 = 2 };
+
 /* ------------------------------------------------------------------ library */
 H3B_API int h3b_version(void);
 H3B_API const char* h3b_status_string(int status);
@@ -286,6 +289,59 @@ H3B_API int h3b_peer_buffer_close(void* dev_ptr);
 H3B_API int h3b_peer_buffer_destroy(void* dev_ptr);
 H3B_API int h3b_amax_exchange(float* amax, const void* slot_table, int rank, int world,
                               int64_t epoch, int64_t limit_us, void* stream);
+
+/* ------------------------------------------------------------------ MXFP4
+ * Microscaled 4-bit floating point, beside the NVFP4 forms above: E2M1 codes,
+ * one E8M0 scale (a power of two) per 32 consecutive values of a row and no
+ * tensor-wide scale.  Per block: e = floor(log2(max |x|)) - 2, not below -127,
+ * stored as the byte e + 127 (0 for a block of zeros, 0xFF = NaN for a block
+ * with an infinity or a NaN); code = E2M1 round-to-nearest-even of x / 2^e,
+ * saturating, sign kept.
+ *   codes   u8 [rows, K/2], low nibble = even K index; K % 32 == 0
+ *   scales  128 x 4 tiles of 512 bytes as for NVFP4 (H3B_SF_SWIZZLED) with
+ *           C = K/32 columns: rows padded to a multiple of 128, columns to a
+ *           multiple of 4; the padding columns of the rows in use are zero.
+ *           pad128(rows) / 128 * ceil(K / 128) * 512 bytes.
+ *
+ * Quantize: x [M, K] of `dtype` (bf16, fp16 or fp32), row stride ldx elements;
+ * x, q and ldx * size are 16-byte aligned.  The scales of the padding rows are
+ * written as zero; codes are written for the M rows only.                    */
+H3B_API int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
+                               void* q, void* sf, void* stream);
+/* out [M, K] of `dtype`, row stride ldo: codes times scales, rounded to dtype. */
+H3B_API int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, void* out,
+                                 int dtype, int64_t ldo, void* stream);
+
+/* D[M, N] (bf16 or fp16, row stride ldd) = act(A B^T + bias) + residual,
+ * accumulated in fp32; A [M, K] and B [N, K] as MXFP4, bias [N] and residual
+ * [M, N] (row stride ldr) optional and of D's type; act is H3B_ACT_NONE or
+ * H3B_ACT_GELU_TANH.  K % 32 == 0, N % 8 == 0, every pointer 16-byte aligned,
+ * ldd and ldr multiples of 8.                                               */
+H3B_API int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B,
+                           const void* sfB, int64_t N, int64_t K, const void* bias, int act,
+                           const void* residual, int64_t ldr, void* D, int dtype, int64_t ldd,
+                           void* stream);
+
+/* h3b_mxfp4_linear: the same with A = x [M, K] of D's type (row stride ldx),
+ * quantized on the way.  `ws`: h3b_mxfp4_linear_ws(M, N, K) bytes of scratch,
+ * 256-byte aligned, private to this call until it has run.                  */
+H3B_API int64_t h3b_mxfp4_linear_ws(int64_t M, int64_t N, int64_t K);
+H3B_API int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const void* B,
+                             const void* sfB, int64_t N, int64_t K, const void* bias, int act,
+                             const void* residual, int64_t ldr, void* D, int64_t ldd, void* ws,
+                             int64_t ws_bytes, void* stream);
+
+/* Gated feed-forward: D[M, N] = Q(v * silu(g)) Bd^T + residual with
+ * [v | g] = Q(x) Bu^T; x [M, N], Bu [2F, N] with its rows in the order that
+ * H3B_ACT_SWIGLU of h3b_nvfp4_gemm describes, Bd [N, F].  v, g and their
+ * product stay in fp32 up to the MXFP4 rounding, which the up projection's
+ * epilogue does itself: the hidden activation exists only as MXFP4.
+ * N % 32 == 0, F % 128 == 0.  `ws`: h3b_mxfp4_ffn_ws(M, N, F) bytes.        */
+H3B_API int64_t h3b_mxfp4_ffn_ws(int64_t M, int64_t N, int64_t F);
+H3B_API int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* Bu,
+                          const void* sfBu, const void* Bd, const void* sfBd, int64_t N,
+                          int64_t F, const void* residual, int64_t ldr, void* D, int64_t ldd,
+                          void* ws, int64_t ws_bytes, void* stream);
 
 #ifdef __cplusplus
 }
