@@ -1,0 +1,327 @@
+// Windowed attention of a few new tokens per sequence against a cache, lengths
+// read on the device (so a captured launch serves every step): the visibility
+// rule of attention_window.cuh for queries at positions len - n_new ... len - 1.
+//
+// Bound by reading the visible keys and values once.  The rows that share a key
+// head, n_new tokens times the group's query heads, form the 16 rows of one
+// mma.sync m16n8k16 tile; a warp's work is a 16-row flash pass over key tiles
+// of kKeys, K and V copied by cp.async into its own ring of stages (no barrier
+// among warps).  A cluster of CTAs along the keys shares a (sequence, key
+// head): tile i belongs to warp i mod (cluster warps), and the partial results
+// (maximum, sum, unnormalised output, all fp32) are joined first in a CTA's
+// shared memory, then across the cluster through distributed shared memory,
+// always in the same order.
+#pragma once
+
+#include "attention_window.cuh"
+
+namespace h3b {
+namespace wdec {
+
+constexpr int kWarps = 4;
+constexpr int kThreads = kWarps * 32;
+constexpr int kRows = 16;
+constexpr int kKeys = 16;           // keys per tile
+constexpr int kMaxCluster = 8;
+
+template <int D>
+struct Smem {
+  static constexpr int kStages = 4;
+  static constexpr int TILE = kKeys * D * 2;                  // K or V of one stage
+  static constexpr int STAGE = 2 * TILE;
+  static constexpr int WARP = kStages * STAGE;
+  static constexpr int RING = kWarps * WARP;
+  // after the pass: per warp and then per CTA 16 x D fp32 plus 16 (max, sum)
+  static constexpr int PART = kRows * D * 4 + kRows * 8;
+  static constexpr int BYTES = RING > kWarps * PART ? RING : kWarps * PART;
+};
+
+struct Args {
+  const void *q, *k, *v;
+  void* out;                        // [B, n_new, H, D] contiguous
+  const int32_t* len;               // [B] keys in use, the new tokens' own included
+  long long q_b, q_t, q_h;          // strides in elements
+  long long k_b, k_s, k_h, v_b, v_s, v_h;
+  int room, n_new, H, kv_heads, group;
+  int left, right, sinks, causal;
+  float scale_log2;
+};
+
+__device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, uint32_t bytes) {
+  asm volatile("cp.async.cg.shared.global [%0], [%1], 16, %2;" ::"r"(dst), "l"(src), "r"(bytes)
+               : "memory");
+}
+__device__ __forceinline__ void cp_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int N>
+__device__ __forceinline__ void cp_wait() {
+  asm volatile("cp.async.wait_group %0;" ::"n"(N) : "memory");
+}
+__device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+__device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
+  asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
+}
+template <typename T>
+__device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
+                                         uint32_t b1) {
+  if constexpr (std::is_same<T, __half>::value)
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, "
+                 "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+  else
+    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, "
+                 "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
+                 : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
+                 : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
+}
+__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
+  float v;
+  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+  return v;
+}
+__device__ __forceinline__ uint32_t cluster_nctarank() {
+  uint32_t r;
+  asm volatile("mov.u32 %0, %%cluster_nctarank;" : "=r"(r));
+  return r;
+}
+
+// Joins (m, l) pairs: the weight of a partial whose maximum is m in a total
+// whose maximum is top; a partial that saw nothing (m = -inf) weighs 0.
+__device__ __forceinline__ float weight(float m, float top) {
+  return m == -INFINITY ? 0.f : attn::ex2(m - top);
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constant__ Args p) {
+  using L = Smem<D>;
+  constexpr int CH = D / 8;                       // 16-byte chunks of a row
+  extern __shared__ __align__(128) uint8_t smem[];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
+  const int rows_all = p.n_new * p.group;
+  const int row_tiles = (rows_all + kRows - 1) / kRows;
+  const int kvh = blockIdx.y / row_tiles;
+  const int row0 = (blockIdx.y % row_tiles) * kRows;
+  const int rows = min(kRows, rows_all - row0);
+  const int b = blockIdx.z;
+  const int n = min(max(__ldg(p.len + b), 0), p.room);
+
+  // keys that any of this tile's rows sees: [0, sink_end) and [lo, end), visited
+  // as one list of `total` keys
+  const int t0 = row0 / p.group, t1 = (row0 + rows - 1) / p.group;
+  const int p0 = n - p.n_new + t0, p1 = n - p.n_new + t1;
+  const int top = p.causal ? min(p1, n - 1) : n - 1;
+  int sink_end = max(0, min(p.sinks, top + 1));
+  int lo = max(0, p0 - p.left);
+  int end = min(top, p1 + p.right) + 1;
+  if (end > lo && sink_end >= lo) {               // they touch: one range from 0
+    end = max(end, sink_end);
+    lo = 0;
+    sink_end = 0;
+  }
+  const int total = sink_end + max(0, end - lo);
+  const int tiles = (total + kKeys - 1) / kKeys;
+
+  // Q as A fragments: rows lane / 4 and + 8, dims (lane % 4) * 2 + {0, 1} and + 8
+  uint32_t qf[D / 16][4];
+  int pos[2];                                     // key position of this lane's two rows
+#pragma unroll
+  for (int i = 0; i < 2; ++i) {
+    const int r = (lane >> 2) + 8 * i;
+    const bool ok = r < rows;
+    const int t = (row0 + min(r, rows - 1)) / p.group;
+    const int g = (row0 + min(r, rows - 1)) % p.group;
+    pos[i] = n - p.n_new + t;
+    const T* q = static_cast<const T*>(p.q) + b * p.q_b + t * p.q_t +
+                 (long long)(kvh * p.group + g) * p.q_h + (lane & 3) * 2;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      qf[kk][i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
+      qf[kk][2 + i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16 + 8)) : 0u;
+    }
+  }
+
+  float o[D / 8][4];
+#pragma unroll
+  for (int i = 0; i < D / 8; ++i)
+#pragma unroll
+    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
+  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+
+  const T* kb = static_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
+  const T* vb = static_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
+  const uint32_t ring = smem_u32(smem) + warp * L::WARP;
+  const int first = rank * kWarps + warp, stride = ranks * kWarps;
+
+  // copy tile i into stage s; keys behind the last are filled with zeros
+  auto fetch = [&](int i, int s) {
+    if (i < tiles) {
+#pragma unroll
+      for (int c = lane; c < kKeys * CH; c += 32) {
+        const int r = c / CH, ch = c % CH;
+        const int u = i * kKeys + r;
+        const bool ok = u < total;
+        const long long key = !ok ? 0 : u < sink_end ? u : lo + (u - sink_end);
+        const uint32_t dst = ring + s * L::STAGE + r * (D * 2) + ((ch ^ (r & 7)) << 4);
+        cp_async16(dst, kb + key * p.k_s + ch * 8, ok ? 16 : 0);
+        cp_async16(dst + L::TILE, vb + key * p.v_s + ch * 8, ok ? 16 : 0);
+      }
+    }
+    cp_commit();
+  };
+  // ldmatrix: lane i of the warp gives the address of row i % 8 of matrix i / 8
+  const int lr = lane & 7, lm = lane >> 3;
+
+#pragma unroll
+  for (int s = 0; s < L::kStages - 1; ++s) fetch(first + s * stride, s);
+  int s = 0;
+  for (int i = first; i < tiles; i += stride) {
+    fetch(i + (L::kStages - 1) * stride, (s + L::kStages - 1) % L::kStages);
+    cp_wait<L::kStages - 1>();
+    __syncwarp();
+    const uint32_t ks = ring + s * L::STAGE, vs = ks + L::TILE;
+    float sc[2][4];                               // S of keys 0-7 and 8-15
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) sc[j][c] = 0.f;
+#pragma unroll
+    for (int kk = 0; kk < D / 16; ++kk) {
+      // matrices: keys 0-7 dims 0-7, dims 8-15, keys 8-15 dims 0-7, dims 8-15
+      const int r = lr + (lm >> 1) * 8, ch = kk * 2 + (lm & 1);
+      uint32_t f[4];
+      ldsm4(ks + r * (D * 2) + ((ch ^ (r & 7)) << 4), f);
+      mma16816<T>(sc[0], qf[kk], f[0], f[1]);
+      mma16816<T>(sc[1], qf[kk], f[2], f[3]);
+    }
+    // visibility and scaling (log2 units)
+    const int u0 = i * kKeys + (lane & 3) * 2;
+    float mx[2] = {-INFINITY, -INFINITY};
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        const int u = u0 + j * 8 + (c & 1);
+        const int key = u < sink_end ? u : lo + (u - sink_end);
+        const int ps = pos[c >> 1];
+        const bool near = key >= ps - p.left && key <= ps + p.right;
+        const bool seen = u < total && (near || key < p.sinks) && (!p.causal || key <= ps);
+        sc[j][c] = seen ? sc[j][c] * p.scale_log2 : -INFINITY;
+        mx[c >> 1] = fmaxf(mx[c >> 1], sc[j][c]);
+      }
+    float al[2], mb[2];
+#pragma unroll
+    for (int h = 0; h < 2; ++h) {
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
+      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
+      const float mn = fmaxf(m[h], mx[h]);
+      mb[h] = mn == -INFINITY ? 0.f : mn;
+      al[h] = attn::ex2(m[h] - mb[h]);            // 0 while nothing was seen
+      m[h] = mn;
+    }
+    uint32_t pf[4];
+    float sum[2] = {0.f, 0.f};
+#pragma unroll
+    for (int j = 0; j < 2; ++j) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        sc[j][c] = attn::ex2(sc[j][c] - mb[c >> 1]);
+        sum[c >> 1] += sc[j][c];
+      }
+      pf[j * 2] = wattn::pack16<T>(sc[j][0], sc[j][1]);
+      pf[j * 2 + 1] = wattn::pack16<T>(sc[j][2], sc[j][3]);
+    }
+#pragma unroll
+    for (int h = 0; h < 2; ++h) l[h] = l[h] * al[h] + sum[h];
+    if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+#pragma unroll
+      for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+        for (int c = 0; c < 4; ++c) o[d][c] *= al[c >> 1];
+    }
+#pragma unroll
+    for (int dd = 0; dd < D / 16; ++dd) {
+      // transposed matrices: keys 0-7 dims 0-7, keys 8-15 dims 0-7, then dims 8-15
+      const int r = lr + (lm & 1) * 8, ch = dd * 2 + (lm >> 1);
+      uint32_t f[4];
+      ldsm4_t(vs + r * (D * 2) + ((ch ^ (r & 7)) << 4), f);
+      mma16816<T>(o[2 * dd], pf, f[0], f[1]);
+      mma16816<T>(o[2 * dd + 1], pf, f[2], f[3]);
+    }
+    __syncwarp();
+    s = (s + 1) % L::kStages;
+  }
+  cp_wait<0>();
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
+    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
+  }
+  __syncthreads();                                // every warp is done with its ring
+
+  // partials: part w at w * PART: O [16][D] fp32, then 16 (m, l)
+  auto part_o = [&](int w) { return reinterpret_cast<float*>(smem + w * L::PART); };
+  auto part_ml = [&](int w) {
+    return reinterpret_cast<float2*>(smem + w * L::PART + kRows * D * 4);
+  };
+  {
+    float* po = part_o(warp);
+#pragma unroll
+    for (int d = 0; d < D / 8; ++d)
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        *reinterpret_cast<float2*>(po + ((lane >> 2) + 8 * h) * D + d * 8 + (lane & 3) * 2) =
+            make_float2(o[d][2 * h], o[d][2 * h + 1]);
+    if ((lane & 3) == 0) {
+#pragma unroll
+      for (int h = 0; h < 2; ++h)
+        part_ml(warp)[(lane >> 2) + 8 * h] = make_float2(m[h], l[h]);
+    }
+  }
+  __syncthreads();
+  // the CTA's own total, into part 0 (each thread owns its elements)
+  float2 ml_tot = make_float2(-INFINITY, 0.f);
+  const int r_own = threadIdx.x & 15;
+  for (int w = 0; w < kWarps; ++w) ml_tot.x = fmaxf(ml_tot.x, part_ml(w)[r_own].x);
+  for (int w = 0; w < kWarps; ++w)
+    ml_tot.y += weight(part_ml(w)[r_own].x, ml_tot.x) * part_ml(w)[r_own].y;
+  for (int e = threadIdx.x; e < rows * D; e += kThreads) {
+    const int r = e / D;
+    float mm = -INFINITY, acc = 0.f;
+    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, part_ml(w)[r].x);
+    for (int w = 0; w < kWarps; ++w) acc += weight(part_ml(w)[r].x, mm) * part_o(w)[e];
+    part_o(0)[e] = acc;
+  }
+  __syncthreads();
+  if (threadIdx.x < kRows) part_ml(0)[threadIdx.x] = ml_tot;
+  // the cluster's total: this CTA's share of the rows' elements
+  cluster_sync_all();
+  const uint32_t base = smem_u32(smem);
+  for (int e = rank * kThreads + threadIdx.x; e < rows * (D / 2); e += ranks * kThreads) {
+    const int r = e / (D / 2), d = (e % (D / 2)) * 2;
+    float mm = -INFINITY, ll = 0.f, a0 = 0.f, a1 = 0.f;
+    for (int c = 0; c < ranks; ++c)
+      mm = fmaxf(mm, ld_cluster_f32(mapa_shared(base + kRows * D * 4 + r * 8, c)));
+    for (int c = 0; c < ranks; ++c) {
+      const uint32_t ml = mapa_shared(base + kRows * D * 4 + r * 8, c);
+      const uint32_t po = mapa_shared(base + (r * D + d) * 4, c);
+      const float w = weight(ld_cluster_f32(ml), mm);
+      ll += w * ld_cluster_f32(ml + 4);
+      a0 += w * ld_cluster_f32(po);
+      a1 += w * ld_cluster_f32(po + 4);
+    }
+    const int t = (row0 + r) / p.group, g = (row0 + r) % p.group;
+    const size_t at = (((size_t)b * p.n_new + t) * p.H + kvh * p.group + g) * D + d;
+    const float inv = 1.0f / ll;
+    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at) =
+        ll != 0.f ? wattn::pack16<T>(a0 * inv, a1 * inv) : 0u;
+  }
+  cluster_sync_all();                             // nobody leaves while its memory is read
+}
+
+}  // namespace wdec
+}  // namespace h3b

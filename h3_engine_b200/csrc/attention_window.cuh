@@ -1,0 +1,543 @@
+// Packed attention with a sliding window and sinks on the 5th-generation
+// tensor cores: bf16 or fp16, head_dim 64 or 128, key heads shared by groups
+// of query heads, fp32 softmax and accumulation.
+//
+// Query i of a document with n_q queries and n_k keys stands at key position
+// p = i + n_k - n_q and sees key j iff
+//     (p - left <= j <= p + right  or  j < sinks)  and  (not causal or j <= p).
+// A query that sees no key gets zeros.
+//
+// One CTA = two 128-row query tiles (A, B) of one head of one document, the
+// roles, TMEM layout and MMA order of attention.cuh.  Of the document's keys it
+// visits only those that some query of the pair sees: the sink keys
+// [0, sink_end) and the window [lo, hi], each in steps of 128 keys that start
+// at 0 and at lo (TMA rows need no alignment, so the first step of the window
+// starts at its first key); the two are one range where they touch.  A step that no query of tile A (or B) sees is skipped for that tile:
+// neither its MMAs nor its softmax run, which is what the window's triangular
+// ends cost least with.  Steps all of whose keys a warp's 32 rows see take the
+// unmasked path; the others build a 128-bit visibility mask per row.
+//
+// Rows of V behind the last visible key of a step (the document's end, the
+// next document, the gap behind the sinks) are cleared in shared memory before
+// the MMA reads them: their P is 0, and 0 times what lies there must be 0.
+#pragma once
+
+#include <cuda_fp16.h>
+
+#include <type_traits>
+
+#include "attention.cuh"
+#include "common.cuh"
+
+namespace h3b {
+namespace wattn {
+
+constexpr int BQ = 128, BK = 128;
+constexpr int THREADS = 384;
+constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
+static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= THREADS * kLaunchRegs, "register split");
+constexpr uint32_t TMEM_COLS = 512;
+constexpr int MAX_DOCS = 64;          // documents per launch
+constexpr int kPrefetchTiles = 4;
+
+template <int D>
+struct Smem {
+  static constexpr int BOX_BYTES = 128 * 128;              // 128 rows x 64 columns
+  static constexpr int TILE_BYTES = (D / 64) * BOX_BYTES;
+  static constexpr int Q_OFF = 0;
+  static constexpr int K_OFF = 2 * TILE_BYTES;
+  static constexpr int V_OFF = K_OFF + 2 * TILE_BYTES;
+  static constexpr int BAR_OFF = V_OFF + 2 * TILE_BYTES;
+  static constexpr int BYTES = BAR_OFF + 256 + 1024;
+};
+
+struct Args {
+  CUtensorMap tmap_q, tmap_k, tmap_v;      // 16-bit [rows, heads * D], box 64 x 128, 128B swizzle
+  void* out;                               // [q rows, ldo]; head h at columns h * D
+  long long ldo;
+  int H, group;                            // query heads; query heads per key head
+  float scale_log2;                        // softmax scale * log2(e)
+  int left, right, sinks, causal;          // left, right < 2^30
+  int ndocs;
+  int q_start[MAX_DOCS], q_len[MAX_DOCS];
+  int k_start[MAX_DOCS], k_len[MAX_DOCS];
+  int item_end[MAX_DOCS];                  // cumulative CTA counts
+};
+
+// What queries at positions [p0, p1] of a document of n_k keys see: sink keys
+// [0, sink_end) and the window [lo, hi] (empty when hi < lo).
+struct Range {
+  int sink_end, lo, hi;
+  __device__ __forceinline__ Range(const Args& p, int n_k, int p0, int p1) {
+    const int top = p.causal ? min(p1, n_k - 1) : n_k - 1;
+    sink_end = max(0, min(p.sinks, top + 1));
+    lo = max(0, p0 - p.left);
+    hi = min(top, p1 + p.right);
+  }
+};
+
+// The key steps of a CTA.
+struct Steps {
+  int n_sink, n, lo, end, sink_end;        // window steps start at lo, end one past the last key
+  __device__ __forceinline__ explicit Steps(const Range& r) {
+    sink_end = r.sink_end;
+    lo = r.lo;
+    end = r.hi + 1;
+    const int ns = (sink_end + BK - 1) / BK;
+    const int nw = end > lo ? (end - lo + BK - 1) / BK : 0;
+    n_sink = ns;
+    n = ns + nw;
+    if (nw > 0 && sink_end >= lo) {                     // they touch: one range
+      n_sink = 0;
+      lo = 0;
+      end = max(end, sink_end);
+      n = (end + BK - 1) / BK;
+    }
+  }
+  __device__ __forceinline__ int base(int j) const {
+    return j < n_sink ? j * BK : lo + (j - n_sink) * BK;
+  }
+  __device__ __forceinline__ int valid(int j) const {
+    return min(BK, (j < n_sink ? sink_end : end) - base(j));
+  }
+  // does a tile that sees `r` see any key of step j
+  __device__ __forceinline__ bool needed(const Range& r, int j) const {
+    const int b = base(j), e = b + valid(j);
+    return b < r.sink_end || (b <= r.hi && e > r.lo && r.hi >= r.lo);
+  }
+};
+
+// 2^x for two lanes on the FMA pipe, as attention.cuh's ex2_poly2 but keeping
+// NaN logits NaN (or at least not finite).
+__device__ __forceinline__ float max_nan(float a, float b) {
+  float d;
+  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
+  return d;
+}
+__device__ __forceinline__ float2 ex2_poly2(float2 x) {
+  x.x = max_nan(x.x, -120.0f);
+  x.y = max_nan(x.y, -120.0f);
+  const float2 magic = make_float2(12582912.0f, 12582912.0f);
+  const float2 t = add2(x, magic);
+  const float2 f = sub2(x, sub2(t, magic));
+  float2 q = fma2(f, make_float2(0.05459282547235489f, 0.05459282547235489f),
+                  make_float2(0.24221783876419067f, 0.24221783876419067f));
+  q = fma2(f, q, make_float2(0.6933686137199402f, 0.6933686137199402f));
+  q = fma2(f, q, make_float2(1.0f, 1.0f));
+  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
+                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
+}
+
+template <typename T>
+__device__ __forceinline__ uint32_t pack16(float lo, float hi) {
+  if constexpr (std::is_same<T, __half>::value) {
+    const __half2 h = __floats2half2_rn(lo, hi);
+    return *reinterpret_cast<const uint32_t*>(&h);
+  } else {
+    return pack_bf16x2(lo, hi);
+  }
+}
+
+// P = 2^(S * scale - m) of one row's 128 keys, stored as 16-bit pairs over the
+// row's S columns; returns the row sum.  P is rounded to 16 bits because the
+// tensor core reads it so; the sum is of the unrounded fp32 values.  MIXED
+// sends 3 of 8 pairs to the polynomial; a step with masked keys (S = -inf) uses
+// the MUFU unit only, which gives exactly 0.
+template <typename T, bool MIXED>
+__device__ __forceinline__ float softmax_store(uint32_t (&sv)[128], float scale_log2, float m,
+                                               uint32_t s_addr, uint32_t half_bar) {
+  const float2 sc = make_float2(scale_log2, scale_log2);
+  const float2 nm = make_float2(-m, -m);
+  float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+#pragma unroll
+  for (int h = 0; h < 2; ++h) {
+    uint32_t pk[32];
+#pragma unroll
+    for (int c = 0; c < 32; ++c) {
+      const int k = h * 64 + 2 * c;
+      const float2 x = fma2(make_float2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc, nm);
+      float2 e;
+      if (MIXED && ((attn::kPolyPairs >> (c & 7)) & 1u)) e = ex2_poly2(x);
+      else e = make_float2(attn::ex2(x.x), attn::ex2(x.y));
+      if (c & 1) acc1 = add2(acc1, e);
+      else acc0 = add2(acc0, e);
+      pk[c] = pack16<T>(e.x, e.y);
+    }
+    tmem_st_32x32b_x32(s_addr + h * 32, pk);
+    if (h == 0) {
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if ((threadIdx.x & 31) == 0) mbar_arrive(half_bar);
+    }
+  }
+  const float2 s = add2(acc0, acc1);
+  return s.x + s.y;
+}
+
+// Bits [a, b] of 32-bit word w of a 128-bit mask (a, b any ints).
+__device__ __forceinline__ uint32_t span_word(int a, int b, int w) {
+  const int lo = max(a - 32 * w, 0), hi = min(b - 32 * w, 31);
+  if (hi < lo) return 0u;
+  return (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
+}
+
+template <int D, typename T>
+__global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constant__ Args p) {
+  using L = Smem<D>;
+  // kind::f16: D fp32 (bit 4), A and B bf16 (bits 7, 10) or fp16 (0)
+  constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
+  constexpr uint32_t IDESC_QK =
+      (1u << 4) | kType | ((uint32_t)(BK >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+  // P V: B = V is MN-major (head dim contiguous): bit 16
+  constexpr uint32_t IDESC_PV =
+      (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
+
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + L::BAR_OFF);
+  // kv_full[j % 2]: V(j) and K(j + 1); kv_empty[j % 2]: after step j's last
+  // MMAs, frees V stage j % 2 and K stage (j + 1) % 2 (K(0)'s release counts
+  // as j = -1).  s_full / p_half / p_full count a tile's needed steps only.
+  uint64_t* q_full = bars;           // 1
+  uint64_t* kv_full = bars + 1;      // 2
+  uint64_t* kv_empty = bars + 3;     // 2
+  uint64_t* s_full = bars + 5;       // 2 (tile A, B)
+  uint64_t* p_full = bars + 7;       // 2
+  uint64_t* pv_done = bars + 9;      // 2
+  uint64_t* drain = bars + 11;       // 1
+  uint64_t* p_half = bars + 12;      // 2
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+
+  int doc = 0;
+  while (doc + 1 < p.ndocs && (int)blockIdx.x >= p.item_end[doc]) ++doc;
+  const int item = (int)blockIdx.x - (doc > 0 ? p.item_end[doc - 1] : 0);
+  const int n_q = p.q_len[doc], n_k = p.k_len[doc];
+  const int pairs = (n_q + 2 * BQ - 1) / (2 * BQ);
+  const int head = item / pairs;
+  const int qp = item - head * pairs;
+  const int q_row = p.q_start[doc] + qp * 2 * BQ;
+  const int k_row = p.k_start[doc];
+  const int pos0 = qp * 2 * BQ + n_k - n_q;               // position of tile A's first row
+  const int rows = min(2 * BQ, n_q - qp * 2 * BQ);        // queries of this pair
+  const Steps st(Range(p, n_k, pos0, pos0 + rows - 1));
+  // what each tile sees; a tile without queries sees nothing
+  auto tile_range = [&](int t) {
+    const int n = min(BQ, rows - t * BQ);
+    Range r(p, n_k, pos0 + t * BQ, pos0 + t * BQ + n - 1);
+    if (n <= 0) {
+      r.sink_end = 0;
+      r.hi = -1;
+      r.lo = 0;
+    }
+    return r;
+  };
+
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(q_full), 1);
+    for (int i = 0; i < 2; ++i) {
+      mbar_init(smem_u32(&kv_full[i]), 1);
+      mbar_init(smem_u32(&kv_empty[i]), 1);
+      mbar_init(smem_u32(&s_full[i]), 1);
+      mbar_init(smem_u32(&p_full[i]), 4);
+      mbar_init(smem_u32(&p_half[i]), 4);
+      mbar_init(smem_u32(&pv_done[i]), 1);
+    }
+    mbar_init(smem_u32(drain), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 9) {
+    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish();
+  }
+  tc_fence_before();
+  __syncthreads();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto fail = [&]() {
+    if (!*abort_flag) {
+      record_error(H3B_ERR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  };
+
+  // Each warpgroup changes its register limit inside its own branch and leaves
+  // through its own copy of the teardown barrier.
+  if (warp >= 8) {
+    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if (warp == 8) {
+      if (lane == 0 && st.n > 0) {
+        prefetch_tmap(&p.tmap_q);
+        prefetch_tmap(&p.tmap_k);
+        prefetch_tmap(&p.tmap_v);
+        const int qx = head * D, kx = (head / p.group) * D;
+        auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+#pragma unroll
+          for (int b = 0; b < D / 64; ++b)
+            tma_load_2d(smem_u32(dst + b * L::BOX_BYTES), map, x + b * 64, y, bar);
+        };
+        const uint32_t qb = smem_u32(q_full);
+        mbar_expect_tx(qb, 3 * L::TILE_BYTES);
+        load(smem + L::Q_OFF, &p.tmap_q, qx, q_row, qb);
+        load(smem + L::Q_OFF + L::TILE_BYTES, &p.tmap_q, qx, q_row + BQ, qb);
+        load(smem + L::K_OFF, &p.tmap_k, kx, k_row + st.base(0), qb);
+        auto prefetch = [&](int j) {
+          if (j < st.n) {
+            const int y = k_row + st.base(j);
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b) {
+              tma_prefetch_2d(&p.tmap_k, kx + b * 64, y);
+              tma_prefetch_2d(&p.tmap_v, kx + b * 64, y);
+            }
+          }
+        };
+        for (int j = 1; j < kPrefetchTiles; ++j) prefetch(j);
+        int issued = 0;
+        bool ok = true;
+        for (int j = 0; j < st.n; ++j) {
+          prefetch(j + kPrefetchTiles);
+          if (j >= 1) {
+            // release r = j - 2 frees K stage (j + 1) % 2 and V stage j % 2
+            const int r = j - 2;
+            const int s = r & 1;
+            const int completion = s ? (r + 1) >> 1 : r >> 1;
+            if (!mbar_wait(smem_u32(&kv_empty[s]), completion & 1, abort_flag)) {
+              ok = false;
+              break;
+            }
+          }
+          const bool more = j + 1 < st.n;
+          const uint32_t b = smem_u32(&kv_full[j & 1]);
+          mbar_expect_tx(b, more ? 2 * L::TILE_BYTES : L::TILE_BYTES);
+          load(smem + L::V_OFF + (j & 1) * L::TILE_BYTES, &p.tmap_v, kx, k_row + st.base(j), b);
+          if (more)
+            load(smem + L::K_OFF + ((j + 1) & 1) * L::TILE_BYTES, &p.tmap_k, kx,
+                 k_row + st.base(j + 1), b);
+          ++issued;
+        }
+        if (!ok) {
+          // no copy may still be landing when the CTA exits
+          fail();
+          mbar_wait(smem_u32(q_full), 0, nullptr);
+          for (int j = issued > 2 ? issued - 2 : 0; j < issued; ++j)
+            mbar_wait(smem_u32(&kv_full[j & 1]), (j >> 1) & 1, nullptr);
+        }
+      }
+    } else if (warp == 9 && st.n > 0) {
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag));
+      };
+      const Range ra = tile_range(0), rb = tile_range(1);
+      int last[2] = {-1, -1};
+      for (int j = 0; j < st.n; ++j) {
+        if (st.needed(ra, j)) last[0] = j;
+        if (st.needed(rb, j)) last[1] = j;
+      }
+      auto need = [&](int t, int j) { return st.needed(t ? rb : ra, j); };
+      auto issue_qk = [&](int t, int j) {
+        const uint64_t qd = desc_kmajor_sw128(smem_u32(smem + L::Q_OFF + t * L::TILE_BYTES));
+        const uint64_t kd = desc_kmajor_sw128(smem_u32(smem + L::K_OFF + (j & 1) * L::TILE_BYTES));
+#pragma unroll
+        for (int kk = 0; kk < D / 16; ++kk) {
+          const uint32_t off = ((kk >> 2) * L::BOX_BYTES + (kk & 3) * 32) >> 4;   // 16 head dims
+          tc_mma_bf16_ss_elect(tmem + attn::s_col(t), qd + off, kd + off, IDESC_QK, kk != 0);
+        }
+        tc_commit_elect(smem_u32(&s_full[t]));
+      };
+      int cnt[2] = {0, 0};                                 // needed steps done per tile
+      auto pv_tile = [&](int t, int j) -> bool {
+        // 16 keys per MMA: P columns kk * 8.. (pairs), V rows kk * 16.. (MN-major:
+        // 64-dim chunks 16 KiB apart, 8-row groups 1 KiB)
+        const uint64_t vd = smem_desc(smem_u32(smem + L::V_OFF + (j & 1) * L::TILE_BYTES),
+                                      L::BOX_BYTES, 1024, 2);
+#pragma unroll
+        for (int h = 0; h < 2; ++h) {
+          if (!wait(h ? &p_full[t] : &p_half[t], cnt[t] & 1)) return false;
+          tc_fence_after();
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const int kk = h * 4 + i;
+            tc_mma_bf16_ts_elect(tmem + attn::o_col(t), tmem + attn::s_col(t) + kk * 8,
+                                 vd + kk * (2048 >> 4), IDESC_PV, (cnt[t] | kk) != 0);
+          }
+        }
+        if (j == last[t]) tc_commit_elect(smem_u32(&pv_done[t]));
+        ++cnt[t];
+        return true;
+      };
+      bool ok = wait(q_full, 0);
+      if (ok) {
+        tc_fence_after();
+        if (need(0, 0)) issue_qk(0, 0);
+        if (need(1, 0)) issue_qk(1, 0);
+        tc_commit_elect(smem_u32(&kv_empty[1]));           // release of K(0)
+      }
+      for (int j = 0; j < st.n && ok; ++j) {
+        const bool more = j + 1 < st.n;
+        if (!wait(&kv_full[j & 1], (j >> 1) & 1)) {
+          ok = false;
+          break;
+        }
+        const int valid = st.valid(j);
+        if (valid < BK) {
+          // V rows that no query sees: 8 chunks of 16 bytes per row and box
+          uint8_t* v = smem + L::V_OFF + (j & 1) * L::TILE_BYTES;
+          for (int c = lane + valid * 8; c < BK * 8; c += 32) {
+#pragma unroll
+            for (int b = 0; b < D / 64; ++b)
+              *reinterpret_cast<uint4*>(v + b * L::BOX_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
+          }
+          fence_proxy_async_smem();
+          __syncwarp();
+        }
+#pragma unroll
+        for (int t = 0; t < 2; ++t) {
+          if (need(t, j) && !pv_tile(t, j)) {
+            ok = false;
+            break;
+          }
+          if (more && need(t, j + 1)) issue_qk(t, j + 1);
+        }
+        if (ok) tc_commit_elect(smem_u32(&kv_empty[j & 1]));
+      }
+      if (!ok) {
+        if (lane == 0) fail();
+        tc_commit_elect(smem_u32(drain));
+        mbar_wait(smem_u32(drain), 0, nullptr);
+      }
+    }
+    tc_fence_before();
+    named_barrier_sync(1, THREADS);
+    if (warp == 9) {
+      __syncwarp();
+      tc_fence_after();
+      tmem_dealloc(tmem, TMEM_COLS);
+    }
+  } else {
+    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    // softmax of tile t: thread = query row (TMEM lane quadrant warp % 4)
+    const int t = warp >> 2;
+    const int qd = warp & 3;
+    const int r = qd * 32 + lane;
+    const uint32_t lane_addr = (uint32_t)(qd * 32) << 16;
+    const uint32_t s_t = tmem + lane_addr + attn::s_col(t);
+    const uint32_t o_t = tmem + lane_addr + attn::o_col(t);
+    const Range rt = tile_range(t);
+    const int pos = pos0 + t * BQ + r;                    // this row's key position
+    const int w_first = pos0 + t * BQ + qd * 32;          // first and last position of the warp
+    const int w_last = w_first + 31;
+    const int top = p.causal ? pos : n_k - 1;             // last key the row may see
+    const int w_top = p.causal ? w_first : n_k - 1;
+    float m_used = -INFINITY, l = 0.f;
+    int cnt = 0;
+    bool ok = true;
+    for (int j = 0; j < st.n; ++j) {
+      if (!st.needed(rt, j)) continue;
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[t]), cnt & 1, abort_flag));
+      if (!ok) break;
+      tc_fence_after();
+      uint32_t sv[128];
+      tmem_ld_32x32b_x64(s_t, sv);
+      tmem_ld_32x32b_x64(s_t + 64, sv + 64);
+      tmem_ld_wait();
+      const int base = st.base(j), valid = st.valid(j);
+      const bool all_seen =                               // warp-uniform
+          valid == BK && base + BK - 1 <= w_top &&
+          (base + BK <= p.sinks || (base >= w_last - p.left && base + BK - 1 <= w_first + p.right));
+      if (!all_seen) {
+        const int a = pos - p.left - base;
+        const int b = min(min(pos + p.right, top) - base, valid - 1);
+        const int s = min(min(p.sinks - 1, top) - base, valid - 1);
+#pragma unroll
+        for (int w = 0; w < 4; ++w) {
+          const uint32_t seen = span_word(a, b, w) | span_word(0, s, w);
+#pragma unroll
+          for (int c = 0; c < 32; ++c)
+            if (!(seen & (1u << c))) sv[w * 32 + c] = 0xff800000u;   // -inf: masked key
+        }
+      }
+      // row max of the scaled logits (scale > 0 commutes with max)
+      float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
+#pragma unroll
+      for (int c = 0; c < 128; c += 8) {
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          m4[u] = attn::max3(m4[u], __uint_as_float(sv[c + 2 * u]), __uint_as_float(sv[c + 2 * u + 1]));
+      }
+      const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
+      const float m_new = fmaxf(m_used, mx);
+      const bool rescale = __any_sync(0xffffffffu, m_new > m_used + attn::kRescaleLog2);
+      float alpha = 1.f;
+      if (rescale) {
+        // a row that has seen nothing yet stays at -inf (its l and O are 0)
+        alpha = m_new == -INFINITY ? 1.f : attn::ex2(m_used - m_new);
+        m_used = m_new;
+      }
+      if (rescale && cnt > 0) {
+        // O is final up to the previous needed step: s_full of this one was
+        // committed after its PV
+#pragma unroll
+        for (int h = 0; h < D / 32; ++h) {
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(o_t + h * 32, ov);
+          tmem_ld_wait();
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+          tmem_st_32x32b_x32(o_t + h * 32, ov);
+        }
+      }
+      const uint32_t hb = smem_u32(&p_half[t]);
+      const float m = m_used == -INFINITY ? 0.f : m_used;   // -inf - (-inf) is no exponent
+      const float s = all_seen ? softmax_store<T, true>(sv, p.scale_log2, m, s_t, hb)
+                               : softmax_store<T, false>(sv, p.scale_log2, m, s_t, hb);
+      l = l * alpha + s;
+      tmem_st_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive(smem_u32(&p_full[t]));
+      ++cnt;
+    }
+    if (ok && cnt > 0)
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), 0, abort_flag));
+    if (!ok) {
+      fail();
+    } else {
+      tc_fence_after();
+      const bool some = l != 0.f;                          // saw a key (or NaN)
+      const float inv_l = 1.0f / l;
+      const bool row_ok = t * BQ + r < rows;
+      T* op = static_cast<T*>(p.out) + (size_t)(q_row + t * BQ + r) * p.ldo + (size_t)head * D;
+#pragma unroll
+      for (int h = 0; h < D / 32; ++h) {
+        uint32_t ov[32];
+        if (cnt > 0) {                                     // warp-uniform
+          tmem_ld_32x32b_x32(o_t + h * 32, ov);
+          tmem_ld_wait();
+        }
+        if (row_ok) {
+#pragma unroll
+          for (int c = 0; c < 4; ++c) {
+            uint32_t w[4];
+#pragma unroll
+            for (int u = 0; u < 4; ++u)
+              w[u] = some ? pack16<T>(__uint_as_float(ov[8 * c + 2 * u]) * inv_l,
+                                      __uint_as_float(ov[8 * c + 2 * u + 1]) * inv_l)
+                          : 0u;
+            *reinterpret_cast<uint4*>(op + h * 32 + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+          }
+        }
+      }
+    }
+    tc_fence_before();
+    named_barrier_sync(1, THREADS);
+  }
+}
+
+}  // namespace wattn
+}  // namespace h3b

@@ -1,0 +1,219 @@
+// Host side of the windowed-attention entry points (declared in include/h3b.h).
+#pragma once
+
+#include "attention_decode.cuh"
+#include "attention_window.cuh"
+#include "mx_host.cuh"
+
+namespace h3b {
+
+constexpr int64_t kMaxKeys = (int64_t)1 << 30;    // positions plus a window stay in 31 bits
+
+static int tmap_16_rows(CUtensorMap* tm, const void* base, int dtype, int64_t rows, int64_t cols,
+                        int64_t stride) {
+  auto fn = encode_fn();
+  if (!fn) return H3B_ERR_UNSUPPORTED;
+  cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
+  cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
+  cuuint32_t box[2] = {64, wattn::BK};
+  cuuint32_t estr[2] = {1, 1};
+  return fn(tm, dtype == H3B_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
+                                    : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
+            2, const_cast<void*>(base), dims, strides, box, estr, CU_TENSOR_MAP_INTERLEAVE_NONE,
+            CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+            CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE) == CUDA_SUCCESS
+             ? H3B_OK
+             : H3B_ERR_INVALID_ARG;
+}
+
+template <int D, typename T>
+static int window_attn_launch(const wattn::Args& a, int items, cudaStream_t st) {
+  auto kernel = wattn::k_window_attn<D, T>;
+  const void* fn = reinterpret_cast<const void*>(kernel);
+  static SmemAttr attr;
+  int rc = attr.set(fn, wattn::Smem<D>::BYTES);
+  if (rc != H3B_OK) return rc;
+  // the kernel's setmaxnreg split draws on this many launch registers
+  static std::atomic<int> regs{0};
+  if (!regs.load(std::memory_order_relaxed)) {
+    cudaFuncAttributes fa;
+    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) return H3B_ERR_CUDA;
+    regs.store(fa.numRegs, std::memory_order_relaxed);
+  }
+  if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
+  kernel<<<(unsigned)items, wattn::THREADS, wattn::Smem<D>::BYTES, st>>>(a);
+  return launched(cudaGetLastError());
+}
+
+static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, float scale) {
+  if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f))
+    return H3B_ERR_INVALID_ARG;
+  return H3B_OK;
+}
+
+static inline int clamp_window(int64_t v) { return (int)std::min<int64_t>(v, kMaxKeys - 1); }
+
+template <int D, typename T>
+static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st) {
+  auto kernel = wdec::k_window_decode<D, T>;
+  static SmemAttr attr;
+  int rc = attr.set(reinterpret_cast<const void*>(kernel), wdec::Smem<D>::BYTES);
+  if (rc != H3B_OK) return rc;
+  const int64_t row_tiles = ((int64_t)a.n_new * a.group + wdec::kRows - 1) / wdec::kRows;
+  const int64_t groups = row_tiles * a.kv_heads;
+  if (groups > 65535 || B > 65535) return H3B_ERR_INVALID_ARG;
+  // CTAs along the keys: enough to cover the SMs once, but not more than give
+  // every warp a tile of a full window
+  const int64_t most =
+      std::min<int64_t>(a.room, (int64_t)a.left + a.right + a.n_new + (int64_t)a.sinks);
+  int split = 1;
+  while (split < wdec::kMaxCluster && groups * B * split * 2 <= num_sms() &&
+         most > (int64_t)split * wdec::kWarps * wdec::kKeys)
+    split *= 2;
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)split, (unsigned)groups, (unsigned)B);
+  cfg.blockDim = dim3(wdec::kThreads);
+  cfg.dynamicSmemBytes = wdec::Smem<D>::BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = 1;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
+}  // namespace h3b
+
+extern "C" {
+
+int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const void* k,
+                         int64_t k_stride, const void* v, int64_t v_stride, int64_t kv_rows,
+                         int dtype, int H, int kv_heads, int D, const int32_t* q_start,
+                         const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
+                         int ndocs, int64_t left, int64_t right, int64_t sinks, int causal,
+                         float scale, void* out, int64_t ldo, void* stream) {
+  if (!dt_16(dtype) || (D != 64 && D != 128) || H <= 0 || kv_heads <= 0 || H % kv_heads ||
+      ndocs < 0 || q_rows < 0 || kv_rows < 0)
+    return H3B_ERR_INVALID_ARG;
+  int rc = window_rule(left, right, sinks, causal, scale);
+  if (rc != H3B_OK) return rc;
+  const int64_t hd = (int64_t)H * D, kd = (int64_t)kv_heads * D;
+  if (q_stride < hd || k_stride < kd || v_stride < kd || ldo < hd || hd > INT32_MAX)
+    return H3B_ERR_INVALID_ARG;
+  if (q_rows > kMaxKeys || kv_rows > kMaxKeys) return H3B_ERR_INVALID_ARG;
+  if ((q_stride | k_stride | v_stride | ldo) % 8) return H3B_ERR_ALIGNMENT;
+  if (ndocs > 0 && (!q_start || !q_len || !k_start || !k_len)) return H3B_ERR_INVALID_ARG;
+  int64_t queries = 0, keys = 0;
+  for (int i = 0; i < ndocs; ++i) {
+    if (q_start[i] < 0 || q_len[i] < 0 || (int64_t)q_start[i] + q_len[i] > q_rows ||
+        k_start[i] < 0 || k_len[i] < 0 || (int64_t)k_start[i] + k_len[i] > kv_rows)
+      return H3B_ERR_INVALID_ARG;
+    queries += q_len[i];
+    keys += k_len[i];
+  }
+  if (queries == 0) return H3B_OK;
+  if (!q || !out || (keys > 0 && (!k || !v))) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out)) return H3B_ERR_ALIGNMENT;
+  rc = check_sm100();
+  if (rc != H3B_OK) return rc;
+
+  wattn::Args a;
+  memset(&a, 0, sizeof(a));
+  rc = tmap_16_rows(&a.tmap_q, q, dtype, q_rows, hd, q_stride);
+  if (rc != H3B_OK) return rc;
+  if (keys > 0) {
+    rc = tmap_16_rows(&a.tmap_k, k, dtype, kv_rows, kd, k_stride);
+    if (rc != H3B_OK) return rc;
+    rc = tmap_16_rows(&a.tmap_v, v, dtype, kv_rows, kd, v_stride);
+    if (rc != H3B_OK) return rc;
+  }
+  a.out = out;
+  a.ldo = ldo;
+  a.H = H;
+  a.group = H / kv_heads;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  a.left = clamp_window(left);
+  a.right = clamp_window(right);
+  a.sinks = clamp_window(sinks);
+  a.causal = causal;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  for (int d0 = 0; d0 < ndocs;) {               // documents in launches of MAX_DOCS
+    int64_t items = 0;
+    int n = 0;
+    for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0) {
+      if (q_len[d0] == 0) continue;
+      items += ((int64_t)q_len[d0] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
+      if (items > INT32_MAX) return H3B_ERR_INVALID_ARG;
+      a.q_start[n] = q_start[d0];
+      a.q_len[n] = q_len[d0];
+      a.k_start[n] = k_start[d0];
+      a.k_len[n] = k_len[d0];
+      a.item_end[n++] = (int)items;
+    }
+    if (n == 0) break;
+    a.ndocs = n;
+    if (D == 128)
+      rc = dtype == H3B_DT_F16 ? window_attn_launch<128, __half>(a, (int)items, st)
+                               : window_attn_launch<128, __nv_bfloat16>(a, (int)items, st);
+    else
+      rc = dtype == H3B_DT_F16 ? window_attn_launch<64, __half>(a, (int)items, st)
+                               : window_attn_launch<64, __nv_bfloat16>(a, (int)items, st);
+    if (rc != H3B_OK) return rc;
+  }
+  return H3B_OK;
+}
+
+int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const void* k,
+                                const int64_t* k_strides, const void* v, const int64_t* v_strides,
+                                const int32_t* len, int64_t B, int64_t room, int64_t n_new,
+                                int dtype, int H, int kv_heads, int D, int64_t left, int64_t right,
+                                int64_t sinks, int causal, float scale, void* out, void* stream) {
+  if (!dt_16(dtype) || (D != 64 && D != 128) || H <= 0 || kv_heads <= 0 || H % kv_heads || B < 0 ||
+      room < 0 || n_new < 0 || room > kMaxKeys || n_new > 65535 || !q_strides || !k_strides ||
+      !v_strides)
+    return H3B_ERR_INVALID_ARG;
+  int rc = window_rule(left, right, sinks, causal, scale);
+  if (rc != H3B_OK) return rc;
+  for (int i = 0; i < 3; ++i) {
+    if (q_strides[i] < 0 || k_strides[i] < 0 || v_strides[i] < 0) return H3B_ERR_INVALID_ARG;
+    if ((q_strides[i] | k_strides[i] | v_strides[i]) % 8) return H3B_ERR_ALIGNMENT;
+  }
+  if (B == 0 || n_new == 0) return H3B_OK;
+  if (!q || !len || !out || (room > 0 && (!k || !v))) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
+      (reinterpret_cast<uintptr_t>(len) & 3u))
+    return H3B_ERR_ALIGNMENT;
+  rc = check_sm100();
+  if (rc != H3B_OK) return rc;
+  wdec::Args a;
+  memset(&a, 0, sizeof(a));
+  a.q = q;
+  a.k = k;
+  a.v = v;
+  a.out = out;
+  a.len = len;
+  a.q_b = q_strides[0], a.q_t = q_strides[1], a.q_h = q_strides[2];
+  a.k_b = k_strides[0], a.k_s = k_strides[1], a.k_h = k_strides[2];
+  a.v_b = v_strides[0], a.v_s = v_strides[1], a.v_h = v_strides[2];
+  a.room = (int)room;
+  a.n_new = (int)n_new;
+  a.H = H;
+  a.kv_heads = kv_heads;
+  a.group = H / kv_heads;
+  a.left = clamp_window(left);
+  a.right = clamp_window(right);
+  a.sinks = clamp_window(sinks);
+  a.causal = causal;
+  a.scale_log2 = scale * 1.4426950408889634f;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (D == 128)
+    return dtype == H3B_DT_F16 ? window_decode_launch<128, __half>(a, B, st)
+                               : window_decode_launch<128, __nv_bfloat16>(a, B, st);
+  return dtype == H3B_DT_F16 ? window_decode_launch<64, __half>(a, B, st)
+                             : window_decode_launch<64, __nv_bfloat16>(a, B, st);
+}
+
+}  // extern "C"

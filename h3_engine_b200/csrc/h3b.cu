@@ -891,3 +891,4 @@ int h3b_rmsnorm_quantize_noalloc(const void* x, int64_t M, int64_t K, int64_t ld
 }  // extern "C"
 
 #include "mx_host.cuh"
+#include "attention_window_host.cuh"

@@ -567,3 +567,124 @@ def mxfp4_ffn(x: torch.Tensor, qu: torch.Tensor, sfu: torch.Tensor, qd: torch.Te
                          device=dev)
         _H3B.mxfp4_ffn(x2, M, x2.stride(0), qu, sfu, qd, sfd, N, F, residual, ldr, o2, ldd, ws)
     return out
+
+
+# ---------------------------------------------------------------- windowed attention
+_ALL_KEYS = (1 << 30) - 1
+
+
+def _window_rule(window, sinks: int, causal: bool) -> tuple[int, int, int, bool]:
+    left, right = window
+    left = _ALL_KEYS if left is None else int(left)
+    right = _ALL_KEYS if right is None else int(right)
+    if left < 0 or right < 0 or sinks < 0:
+        raise ValueError("window sides and sinks must not be negative")
+    return left, right, int(sinks), bool(causal)
+
+
+def _heads_dim(heads: int, kv_heads: int, head_dim: int) -> None:
+    if head_dim not in (64, 128):
+        raise ValueError(f"head_dim must be 64 or 128, not {head_dim}")
+    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
+        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
+
+
+def _ranges(cu, rows: int, what: str) -> tuple[list[int], list[int]]:
+    """(starts, lengths) of the documents that host boundaries give."""
+    cu = [int(c) for c in (cu.tolist() if hasattr(cu, "tolist") else cu)]
+    if not cu or cu[0] < 0 or cu[-1] > rows or any(b < a for a, b in zip(cu, cu[1:])):
+        raise ValueError(f"{what} must rise from 0 or more to at most {rows}")
+    return cu[:-1], [b - a for a, b in zip(cu, cu[1:])]
+
+
+def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, head_dim: int,
+                     cu_seqlens, *, kv_heads: int | None = None, cu_seqlens_k=None,
+                     window: tuple = (None, None), sinks: int = 0, causal: bool = False,
+                     scale: float | None = None,
+                     out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention per document with a sliding window and sinks, over separate
+    ``q`` [rows, heads*head_dim] and ``k``, ``v`` [kv_rows, kv_heads*head_dim]
+    activations (bf16 or fp16, head_dim 64 or 128, any row strides).
+
+    Query i of a document with n_q queries and n_k keys stands at key position
+    ``p = i + n_k - n_q`` and sees key j iff ``p - left <= j <= p + right`` or
+    ``j < sinks``, and, if ``causal``, ``j <= p``; ``window = (left, right)``,
+    None meaning no limit.  A query that sees nothing gets zeros.
+    ``cu_seqlens`` (queries) and ``cu_seqlens_k`` (keys, default the same) are
+    host boundaries; rows of ``out`` outside them are left as they were (zeros
+    when ``out`` is allocated here)."""
+    dev = _need_cuda(q, k, v, out)
+    kv_heads = heads if kv_heads is None else kv_heads
+    _heads_dim(heads, kv_heads, head_dim)
+    left, right, sinks, causal = _window_rule(window, sinks, causal)
+    q2, k2, v2 = _mx_rows(q), _mx_rows(k), _mx_rows(v)
+    if q2.dtype not in _16BIT or k2.dtype != q2.dtype or v2.dtype != q2.dtype:
+        raise TypeError("q, k, v must be bf16 or fp16, of one type")
+    rows, hd = q2.shape
+    if hd != heads * head_dim or k2.shape != v2.shape or k2.shape[1] != kv_heads * head_dim:
+        raise ValueError("q must be [rows, heads * head_dim], k and v [rows, kv_heads * head_dim]")
+    qs, ql = _ranges(cu_seqlens, rows, "cu_seqlens")
+    ks, kl = _ranges(cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, k2.shape[0],
+                     "cu_seqlens_k")
+    if len(ks) != len(qs):
+        raise ValueError("cu_seqlens and cu_seqlens_k name different numbers of documents")
+    sc = float(scale) if scale is not None else head_dim ** -0.5
+    if not sc > 0:
+        raise ValueError("scale must be positive")
+    if out is None:
+        covered = sum(ql) == rows
+        out = (torch.empty if covered else torch.zeros)(rows, hd, dtype=q2.dtype, device=dev)
+        o2 = out
+    else:
+        out, o2, _ = _mx_out(out, rows, hd, q2.dtype, dev, q.shape[:-1])
+    if sum(ql):
+        _H3B.attention_window(q2, k2, v2, heads, kv_heads, head_dim, qs, ql, ks, kl, left, right,
+                              sinks, causal, sc, o2)
+    return out
+
+
+def attention_window_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
+                            kv_len: torch.Tensor, *, window: tuple = (None, None), sinks: int = 0,
+                            causal: bool = True, scale: float | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """The window rule of ``attention_window`` for the newest tokens of each
+    sequence against its cache: ``q`` [B, n_new, heads, D], ``k`` and ``v``
+    [B, room, kv_heads, D] (any strides that keep D contiguous and rows 16-byte
+    aligned; caches are never copied), ``kv_len`` int32 [B] on the device: the
+    keys in use, the new tokens' own included, so token t stands at position
+    ``kv_len - n_new + t``.  Lengths are read when the kernel runs (a captured
+    call follows them) and clamped to [0, room].  Returns [B, n_new, heads, D]."""
+    dev = _need_cuda(q, k, v, kv_len, out)
+    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
+        raise ValueError("q must be [B, n_new, heads, D], k and v [B, room, kv_heads, D]")
+    B, n, heads, D = q.shape
+    if k.shape[0] != B or k.shape[3] != D:
+        raise ValueError("q, k and v must agree on batch and head_dim")
+    _heads_dim(heads, k.shape[2], D)
+    if q.dtype not in _16BIT or k.dtype != q.dtype or v.dtype != q.dtype:
+        raise TypeError("q, k, v must be bf16 or fp16, of one type")
+    if kv_len.dtype != torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous():
+        raise ValueError(f"kv_len must be a contiguous int32 [{B}]")
+    left, right, sinks, causal = _window_rule(window, sinks, causal)
+    if not _decode_strides(q):
+        q = q.clone(memory_format=torch.contiguous_format)
+    if not (_decode_strides(k) and _decode_strides(v)):
+        raise ValueError("caches need a contiguous head_dim and 16-byte aligned rows")
+    sc = float(scale) if scale is not None else D ** -0.5
+    if not sc > 0:
+        raise ValueError("scale must be positive")
+    if out is None:
+        out = torch.empty(B, n, heads, D, dtype=q.dtype, device=dev)
+    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() \
+            or out.storage_offset() % 8:
+        raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)}")
+    else:
+        torch.autograd.graph.increment_version(out)
+    if B and n:
+        _H3B.attention_window_decode(q, k, v, kv_len, left, right, sinks, causal, sc, out)
+    return out
+
+
+def _decode_strides(t: torch.Tensor) -> bool:
+    s = t.stride()
+    return s[3] == 1 and not (s[0] | s[1] | s[2]) % 8 and not t.storage_offset() % 8

@@ -14,6 +14,7 @@ is a dispatch error, never a silent fallback.  The tensor-level wrappers in
 ``ops.py`` allocate outputs, check shapes and call these operators; they are
 the functions the rest of the package uses.
 """
+import ctypes
 from typing import Optional
 
 import torch
@@ -256,3 +257,31 @@ def mxfp4_ffn(x, m, ldx, qu, sfu, qd, sfd, n, f, residual, ldr, out, ldd, ws):
     """Q(v * silu(g)) Wd^T + residual, [v | g] = Q(x) Wu^T (h3b_mxfp4_ffn)."""
     _call(out, "h3b_mxfp4_ffn", _p(x), DTYPES[x.dtype], m, ldx, _p(qu), _p(sfu), _p(qd), _p(sfd),
           n, f, _p(residual), ldr, _p(out), ldd, _p(ws), ws.numel())
+
+
+def _i32s(v):
+    return (ctypes.c_int32 * max(len(v), 1))(*v)
+
+
+@_light("attention_window(Tensor q, Tensor k, Tensor v, int heads, int kv_heads, int head_dim, "
+        "int[] q_start, int[] q_len, int[] k_start, int[] k_len, int left, int right, int sinks, "
+        "bool causal, float scale, Tensor(a!) out) -> ()")
+def attention_window(q, k, v, heads, kv_heads, head_dim, q_start, q_len, k_start, k_len, left,
+                     right, sinks, causal, scale, out):
+    """Packed windowed attention over host row ranges (h3b_attention_window)."""
+    _call(out, "h3b_attention_window", _p(q), q.shape[0], q.stride(0), _p(k), k.stride(0), _p(v),
+          v.stride(0), k.shape[0], DTYPES[q.dtype], heads, kv_heads, head_dim, _i32s(q_start),
+          _i32s(q_len), _i32s(k_start), _i32s(k_len), len(q_start), left, right, sinks,
+          int(causal), scale, _p(out), out.stride(0))
+
+
+@_light("attention_window_decode(Tensor q, Tensor k, Tensor v, Tensor kv_len, int left, "
+        "int right, int sinks, bool causal, float scale, Tensor(a!) out) -> ()")
+def attention_window_decode(q, k, v, kv_len, left, right, sinks, causal, scale, out):
+    """Windowed attention of new tokens against a cache with device lengths
+    (h3b_attention_window_decode); q [B, n, H, D], k and v [B, room, kv_heads, D]."""
+    b, n, h, d = q.shape
+    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
+    _call(out, "h3b_attention_window_decode", _p(q), strides[0], _p(k), strides[1], _p(v),
+          strides[2], _p(kv_len), b, k.shape[1], n, DTYPES[q.dtype], h, k.shape[2], d, left, right,
+          sinks, int(causal), scale, _p(out))

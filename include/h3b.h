@@ -343,6 +343,43 @@ H3B_API int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, cons
                           int64_t F, const void* residual, int64_t ldr, void* D, int64_t ldd,
                           void* ws, int64_t ws_bytes, void* stream);
 
+/* ------------------------------------------------------------------ windowed attention
+ * Query i of a document with n_q queries and n_k keys stands at key position
+ * p = i + n_k - n_q and sees key j iff
+ *   (p - left <= j <= p + right  or  j < sinks)  and  (not causal or j <= p);
+ * softmax(scale * q k^T) v over the keys it sees, zeros where it sees none.
+ * bf16 or fp16, D 64 or 128, H query heads over kv_heads key heads (H a
+ * multiple; query head h reads key head h / (H / kv_heads)).
+ * A value row that some query sees must be finite to leave the other queries
+ * of the same 256-row tile finite; what lies in rows that no query of the
+ * tile sees (past a document's end, outside every window) does not matter.
+ *
+ * Packed documents: q [q_rows, H*D], k and v [kv_rows, kv_heads*D], row
+ * strides in elements (multiples of 8, 16-byte aligned bases); q_start, q_len,
+ * k_start, k_len: HOST arrays of ndocs row ranges.  Rows of out that belong to
+ * no document are left as they were.                                        */
+H3B_API int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const void* k,
+                                 int64_t k_stride, const void* v, int64_t v_stride,
+                                 int64_t kv_rows, int dtype, int H, int kv_heads, int D,
+                                 const int32_t* q_start, const int32_t* q_len,
+                                 const int32_t* k_start, const int32_t* k_len, int ndocs,
+                                 int64_t left, int64_t right, int64_t sinks, int causal,
+                                 float scale, void* out, int64_t ldo, void* stream);
+
+/* A few new tokens per sequence against a cache: q [B, n_new, H, D], k and v
+ * [B, room, kv_heads, D], each with HOST strides {batch, row, head} in
+ * elements (multiples of 8; the last dimension contiguous), out [B, n_new, H,
+ * D] contiguous.  len: DEVICE int32 [B], the keys in use per sequence with the
+ * new tokens' own (read when the kernel runs, clamped to [0, room]), so that
+ * token t stands at position len - n_new + t.                               */
+H3B_API int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const void* k,
+                                        const int64_t* k_strides, const void* v,
+                                        const int64_t* v_strides, const int32_t* len, int64_t B,
+                                        int64_t room, int64_t n_new, int dtype, int H,
+                                        int kv_heads, int D, int64_t left, int64_t right,
+                                        int64_t sinks, int causal, float scale, void* out,
+                                        void* stream);
+
 #ifdef __cplusplus
 }
 #endif
