@@ -400,5 +400,266 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm_mxfp4(const __grid_constant
   }
 }
 
+// ============================================================================
+// CTA-pair kernel (cluster of 2): one 256 x 256 tile per pair, the MMA in its
+// cta_group::2 form.  CTA r loads rows m0 + 128 r .. of A with their scales,
+// rows n0 + 128 r .. of B (its half of the tile's N) and the scales of all 256
+// B rows; every load counts its bytes on the leader's full barrier
+// (cta_group::2 form, no multicast).  The leader's MMA warp alone issues, for
+// both SMs: per 128 values of K three scale copies and two MMAs.  Scale tiles
+// come through tensor maps so that rows and columns outside the operand read
+// as zeros.  Protocol, bounds and teardown as in the NVFP4 pair kernel.
+// ============================================================================
+constexpr int P_STAGES = 5;
+constexpr int P_A_BYTES = 128 * KB_BYTES;
+constexpr int P_B_BYTES = 128 * KB_BYTES;
+constexpr int P_SFA_BYTES = KB_ATOMS * SF_ATOM;
+constexpr int P_SFB_BYTES = 2 * KB_ATOMS * SF_ATOM;
+constexpr int P_STAGE_BYTES = P_A_BYTES + P_B_BYTES + P_SFA_BYTES + P_SFB_BYTES;
+constexpr int P_OUT_OFFSET = P_STAGES * P_STAGE_BYTES;
+constexpr int P_BAR_OFFSET = P_OUT_OFFSET + EPI_WARPS * OUT_WARP_BYTES;
+constexpr int P_SMEM_BYTES = P_BAR_OFFSET + 256 + 1024;
+static_assert(P_STAGE_BYTES % 1024 == 0 && P_OUT_OFFSET % 1024 == 0, "swizzle alignment");
+static_assert(SF_COL + P_STAGES * SF_STAGE_COLS <= TMEM_COLS, "TMEM budget");
+static_assert(P_SMEM_BYTES <= 232448, "shared memory budget");
+
+struct PairArgs {
+  Args base;               // tmap_a and tmap_b: box 128 B x 128 rows
+  CUtensorMap tmap_sfa;    // u64 [128-row blocks, scale tiles * 64], box 128 x 1 (one k-block)
+  CUtensorMap tmap_sfb;    // the same for B, box 128 x 2
+  int m_tiles;             // 256-row tiles
+  int group;               // tile rows per raster group
+};
+
+// Tile t of the raster: groups of `group` tile rows, column by column inside a
+// group, so that the tiles running at one time share A rows and B columns.
+__device__ __forceinline__ void pair_tile(const PairArgs& p, int t, int& m, int& n) {
+  const int per = p.group * p.base.n_tiles;
+  const int g = t / per, r = t - g * per;
+  const int rows = min(p.group, p.m_tiles - g * p.group);
+  n = r / rows;
+  m = g * p.group + (r - n * rows);
+}
+
+__device__ __forceinline__ void kpair_pair_elect(uint32_t sfa_t, uint64_t sfa_d, uint32_t sfb_t,
+                                                 uint64_t sfb_d0, uint64_t sfb_d1, uint32_t d_tmem,
+                                                 uint64_t a_desc, uint64_t b_desc,
+                                                 uint32_t accumulate, uint32_t second) {
+  asm volatile(
+      "{\n\t.reg .pred p, e, f;\n\t"
+      "setp.ne.b32 p, %9, 0;\n\t"
+      "elect.sync _|e, 0xffffffff;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%0], %1;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%2], %3;\n\t"
+      "@e tcgen05.cp.cta_group::2.32x128b.warpx4 [%4], %5;\n\t"
+      "@e tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
+      " [%6], %7, %8, %10, [%0], [%2], p;\n\t"
+      "setp.ne.and.b32 f, %12, 0, e;\n\t"
+      "setp.eq.u32 p, 0, 0;\n\t"
+      "@f tcgen05.mma.cta_group::2.kind::mxf4.block_scale.scale_vec::2X"
+      " [%6], %13, %14, %11, [%0], [%2], p;\n\t}" ::"r"(sfa_t),
+      "l"(sfa_d), "r"(sfb_t), "l"(sfb_d0), "r"(sfb_t + 4), "l"(sfb_d1), "r"(d_tmem), "l"(a_desc),
+      "l"(b_desc), "r"(accumulate), "r"(idesc(256, 256, 0)), "r"(idesc(256, 256, 2)),
+      "r"(second), "l"(a_desc + 2), "l"(b_desc + 2)
+      : "memory");
+}
+
+template <typename T, int EPI>
+__global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
+    k_gemm_mxfp4_pair(const __grid_constant__ PairArgs pa) {
+  const Args& p = pa.base;
+  extern __shared__ uint8_t smem_raw[];
+  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
+                                             ~uintptr_t(1023));
+  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + P_BAR_OFFSET);
+  uint64_t* full = bars;                       // leader: both CTAs' loads of a stage
+  uint64_t* empty = bars + P_STAGES;           // both: stage consumed (leader's commit)
+  uint64_t* acc_full = bars + 2 * P_STAGES;    // both: accumulator ready
+  uint64_t* acc_empty = bars + 2 * P_STAGES + 1;   // leader: both CTAs drained it
+  uint64_t* drain = bars + 2 * P_STAGES + 2;
+  uint64_t* bye = bars + 2 * P_STAGES + 3;     // both: the peer is done
+  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * P_STAGES + 4);
+  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
+  const uint32_t rank = cluster_ctarank();
+  const int num_kb = (p.K + KB_ELEMS - 1) / KB_ELEMS;
+  const int pair_id = (int)(blockIdx.x >> 1);
+  const int num_pairs = (int)(gridDim.x >> 1);
+  const int num_tiles = pa.m_tiles * p.n_tiles;
+
+  auto sA = [&](int s) { return smem + s * P_STAGE_BYTES; };
+  auto sB = [&](int s) { return smem + s * P_STAGE_BYTES + P_A_BYTES; };
+  auto sSFA = [&](int s) { return smem + s * P_STAGE_BYTES + P_A_BYTES + P_B_BYTES; };
+  auto sSFB = [&](int s) {
+    return smem + s * P_STAGE_BYTES + P_A_BYTES + P_B_BYTES + P_SFA_BYTES;
+  };
+
+  if (threadIdx.x == 0) {
+    for (int s = 0; s < P_STAGES; ++s) {
+      mbar_init(smem_u32(&full[s]), 1);
+      mbar_init(smem_u32(&empty[s]), 1);
+    }
+    mbar_init(smem_u32(acc_full), 1);
+    mbar_init(smem_u32(acc_empty), 2 * EPI_WARPS);
+    mbar_init(smem_u32(drain), 1);
+    mbar_init(smem_u32(bye), 1);
+    *abort_flag = 0;
+    fence_mbar_init();
+  }
+  if (warp == 1) {
+    tmem_alloc_pair(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_relinquish_pair();
+  }
+  tc_fence_before();
+  // both CTAs' barriers exist before any load or arrival reaches them
+  cluster_sync_all();
+  tc_fence_after();
+  const uint32_t tmem = *tmem_slot;
+
+  auto fail = [&]() {
+    if (!*abort_flag) {
+      record_error(H3B_ERR_TIMEOUT);
+      *abort_flag = 1;
+    }
+  };
+
+  if (warp == 0) {
+    if (lane == 0) {
+      prefetch_tmap(&p.tmap_a);
+      prefetch_tmap(&p.tmap_b);
+      prefetch_tmap(&pa.tmap_sfa);
+      prefetch_tmap(&pa.tmap_sfb);
+      uint32_t g = 0;
+      bool ok = true;
+      for (int t = pair_id; t < num_tiles && ok; t += num_pairs) {
+        int mt, nt;
+        pair_tile(pa, t, mt, nt);
+        const int m0 = mt * 256, n0 = nt * BN;
+        for (int kb = 0; kb < num_kb; ++kb, ++g) {
+          const int s = g % P_STAGES;
+          const uint32_t ph = (g / P_STAGES) & 1;
+          if (g >= P_STAGES && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, abort_flag)) {
+            fail();
+            ok = false;
+            break;
+          }
+          const uint32_t lb = mapa_shared(smem_u32(&full[s]), 0);
+          if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * P_STAGE_BYTES);
+          tma_load_2d_pair(smem_u32(sA(s)), &p.tmap_a, kb * KB_BYTES, m0 + 128 * (int)rank, lb);
+          tma_load_2d_pair(smem_u32(sB(s)), &p.tmap_b, kb * KB_BYTES, n0 + 128 * (int)rank, lb);
+          tma_load_2d_pair(smem_u32(sSFA(s)), &pa.tmap_sfa, kb * KB_ATOMS * 64,
+                           m0 / 128 + (int)rank, lb);
+          tma_load_2d_pair(smem_u32(sSFB(s)), &pa.tmap_sfb, kb * KB_ATOMS * 64, n0 / 128, lb);
+        }
+      }
+      // tail: the release of every stage this CTA filled has arrived (the
+      // leader's last commits reach this CTA's barriers before it can exit)
+      for (uint32_t q = g > (uint32_t)P_STAGES ? g - P_STAGES : 0; q < g && ok; ++q) {
+        if (!mbar_wait(smem_u32(&empty[q % P_STAGES]), (q / P_STAGES) & 1, abort_flag)) {
+          fail();
+          ok = false;
+        }
+      }
+    }
+  } else if (warp == 1) {
+    if (rank == 0) {
+      auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
+        return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag));
+      };
+      const int last_steps = (p.K - (num_kb - 1) * KB_ELEMS + 63) >> 6;
+      uint32_t g = 0, i = 0;
+      bool ok = true;
+      for (int t = pair_id; t < num_tiles && ok; t += num_pairs, ++i) {
+        if (i > 0 && !wait(acc_empty, (i - 1) & 1)) {
+          ok = false;
+          break;
+        }
+        tc_fence_after();
+        for (int kb = 0; kb < num_kb; ++kb, ++g) {
+          const int s = g % P_STAGES;
+          const uint32_t ph = (g / P_STAGES) & 1;
+          if (!wait(&full[s], ph)) {
+            ok = false;
+            break;
+          }
+          tc_fence_after();
+          const int steps = kb == num_kb - 1 ? last_steps : 4;
+          const uint32_t sf_t = tmem + SF_COL + s * SF_STAGE_COLS;
+          const uint64_t sfa_d = desc_sf_atom(smem_u32(sSFA(s)));
+          const uint64_t sfb_d = desc_sf_atom(smem_u32(sSFB(s)));
+          const uint64_t a_d = desc_kmajor_sw128(smem_u32(sA(s)));
+          const uint64_t b_d = desc_kmajor_sw128(smem_u32(sB(s)));
+#pragma unroll
+          for (int h = 0; h < 2; ++h) {
+            if (h * 2 < steps)
+              kpair_pair_elect(sf_t + h * 4, sfa_d + ((h * SF_ATOM) >> 4), sf_t + 8 + h * 8,
+                               sfb_d + ((h * SF_ATOM) >> 4),
+                               sfb_d + (((KB_ATOMS + h) * SF_ATOM) >> 4), tmem + ACC_COL,
+                               a_d + h * 4, b_d + h * 4, (kb | h) != 0, h * 2 + 1 < steps);
+          }
+          tc_commit_pair_elect(smem_u32(&empty[s]), 0x3);
+        }
+        if (!ok) break;
+        tc_commit_pair_elect(smem_u32(acc_full), 0x3);
+      }
+      if (!ok) {
+        if (lane == 0) fail();
+        tc_commit_pair_elect(smem_u32(drain), 0x1);
+        mbar_wait(smem_u32(drain), 0, nullptr);
+      }
+    }
+  } else {
+    const int ew = warp - 2;
+    const int qd = warp & 3;
+    const int half = ew >> 2;
+    uint8_t* stage = smem + P_OUT_OFFSET + ew * OUT_WARP_BYTES;
+    const uint32_t stage_s = smem_u32(stage);
+    const uint32_t leader_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
+    uint32_t i = 0;
+    if (EPI == kOut && lane == 0) prefetch_tmap(&p.tmap_d);
+    for (int t = pair_id; t < num_tiles; t += num_pairs, ++i) {
+      int mt, nt;
+      pair_tile(pa, t, mt, nt);
+      const int m0 = mt * 256 + 128 * (int)rank, n0 = nt * BN;
+      const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(acc_full), i & 1, abort_flag));
+      if (!ready) {
+        fail();
+        break;
+      }
+      tc_fence_after();
+      uint32_t acc[128];
+      const uint32_t taddr = tmem + ACC_COL + ((uint32_t)(qd * 32) << 16) + half * 128;
+      tmem_ld_32x32b_x64(taddr, acc);
+      tmem_ld_32x32b_x64(taddr + 64, acc + 64);
+      tmem_ld_wait();
+      tc_fence_before();
+      __syncwarp();
+      if (lane == 0) mbar_arrive_cluster(leader_acc_empty);
+      if (EPI == kOut)
+        epilogue_out<T>(p, acc, m0, n0, half, qd, lane, stage, stage_s);
+      else
+        epilogue_swiglu_quant(p, acc, m0, n0, half, qd, lane);
+    }
+    if (EPI == kOut && lane == 0) bulk_wait0();
+  }
+
+  tc_fence_before();
+  __syncthreads();
+  // the pair meets before either frees tensor memory or exits: the peer's
+  // accumulator is written by the leader's MMAs, its loads count on the
+  // leader's barriers
+  if (threadIdx.x == 0) {
+    mbar_arrive_cluster(mapa_shared(smem_u32(bye), rank ^ 1u));
+    if (!mbar_wait(smem_u32(bye), 0, nullptr)) record_error(H3B_ERR_TIMEOUT);
+  }
+  __syncthreads();
+  if (warp == 1) {
+    __syncwarp();
+    tc_fence_after();
+    tmem_dealloc_pair(tmem, TMEM_COLS);
+  }
+}
+
 }  // namespace mxgemm
 }  // namespace h3b

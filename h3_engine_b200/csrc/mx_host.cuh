@@ -67,20 +67,27 @@ static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64
       static_cast<T*>(out), ldo);
 }
 
-// Operands of both MXFP4 GEMM forms: shapes and alignment.
-static int mx_gemm_args(mxgemm::Args& a, const void* A, const void* sfA, int64_t M, const void* B,
-                        const void* sfB, int64_t N, int64_t K) {
+// CTA pairs wherever there are two 128-row blocks to share a B tile: 13383 x
+// 5376 x 7168 takes 196 us on them and 212 on single CTAs, 13383 x 28672 x 5376
+// 793 and 1048.
+static bool mx_use_pair(int64_t M, int64_t N) { return M > mxgemm::BM && N > 128; }
+
+// Operands of both MXFP4 GEMM kernels: shapes and alignment.
+static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, int64_t M,
+                        const void* B, const void* sfB, int64_t N, int64_t K) {
   if (!A || !sfA || !B || !sfB) return H3B_ERR_INVALID_ARG;
   if (!aligned16(A) || !aligned16(sfA) || !aligned16(B) || !aligned16(sfB))
     return H3B_ERR_ALIGNMENT;
   int rc = check_sm100();
   if (rc != H3B_OK) return rc;
-  memset(&a, 0, sizeof(a));
+  memset(&pa, 0, sizeof(pa));
+  mxgemm::Args& a = pa.base;
+  const bool pair = mx_use_pair(M, N);
   rc = make_tmap_u8_sw128(&a.tmap_a, A, (uint64_t)M, (uint64_t)(K / 2), (uint64_t)(K / 2),
                           mxgemm::KB_BYTES, mxgemm::BM);
   if (rc != H3B_OK) return rc;
   rc = make_tmap_u8_sw128(&a.tmap_b, B, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)(K / 2),
-                          mxgemm::KB_BYTES, mxgemm::BN);
+                          mxgemm::KB_BYTES, pair ? 128 : mxgemm::BN);
   if (rc != H3B_OK) return rc;
   a.sfa = static_cast<const uint8_t*>(sfA);
   a.sfb = static_cast<const uint8_t*>(sfB);
@@ -92,11 +99,37 @@ static int mx_gemm_args(mxgemm::Args& a, const void* A, const void* sfA, int64_t
   const int64_t tiles = (int64_t)a.n_tiles * ((M + mxgemm::BM - 1) / mxgemm::BM);
   if (tiles > INT32_MAX) return H3B_ERR_INVALID_ARG;
   a.num_tiles = (int)tiles;
+  if (pair) {
+    const uint64_t width = (uint64_t)a.sf_tiles_k * (mxgemm::SF_ATOM / 8);
+    rc = make_tmap_u64(&pa.tmap_sfa, sfA, (uint64_t)((M + 127) / 128), width,
+                       mxgemm::KB_ATOMS * 64, 1);
+    if (rc != H3B_OK) return rc;
+    rc = make_tmap_u64(&pa.tmap_sfb, sfB, (uint64_t)((N + 127) / 128), width,
+                       mxgemm::KB_ATOMS * 64, 2);
+    if (rc != H3B_OK) return rc;
+    pa.m_tiles = (int)((M + 255) / 256);
+    // 16 tile rows per raster group: the 74 pairs then work on 16 row and about
+    // 5 column tiles at a time (13383 x 28672 x 5376: 889 us with groups of
+    // one, 843 of 4, 811 of 8, 793 of 16, 784 of 32; shorter N, 193-198)
+    pa.group = 16;
+  }
   return H3B_OK;
 }
 
 template <typename T, int EPI>
-static int mx_gemm_launch(const mxgemm::Args& a, cudaStream_t st) {
+static int mx_gemm_launch(const mxgemm::PairArgs& pa, cudaStream_t st) {
+  const mxgemm::Args& a = pa.base;
+  if (pa.m_tiles > 0) {
+    static SmemAttr attr;
+    const int rc = attr.set(reinterpret_cast<const void*>(&mxgemm::k_gemm_mxfp4_pair<T, EPI>),
+                            mxgemm::P_SMEM_BYTES);
+    if (rc != H3B_OK) return rc;
+    const int64_t tiles = (int64_t)pa.m_tiles * a.n_tiles;
+    const int pairs = (int)std::min<int64_t>(tiles, num_sms() / 2);
+    mxgemm::k_gemm_mxfp4_pair<T, EPI>
+        <<<2 * pairs, mxgemm::THREADS, mxgemm::P_SMEM_BYTES, st>>>(pa);
+    return launched(cudaGetLastError());
+  }
   static SmemAttr attr;
   const int rc = attr.set(reinterpret_cast<const void*>(&mxgemm::k_gemm_mxfp4<T, EPI>),
                           mxgemm::SMEM_BYTES);
@@ -133,9 +166,10 @@ static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* 
 static int mx_gemm_out(const void* A, const void* sfA, int64_t M, const void* B, const void* sfB,
                        int64_t N, int64_t K, const void* bias, int act, const void* residual,
                        int64_t ldr, void* D, int dtype, int64_t ldd, cudaStream_t st) {
-  mxgemm::Args a;
-  int rc = mx_gemm_args(a, A, sfA, M, B, sfB, N, K);
+  mxgemm::PairArgs pa;
+  int rc = mx_gemm_args(pa, A, sfA, M, B, sfB, N, K);
   if (rc != H3B_OK) return rc;
+  mxgemm::Args& a = pa.base;
   rc = make_tmap_16_sw128(&a.tmap_d, D, dtype, (uint64_t)M, (uint64_t)N, (uint64_t)ldd,
                           mxgemm::OUT_COLS, 32);
   if (rc != H3B_OK) return rc;
@@ -143,8 +177,8 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t M, const void* B,
   a.residual = residual;
   a.ldr = residual ? ldr : 0;
   a.act = act;
-  return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(a, st)
-                             : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(a, st);
+  return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(pa, st)
+                             : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(pa, st);
 }
 
 }  // namespace h3b
@@ -230,12 +264,12 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   uint8_t* sfh = qh + mx_code_bytes(M, F);
   rc = h3b_mxfp4_quantize(x, dtype, M, N, ldx, q, sf, stream);
   if (rc != H3B_OK) return rc;
-  mxgemm::Args a;
-  rc = mx_gemm_args(a, q, sf, M, Bu, sfBu, 2 * F, N);
+  mxgemm::PairArgs up;
+  rc = mx_gemm_args(up, q, sf, M, Bu, sfBu, 2 * F, N);
   if (rc != H3B_OK) return rc;
-  a.q_out = qh;
-  a.sf_out = sfh;
-  rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(a, static_cast<cudaStream_t>(stream));
+  up.base.q_out = qh;
+  up.base.sf_out = sfh;
+  rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, static_cast<cudaStream_t>(stream));
   if (rc != H3B_OK) return rc;
   return mx_gemm_out(qh, sfh, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D, dtype,
                      ldd, static_cast<cudaStream_t>(stream));
