@@ -3,6 +3,7 @@
 #pragma once
 
 #include "gemm_mxfp4.cuh"
+#include "gemm_mxfp4_rows.cuh"
 #include "quant_mx.cuh"
 
 namespace h3b {
@@ -49,12 +50,31 @@ constexpr int64_t kMxMaxDim = (int64_t)INT32_MAX - 512;
 
 template <typename T>
 static void mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
-                               int64_t Mpad, cudaStream_t st) {
-  int64_t blocks = (Mpad + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
+                               int64_t Mpad, bool early, cudaStream_t st) {
+  constexpr int kUnroll = 4;
+  const int64_t per_row = (mx::sf_tiles(K) * 128 + 256 * kUnroll - 1) / (256 * kUnroll);
+  int64_t blocks = (Mpad * per_row + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
   blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
-  mx::k_mxfp4_quantize<T, 4><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
+  mx::k_mxfp4_quantize<T, kUnroll><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
       static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
-      Mpad);
+      Mpad, (uint32_t)per_row, early);
+}
+
+static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
+                       void* sf, bool early, cudaStream_t st) {
+  if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldx < K) return H3B_ERR_INVALID_ARG;
+  if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
+  if (M == 0) return H3B_OK;
+  if (!x || !q || !sf) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(x) || !aligned16(q) || (ldx * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
+  const int64_t Mpad = (M + 127) / 128 * 128;
+  if (dtype == H3B_DT_BF16)
+    mx_quantize_launch<__nv_bfloat16>(x, M, K, ldx, q, sf, Mpad, early, st);
+  else if (dtype == H3B_DT_F16)
+    mx_quantize_launch<__half>(x, M, K, ldx, q, sf, Mpad, early, st);
+  else
+    mx_quantize_launch<float>(x, M, K, ldx, q, sf, Mpad, early, st);
+  return launched(cudaGetLastError());
 }
 
 template <typename T>
@@ -139,6 +159,71 @@ static int mx_gemm_launch(const mxgemm::PairArgs& pa, cudaStream_t st) {
   return launched(cudaGetLastError());
 }
 
+// ---- up to 128 rows: the weight-streaming kernel
+template <int MT, typename T, int EPI, bool FUSED>
+static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool chained,
+                          cudaStream_t st) {
+  int rc = make_tmap_u8_sw128(&a.tmap_w, B, (uint64_t)a.N, (uint64_t)(a.K / 2),
+                              (uint64_t)(a.K / 2), mxrows::KB_BYTES, mxrows::BN);
+  if (rc != H3B_OK) return rc;
+  if (!FUSED) {
+    rc = make_tmap_u8_sw128(&a.tmap_x, A, (uint64_t)a.M, (uint64_t)(a.K / 2),
+                            (uint64_t)(a.K / 2), mxrows::KB_BYTES, MT);
+    if (rc != H3B_OK) return rc;
+  }
+  auto kernel = mxrows::k_gemm_mxfp4_rows<MT, T, EPI, FUSED>;
+  static SmemAttr attr;
+  rc = attr.set(reinterpret_cast<const void*>(kernel), mxrows::Ring<MT>::BYTES);
+  if (rc != H3B_OK) return rc;
+  const int tiles = (a.N + mxrows::BN - 1) / mxrows::BN;
+  const int num_kb = (a.K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS;
+  // as many CTAs along K as two per SM allow
+  int split = std::max(1, 2 * num_sms() / tiles);
+  split = std::min(split, std::min(num_kb, mxrows::kMaxSplit));
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)split, (unsigned)tiles, 1);
+  cfg.blockDim = dim3(mxrows::THREADS);
+  cfg.dynamicSmemBytes = mxrows::Ring<MT>::BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  at[0].id = cudaLaunchAttributeClusterDimension;
+  at[0].val.clusterDim.x = (unsigned)split;
+  at[0].val.clusterDim.y = 1;
+  at[0].val.clusterDim.z = 1;
+  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[1].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 2 : 1;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
+// Operands of the rows kernel: A as codes and scales, or (sfA NULL) as 16-bit
+// rows of stride ldx that the kernel quantizes itself.
+template <typename T, int EPI>
+static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t ldx, int64_t M,
+                        const void* B, const void* sfB, int64_t N, int64_t K, bool chained,
+                        cudaStream_t st) {
+  if (!A || !B || !sfB) return H3B_ERR_INVALID_ARG;
+  if (!aligned16(A) || !aligned16(sfA) || !aligned16(B) || !aligned16(sfB))
+    return H3B_ERR_ALIGNMENT;
+  if ((N + mxrows::BN - 1) / mxrows::BN > 65535) return H3B_ERR_INVALID_ARG;
+  const int rc = check_sm100();
+  if (rc != H3B_OK) return rc;
+  a.sfw = static_cast<const uint8_t*>(sfB);
+  a.sfx = static_cast<const uint8_t*>(sfA);
+  a.x = A;
+  a.ldx = ldx;
+  a.M = (int)M;
+  a.N = (int)N;
+  a.K = (int)K;
+  a.sf_tiles_k = (int)mx::sf_tiles(K);
+  if (!sfA) return mx_rows_launch<16, T, EPI, true>(a, A, B, chained, st);
+  if (M <= 16) return mx_rows_launch<16, T, EPI, false>(a, A, B, chained, st);
+  if (M <= 32) return mx_rows_launch<32, T, EPI, false>(a, A, B, chained, st);
+  if (M <= 64) return mx_rows_launch<64, T, EPI, false>(a, A, B, chained, st);
+  return mx_rows_launch<128, T, EPI, false>(a, A, B, chained, st);
+}
+
 // Bytes of an activation's codes and blocked scales in a workspace, each part
 // rounded up to 256 bytes.
 static inline int64_t mx_code_bytes(int64_t rows, int64_t k) {
@@ -163,9 +248,27 @@ static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* 
   return H3B_OK;
 }
 
-static int mx_gemm_out(const void* A, const void* sfA, int64_t M, const void* B, const void* sfB,
-                       int64_t N, int64_t K, const void* bias, int act, const void* residual,
-                       int64_t ldr, void* D, int dtype, int64_t ldd, cudaStream_t st) {
+// D = act(A B^T + bias) + residual.  sfA NULL (M <= kFusedRows): A is 16-bit
+// rows of stride ldx.  chained: the launch before is of the same entry point.
+static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, const void* B,
+                       const void* sfB, int64_t N, int64_t K, const void* bias, int act,
+                       const void* residual, int64_t ldr, void* D, int dtype, int64_t ldd,
+                       bool chained, cudaStream_t st) {
+  ldr = residual ? ldr : 0;
+  if (M <= mxrows::kMaxRows) {
+    mxrows::Args a;
+    memset(&a, 0, sizeof(a));
+    a.bias = bias;
+    a.residual = residual;
+    a.out = D;
+    a.ldr = ldr;
+    a.ldd = ldd;
+    a.act = act;
+    return dtype == H3B_DT_F16
+               ? mx_rows_gemm<__half, mxgemm::kOut>(a, A, sfA, ldx, M, B, sfB, N, K, chained, st)
+               : mx_rows_gemm<__nv_bfloat16, mxgemm::kOut>(a, A, sfA, ldx, M, B, sfB, N, K,
+                                                           chained, st);
+  }
   mxgemm::PairArgs pa;
   int rc = mx_gemm_args(pa, A, sfA, M, B, sfB, N, K);
   if (rc != H3B_OK) return rc;
@@ -175,10 +278,16 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t M, const void* B,
   if (rc != H3B_OK) return rc;
   a.bias = bias;
   a.residual = residual;
-  a.ldr = residual ? ldr : 0;
+  a.ldr = ldr;
   a.act = act;
   return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(pa, st)
                              : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(pa, st);
+}
+
+// 16-bit rows that a product can quantize itself.
+static int mx_input_check(const void* x, int64_t ldx, int64_t K) {
+  if (!x || ldx < K) return H3B_ERR_INVALID_ARG;
+  return !aligned16(x) || ldx % 8 ? H3B_ERR_ALIGNMENT : H3B_OK;
 }
 
 }  // namespace h3b
@@ -187,17 +296,7 @@ extern "C" {
 
 int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
                        void* sf, void* stream) {
-  if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldx < K) return H3B_ERR_INVALID_ARG;
-  if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
-  if (M == 0) return H3B_OK;
-  if (!x || !q || !sf) return H3B_ERR_INVALID_ARG;
-  if (!aligned16(x) || !aligned16(q) || (ldx * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
-  const int64_t Mpad = (M + 127) / 128 * 128;
-  cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == H3B_DT_BF16) mx_quantize_launch<__nv_bfloat16>(x, M, K, ldx, q, sf, Mpad, st);
-  else if (dtype == H3B_DT_F16) mx_quantize_launch<__half>(x, M, K, ldx, q, sf, Mpad, st);
-  else mx_quantize_launch<float>(x, M, K, ldx, q, sf, Mpad, st);
-  return launched(cudaGetLastError());
+  return mx_quantize(x, dtype, M, K, ldx, q, sf, false, static_cast<cudaStream_t>(stream));
 }
 
 int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, void* out, int dtype,
@@ -219,7 +318,8 @@ int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, con
                    int64_t ldr, void* D, int dtype, int64_t ldd, void* stream) {
   const int rc = mx_out_check(dtype, M, N, K, bias, act, residual, ldr, D, ldd);
   if (rc != H3B_OK || M == 0) return rc;
-  return mx_gemm_out(A, sfA, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
+  if (!sfA) return H3B_ERR_INVALID_ARG;
+  return mx_gemm_out(A, sfA, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, false,
                      static_cast<cudaStream_t>(stream));
 }
 
@@ -236,12 +336,17 @@ int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const voi
   if (rc != H3B_OK || M == 0) return rc;
   if (!ws || ws_bytes < h3b_mxfp4_linear_ws(M, N, K)) return H3B_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(ws) & 255u) return H3B_ERR_ALIGNMENT;
+  rc = mx_input_check(x, ldx, K);
+  if (rc != H3B_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
+  if (M <= mxrows::kFusedRows)
+    return mx_gemm_out(x, nullptr, ldx, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
+                       false, st);
   uint8_t* q = static_cast<uint8_t*>(ws);
   uint8_t* sf = q + mx_code_bytes(M, K);
-  rc = h3b_mxfp4_quantize(x, dtype, M, K, ldx, q, sf, stream);
+  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, M <= mxrows::kMaxRows, st);
   if (rc != H3B_OK) return rc;
-  return mx_gemm_out(q, sf, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
-                     static_cast<cudaStream_t>(stream));
+  return mx_gemm_out(q, sf, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, true, st);
 }
 
 int64_t h3b_mxfp4_ffn_ws(int64_t M, int64_t N, int64_t F) {
@@ -258,21 +363,42 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   if (rc != H3B_OK || M == 0) return rc;
   if (!ws || ws_bytes < h3b_mxfp4_ffn_ws(M, N, F)) return H3B_ERR_INVALID_ARG;
   if (reinterpret_cast<uintptr_t>(ws) & 255u) return H3B_ERR_ALIGNMENT;
+  rc = mx_input_check(x, ldx, N);
+  if (rc != H3B_OK) return rc;
+  cudaStream_t st = static_cast<cudaStream_t>(stream);
   uint8_t* q = static_cast<uint8_t*>(ws);
   uint8_t* sf = q + mx_code_bytes(M, N);
   uint8_t* qh = q + mx_operand_bytes(M, N);
   uint8_t* sfh = qh + mx_code_bytes(M, F);
-  rc = h3b_mxfp4_quantize(x, dtype, M, N, ldx, q, sf, stream);
+  const bool fused = M <= mxrows::kFusedRows;
+  if (!fused) {
+    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, M <= mxrows::kMaxRows, st);
+    if (rc != H3B_OK) return rc;
+  }
+  if (M <= mxrows::kMaxRows) {
+    mxrows::Args a;
+    memset(&a, 0, sizeof(a));
+    a.q_out = qh;
+    a.sf_out = sfh;
+    a.early = 1;
+    const void* A = fused ? x : q;
+    const void* sfA = fused ? nullptr : sf;
+    rc = dtype == H3B_DT_F16
+             ? mx_rows_gemm<__half, mxgemm::kSwigluQuant>(a, A, sfA, ldx, M, Bu, sfBu, 2 * F, N,
+                                                          !fused, st)
+             : mx_rows_gemm<__nv_bfloat16, mxgemm::kSwigluQuant>(a, A, sfA, ldx, M, Bu, sfBu,
+                                                                 2 * F, N, !fused, st);
+  } else {
+    mxgemm::PairArgs up;
+    rc = mx_gemm_args(up, q, sf, M, Bu, sfBu, 2 * F, N);
+    if (rc != H3B_OK) return rc;
+    up.base.q_out = qh;
+    up.base.sf_out = sfh;
+    rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, st);
+  }
   if (rc != H3B_OK) return rc;
-  mxgemm::PairArgs up;
-  rc = mx_gemm_args(up, q, sf, M, Bu, sfBu, 2 * F, N);
-  if (rc != H3B_OK) return rc;
-  up.base.q_out = qh;
-  up.base.sf_out = sfh;
-  rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, static_cast<cudaStream_t>(stream));
-  if (rc != H3B_OK) return rc;
-  return mx_gemm_out(qh, sfh, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D, dtype,
-                     ldd, static_cast<cudaStream_t>(stream));
+  return mx_gemm_out(qh, sfh, 0, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D,
+                     dtype, ldd, true, st);
 }
 
 }  // extern "C"

@@ -121,49 +121,59 @@ __device__ __forceinline__ uint32_t absmax_bits8(const float (&v)[8]) {
   return m;
 }
 
+// Lets the next launch of the stream start before this one is done, where that
+// launch waits for this one before it reads its results.
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
 // ---------------------------------------------------------------- quantize
 constexpr int kThreads = 256;
 
-// One warp per row (grid-stride), four lanes per 32-value block, each lane 8
-// values per step, UNROLL steps in flight.  A warp reads 256 consecutive
-// values and writes 128 consecutive code bytes per step.  Scales of rows in
-// [M, Mpad) and of the columns that pad a row's last tile are written as 0.
+// A warp's unit of work is UNROLL * 256 consecutive values of a row (units
+// grid-stride over rows and pieces alike, so one long row spreads over many
+// warps): four lanes per 32-value block, each lane 8 values per step, UNROLL
+// loads in flight.  Scales of rows in [M, Mpad) and of the columns that pad a
+// row's last tile are written as 0.
 template <typename T, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     k_mxfp4_quantize(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                     uint8_t* __restrict__ q, uint8_t* __restrict__ sf, int64_t Mpad) {
+                     uint8_t* __restrict__ q, uint8_t* __restrict__ sf, int64_t Mpad,
+                     uint32_t units_per_row, int early) {
+  if (early) grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int steps = (int)(K >> 3);                 // 8-value pieces of a row
   const int64_t c4 = sf_tiles(K);
   const int padded = (int)(c4 * 16);               // pieces up to the padded width
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < Mpad;
-       r += warps) {
+  const int64_t units = Mpad * units_per_row;
+  for (int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < units;
+       w += warps) {
+    const int64_t r = w / units_per_row;
+    const int h0 = (int)(w - r * units_per_row) * (32 * UNROLL);
     const bool real = r < M;
     const T* xr = x + r * ldx;
     uint8_t* qr = q + r * (K >> 1);
-    for (int h0 = 0; h0 < padded; h0 += 32 * UNROLL) {
-      Vec8<T> raw[UNROLL];
+    Vec8<T> raw[UNROLL];
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int h = h0 + u * 32 + lane;
-        raw[u].zero();
-        if (real && h < steps) raw[u].load(xr + (int64_t)h * 8);
-      }
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * 32 + lane;
+      raw[u].zero();
+      if (real && h < steps) raw[u].load(xr + (int64_t)h * 8);
+    }
 #pragma unroll
-      for (int u = 0; u < UNROLL; ++u) {
-        const int h = h0 + u * 32 + lane;
-        float v[8];
-        raw[u].get(v);
-        uint32_t m = absmax_bits8(v);
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-        m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
-        const uint32_t s = scale_byte(m);
-        if (real && h < steps)
-          *reinterpret_cast<uint32_t*>(qr + (int64_t)h * 4) = codes8(v, scale_inverse(s));
-        if ((lane & 3) == 0 && h < padded)
-          sf[sf_swizzled_offset(r, h >> 2, c4)] = static_cast<uint8_t>(s);
-      }
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * 32 + lane;
+      float v[8];
+      raw[u].get(v);
+      uint32_t m = absmax_bits8(v);
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
+      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const uint32_t s = scale_byte(m);
+      if (real && h < steps)
+        *reinterpret_cast<uint32_t*>(qr + (int64_t)h * 4) = codes8(v, scale_inverse(s));
+      if ((lane & 3) == 0 && h < padded)
+        sf[sf_swizzled_offset(r, h >> 2, c4)] = static_cast<uint8_t>(s);
     }
   }
 }
