@@ -1,10 +1,11 @@
-"""Build libh3b.so (sm_100a) in-tree with nvcc.
+"""Build libh3b.so (sm_100a) in-tree with nvcc, and _h3b_torch.so with g++.
 
     python -m h3_engine_b200.csrc.build [--verbose]
 
 The library is one translation unit (h3b.cu includes every kernel header) so
 all kernels share the device error word.  cudart is linked statically: the
-library only needs the CUDA driver at run time.
+library only needs the CUDA driver at run time.  _h3b_torch.so holds the torch
+operators that are written in C++; it links libh3b.so and torch.
 """
 from __future__ import annotations
 
@@ -18,6 +19,7 @@ HERE = Path(__file__).resolve().parent
 PKG = HERE.parent
 ROOT = PKG.parent
 LIB = PKG / "libh3b.so"
+EXT = PKG / "_h3b_torch.so"
 
 ARCH_FLAGS = ["-gencode", "arch=compute_100a,code=sm_100a"]
 NVCC_FLAGS = [
@@ -32,6 +34,16 @@ def nvcc() -> str:
         if cand and Path(cand).exists():
             return cand
     raise RuntimeError("nvcc not found")
+
+
+def cxx() -> str:
+    """The system's g++, whose C++ runtime is the one that torch loads at run
+    time (a newer compiler named by $CXX links parts of its own runtime in,
+    and the two crash on each other's streams)."""
+    for cand in ("/usr/bin/g++", shutil.which("g++")):
+        if cand and Path(cand).exists():
+            return cand
+    raise RuntimeError("g++ not found")
 
 
 def sources() -> list[Path]:
@@ -65,7 +77,33 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
     return LIB
 
 
+def build_ext(force: bool = False, verbose: bool = False) -> Path:
+    """_h3b_torch.so from torch_ext.cpp, against the installed torch and LIB."""
+    import torch
+    src = [HERE / "torch_ext.cpp", ROOT / "include" / "h3b.h"]
+    if not force and EXT.exists() and all(p.stat().st_mtime <= EXT.stat().st_mtime for p in src):
+        return EXT
+    troot = Path(torch.__file__).resolve().parent
+    cuda = Path(nvcc()).resolve().parent.parent
+    tmp = EXT.with_suffix(".so.tmp")
+    cmd = [cxx(), "-O2", "-std=c++17", "-fPIC", "-shared",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-I", str(ROOT / "include"), "-isystem", str(troot / "include"),
+           "-isystem", str(cuda / "include"), str(src[0]), "-o", str(tmp),
+           "-L", str(PKG), "-lh3b", "-L", str(troot / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
+           "-ltorch", "-Wl,-rpath,$ORIGIN"]
+    if verbose:
+        print(" ".join(cmd), flush=True)
+    r = subprocess.run(cmd, capture_output=True, text=True)
+    if r.returncode != 0:
+        sys.stderr.write(r.stdout + r.stderr)
+        raise RuntimeError(f"{cmd[0]} failed with exit code {r.returncode}")
+    os.replace(tmp, EXT)
+    return EXT
+
+
 if __name__ == "__main__":
     build(force="--force" in sys.argv, verbose="--verbose" in sys.argv,
           ptxas_v="--ptxas-v" in sys.argv)
+    build_ext(force="--force" in sys.argv, verbose="--verbose" in sys.argv)
     print(LIB)

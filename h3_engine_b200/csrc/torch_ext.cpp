@@ -1,0 +1,554 @@
+// torch operators (namespace h3b) of the MXFP4 and windowed-attention entry
+// points, in C++: these serve single tokens, where an operator written in
+// Python costs several times the kernel it launches.  Each checks its tensors
+// (ValueError, TypeError), allocates results and workspaces from torch's
+// caching allocator, and calls the C ABI of libh3b.so on the current stream of
+// its tensors' device.  Only CUDA implementations are registered.  Built as
+// _h3b_torch.so beside libh3b.so, which it links.
+#include <ATen/ATen.h>
+#include <c10/cuda/CUDAGuard.h>
+#include <c10/cuda/CUDAStream.h>
+#include <torch/library.h>
+
+#include <vector>
+
+#include "h3b.h"
+
+namespace {
+
+using at::Tensor;
+using std::optional;
+
+void check(int status, const char* what) {
+  TORCH_CHECK(status == H3B_OK, what, " failed: status ", status, " (", h3b_status_string(status),
+              ")");
+}
+
+// The call's device, current stream and guard; every tensor has to live there.
+struct Call {
+  c10::cuda::CUDAGuard guard;
+  c10::Device dev;
+  explicit Call(const Tensor& t) : guard(on_cuda(t)), dev(t.device()) {}
+  static c10::Device on_cuda(const Tensor& t) {
+    TORCH_CHECK_VALUE(t.is_cuda(), "h3b ops take CUDA tensors (there is no CPU path)");
+    return t.device();
+  }
+  void same(const Tensor& t) const {
+    TORCH_CHECK_VALUE(t.device() == dev, "tensors on different devices: ", dev, " vs ", t.device());
+  }
+  void same(const optional<Tensor>& t) const {
+    if (t) same(*t);
+  }
+  void* stream() const { return c10::cuda::getCurrentCUDAStream(dev.index()).stream(); }
+};
+
+int dtype_code(const Tensor& t, bool f32_too, const char* what) {
+  switch (t.scalar_type()) {
+    case at::kBFloat16: return H3B_DT_BF16;
+    case at::kHalf: return H3B_DT_F16;
+    case at::kFloat:
+      if (f32_too) return H3B_DT_F32;
+      break;
+    default: break;
+  }
+  TORCH_CHECK_TYPE(false, what, " takes ", f32_too ? "bf16, fp16 or fp32" : "bf16 or fp16",
+                   ", not ", t.scalar_type());
+}
+
+bool aligned(const void* p) { return (reinterpret_cast<uintptr_t>(p) & 15u) == 0; }
+
+bool rows_aligned(const Tensor& t) {
+  return t.stride(1) == 1 && t.stride(0) >= t.size(1) &&
+         t.stride(0) * (int64_t)t.element_size() % 16 == 0 && aligned(t.data_ptr());
+}
+
+// A [rows, C] view with contiguous, 16-byte aligned rows (a copy only when the
+// layout needs one).
+Tensor rows2d(const Tensor& t) {
+  TORCH_CHECK_VALUE(t.dim() >= 1, "a tensor of rows is expected");
+  Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
+  return r.numel() == 0 || rows_aligned(r) ? r : r.clone(at::MemoryFormat::Contiguous);
+}
+
+int64_t sf_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * ((k + 127) / 128) * 512; }
+
+void check_operand(const Tensor& q, const Tensor& sf, int64_t rows, int64_t k, const char* what) {
+  TORCH_CHECK_TYPE(q.scalar_type() == at::kByte && sf.scalar_type() == at::kByte, what,
+                   ": codes and scales must be uint8");
+  TORCH_CHECK_VALUE(k > 0 && k % 32 == 0, what, ": K = ", k, " must be a positive multiple of 32");
+  TORCH_CHECK_VALUE(rows >= 0, what, ": negative row count");
+  TORCH_CHECK_VALUE(q.is_contiguous() && sf.is_contiguous(), what,
+                    ": codes and scales must be contiguous");
+  TORCH_CHECK_VALUE(q.numel() >= rows * (k / 2) && sf.numel() >= sf_bytes(rows, k), what,
+                    ": codes or scales too small for ", rows, " x ", k, " values");
+}
+
+void check_n(int64_t n) {
+  TORCH_CHECK_VALUE(n > 0 && n % 8 == 0, "N = ", n, " must be a positive multiple of 8");
+}
+
+Tensor new_out(const Tensor& like, int64_t n, at::ScalarType type) {
+  auto shape = like.sizes().vec();
+  shape.back() = n;
+  return at::empty(shape, like.options().dtype(type));
+}
+
+// The [m, n] view of a caller's output.
+Tensor out_rows(const Tensor& out, at::IntArrayRef lead, int64_t m, int64_t n,
+                at::ScalarType type) {
+  auto shape = lead.vec();
+  shape.push_back(n);
+  TORCH_CHECK_VALUE(out.scalar_type() == type && out.sizes() == at::IntArrayRef(shape),
+                    "out must be ", type, " ", at::IntArrayRef(shape));
+  Tensor o = out.dim() == 2 ? out : out.view({m, n});
+  TORCH_CHECK_VALUE(m == 0 || rows_aligned(o), "out must have contiguous, 16-byte aligned rows");
+  out.unsafeGetTensorImpl()->bump_version();
+  return o;
+}
+
+struct Extras {
+  Tensor bias, residual;
+  const void* b = nullptr;
+  const void* r = nullptr;
+  int64_t ldr = 0;
+  Extras(const optional<Tensor>& bias_in, const optional<Tensor>& res_in, int64_t m, int64_t n,
+         at::ScalarType type) {
+    if (bias_in) {
+      TORCH_CHECK_VALUE(bias_in->scalar_type() == type && bias_in->dim() == 1 &&
+                            bias_in->size(0) == n,
+                        "bias must be ", type, " [", n, "]");
+      bias = *bias_in;
+      if (bias.stride(0) != 1 || !aligned(bias.data_ptr()))
+        bias = bias.clone(at::MemoryFormat::Contiguous);
+      b = bias.data_ptr();
+    }
+    if (res_in) {
+      TORCH_CHECK_VALUE(res_in->scalar_type() == type && res_in->numel() == m * n &&
+                            res_in->dim() >= 1 && res_in->size(-1) == n,
+                        "residual must be ", type, " with ", m, " rows of ", n);
+      residual = rows2d(*res_in);
+      r = residual.data_ptr();
+      ldr = residual.stride(0);
+    }
+  }
+};
+
+void check_act(int64_t act) {
+  TORCH_CHECK_VALUE(act == H3B_ACT_NONE || act == H3B_ACT_GELU_TANH,
+                    "the MXFP4 products take ACT_NONE or ACT_GELU_TANH");
+}
+
+// ---------------------------------------------------------------- MXFP4
+void quantize_into(const Call& c, const Tensor& x2, int64_t k, const Tensor& q, const Tensor& sf) {
+  const int64_t m = x2.size(0);
+  if (m == 0) return;
+  check(h3b_mxfp4_quantize(x2.data_ptr(), dtype_code(x2, true, "mxfp4_quantize"), m, k,
+                           x2.stride(0), q.data_ptr(), sf.data_ptr(), c.stream()),
+        "h3b_mxfp4_quantize");
+}
+
+Tensor quantize_input(const Tensor& x) {
+  dtype_code(x, true, "mxfp4_quantize");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) > 0 && x.size(-1) % 32 == 0,
+                    "K must be a positive multiple of 32");
+  return rows2d(x);
+}
+
+std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x) {
+  Call c(x);
+  const Tensor x2 = quantize_input(x);
+  const int64_t m = x2.size(0), k = x2.size(1);
+  const auto u8 = x.options().dtype(at::kByte);
+  Tensor q = at::empty({m, k / 2}, u8), sf = at::empty({sf_bytes(m, k)}, u8);
+  quantize_into(c, x2, k, q, sf);
+  return {q, sf};
+}
+
+void mxfp4_quantize_out(const Tensor& x, Tensor q, Tensor sf) {
+  Call c(x);
+  c.same(q);
+  c.same(sf);
+  const Tensor x2 = quantize_input(x);
+  check_operand(q, sf, x2.size(0), x2.size(1), "mxfp4_quantize");
+  q.unsafeGetTensorImpl()->bump_version();
+  sf.unsafeGetTensorImpl()->bump_version();
+  quantize_into(c, x2, x2.size(1), q, sf);
+}
+
+void dequantize_into(const Call& c, const Tensor& q, const Tensor& sf, int64_t m, int64_t k,
+                     const Tensor& out) {
+  if (m == 0) return;
+  check(h3b_mxfp4_dequantize(q.data_ptr(), sf.data_ptr(), m, k, out.data_ptr(),
+                             dtype_code(out, true, "mxfp4_dequantize"), out.stride(0), c.stream()),
+        "h3b_mxfp4_dequantize");
+}
+
+Tensor mxfp4_dequantize(const Tensor& q, const Tensor& sf, int64_t m, int64_t k,
+                        at::ScalarType dtype) {
+  Call c(q);
+  c.same(sf);
+  check_operand(q, sf, m, k, "mxfp4_dequantize");
+  TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
+                   "mxfp4_dequantize gives bf16, fp16 or fp32, not ", dtype);
+  Tensor out = at::empty({m, k}, q.options().dtype(dtype));
+  dequantize_into(c, q, sf, m, k, out);
+  return out;
+}
+
+void mxfp4_dequantize_out(const Tensor& q, const Tensor& sf, int64_t m, int64_t k, Tensor out) {
+  Call c(q);
+  c.same(sf);
+  c.same(out);
+  check_operand(q, sf, m, k, "mxfp4_dequantize");
+  dequantize_into(c, q, sf, m, k, out_rows(out, {m}, m, k, out.scalar_type()));
+}
+
+void gemm_into(const Call& c, const Tensor& qa, const Tensor& sfa, int64_t m, const Tensor& qb,
+               const Tensor& sfb, int64_t n, int64_t k, const Extras& e, int64_t act,
+               const Tensor& o) {
+  if (m == 0) return;
+  check(h3b_mxfp4_gemm(qa.data_ptr(), sfa.data_ptr(), m, qb.data_ptr(), sfb.data_ptr(), n, k, e.b,
+                       (int)act, e.r, e.ldr, o.data_ptr(), dtype_code(o, false, "mxfp4_gemm"),
+                       o.stride(0), c.stream()),
+        "h3b_mxfp4_gemm");
+}
+
+void gemm_checks(const Call& c, const Tensor& sfa, const Tensor& qa, int64_t m, const Tensor& qb,
+                 const Tensor& sfb, int64_t n, int64_t k, const optional<Tensor>& bias,
+                 int64_t act, const optional<Tensor>& residual) {
+  c.same(sfa);
+  c.same(qb);
+  c.same(sfb);
+  c.same(bias);
+  c.same(residual);
+  check_n(n);
+  check_act(act);
+  check_operand(qa, sfa, m, k, "mxfp4_gemm: A");
+  check_operand(qb, sfb, n, k, "mxfp4_gemm: B");
+}
+
+Tensor mxfp4_gemm(const Tensor& qa, const Tensor& sfa, int64_t m, const Tensor& qb,
+                  const Tensor& sfb, int64_t n, int64_t k, const optional<Tensor>& bias,
+                  int64_t act, const optional<Tensor>& residual, at::ScalarType dtype) {
+  Call c(qa);
+  gemm_checks(c, sfa, qa, m, qb, sfb, n, k, bias, act, residual);
+  TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kHalf,
+                   "mxfp4_gemm gives bf16 or fp16, not ", dtype);
+  const Extras e(bias, residual, m, n, dtype);
+  Tensor out = at::empty({m, n}, qa.options().dtype(dtype));
+  gemm_into(c, qa, sfa, m, qb, sfb, n, k, e, act, out);
+  return out;
+}
+
+void mxfp4_gemm_out(const Tensor& qa, const Tensor& sfa, int64_t m, const Tensor& qb,
+                    const Tensor& sfb, int64_t n, int64_t k, const optional<Tensor>& bias,
+                    int64_t act, const optional<Tensor>& residual, Tensor out) {
+  Call c(qa);
+  gemm_checks(c, sfa, qa, m, qb, sfb, n, k, bias, act, residual);
+  c.same(out);
+  dtype_code(out, false, "mxfp4_gemm");
+  const Extras e(bias, residual, m, n, out.scalar_type());
+  gemm_into(c, qa, sfa, m, qb, sfb, n, k, e, act, out_rows(out, {m}, m, n, out.scalar_type()));
+}
+
+Tensor product_input(const Tensor& x, int64_t k) {
+  dtype_code(x, false, "an MXFP4 product");
+  TORCH_CHECK_VALUE(x.dim() >= 1 && x.size(-1) == k, "activation width ",
+                    x.dim() ? x.size(-1) : 0, " != in_features ", k);
+  return rows2d(x);
+}
+
+void linear_into(const Call& c, const Tensor& x2, const Tensor& qb, const Tensor& sfb, int64_t n,
+                 int64_t k, const Extras& e, int64_t act, const Tensor& o, int64_t ldo) {
+  const int64_t m = x2.size(0);
+  if (m == 0) return;
+  const int64_t bytes = h3b_mxfp4_linear_ws(m, n, k);
+  const Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));
+  check(h3b_mxfp4_linear(x2.data_ptr(), dtype_code(x2, false, "mxfp4_linear"), m, x2.stride(0),
+                         qb.data_ptr(), sfb.data_ptr(), n, k, e.b, (int)act, e.r, e.ldr,
+                         o.data_ptr(), ldo, ws.data_ptr(), bytes, c.stream()),
+        "h3b_mxfp4_linear");
+}
+
+void linear_checks(const Call& c, const Tensor& qb, const Tensor& sfb, int64_t n, int64_t k,
+                   const optional<Tensor>& bias, int64_t act, const optional<Tensor>& residual) {
+  c.same(qb);
+  c.same(sfb);
+  c.same(bias);
+  c.same(residual);
+  check_n(n);
+  check_act(act);
+  check_operand(qb, sfb, n, k, "mxfp4_linear: weight");
+}
+
+Tensor mxfp4_linear(const Tensor& x, const Tensor& qb, const Tensor& sfb, int64_t n, int64_t k,
+                    const optional<Tensor>& bias, int64_t act, const optional<Tensor>& residual) {
+  Call c(x);
+  linear_checks(c, qb, sfb, n, k, bias, act, residual);
+  const Tensor x2 = product_input(x, k);
+  const Extras e(bias, residual, x2.size(0), n, x.scalar_type());
+  Tensor out = new_out(x, n, x.scalar_type());
+  linear_into(c, x2, qb, sfb, n, k, e, act, out, n);
+  return out;
+}
+
+void mxfp4_linear_out(const Tensor& x, const Tensor& qb, const Tensor& sfb, int64_t n, int64_t k,
+                      const optional<Tensor>& bias, int64_t act, const optional<Tensor>& residual,
+                      Tensor out) {
+  Call c(x);
+  linear_checks(c, qb, sfb, n, k, bias, act, residual);
+  c.same(out);
+  const Tensor x2 = product_input(x, k);
+  const Extras e(bias, residual, x2.size(0), n, x.scalar_type());
+  const Tensor o = out_rows(out, x.sizes().slice(0, x.dim() - 1), x2.size(0), n, x.scalar_type());
+  linear_into(c, x2, qb, sfb, n, k, e, act, o, o.dim() == 2 ? o.stride(0) : n);
+}
+
+void ffn_into(const Call& c, const Tensor& x2, const Tensor& qu, const Tensor& sfu,
+              const Tensor& qd, const Tensor& sfd, int64_t n, int64_t f, const Extras& e,
+              const Tensor& o, int64_t ldo) {
+  const int64_t m = x2.size(0);
+  if (m == 0) return;
+  const int64_t bytes = h3b_mxfp4_ffn_ws(m, n, f);
+  const Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));
+  check(h3b_mxfp4_ffn(x2.data_ptr(), dtype_code(x2, false, "mxfp4_ffn"), m, x2.stride(0),
+                      qu.data_ptr(), sfu.data_ptr(), qd.data_ptr(), sfd.data_ptr(), n, f, e.r,
+                      e.ldr, o.data_ptr(), ldo, ws.data_ptr(), bytes, c.stream()),
+        "h3b_mxfp4_ffn");
+}
+
+void ffn_checks(const Call& c, const Tensor& qu, const Tensor& sfu, const Tensor& qd,
+                const Tensor& sfd, int64_t n, int64_t f, const optional<Tensor>& residual) {
+  c.same(qu);
+  c.same(sfu);
+  c.same(qd);
+  c.same(sfd);
+  c.same(residual);
+  TORCH_CHECK_VALUE(f > 0 && f % 128 == 0, "feed-forward width ", f,
+                    " must be a positive multiple of 128");
+  check_operand(qu, sfu, 2 * f, n, "mxfp4_ffn: up projection");
+  check_operand(qd, sfd, n, f, "mxfp4_ffn: down projection");
+}
+
+Tensor mxfp4_ffn(const Tensor& x, const Tensor& qu, const Tensor& sfu, const Tensor& qd,
+                 const Tensor& sfd, int64_t n, int64_t f, const optional<Tensor>& residual) {
+  Call c(x);
+  ffn_checks(c, qu, sfu, qd, sfd, n, f, residual);
+  const Tensor x2 = product_input(x, n);
+  const Extras e(std::nullopt, residual, x2.size(0), n, x.scalar_type());
+  Tensor out = new_out(x, n, x.scalar_type());
+  ffn_into(c, x2, qu, sfu, qd, sfd, n, f, e, out, n);
+  return out;
+}
+
+void mxfp4_ffn_out(const Tensor& x, const Tensor& qu, const Tensor& sfu, const Tensor& qd,
+                   const Tensor& sfd, int64_t n, int64_t f, const optional<Tensor>& residual,
+                   Tensor out) {
+  Call c(x);
+  ffn_checks(c, qu, sfu, qd, sfd, n, f, residual);
+  c.same(out);
+  const Tensor x2 = product_input(x, n);
+  const Extras e(std::nullopt, residual, x2.size(0), n, x.scalar_type());
+  const Tensor o = out_rows(out, x.sizes().slice(0, x.dim() - 1), x2.size(0), n, x.scalar_type());
+  ffn_into(c, x2, qu, sfu, qd, sfd, n, f, e, o, o.stride(0));
+}
+
+// ---------------------------------------------------------------- windowed attention
+struct Rule {
+  int64_t left, right, sinks;
+  bool causal;
+  double scale;
+};
+
+void check_rule(const Rule& r, int64_t heads, int64_t kv_heads, int64_t d) {
+  TORCH_CHECK_VALUE(d == 64 || d == 128, "head_dim must be 64 or 128, not ", d);
+  TORCH_CHECK_VALUE(heads > 0 && kv_heads > 0 && heads % kv_heads == 0, heads,
+                    " query heads are not a multiple of ", kv_heads, " key heads");
+  TORCH_CHECK_VALUE(r.left >= 0 && r.right >= 0 && r.sinks >= 0,
+                    "window sides and sinks must not be negative");
+  TORCH_CHECK_VALUE(r.scale > 0, "scale must be positive");
+}
+
+// Row ranges of the documents that boundaries give.
+struct Docs {
+  std::vector<int32_t> start, len;
+  int64_t covered = 0;
+  Docs(at::IntArrayRef cu, int64_t rows, const char* what) {
+    bool ok = !cu.empty() && cu.front() >= 0 && cu.back() <= rows && rows <= (1 << 30);
+    for (size_t i = 0; ok && i + 1 < cu.size(); ++i) ok = cu[i] <= cu[i + 1];
+    TORCH_CHECK_VALUE(ok, what, " must rise from 0 or more to at most ", rows);
+    start.reserve(cu.size());
+    len.reserve(cu.size());
+    for (size_t i = 0; i + 1 < cu.size(); ++i) {
+      start.push_back((int32_t)cu[i]);
+      len.push_back((int32_t)(cu[i + 1] - cu[i]));
+      covered += len.back();
+    }
+  }
+};
+
+struct Packed {
+  Tensor q, k, v;
+  Docs qd, kd;
+  static at::IntArrayRef keys(at::IntArrayRef cu, const at::OptionalIntArrayRef& cu_k) {
+    return cu_k ? *cu_k : cu;
+  }
+  Packed(const Call& c, const Tensor& q_, const Tensor& k_, const Tensor& v_, int64_t heads,
+         int64_t kv_heads, int64_t d, at::IntArrayRef cu, const at::OptionalIntArrayRef& cu_k,
+         const Rule& r)
+      : q(ready(c, q_)),
+        k(ready(c, k_)),
+        v(ready(c, v_)),
+        qd(cu, q.size(0), "cu_seqlens"),
+        kd(keys(cu, cu_k), k.size(0), "cu_seqlens_k") {
+    check_rule(r, heads, kv_heads, d);
+    dtype_code(q, false, "attention");
+    TORCH_CHECK_TYPE(k.scalar_type() == q.scalar_type() && v.scalar_type() == q.scalar_type(),
+                     "q, k, v must be of one type");
+    TORCH_CHECK_VALUE(q.size(1) == heads * d && k.sizes() == v.sizes() &&
+                          k.size(1) == kv_heads * d,
+                      "q must be [rows, heads * head_dim], k and v [rows, kv_heads * head_dim]");
+    TORCH_CHECK_VALUE(qd.start.size() == kd.start.size(),
+                      "cu_seqlens and cu_seqlens_k name different numbers of documents");
+  }
+  static Tensor ready(const Call& c, const Tensor& t) {
+    c.same(t);
+    return rows2d(t);
+  }
+};
+
+void window_into(const Call& c, const Packed& p, int64_t heads, int64_t kv_heads, int64_t d,
+                 const Rule& r, const Tensor& o) {
+  if (p.qd.covered == 0) return;
+  check(h3b_attention_window(p.q.data_ptr(), p.q.size(0), p.q.stride(0), p.k.data_ptr(),
+                             p.k.stride(0), p.v.data_ptr(), p.v.stride(0), p.k.size(0),
+                             dtype_code(p.q, false, "attention"), (int)heads, (int)kv_heads,
+                             (int)d, p.qd.start.data(), p.qd.len.data(), p.kd.start.data(),
+                             p.kd.len.data(), (int)p.qd.start.size(), r.left, r.right, r.sinks,
+                             r.causal, (float)r.scale, o.data_ptr(), o.stride(0), c.stream()),
+        "h3b_attention_window");
+}
+
+Tensor attention_window(const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads,
+                        int64_t kv_heads, int64_t d, at::IntArrayRef cu,
+                        at::OptionalIntArrayRef cu_k, int64_t left, int64_t right, int64_t sinks,
+                        bool causal, double scale) {
+  Call c(q);
+  const Rule r{left, right, sinks, causal, scale};
+  const Packed p(c, q, k, v, heads, kv_heads, d, cu, cu_k, r);
+  // rows of no document read as zeros
+  Tensor out = p.qd.covered == p.q.size(0) ? at::empty({p.q.size(0), heads * d}, q.options())
+                                           : at::zeros({p.q.size(0), heads * d}, q.options());
+  window_into(c, p, heads, kv_heads, d, r, out);
+  return out;
+}
+
+void attention_window_out(const Tensor& q, const Tensor& k, const Tensor& v, int64_t heads,
+                          int64_t kv_heads, int64_t d, at::IntArrayRef cu,
+                          at::OptionalIntArrayRef cu_k, int64_t left, int64_t right,
+                          int64_t sinks, bool causal, double scale, Tensor out) {
+  Call c(q);
+  c.same(out);
+  const Rule r{left, right, sinks, causal, scale};
+  const Packed p(c, q, k, v, heads, kv_heads, d, cu, cu_k, r);
+  const int64_t rows = p.q.size(0);
+  window_into(c, p, heads, kv_heads, d, r,
+              out_rows(out, {rows}, rows, heads * d, q.scalar_type()));
+}
+
+bool decode_strides(const Tensor& t) {
+  return t.stride(3) == 1 && (t.stride(0) | t.stride(1) | t.stride(2)) % 8 == 0 &&
+         aligned(t.data_ptr());
+}
+
+void decode_into(const Call& c, const Tensor& q_in, const Tensor& k, const Tensor& v,
+                 const Tensor& len, const Rule& r, const Tensor& out) {
+  c.same(k);
+  c.same(v);
+  c.same(len);
+  TORCH_CHECK_VALUE(q_in.dim() == 4 && k.dim() == 4 && k.sizes() == v.sizes(),
+                    "q must be [B, n_new, heads, D], k and v [B, room, kv_heads, D]");
+  const int64_t B = q_in.size(0), n = q_in.size(1), heads = q_in.size(2), d = q_in.size(3);
+  TORCH_CHECK_VALUE(k.size(0) == B && k.size(3) == d, "q, k and v must agree on batch and head_dim");
+  check_rule(r, heads, k.size(2), d);
+  const int dt = dtype_code(q_in, false, "attention");
+  TORCH_CHECK_TYPE(k.scalar_type() == q_in.scalar_type() && v.scalar_type() == q_in.scalar_type(),
+                   "q, k, v must be of one type");
+  TORCH_CHECK_VALUE(len.scalar_type() == at::kInt && len.dim() == 1 && len.size(0) == B &&
+                        len.is_contiguous(),
+                    "kv_len must be a contiguous int32 [", B, "]");
+  TORCH_CHECK_VALUE(out.scalar_type() == q_in.scalar_type() && out.sizes() == q_in.sizes() &&
+                        out.is_contiguous() && aligned(out.data_ptr()),
+                    "out must be a contiguous, 16-byte aligned ", q_in.scalar_type(), " ",
+                    q_in.sizes());
+  TORCH_CHECK_VALUE(k.numel() == 0 || (decode_strides(k) && decode_strides(v)),
+                    "caches need a contiguous head_dim and 16-byte aligned rows");
+  if (out.numel() == 0) return;
+  const Tensor q = decode_strides(q_in) ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
+  check(h3b_attention_window_decode(q.data_ptr(), q.strides().data(), k.data_ptr(),
+                                    k.strides().data(), v.data_ptr(), v.strides().data(),
+                                    len.const_data_ptr<int32_t>(), B, k.size(1), n, dt, (int)heads,
+                                    (int)k.size(2), (int)d, r.left, r.right, r.sinks, r.causal,
+                                    (float)r.scale, out.data_ptr(), c.stream()),
+        "h3b_attention_window_decode");
+}
+
+Tensor attention_window_decode(const Tensor& q, const Tensor& k, const Tensor& v,
+                               const Tensor& len, int64_t left, int64_t right, int64_t sinks,
+                               bool causal, double scale) {
+  Call c(q);
+  Tensor out = at::empty(q.sizes(), q.options());
+  decode_into(c, q, k, v, len, Rule{left, right, sinks, causal, scale}, out);
+  return out;
+}
+
+void attention_window_decode_out(const Tensor& q, const Tensor& k, const Tensor& v,
+                                 const Tensor& len, int64_t left, int64_t right, int64_t sinks,
+                                 bool causal, double scale, Tensor out) {
+  Call c(q);
+  c.same(out);
+  decode_into(c, q, k, v, len, Rule{left, right, sinks, causal, scale}, out);
+  out.unsafeGetTensorImpl()->bump_version();
+}
+
+}  // namespace
+
+#define MX_GEMM "Tensor qa, Tensor sfa, int m, Tensor qb, Tensor sfb, int n, int k, Tensor? bias, int act, Tensor? residual"
+#define MX_LINEAR "Tensor x, Tensor qb, Tensor sfb, int n, int k, Tensor? bias, int act, Tensor? residual"
+#define MX_FFN "Tensor x, Tensor qu, Tensor sfu, Tensor qd, Tensor sfd, int n, int f, Tensor? residual"
+#define WINDOW "Tensor q, Tensor k, Tensor v, int heads, int kv_heads, int head_dim, int[] cu_seqlens, int[]? cu_seqlens_k, int left, int right, int sinks, bool causal, float scale"
+#define DECODE "Tensor q, Tensor k, Tensor v, Tensor kv_len, int left, int right, int sinks, bool causal, float scale"
+
+TORCH_LIBRARY_FRAGMENT(h3b, m) {
+  m.def("mxfp4_quantize(Tensor x) -> (Tensor, Tensor)");
+  m.def("mxfp4_quantize_out(Tensor x, Tensor(a!) q, Tensor(b!) sf) -> ()");
+  m.def("mxfp4_dequantize(Tensor q, Tensor sf, int m, int k, ScalarType dtype) -> Tensor");
+  m.def("mxfp4_dequantize_out(Tensor q, Tensor sf, int m, int k, Tensor(a!) out) -> ()");
+  m.def("mxfp4_gemm(" MX_GEMM ", ScalarType dtype) -> Tensor");
+  m.def("mxfp4_gemm_out(" MX_GEMM ", Tensor(a!) out) -> ()");
+  m.def("mxfp4_linear(" MX_LINEAR ") -> Tensor");
+  m.def("mxfp4_linear_out(" MX_LINEAR ", Tensor(a!) out) -> ()");
+  m.def("mxfp4_ffn(" MX_FFN ") -> Tensor");
+  m.def("mxfp4_ffn_out(" MX_FFN ", Tensor(a!) out) -> ()");
+  m.def("attention_window(" WINDOW ") -> Tensor");
+  m.def("attention_window_out(" WINDOW ", Tensor(a!) out) -> ()");
+  m.def("attention_window_decode(" DECODE ") -> Tensor");
+  m.def("attention_window_decode_out(" DECODE ", Tensor(a!) out) -> ()");
+}
+
+TORCH_LIBRARY_IMPL(h3b, CUDA, m) {
+  m.impl("mxfp4_quantize", &mxfp4_quantize);
+  m.impl("mxfp4_quantize_out", &mxfp4_quantize_out);
+  m.impl("mxfp4_dequantize", &mxfp4_dequantize);
+  m.impl("mxfp4_dequantize_out", &mxfp4_dequantize_out);
+  m.impl("mxfp4_gemm", &mxfp4_gemm);
+  m.impl("mxfp4_gemm_out", &mxfp4_gemm_out);
+  m.impl("mxfp4_linear", &mxfp4_linear);
+  m.impl("mxfp4_linear_out", &mxfp4_linear_out);
+  m.impl("mxfp4_ffn", &mxfp4_ffn);
+  m.impl("mxfp4_ffn_out", &mxfp4_ffn_out);
+  m.impl("attention_window", &attention_window);
+  m.impl("attention_window_out", &attention_window_out);
+  m.impl("attention_window_decode", &attention_window_decode);
+  m.impl("attention_window_decode_out", &attention_window_decode_out);
+}

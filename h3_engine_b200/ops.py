@@ -368,8 +368,25 @@ def ada_modulate(x: torch.Tensor, scale: torch.Tensor, shift: torch.Tensor,
 
 
 # ---------------------------------------------------------------- MXFP4
+# Checks of shapes, types and strides are the operators' own (ValueError,
+# TypeError); a layout that a kernel cannot read is copied, an output or a
+# cache of that kind is refused.
 MX_BLOCK = 32
-_16BIT = (torch.bfloat16, torch.float16)
+
+_QUANTIZE, _QUANTIZE_OUT = (torch_ops.ext_op(n) for n in ("mxfp4_quantize", "mxfp4_quantize_out"))
+_DEQUANTIZE, _DEQUANTIZE_OUT = (torch_ops.ext_op(n)
+                                for n in ("mxfp4_dequantize", "mxfp4_dequantize_out"))
+_GEMM, _GEMM_OUT = (torch_ops.ext_op(n) for n in ("mxfp4_gemm", "mxfp4_gemm_out"))
+_LINEAR, _LINEAR_OUT = (torch_ops.ext_op(n) for n in ("mxfp4_linear", "mxfp4_linear_out"))
+_FFN, _FFN_OUT = (torch_ops.ext_op(n) for n in ("mxfp4_ffn", "mxfp4_ffn_out"))
+_WINDOW, _WINDOW_OUT = (torch_ops.ext_op(n) for n in ("attention_window", "attention_window_out"))
+_DECODE, _DECODE_OUT = (torch_ops.ext_op(n) for n in ("attention_window_decode",
+                                                      "attention_window_decode_out"))
+
+
+def _cuda_only(t: torch.Tensor) -> None:
+    if not t.is_cuda:
+        raise ValueError("h3b ops take CUDA tensors (there is no CPU path)")
 
 
 def mxfp4_sf_bytes(rows: int, k: int) -> int:
@@ -378,94 +395,21 @@ def mxfp4_sf_bytes(rows: int, k: int) -> int:
     return pad_m(rows) // 128 * (-(-k // 128)) * 512
 
 
-def _mx_rows(t: torch.Tensor) -> torch.Tensor:
-    """A [rows, K] view with a contiguous last dim and 16-byte aligned rows (a
-    copy only when the layout needs one)."""
-    t2 = t if t.dim() == 2 else t.reshape(-1, t.shape[-1])
-    size = t2.element_size()
-    if t2.stride(1) != 1 or t2.stride(0) * size % 16 or t2.storage_offset() * size % 16 \
-            or t2.stride(0) < t2.shape[1]:
-        t2 = t2.clone(memory_format=torch.contiguous_format)
-    return t2
-
-
-def _mx_operand(q: torch.Tensor, sf: torch.Tensor, rows: int, k: int, what: str) -> None:
-    if q.dtype != torch.uint8 or sf.dtype != torch.uint8:
-        raise TypeError(f"{what}: codes and scales must be uint8")
-    if k <= 0 or k % MX_BLOCK:
-        raise ValueError(f"{what}: K = {k} must be a positive multiple of {MX_BLOCK}")
-    if not (q.is_contiguous() and sf.is_contiguous()):
-        raise ValueError(f"{what}: codes and scales must be contiguous")
-    if q.numel() < rows * (k // 2) or sf.numel() < mxfp4_sf_bytes(rows, k):
-        raise ValueError(f"{what}: codes or scales too small for {rows} x {k} values")
-
-
-def _mx_out(out: torch.Tensor | None, m: int, n: int, dtype: torch.dtype, dev,
-            lead: torch.Size) -> tuple[torch.Tensor, torch.Tensor, int]:
-    """(the tensor to return, the [m, n] view the kernel writes, its row stride)."""
-    if out is None:
-        out = torch.empty(*lead, n, dtype=dtype, device=dev)
-        return out, out, n
-    if out.dtype != dtype or out.shape != (*lead, n):
-        raise ValueError(f"out must be {dtype} {(*lead, n)}")
-    o2 = out if out.dim() == 2 else out.view(m, n)
-    size = o2.element_size()
-    if m and (o2.stride(1) != 1 or o2.stride(0) * size % 16 or o2.stride(0) < n
-              or o2.storage_offset() * size % 16):
-        raise ValueError("out must have contiguous, 16-byte aligned rows")
-    torch.autograd.graph.increment_version(out)
-    return out, o2, o2.stride(0)
-
-
-def _mx_residual(residual: torch.Tensor | None, m: int, n: int, dtype: torch.dtype):
-    if residual is None:
-        return None, 0
-    if residual.dtype != dtype or residual.numel() != m * n or residual.shape[-1] != n:
-        raise ValueError(f"residual must be {dtype} with {m} rows of {n}")
-    r2 = _mx_rows(residual)
-    return r2, r2.stride(0)
-
-
-def _mx_bias(bias: torch.Tensor | None, n: int, dtype: torch.dtype) -> torch.Tensor | None:
-    if bias is None:
-        return None
-    if bias.dtype != dtype or bias.shape != (n,):
-        raise ValueError(f"bias must be {dtype} [{n}]")
-    if bias.stride(0) != 1 or bias.storage_offset() % 8:
-        bias = bias.clone(memory_format=torch.contiguous_format)
-    return bias
-
-
-def _mx_act(act: int) -> None:
-    if act not in (ACT_NONE, ACT_GELU_TANH):
-        raise ValueError("the MXFP4 products take ACT_NONE or ACT_GELU_TANH")
-
-
 def mxfp4_quantize(x: torch.Tensor, *, q_out: torch.Tensor | None = None,
                    sf_out: torch.Tensor | None = None):
     """bf16, fp16 or fp32 ``[..., K]`` -> (codes u8 ``[M, K/2]``, blocked E8M0
     scales u8, flat): MXFP4, one power-of-two scale per 32 values and no
     tensor-wide scale, so no amax pass.  ``K % 32 == 0``.  A block holding an
     infinity or a NaN becomes NaN as a whole."""
-    dev = _need_cuda(x, q_out, sf_out)
-    if x.dtype not in torch_ops.DTYPES:
-        raise TypeError(f"mxfp4_quantize takes bf16, fp16 or fp32, not {x.dtype}")
-    K = x.shape[-1]
-    if K <= 0 or K % MX_BLOCK:
-        raise ValueError(f"K = {K} must be a positive multiple of {MX_BLOCK}")
-    x2 = _mx_rows(x)
-    M = x2.shape[0]
+    _cuda_only(x)
+    if q_out is None and sf_out is None:
+        return _QUANTIZE(x)
+    rows, k = x.numel() // max(x.shape[-1], 1), x.shape[-1]
     if q_out is None:
-        q_out = torch.empty(M, K // 2, dtype=torch.uint8, device=dev)
-    else:
-        torch.autograd.graph.increment_version(q_out)
+        q_out = torch.empty(rows, k // 2, dtype=torch.uint8, device=x.device)
     if sf_out is None:
-        sf_out = torch.empty(mxfp4_sf_bytes(M, K), dtype=torch.uint8, device=dev)
-    else:
-        torch.autograd.graph.increment_version(sf_out)
-    _mx_operand(q_out, sf_out, M, K, "mxfp4_quantize")
-    if M:
-        _H3B.mxfp4_quantize(x2, M, K, x2.stride(0), q_out, sf_out)
+        sf_out = torch.empty(mxfp4_sf_bytes(rows, k), dtype=torch.uint8, device=x.device)
+    _QUANTIZE_OUT(x, q_out, sf_out)
     return q_out, sf_out
 
 
@@ -473,14 +417,11 @@ def mxfp4_dequantize(q: torch.Tensor, sf: torch.Tensor, M: int, K: int, *,
                      dtype: torch.dtype = torch.bfloat16,
                      out: torch.Tensor | None = None) -> torch.Tensor:
     """``[M, K]`` values of MXFP4 codes and blocked scales (exact in bf16 and
-    fp32, rounded in fp16)."""
-    dev = _need_cuda(q, sf, out)
-    if dtype not in torch_ops.DTYPES:
-        raise TypeError(f"mxfp4_dequantize gives bf16, fp16 or fp32, not {dtype}")
-    _mx_operand(q, sf, M, K, "mxfp4_dequantize")
-    out, o2, ldo = _mx_out(out, M, K, dtype, dev, (M,))
-    if M:
-        _H3B.mxfp4_dequantize(q, sf, M, K, o2, ldo)
+    fp32, rounded in fp16); ``out``, when given, names the type."""
+    _cuda_only(q)
+    if out is None:
+        return _DEQUANTIZE(q, sf, M, K, dtype)
+    _DEQUANTIZE_OUT(q, sf, M, K, out)
     return out
 
 
@@ -490,29 +431,12 @@ def mxfp4_gemm(qa: torch.Tensor, sfa: torch.Tensor, M: int, qb: torch.Tensor, sf
                out: torch.Tensor | None = None) -> torch.Tensor:
     """``act(deq(qa) @ deq(qb)^T + bias) + residual`` in bf16 or fp16
     ``[M, N]``, accumulated in fp32, both operands MXFP4 (``mxfp4_quantize``).
-    ``K % 32 == 0``, ``N % 8 == 0``."""
-    dev = _need_cuda(qa, sfa, qb, sfb, bias, residual, out)
-    if dtype not in _16BIT:
-        raise TypeError(f"mxfp4_gemm gives bf16 or fp16, not {dtype}")
-    if N <= 0 or N % 8:
-        raise ValueError(f"N = {N} must be a positive multiple of 8")
-    _mx_act(act)
-    _mx_operand(qa, sfa, M, K, "mxfp4_gemm: A")
-    _mx_operand(qb, sfb, N, K, "mxfp4_gemm: B")
-    bias = _mx_bias(bias, N, dtype)
-    residual, ldr = _mx_residual(residual, M, N, dtype)
-    out, o2, ldd = _mx_out(out, M, N, dtype, dev, (M,))
-    if M:
-        _H3B.mxfp4_gemm(qa, sfa, M, qb, sfb, N, K, bias, act, residual, ldr, o2, ldd)
+    ``K % 32 == 0``, ``N % 8 == 0``; ``out``, when given, names the type."""
+    _cuda_only(qa)
+    if out is None:
+        return _GEMM(qa, sfa, M, qb, sfb, N, K, bias, act, residual, dtype)
+    _GEMM_OUT(qa, sfa, M, qb, sfb, N, K, bias, act, residual, out)
     return out
-
-
-def _mx_input(x: torch.Tensor, K: int) -> torch.Tensor:
-    if x.dtype not in _16BIT:
-        raise TypeError(f"MXFP4 products take bf16 or fp16 activations, not {x.dtype}")
-    if x.shape[-1] != K:
-        raise ValueError(f"activation width {x.shape[-1]} != in_features {K}")
-    return _mx_rows(x)
 
 
 def mxfp4_linear(x: torch.Tensor, qb: torch.Tensor, sfb: torch.Tensor, N: int, K: int, *,
@@ -522,27 +446,11 @@ def mxfp4_linear(x: torch.Tensor, qb: torch.Tensor, sfb: torch.Tensor, N: int, K
     """``act(Q(x) @ deq(qb)^T + bias) + residual`` in x's type for ``x``
     ``[..., K]`` bf16 or fp16: quantization and product in one call, from one
     token to whole sequences."""
-    dev = _need_cuda(x, qb, sfb, bias, residual, out)
-    if N <= 0 or N % 8:
-        raise ValueError(f"N = {N} must be a positive multiple of 8")
-    _mx_act(act)
-    _mx_operand(qb, sfb, N, K, "mxfp4_linear: weight")
-    x2 = _mx_input(x, K)
-    M = x2.shape[0]
-    bias = _mx_bias(bias, N, x.dtype)
-    residual, ldr = _mx_residual(residual, M, N, x.dtype)
-    out, o2, ldd = _mx_out(out, M, N, x.dtype, dev, x.shape[:-1])
-    if M:
-        ws = torch.empty(_mx_operand_bytes(M, K), dtype=torch.uint8, device=dev)
-        _H3B.mxfp4_linear(x2, M, x2.stride(0), qb, sfb, N, K, bias, act, residual, ldr, o2, ldd,
-                          ws)
+    _cuda_only(x)
+    if out is None:
+        return _LINEAR(x, qb, sfb, N, K, bias, act, residual)
+    _LINEAR_OUT(x, qb, sfb, N, K, bias, act, residual, out)
     return out
-
-
-def _mx_operand_bytes(rows: int, k: int) -> int:
-    """Workspace of one quantized activation (h3b_mxfp4_linear_ws): its codes,
-    rounded up to 256 bytes, and its blocked scales."""
-    return -(-rows * (k // 2) // 256) * 256 + mxfp4_sf_bytes(rows, k)
 
 
 def mxfp4_ffn(x: torch.Tensor, qu: torch.Tensor, sfu: torch.Tensor, qd: torch.Tensor,
@@ -553,19 +461,10 @@ def mxfp4_ffn(x: torch.Tensor, qu: torch.Tensor, sfu: torch.Tensor, qd: torch.Te
     the up projection's 2F rows in ``swiglu_rows`` order, ``qd`` ``[N, F]``.
     The hidden activation is quantized in the up projection's epilogue.
     ``N % 32 == 0``, ``F % 128 == 0``."""
-    dev = _need_cuda(x, qu, sfu, qd, sfd, residual, out)
-    if F <= 0 or F % 128:
-        raise ValueError(f"feed-forward width {F} must be a positive multiple of 128")
-    _mx_operand(qu, sfu, 2 * F, N, "mxfp4_ffn: up projection")
-    _mx_operand(qd, sfd, N, F, "mxfp4_ffn: down projection")
-    x2 = _mx_input(x, N)
-    M = x2.shape[0]
-    residual, ldr = _mx_residual(residual, M, N, x.dtype)
-    out, o2, ldd = _mx_out(out, M, N, x.dtype, dev, x.shape[:-1])
-    if M:
-        ws = torch.empty(_mx_operand_bytes(M, N) + _mx_operand_bytes(M, F), dtype=torch.uint8,
-                         device=dev)
-        _H3B.mxfp4_ffn(x2, M, x2.stride(0), qu, sfu, qd, sfd, N, F, residual, ldr, o2, ldd, ws)
+    _cuda_only(x)
+    if out is None:
+        return _FFN(x, qu, sfu, qd, sfd, N, F, residual)
+    _FFN_OUT(x, qu, sfu, qd, sfd, N, F, residual, out)
     return out
 
 
@@ -573,28 +472,8 @@ def mxfp4_ffn(x: torch.Tensor, qu: torch.Tensor, sfu: torch.Tensor, qd: torch.Te
 _ALL_KEYS = (1 << 30) - 1
 
 
-def _window_rule(window, sinks: int, causal: bool) -> tuple[int, int, int, bool]:
-    left, right = window
-    left = _ALL_KEYS if left is None else int(left)
-    right = _ALL_KEYS if right is None else int(right)
-    if left < 0 or right < 0 or sinks < 0:
-        raise ValueError("window sides and sinks must not be negative")
-    return left, right, int(sinks), bool(causal)
-
-
-def _heads_dim(heads: int, kv_heads: int, head_dim: int) -> None:
-    if head_dim not in (64, 128):
-        raise ValueError(f"head_dim must be 64 or 128, not {head_dim}")
-    if heads <= 0 or kv_heads <= 0 or heads % kv_heads:
-        raise ValueError(f"{heads} query heads are not a multiple of {kv_heads} key heads")
-
-
-def _ranges(cu, rows: int, what: str) -> tuple[list[int], list[int]]:
-    """(starts, lengths) of the documents that host boundaries give."""
-    cu = [int(c) for c in (cu.tolist() if hasattr(cu, "tolist") else cu)]
-    if not cu or cu[0] < 0 or cu[-1] > rows or any(b < a for a, b in zip(cu, cu[1:])):
-        raise ValueError(f"{what} must rise from 0 or more to at most {rows}")
-    return cu[:-1], [b - a for a, b in zip(cu, cu[1:])]
+def _host_ints(cu):
+    return None if cu is None else [int(c) for c in (cu.tolist() if hasattr(cu, "tolist") else cu)]
 
 
 def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: int, head_dim: int,
@@ -612,34 +491,18 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     None meaning no limit.  A query that sees nothing gets zeros.
     ``cu_seqlens`` (queries) and ``cu_seqlens_k`` (keys, default the same) are
     host boundaries; rows of ``out`` outside them are left as they were (zeros
-    when ``out`` is allocated here)."""
-    dev = _need_cuda(q, k, v, out)
-    kv_heads = heads if kv_heads is None else kv_heads
-    _heads_dim(heads, kv_heads, head_dim)
-    left, right, sinks, causal = _window_rule(window, sinks, causal)
-    q2, k2, v2 = _mx_rows(q), _mx_rows(k), _mx_rows(v)
-    if q2.dtype not in _16BIT or k2.dtype != q2.dtype or v2.dtype != q2.dtype:
-        raise TypeError("q, k, v must be bf16 or fp16, of one type")
-    rows, hd = q2.shape
-    if hd != heads * head_dim or k2.shape != v2.shape or k2.shape[1] != kv_heads * head_dim:
-        raise ValueError("q must be [rows, heads * head_dim], k and v [rows, kv_heads * head_dim]")
-    qs, ql = _ranges(cu_seqlens, rows, "cu_seqlens")
-    ks, kl = _ranges(cu_seqlens if cu_seqlens_k is None else cu_seqlens_k, k2.shape[0],
-                     "cu_seqlens_k")
-    if len(ks) != len(qs):
-        raise ValueError("cu_seqlens and cu_seqlens_k name different numbers of documents")
-    sc = float(scale) if scale is not None else head_dim ** -0.5
-    if not sc > 0:
-        raise ValueError("scale must be positive")
+    when ``out`` is allocated here).  Values that some query sees have to be
+    finite for the other queries of its 256-row tile; what no query of a tile
+    sees does not matter."""
+    _cuda_only(q)
+    left, right = window
+    args = (q, k, v, heads, heads if kv_heads is None else kv_heads, head_dim,
+            _host_ints(cu_seqlens), _host_ints(cu_seqlens_k),
+            _ALL_KEYS if left is None else left, _ALL_KEYS if right is None else right, sinks,
+            causal, head_dim ** -0.5 if scale is None else scale)
     if out is None:
-        covered = sum(ql) == rows
-        out = (torch.empty if covered else torch.zeros)(rows, hd, dtype=q2.dtype, device=dev)
-        o2 = out
-    else:
-        out, o2, _ = _mx_out(out, rows, hd, q2.dtype, dev, q.shape[:-1])
-    if sum(ql):
-        _H3B.attention_window(q2, k2, v2, heads, kv_heads, head_dim, qs, ql, ks, kl, left, right,
-                              sinks, causal, sc, o2)
+        return _WINDOW(*args)
+    _WINDOW_OUT(*args, out)
     return out
 
 
@@ -654,37 +517,12 @@ def attention_window_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     keys in use, the new tokens' own included, so token t stands at position
     ``kv_len - n_new + t``.  Lengths are read when the kernel runs (a captured
     call follows them) and clamped to [0, room].  Returns [B, n_new, heads, D]."""
-    dev = _need_cuda(q, k, v, kv_len, out)
-    if q.dim() != 4 or k.dim() != 4 or k.shape != v.shape:
-        raise ValueError("q must be [B, n_new, heads, D], k and v [B, room, kv_heads, D]")
-    B, n, heads, D = q.shape
-    if k.shape[0] != B or k.shape[3] != D:
-        raise ValueError("q, k and v must agree on batch and head_dim")
-    _heads_dim(heads, k.shape[2], D)
-    if q.dtype not in _16BIT or k.dtype != q.dtype or v.dtype != q.dtype:
-        raise TypeError("q, k, v must be bf16 or fp16, of one type")
-    if kv_len.dtype != torch.int32 or kv_len.shape != (B,) or not kv_len.is_contiguous():
-        raise ValueError(f"kv_len must be a contiguous int32 [{B}]")
-    left, right, sinks, causal = _window_rule(window, sinks, causal)
-    if not _decode_strides(q):
-        q = q.clone(memory_format=torch.contiguous_format)
-    if not (_decode_strides(k) and _decode_strides(v)):
-        raise ValueError("caches need a contiguous head_dim and 16-byte aligned rows")
-    sc = float(scale) if scale is not None else D ** -0.5
-    if not sc > 0:
-        raise ValueError("scale must be positive")
+    _cuda_only(q)
+    left, right = window
+    left = _ALL_KEYS if left is None else left
+    right = _ALL_KEYS if right is None else right
+    scale = q.shape[-1] ** -0.5 if scale is None else scale
     if out is None:
-        out = torch.empty(B, n, heads, D, dtype=q.dtype, device=dev)
-    elif out.dtype != q.dtype or out.shape != q.shape or not out.is_contiguous() \
-            or out.storage_offset() % 8:
-        raise ValueError(f"out must be a contiguous, 16-byte aligned {q.dtype} {tuple(q.shape)}")
-    else:
-        torch.autograd.graph.increment_version(out)
-    if B and n:
-        _H3B.attention_window_decode(q, k, v, kv_len, left, right, sinks, causal, sc, out)
+        return _DECODE(q, k, v, kv_len, left, right, sinks, causal, scale)
+    _DECODE_OUT(q, k, v, kv_len, left, right, sinks, causal, scale, out)
     return out
-
-
-def _decode_strides(t: torch.Tensor) -> bool:
-    s = t.stride()
-    return s[3] == 1 and not (s[0] | s[1] | s[2]) % 8 and not t.storage_offset() % 8

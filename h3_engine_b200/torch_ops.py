@@ -14,7 +14,6 @@ is a dispatch error, never a silent fallback.  The tensor-level wrappers in
 ``ops.py`` allocate outputs, check shapes and call these operators; they are
 the functions the rest of the package uses.
 """
-import ctypes
 from typing import Optional
 
 import torch
@@ -190,98 +189,56 @@ def amax_exchange(amax: torch.Tensor, slot_table: torch.Tensor, rank: int, world
 
 
 # ---------------------------------------------------------------- MXFP4 and windowed attention
-# These operators serve single tokens too, where the dispatch costs as much as
-# the kernel, so they are registered with the lighter ``torch.library.Library``
-# interface (same schema rules: mutated outputs declared, CUDA only, fake
-# implementations).  Their wrappers in ops.py bump the version counter of an
-# output that the caller passed in.
-_LIGHT = torch.library.Library("h3b", "FRAGMENT")
-DTYPES = {torch.bfloat16: 0, torch.float16: 1, torch.float32: 2}
+# These operators serve single tokens, where a dispatch through Python costs
+# several times the kernel, so they are written in C++ (csrc/torch_ext.cpp):
+# they check their tensors, allocate results and workspaces, and call the C ABI.
+# ``X`` returns new tensors, ``X_out`` writes the caller's.
+EXT_PATH = _lib.LIB_PATH.with_name("_h3b_torch.so")
 
 
-def _light(schema: str):
-    def wrap(fn):
-        name = schema.split("(", 1)[0]
-        _LIGHT.define(schema)
-        _LIGHT.impl(name, fn, "CUDA")
-        torch.library.register_fake(f"h3b::{name}", _no_output, lib=_LIGHT)
-        return fn
-    return wrap
+def _fake_rows(x: torch.Tensor, n: int, dtype=None) -> torch.Tensor:
+    return x.new_empty((*x.shape[:-1], n), dtype=dtype or x.dtype)
 
 
-def _call(t: torch.Tensor, name: str, *args) -> None:
-    """As ``_run``, entering the device guard only when it changes anything."""
-    dev = t.device.index
-    fn = getattr(_lib.lib(), name)
-    if dev == torch.cuda.current_device():
-        st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    else:
-        with torch.cuda.device(dev):
-            st = fn(*args, torch._C._cuda_getCurrentRawStream(dev))
-    if st:
-        _lib.check(st, name)
+def _fake_quantize(x):
+    m, k = x.numel() // x.shape[-1], x.shape[-1]
+    return (x.new_empty((m, k // 2), dtype=torch.uint8),
+            x.new_empty(((m + 127) // 128 * ((k + 127) // 128) * 512,), dtype=torch.uint8))
 
 
-@_light("mxfp4_quantize(Tensor x, int rows, int cols, int ldx, Tensor(a!) q, Tensor(b!) sf) -> ()")
-def mxfp4_quantize(x, rows, cols, ldx, q, sf):
-    """E2M1 codes and blocked E8M0 scales of a [rows, cols] view (h3b_mxfp4_quantize)."""
-    _call(q, "h3b_mxfp4_quantize", _p(x), DTYPES[x.dtype], rows, cols, ldx, _p(q), _p(sf))
+_FAKES = {
+    "mxfp4_quantize": _fake_quantize,
+    "mxfp4_dequantize": lambda q, sf, m, k, dtype: q.new_empty((m, k), dtype=dtype),
+    "mxfp4_gemm": lambda qa, sfa, m, qb, sfb, n, k, bias, act, residual, dtype:
+        qa.new_empty((m, n), dtype=dtype),
+    "mxfp4_linear": lambda x, qb, sfb, n, k, bias, act, residual: _fake_rows(x, n),
+    "mxfp4_ffn": lambda x, qu, sfu, qd, sfd, n, f, residual: _fake_rows(x, n),
+    "attention_window": lambda q, k, v, heads, kv_heads, head_dim, *_:
+        q.new_empty((q.numel() // q.shape[-1], heads * head_dim)),
+    "attention_window_decode": lambda q, *_: q.new_empty(q.shape),
+}
 
 
-@_light("mxfp4_dequantize(Tensor q, Tensor sf, int rows, int cols, Tensor(a!) out, int ldo) -> ()")
-def mxfp4_dequantize(q, sf, rows, cols, out, ldo):
-    """Codes times scales in out's type (h3b_mxfp4_dequantize)."""
-    _call(out, "h3b_mxfp4_dequantize", _p(q), _p(sf), rows, cols, _p(out), DTYPES[out.dtype], ldo)
+def _load_ext() -> bool:
+    if not EXT_PATH.exists():
+        return False
+    torch.ops.load_library(str(EXT_PATH))
+    for name, fake in _FAKES.items():
+        torch.library.register_fake(f"h3b::{name}", fake)
+        torch.library.register_fake(f"h3b::{name}_out", _no_output)
+    return True
 
 
-@_light("mxfp4_gemm(Tensor qa, Tensor sfa, int m, Tensor qb, Tensor sfb, int n, int k, "
-        "Tensor? bias, int act, Tensor? residual, int ldr, Tensor(a!) out, int ldd) -> ()")
-def mxfp4_gemm(qa, sfa, m, qb, sfb, n, k, bias, act, residual, ldr, out, ldd):
-    """Block-scaled MXFP4 GEMM with the fused epilogue (h3b_mxfp4_gemm)."""
-    _call(out, "h3b_mxfp4_gemm", _p(qa), _p(sfa), m, _p(qb), _p(sfb), n, k, _p(bias), act,
-          _p(residual), ldr, _p(out), DTYPES[out.dtype], ldd)
+_EXT_LOADED = _load_ext()
 
 
-@_light("mxfp4_linear(Tensor x, int m, int ldx, Tensor qb, Tensor sfb, int n, int k, "
-        "Tensor? bias, int act, Tensor? residual, int ldr, Tensor(a!) out, int ldd, "
-        "Tensor(b!) ws) -> ()")
-def mxfp4_linear(x, m, ldx, qb, sfb, n, k, bias, act, residual, ldr, out, ldd, ws):
-    """act(Q(x) W^T + bias) + residual (h3b_mxfp4_linear)."""
-    _call(out, "h3b_mxfp4_linear", _p(x), DTYPES[x.dtype], m, ldx, _p(qb), _p(sfb), n, k, _p(bias),
-          act, _p(residual), ldr, _p(out), ldd, _p(ws), ws.numel())
+def ext_op(name: str):
+    """The C++ operator ``h3b::name``; without the built extension a callable
+    that raises (there is no other path)."""
+    if _EXT_LOADED:
+        return getattr(torch.ops.h3b, name).default
 
-
-@_light("mxfp4_ffn(Tensor x, int m, int ldx, Tensor qu, Tensor sfu, Tensor qd, Tensor sfd, int n, "
-        "int f, Tensor? residual, int ldr, Tensor(a!) out, int ldd, Tensor(b!) ws) -> ()")
-def mxfp4_ffn(x, m, ldx, qu, sfu, qd, sfd, n, f, residual, ldr, out, ldd, ws):
-    """Q(v * silu(g)) Wd^T + residual, [v | g] = Q(x) Wu^T (h3b_mxfp4_ffn)."""
-    _call(out, "h3b_mxfp4_ffn", _p(x), DTYPES[x.dtype], m, ldx, _p(qu), _p(sfu), _p(qd), _p(sfd),
-          n, f, _p(residual), ldr, _p(out), ldd, _p(ws), ws.numel())
-
-
-def _i32s(v):
-    return (ctypes.c_int32 * max(len(v), 1))(*v)
-
-
-@_light("attention_window(Tensor q, Tensor k, Tensor v, int heads, int kv_heads, int head_dim, "
-        "int[] q_start, int[] q_len, int[] k_start, int[] k_len, int left, int right, int sinks, "
-        "bool causal, float scale, Tensor(a!) out) -> ()")
-def attention_window(q, k, v, heads, kv_heads, head_dim, q_start, q_len, k_start, k_len, left,
-                     right, sinks, causal, scale, out):
-    """Packed windowed attention over host row ranges (h3b_attention_window)."""
-    _call(out, "h3b_attention_window", _p(q), q.shape[0], q.stride(0), _p(k), k.stride(0), _p(v),
-          v.stride(0), k.shape[0], DTYPES[q.dtype], heads, kv_heads, head_dim, _i32s(q_start),
-          _i32s(q_len), _i32s(k_start), _i32s(k_len), len(q_start), left, right, sinks,
-          int(causal), scale, _p(out), out.stride(0))
-
-
-@_light("attention_window_decode(Tensor q, Tensor k, Tensor v, Tensor kv_len, int left, "
-        "int right, int sinks, bool causal, float scale, Tensor(a!) out) -> ()")
-def attention_window_decode(q, k, v, kv_len, left, right, sinks, causal, scale, out):
-    """Windowed attention of new tokens against a cache with device lengths
-    (h3b_attention_window_decode); q [B, n, H, D], k and v [B, room, kv_heads, D]."""
-    b, n, h, d = q.shape
-    strides = [(ctypes.c_int64 * 3)(*t.stride()[:3]) for t in (q, k, v)]
-    _call(out, "h3b_attention_window_decode", _p(q), strides[0], _p(k), strides[1], _p(v),
-          strides[2], _p(kv_len), b, k.shape[1], n, DTYPES[q.dtype], h, k.shape[2], d, left, right,
-          sinks, int(causal), scale, _p(out))
+    def missing(*_args, **_kwargs):
+        raise RuntimeError(f"{EXT_PATH} is missing: build it with "
+                           "`python -m h3_engine_b200.csrc.build`")
+    return missing

@@ -116,9 +116,19 @@ def test_cpu_tensors_are_refused():
 
 @pytest.mark.parametrize("name", ["attention_window", "attention_window_decode"])
 def test_operators_declare_their_outputs(name):
-    schema = getattr(torch.ops.h3b, name).default._schema
+    schema = getattr(torch.ops.h3b, name + "_out").default._schema
     assert {a.name for a in schema.arguments
             if a.alias_info is not None and a.alias_info.is_write} == {"out"}
+
+
+def test_operators_trace_without_a_gpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        q = torch.empty(10, 256, dtype=BF16, device="cuda")
+        assert ops.attention_window(q, q, q, 2, 128, [0, 10]).shape == (10, 256)
+        c = torch.empty(2, 8, 2, 64, dtype=BF16, device="cuda")
+        n = torch.empty(2, dtype=torch.int32, device="cuda")
+        assert ops.attention_window_decode(c[:, :1], c, c, n).shape == (2, 1, 2, 64)
 
 
 # ---------------------------------------------------------------- GPU: packed

@@ -42,12 +42,12 @@ def test_host_checks_refuse_without_a_gpu():
     assert g(p, p, 0, p, p, 16, 64, None, 0, None, 0, p, 0, 16, None) == 0
     lin = lib.h3b_mxfp4_linear
     need = lib.h3b_mxfp4_linear_ws(4, 16, 64)
-    assert need == ops._mx_operand_bytes(4, 64)
+    assert need == 256 + 512                              # codes to 256 bytes, one scale tile
     assert lin(p, 0, 4, 64, p, p, 16, 64, None, 0, None, 0, p, 16, p, need - 1, None) == 1
     assert lin(p, 0, 4, 64, p, p, 16, 64, None, 0, None, 0, p, 16, odd, need, None) == 2
     f = lib.h3b_mxfp4_ffn
     need = lib.h3b_mxfp4_ffn_ws(4, 64, 128)
-    assert need == ops._mx_operand_bytes(4, 64) + ops._mx_operand_bytes(4, 128)
+    assert need == 2 * (256 + 512)
     assert f(p, 0, 4, 64, p, p, p, p, 64, 192, None, 0, p, 64, p, 1 << 30, None) == 1   # F % 128
     assert f(p, 0, 4, 64, p, p, p, p, 48, 128, None, 0, p, 48, p, 1 << 30, None) == 1   # N % 32
     assert f(p, 0, 4, 64, p, p, p, p, 64, 128, None, 0, p, 64, p, need - 1, None) == 1
@@ -58,17 +58,33 @@ def test_cpu_tensors_are_refused():
     with pytest.raises(ValueError):
         ops.mxfp4_quantize(x)
     with pytest.raises((NotImplementedError, RuntimeError)):
-        torch.ops.h3b.mxfp4_quantize(x, 4, 64, 64, x, x)
+        torch.ops.h3b.mxfp4_quantize(x)
 
 
 @pytest.mark.parametrize("name,outs", [
     ("mxfp4_quantize", {"q", "sf"}), ("mxfp4_dequantize", {"out"}), ("mxfp4_gemm", {"out"}),
-    ("mxfp4_linear", {"out", "ws"}), ("mxfp4_ffn", {"out", "ws"})])
+    ("mxfp4_linear", {"out"}), ("mxfp4_ffn", {"out"})])
 def test_operators_declare_their_outputs(name, outs):
-    schema = getattr(torch.ops.h3b, name).default._schema
+    schema = getattr(torch.ops.h3b, name + "_out").default._schema
     assert {a.name for a in schema.arguments
             if a.alias_info is not None and a.alias_info.is_write} == outs
     assert not schema.returns
+    assert not any(a.alias_info for a in getattr(torch.ops.h3b, name).default._schema.arguments)
+
+
+def test_operators_trace_without_a_gpu():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+    with FakeTensorMode():
+        x = torch.empty(3, 5, 96, dtype=BF16, device="cuda")
+        q, sf = ops.mxfp4_quantize(x)
+        assert q.shape == (15, 48) and sf.shape == (512,)
+        assert ops.mxfp4_dequantize(q, sf, 15, 96, dtype=F32).shape == (15, 96)
+        w = mxfp4.MXFP4Weight(torch.empty(64, 96, dtype=BF16, device="cuda"))
+        assert mxfp4.mxfp4_linear(w, x).shape == (3, 5, 64)
+        assert ops.mxfp4_gemm(q, sf, 15, w.qdata, w.scale, 64, 96, dtype=F16).dtype == F16
+        up = mxfp4.gated_up_weight(torch.empty(256, 96, dtype=BF16, device="cuda"))
+        down = mxfp4.MXFP4Weight(torch.empty(96, 128, dtype=BF16, device="cuda"))
+        assert mxfp4.gated_ffn(up, down, x, out=torch.empty_like(x)).shape == x.shape
 
 
 # ---------------------------------------------------------------- GPU
