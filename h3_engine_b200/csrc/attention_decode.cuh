@@ -18,7 +18,7 @@
 namespace h3b {
 namespace wdec {
 
-constexpr int kWarps = 4;
+constexpr int kWarps = 4;            // 96 KiB of rings (D = 128): two CTAs per SM
 constexpr int kThreads = kWarps * 32;
 constexpr int kRows = 16;
 constexpr int kKeys = 16;           // keys per tile
@@ -26,7 +26,7 @@ constexpr int kMaxCluster = 8;
 
 template <int D>
 struct Smem {
-  static constexpr int kStages = 4;
+  static constexpr int kStages = 3;
   static constexpr int TILE = kKeys * D * 2;                  // K or V of one stage
   static constexpr int STAGE = 2 * TILE;
   static constexpr int WARP = kStages * STAGE;
@@ -78,9 +78,10 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float ld_cluster_f32(uint32_t addr) {
-  float v;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(v) : "r"(addr) : "memory");
+__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
+  float2 v;
+  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
+               : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
   return v;
 }
 __device__ __forceinline__ uint32_t cluster_nctarank() {
@@ -100,6 +101,7 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   using L = Smem<D>;
   constexpr int CH = D / 8;                       // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t smem[];
+  __shared__ float2 total_ml[kRows];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
   const int rows_all = p.n_new * p.group;
@@ -283,36 +285,61 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
     }
   }
   __syncthreads();
-  // the CTA's own total, into part 0 (each thread owns its elements)
-  float2 ml_tot = make_float2(-INFINITY, 0.f);
-  const int r_own = threadIdx.x & 15;
-  for (int w = 0; w < kWarps; ++w) ml_tot.x = fmaxf(ml_tot.x, part_ml(w)[r_own].x);
-  for (int w = 0; w < kWarps; ++w)
-    ml_tot.y += weight(part_ml(w)[r_own].x, ml_tot.x) * part_ml(w)[r_own].y;
-  for (int e = threadIdx.x; e < rows * D; e += kThreads) {
-    const int r = e / D;
-    float mm = -INFINITY, acc = 0.f;
-    for (int w = 0; w < kWarps; ++w) mm = fmaxf(mm, part_ml(w)[r].x);
-    for (int w = 0; w < kWarps; ++w) acc += weight(part_ml(w)[r].x, mm) * part_o(w)[e];
-    part_o(0)[e] = acc;
+  // the CTA's own total, over part 0: each warp's weight per row once, in the
+  // place of its maximum, then the elements
+  if (threadIdx.x < kRows) {
+    const int r = threadIdx.x;
+    float2 ml[kWarps];
+    float mm = -INFINITY, ll = 0.f;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      ml[w] = part_ml(w)[r];
+      mm = fmaxf(mm, ml[w].x);
+    }
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = weight(ml[w].x, mm);
+      ll += f * ml[w].y;
+      part_ml(w)[r].x = f;
+    }
+    total_ml[r] = make_float2(mm, ll);
   }
   __syncthreads();
-  if (threadIdx.x < kRows) part_ml(0)[threadIdx.x] = ml_tot;
-  // the cluster's total: this CTA's share of the rows' elements
+  for (int e = threadIdx.x * 4; e < rows * D; e += kThreads * 4) {
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float f = part_ml(w)[e / D].x;
+      const float4 v = *reinterpret_cast<const float4*>(part_o(w) + e);
+      acc = make_float4(acc.x + f * v.x, acc.y + f * v.y, acc.z + f * v.z, acc.w + f * v.w);
+    }
+    *reinterpret_cast<float4*>(part_o(0) + e) = acc;
+  }
+  // the cluster's total: this CTA's share of the rows' elements, every rank's
+  // part in flight at once
   cluster_sync_all();
-  const uint32_t base = smem_u32(smem);
+  const uint32_t base = smem_u32(smem), mls = smem_u32(total_ml);
   for (int e = rank * kThreads + threadIdx.x; e < rows * (D / 2); e += ranks * kThreads) {
     const int r = e / (D / 2), d = (e % (D / 2)) * 2;
+    float2 ml[kMaxCluster], po[kMaxCluster];
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      ml[c] = make_float2(-INFINITY, 0.f);
+      po[c] = make_float2(0.f, 0.f);
+      if (c < ranks) {
+        ml[c] = ld_cluster_f2(mapa_shared(mls + r * 8, c));
+        po[c] = ld_cluster_f2(mapa_shared(base + (r * D + d) * 4, c));
+      }
+    }
     float mm = -INFINITY, ll = 0.f, a0 = 0.f, a1 = 0.f;
-    for (int c = 0; c < ranks; ++c)
-      mm = fmaxf(mm, ld_cluster_f32(mapa_shared(base + kRows * D * 4 + r * 8, c)));
-    for (int c = 0; c < ranks; ++c) {
-      const uint32_t ml = mapa_shared(base + kRows * D * 4 + r * 8, c);
-      const uint32_t po = mapa_shared(base + (r * D + d) * 4, c);
-      const float w = weight(ld_cluster_f32(ml), mm);
-      ll += w * ld_cluster_f32(ml + 4);
-      a0 += w * ld_cluster_f32(po);
-      a1 += w * ld_cluster_f32(po + 4);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) mm = fmaxf(mm, ml[c].x);
+#pragma unroll
+    for (int c = 0; c < kMaxCluster; ++c) {
+      const float f = weight(ml[c].x, mm);
+      ll += f * ml[c].y;
+      a0 += f * po[c].x;
+      a1 += f * po[c].y;
     }
     const int t = (row0 + r) / p.group, g = (row0 + r) % p.group;
     const size_t at = (((size_t)b * p.n_new + t) * p.H + kvh * p.group + g) * D + d;

@@ -62,13 +62,15 @@ static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st)
   const int64_t row_tiles = ((int64_t)a.n_new * a.group + wdec::kRows - 1) / wdec::kRows;
   const int64_t groups = row_tiles * a.kv_heads;
   if (groups > 65535 || B > 65535) return H3B_ERR_INVALID_ARG;
-  // CTAs along the keys: enough to cover the SMs once, but not more than give
-  // every warp a tile of a full window
+  // CTAs along the keys: until there are two per SM, which run at a time (32
+  // uneven sequences of 8 key heads: 135 us without a split, 84 with 512 CTAs,
+  // 89 with 1024, 106 with 2048), but no more than give every warp two tiles
+  // of a full window
   const int64_t most =
       std::min<int64_t>(a.room, (int64_t)a.left + a.right + a.n_new + (int64_t)a.sinks);
   int split = 1;
-  while (split < wdec::kMaxCluster && groups * B * split * 2 <= num_sms() &&
-         most > (int64_t)split * wdec::kWarps * wdec::kKeys)
+  while (split < wdec::kMaxCluster && groups * B * split < 2 * (int64_t)num_sms() &&
+         most > (int64_t)split * wdec::kWarps * wdec::kKeys * 2)
     split *= 2;
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)split, (unsigned)groups, (unsigned)B);

@@ -80,11 +80,13 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
 template <typename T>
 static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
                                  int64_t ldo, cudaStream_t st) {
-  int64_t blocks = (M + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
+  constexpr int kUnroll = 4;
+  const int64_t per_row = (K + 256 * kUnroll - 1) / (256 * kUnroll);
+  int64_t blocks = (M * per_row + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
   blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
-  mx::k_mxfp4_dequantize<T><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
+  mx::k_mxfp4_dequantize<T, kUnroll><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
       static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
-      static_cast<T*>(out), ldo);
+      static_cast<T*>(out), ldo, (uint32_t)per_row);
 }
 
 // CTA pairs wherever there are two 128-row blocks to share a B tile: 13383 x

@@ -213,41 +213,42 @@ __device__ __forceinline__ void values8(uint32_t codes, float s, float (&v)[8]) 
   }
 }
 
-// One warp per row (grid-stride), lane l takes the 8-value pieces l, l + 32,
-// ... of the row, four in flight.
-template <typename T>
+// Units of UNROLL * 256 values as in the quantizer: lane l takes the 8-value
+// pieces l, l + 32, ... of the unit, all loads in flight.
+template <typename T, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     k_mxfp4_dequantize(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int64_t M,
-                       int64_t K, T* __restrict__ out, int64_t ldo) {
-  constexpr int U = 4;
+                       int64_t K, T* __restrict__ out, int64_t ldo, uint32_t units_per_row) {
   const int lane = threadIdx.x & 31;
   const int steps = (int)(K >> 3);
   const int64_t c4 = sf_tiles(K);
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
-  for (int64_t r = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); r < M; r += warps) {
+  const int64_t units = M * units_per_row;
+  for (int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < units;
+       w += warps) {
+    const int64_t r = w / units_per_row;
+    const int h0 = (int)(w - r * units_per_row) * (32 * UNROLL) + lane;
     const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + r * (K >> 1));
     T* orow = out + r * ldo;
-    for (int h0 = lane; h0 < steps; h0 += 32 * U) {
-      uint32_t codes[U];
-      uint8_t s[U];
+    uint32_t codes[UNROLL];
+    uint8_t s[UNROLL];
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * 32;
-        codes[u] = 0;
-        s[u] = 0;
-        if (h < steps) {
-          codes[u] = __ldg(qr + h);
-          s[u] = __ldg(sf + sf_swizzled_offset(r, h >> 2, c4));
-        }
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * 32;
+      codes[u] = 0;
+      s[u] = 0;
+      if (h < steps) {
+        codes[u] = __ldg(qr + h);
+        s[u] = __ldg(sf + sf_swizzled_offset(r, h >> 2, c4));
       }
+    }
 #pragma unroll
-      for (int u = 0; u < U; ++u) {
-        const int h = h0 + u * 32;
-        if (h >= steps) break;
-        float v[8];
-        values8(codes[u], scale_value(s[u]), v);
-        store8(orow + (int64_t)h * 8, v);
-      }
+    for (int u = 0; u < UNROLL; ++u) {
+      const int h = h0 + u * 32;
+      if (h >= steps) break;
+      float v[8];
+      values8(codes[u], scale_value(s[u]), v);
+      store8(orow + (int64_t)h * 8, v);
     }
   }
 }
