@@ -76,7 +76,8 @@ SIGNATURES: dict[str, tuple] = {
     "h3b_attention_window": (_i32, [_c_void_p, _i64, _i64, _c_void_p, _i64, _c_void_p, _i64, _i64,
                                     _i32, _i32, _i32, _i32, _c_void_p, _c_void_p, _c_void_p,
                                     _c_void_p, _i32, _i64, _i64, _i64, _i32, _f32, _c_void_p,
-                                    _i64, _c_void_p]),
+                                    _i64, _c_void_p, _i64, _c_void_p]),
+    "h3b_attention_window_ws": (_i64, [_c_void_p, _c_void_p, _i32, _i32, _i32, _i64, _i64, _i64]),
     "h3b_attention_window_decode": (_i32, [_c_void_p, _c_void_p, _c_void_p, _c_void_p, _c_void_p,
                                            _c_void_p, _c_void_p, _i64, _i64, _i64, _i32, _i32,
                                            _i32, _i32, _i64, _i64, _i64, _i32, _f32, _c_void_p,

@@ -14,8 +14,14 @@
 // at 0 and at lo (TMA rows need no alignment, so the first step of the window
 // starts at its first key); the two are one range where they touch.  A step that no query of tile A (or B) sees is skipped for that tile:
 // neither its MMAs nor its softmax run, which is what the window's triangular
-// ends cost least with.  Steps all of whose keys a warp's 32 rows see take the
-// unmasked path; the others build a 128-bit visibility mask per row.
+// ends cost least with.  Within a step a row's 128 keys are four words of 32, of
+// which only those that some row of the warp does not see whole are masked.
+//
+// The grid is a number of full waves of items, one CTA per SM, and a last
+// partial wave whose items are split along their keys so that it fills the SMs
+// too: the parts leave their unnormalised O, row maximum and sum (fp32) in a
+// workspace, and the part that finishes last adds them up, in part order, so
+// the result does not depend on which one that is.
 //
 // Rows of V behind the last visible key of a step (the document's end, the
 // next document, the gap behind the sinks) are cleared in shared memory before
@@ -58,6 +64,9 @@ struct Args {
   int H, group;                            // query heads; query heads per key head
   float scale_log2;                        // softmax scale * log2(e)
   int left, right, sinks, causal;          // left, right < 2^30
+  int whole, parts;                        // items [0, whole) are whole, the others in `parts`
+  float* partial;                          // [split item][part]: O [D/4][256][4], then (m, l) [256]
+  int* done;                               // [split item]: parts finished (0 between launches)
   int ndocs;
   int q_start[MAX_DOCS], q_len[MAX_DOCS];
   int k_start[MAX_DOCS], k_len[MAX_DOCS];
@@ -79,6 +88,7 @@ struct Range {
 // The key steps of a CTA.
 struct Steps {
   int n_sink, n, lo, end, sink_end;        // window steps start at lo, end one past the last key
+  int first = 0;                           // of this CTA's part; n counts its own
   __device__ __forceinline__ explicit Steps(const Range& r) {
     sink_end = r.sink_end;
     lo = r.lo;
@@ -94,11 +104,16 @@ struct Steps {
       n = (end + BK - 1) / BK;
     }
   }
+  __device__ __forceinline__ void take(int part, int parts) {
+    first = n * part / parts;
+    n = n * (part + 1) / parts - first;
+  }
   __device__ __forceinline__ int base(int j) const {
+    j += first;
     return j < n_sink ? j * BK : lo + (j - n_sink) * BK;
   }
   __device__ __forceinline__ int valid(int j) const {
-    return min(BK, (j < n_sink ? sink_end : end) - base(j));
+    return min(BK, (j + first < n_sink ? sink_end : end) - base(j));
   }
   // does a tile that sees `r` see any key of step j
   __device__ __forceinline__ bool needed(const Range& r, int j) const {
@@ -138,14 +153,15 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
-// P = 2^(S * scale - m) of one row's 128 keys, stored as 16-bit pairs over the
-// row's S columns; returns the row sum.  P is rounded to 16 bits because the
-// tensor core reads it so; the sum is of the unrounded fp32 values.  MIXED
-// sends 3 of 8 pairs to the polynomial; a step with masked keys (S = -inf) uses
-// the MUFU unit only, which gives exactly 0.
-template <typename T, bool MIXED>
+// P = 2^(S * scale - m) of one row's 128 keys, stored as 16-bit pairs over 64
+// columns of tensor memory; returns the row sum.  P is rounded to 16 bits
+// because the tensor core reads it so; the sum is of the unrounded fp32 values.
+// 3 of 8 pairs go to the polynomial; a masked key (S = -inf) that falls there
+// gives 2^-120 instead of 0, which no sum of 2^0 or more notices (a row's sum
+// holds its maximum's 2^0, and a row that sees nothing is told by its range).
+template <typename T>
 __device__ __forceinline__ float softmax_store(uint32_t (&sv)[128], float scale_log2, float m,
-                                               uint32_t s_addr, uint32_t half_bar) {
+                                               uint32_t p_addr, uint32_t half_bar) {
   const float2 sc = make_float2(scale_log2, scale_log2);
   const float2 nm = make_float2(-m, -m);
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
@@ -157,13 +173,13 @@ __device__ __forceinline__ float softmax_store(uint32_t (&sv)[128], float scale_
       const int k = h * 64 + 2 * c;
       const float2 x = fma2(make_float2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc, nm);
       float2 e;
-      if (MIXED && ((attn::kPolyPairs >> (c & 7)) & 1u)) e = ex2_poly2(x);
+      if ((attn::kPolyPairs >> (c & 7)) & 1u) e = ex2_poly2(x);
       else e = make_float2(attn::ex2(x.x), attn::ex2(x.y));
       if (c & 1) acc1 = add2(acc1, e);
       else acc0 = add2(acc0, e);
       pk[c] = pack16<T>(e.x, e.y);
     }
-    tmem_st_32x32b_x32(s_addr + h * 32, pk);
+    tmem_st_32x32b_x32(p_addr + h * 32, pk);
     if (h == 0) {
       tmem_st_wait();
       tc_fence_before();
@@ -193,6 +209,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   constexpr uint32_t IDESC_PV =
       (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
 
+  // head_dim 64 leaves 128 columns of tensor memory, which hold P apart from S:
+  // S(j + 1) is then computed under the exponentials of step j.
+  constexpr bool SEP = D == 64;
+  auto p_col = [](int t) { return SEP ? 320u + (uint32_t)t * 128u : attn::s_col(t); };
+
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
                                              ~uintptr_t(1023));
@@ -205,17 +226,23 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   uint64_t* kv_empty = bars + 3;     // 2
   uint64_t* s_full = bars + 5;       // 2 (tile A, B)
   uint64_t* p_full = bars + 7;       // 2
-  uint64_t* pv_done = bars + 9;      // 2
+  uint64_t* pv_done = bars + 9;      // 2: the last PV of a tile (SEP: every PV)
   uint64_t* drain = bars + 11;       // 1
   uint64_t* p_half = bars + 12;      // 2
+  uint64_t* s_free = bars + 14;      // 2 (SEP): S has been read
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  // work item (document, query-tile pair, head) and the part of its keys
+  const int split = max(0, (int)blockIdx.x - p.whole) / p.parts;     // index of a split item
+  const bool whole = (int)blockIdx.x < p.whole;
+  const int part = whole ? 0 : ((int)blockIdx.x - p.whole) % p.parts;
+  const int idx = whole ? (int)blockIdx.x : p.whole + split;
   int doc = 0;
-  while (doc + 1 < p.ndocs && (int)blockIdx.x >= p.item_end[doc]) ++doc;
-  const int item = (int)blockIdx.x - (doc > 0 ? p.item_end[doc - 1] : 0);
+  while (doc + 1 < p.ndocs && idx >= p.item_end[doc]) ++doc;
+  const int item = idx - (doc > 0 ? p.item_end[doc - 1] : 0);
   const int n_q = p.q_len[doc], n_k = p.k_len[doc];
   const int pairs = (n_q + 2 * BQ - 1) / (2 * BQ);
   const int head = item / pairs;
@@ -224,7 +251,8 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   const int k_row = p.k_start[doc];
   const int pos0 = qp * 2 * BQ + n_k - n_q;               // position of tile A's first row
   const int rows = min(2 * BQ, n_q - qp * 2 * BQ);        // queries of this pair
-  const Steps st(Range(p, n_k, pos0, pos0 + rows - 1));
+  Steps st(Range(p, n_k, pos0, pos0 + rows - 1));
+  if (!whole) st.take(part, p.parts);
   // what each tile sees; a tile without queries sees nothing
   auto tile_range = [&](int t) {
     const int n = min(BQ, rows - t * BQ);
@@ -237,7 +265,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
     return r;
   };
 
-  if (threadIdx.x == 0) {
+  const int qx = head * D, kx = (head / p.group) * D;
+  auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+#pragma unroll
+    for (int b = 0; b < D / 64; ++b)
+      tma_load_2d(smem_u32(dst + b * L::BOX_BYTES), map, x + b * 64, y, bar);
+  };
+  if (warp == 8 && lane == 0) {
     mbar_init(smem_u32(q_full), 1);
     for (int i = 0; i < 2; ++i) {
       mbar_init(smem_u32(&kv_full[i]), 1);
@@ -246,10 +280,19 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&p_half[i]), 4);
       mbar_init(smem_u32(&pv_done[i]), 1);
+      mbar_init(smem_u32(&s_free[i]), 4);
     }
     mbar_init(smem_u32(drain), 1);
     *abort_flag = 0;
     fence_mbar_init();
+    if (st.n > 0) {
+      // the first loads run while tensor memory is allocated
+      const uint32_t qb = smem_u32(q_full);
+      mbar_expect_tx(qb, 3 * L::TILE_BYTES);
+      load(smem + L::Q_OFF, &p.tmap_q, qx, q_row, qb);
+      load(smem + L::K_OFF, &p.tmap_k, kx, k_row + st.base(0), qb);
+      load(smem + L::Q_OFF + L::TILE_BYTES, &p.tmap_q, qx, q_row + BQ, qb);
+    }
   }
   if (warp == 9) {
     tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
@@ -273,20 +316,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
     asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
     if (warp == 8) {
       if (lane == 0 && st.n > 0) {
-        prefetch_tmap(&p.tmap_q);
-        prefetch_tmap(&p.tmap_k);
-        prefetch_tmap(&p.tmap_v);
-        const int qx = head * D, kx = (head / p.group) * D;
-        auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
-#pragma unroll
-          for (int b = 0; b < D / 64; ++b)
-            tma_load_2d(smem_u32(dst + b * L::BOX_BYTES), map, x + b * 64, y, bar);
-        };
-        const uint32_t qb = smem_u32(q_full);
-        mbar_expect_tx(qb, 3 * L::TILE_BYTES);
-        load(smem + L::Q_OFF, &p.tmap_q, qx, q_row, qb);
-        load(smem + L::Q_OFF + L::TILE_BYTES, &p.tmap_q, qx, q_row + BQ, qb);
-        load(smem + L::K_OFF, &p.tmap_k, kx, k_row + st.base(0), qb);
         auto prefetch = [&](int j) {
           if (j < st.n) {
             const int y = k_row + st.base(j);
@@ -363,11 +392,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int kk = h * 4 + i;
-            tc_mma_bf16_ts_elect(tmem + attn::o_col(t), tmem + attn::s_col(t) + kk * 8,
+            tc_mma_bf16_ts_elect(tmem + attn::o_col(t), tmem + p_col(t) + kk * 8,
                                  vd + kk * (2048 >> 4), IDESC_PV, (cnt[t] | kk) != 0);
           }
         }
-        if (j == last[t]) tc_commit_elect(smem_u32(&pv_done[t]));
+        if (SEP || j == last[t]) tc_commit_elect(smem_u32(&pv_done[t]));
         ++cnt[t];
         return true;
       };
@@ -396,13 +425,28 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
           fence_proxy_async_smem();
           __syncwarp();
         }
+        if (SEP) {
+#pragma unroll
+          for (int t = 0; t < 2; ++t) {
+            if (!(more && need(t, j + 1))) continue;
+            // S of the tile's latest step has been read (none yet: nothing to wait for)
+            const int read = cnt[t] + (need(t, j) ? 1 : 0);
+            if (read > 0 && !wait(&s_free[t], (read - 1) & 1)) {
+              ok = false;
+              break;
+            }
+            tc_fence_after();
+            issue_qk(t, j + 1);
+          }
+        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
+          if (!ok) break;
           if (need(t, j) && !pv_tile(t, j)) {
             ok = false;
             break;
           }
-          if (more && need(t, j + 1)) issue_qk(t, j + 1);
+          if (!SEP && more && need(t, j + 1)) issue_qk(t, j + 1);
         }
         if (ok) tc_commit_elect(smem_u32(&kv_empty[j & 1]));
       }
@@ -428,6 +472,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
     const uint32_t lane_addr = (uint32_t)(qd * 32) << 16;
     const uint32_t s_t = tmem + lane_addr + attn::s_col(t);
     const uint32_t o_t = tmem + lane_addr + attn::o_col(t);
+    const uint32_t p_t = tmem + lane_addr + p_col(t);
     const Range rt = tile_range(t);
     const int pos = pos0 + t * BQ + r;                    // this row's key position
     const int w_first = pos0 + t * BQ + qd * 32;          // first and last position of the warp
@@ -446,6 +491,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       tmem_ld_32x32b_x64(s_t, sv);
       tmem_ld_32x32b_x64(s_t + 64, sv + 64);
       tmem_ld_wait();
+      if (SEP) {
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&s_free[t]));
+      }
       const int base = st.base(j), valid = st.valid(j);
       const bool all_seen =                               // warp-uniform
           valid == BK && base + BK - 1 <= w_top &&
@@ -457,9 +507,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
           const uint32_t seen = span_word(a, b, w) | span_word(0, s, w);
+          if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
-          for (int c = 0; c < 32; ++c)
-            if (!(seen & (1u << c))) sv[w * 32 + c] = 0xff800000u;   // -inf: masked key
+            for (int c = 0; c < 32; ++c)
+              if (!(seen & (1u << c))) sv[w * 32 + c] = 0xff800000u;   // -inf: masked key
+          }
         }
       }
       // row max of the scaled logits (scale > 0 commutes with max)
@@ -479,9 +531,15 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
         alpha = m_new == -INFINITY ? 1.f : attn::ex2(m_used - m_new);
         m_used = m_new;
       }
+      if (SEP && cnt > 0) {
+        // the previous PV has read its P and written O
+        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), (cnt - 1) & 1, abort_flag));
+        if (!ok) break;
+        tc_fence_after();
+      }
       if (rescale && cnt > 0) {
-        // O is final up to the previous needed step: s_full of this one was
-        // committed after its PV
+        // O is final up to the previous needed step (without SEP: s_full of this
+        // one was committed after its PV)
 #pragma unroll
         for (int h = 0; h < D / 32; ++h) {
           uint32_t ov[32];
@@ -494,9 +552,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       }
       const uint32_t hb = smem_u32(&p_half[t]);
       const float m = m_used == -INFINITY ? 0.f : m_used;   // -inf - (-inf) is no exponent
-      const float s = all_seen ? softmax_store<T, true>(sv, p.scale_log2, m, s_t, hb)
-                               : softmax_store<T, false>(sv, p.scale_log2, m, s_t, hb);
-      l = l * alpha + s;
+      l = l * alpha + softmax_store<T>(sv, p.scale_log2, m, p_t, hb);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -504,34 +560,133 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       ++cnt;
     }
     if (ok && cnt > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), 0, abort_flag));
-    if (!ok) {
-      fail();
-    } else {
-      tc_fence_after();
-      const bool some = l != 0.f;                          // saw a key (or NaN)
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), SEP ? (cnt - 1) & 1 : 0,
+                                             abort_flag));
+    if (!ok) fail();
+    tc_fence_after();
+    const int row = t * BQ + r;                            // of the pair's 256
+    // does the row see any key at all
+    const bool some = min(p.sinks, top + 1) > 0 ||
+                      min(pos + p.right, min(top, n_k - 1)) >= max(0, pos - p.left);
+    // The output leaves through the tile's Q buffer (all its MMAs are done), a
+    // warp's 32 rows at a time: written a row per lane, 16-byte chunk c of row r
+    // at chunk c ^ (r % 8), and copied out whole rows at a time.
+    constexpr int CH = D / 8;                              // 16-byte chunks of a row
+    uint4* const ostage = reinterpret_cast<uint4*>(smem + L::Q_OFF + t * L::TILE_BYTES) + qd * 32 * CH;
+    auto stage = [&](int h, const uint32_t (&ov)[32], float inv_l) {
+#pragma unroll
+      for (int c = 0; c < 4; ++c) {
+        uint32_t w[4];
+#pragma unroll
+        for (int u = 0; u < 4; ++u)
+          w[u] = some ? pack16<T>(__uint_as_float(ov[8 * c + 2 * u]) * inv_l,
+                                  __uint_as_float(ov[8 * c + 2 * u + 1]) * inv_l)
+                      : 0u;
+        ostage[lane * CH + ((h * 4 + c) ^ (lane & 7))] = make_uint4(w[0], w[1], w[2], w[3]);
+      }
+    };
+    // a part without a step of its own may have Q landing in that buffer still
+    auto direct = [&](int h, const float (&acc)[32], float inv_l) {
+      T* op = static_cast<T*>(p.out) + (size_t)(q_row + row) * p.ldo + (size_t)head * D + h * 32;
+#pragma unroll
+      for (int c = 0; c < 32; c += 2)
+        *reinterpret_cast<uint32_t*>(op + c) =
+            some ? pack16<T>(acc[c] * inv_l, acc[c + 1] * inv_l) : 0u;
+    };
+    auto copy_out = [&](bool zeros) {
+      T* op = static_cast<T*>(p.out) + (size_t)(q_row + t * BQ + qd * 32) * p.ldo + (size_t)head * D;
+      const int n = min(32, rows - t * BQ - qd * 32);      // rows of this warp
+      __syncwarp();
+#pragma unroll 4
+      for (int i = lane; i < 32 * CH; i += 32) {
+        const int rr = i / CH, c = i % CH;
+        if (rr < n)
+          *reinterpret_cast<uint4*>(op + (size_t)rr * p.ldo + c * 8) =
+              zeros ? make_uint4(0, 0, 0, 0) : ostage[rr * CH + (c ^ (rr & 7))];
+      }
+    };
+    if (whole) {
       const float inv_l = 1.0f / l;
-      const bool row_ok = t * BQ + r < rows;
-      T* op = static_cast<T*>(p.out) + (size_t)(q_row + t * BQ + r) * p.ldo + (size_t)head * D;
+#pragma unroll
+      for (int h = 0; h < D / 32; ++h) {
+        if (ok && cnt > 0) {                               // warp-uniform
+          uint32_t ov[32];
+          tmem_ld_32x32b_x32(o_t + h * 32, ov);
+          tmem_ld_wait();
+          stage(h, ov, inv_l);
+        }
+      }
+      if (ok) copy_out(cnt == 0);    // without a step Q may still be landing: zeros, no staging
+    } else {
+      // this part's O, m and l; the last part to arrive here adds all of them up
+      constexpr int kPart = 256 * D + 512;                 // floats of a part
+      float* mine = p.partial + ((size_t)split * p.parts + part) * kPart;
 #pragma unroll
       for (int h = 0; h < D / 32; ++h) {
         uint32_t ov[32];
-        if (cnt > 0) {                                     // warp-uniform
+        if (ok && cnt > 0) {
           tmem_ld_32x32b_x32(o_t + h * 32, ov);
           tmem_ld_wait();
+        } else {
+#pragma unroll
+          for (int c = 0; c < 32; ++c) ov[c] = 0u;
         }
-        if (row_ok) {
 #pragma unroll
-          for (int c = 0; c < 4; ++c) {
-            uint32_t w[4];
+        for (int c = 0; c < 8; ++c)
+          *reinterpret_cast<uint4*>(mine + ((h * 8 + c) * 256 + row) * 4) =
+              make_uint4(ov[4 * c], ov[4 * c + 1], ov[4 * c + 2], ov[4 * c + 3]);
+      }
+      *reinterpret_cast<float2*>(mine + 256 * D + row * 2) = make_float2(m_used, l);
+      __threadfence();
+      named_barrier_sync(2, 256);
+      volatile int* last = reinterpret_cast<volatile int*>(tmem_slot + 2);
+      if (threadIdx.x == 0) {
+        const bool is_last = atomicAdd(p.done + split, 1) == p.parts - 1;
+        if (is_last) p.done[split] = 0;                    // for the next launch
+        *last = is_last;
+      }
+      named_barrier_sync(2, 256);
+      if (*last) {
+        __threadfence();
+        const float* all = p.partial + (size_t)split * p.parts * kPart;
+        float mm = -INFINITY, ll = 0.f;
+        for (int i = 0; i < p.parts; ++i)
+          mm = fmaxf(mm, __ldcg(all + (size_t)i * kPart + 256 * D + row * 2));
+        for (int i = 0; i < p.parts; ++i) {
+          const float* ml = all + (size_t)i * kPart + 256 * D + row * 2;
+          const float mi = __ldcg(ml);
+          ll += mi == -INFINITY ? 0.f : attn::ex2(mi - mm) * __ldcg(ml + 1);
+        }
+        const float inv_l = 1.0f / ll;
 #pragma unroll
-            for (int u = 0; u < 4; ++u)
-              w[u] = some ? pack16<T>(__uint_as_float(ov[8 * c + 2 * u]) * inv_l,
-                                      __uint_as_float(ov[8 * c + 2 * u + 1]) * inv_l)
-                          : 0u;
-            *reinterpret_cast<uint4*>(op + h * 32 + c * 8) = make_uint4(w[0], w[1], w[2], w[3]);
+        for (int h = 0; h < D / 32; ++h) {
+          float acc[32];
+#pragma unroll
+          for (int c = 0; c < 32; ++c) acc[c] = 0.f;
+          for (int i = 0; i < p.parts; ++i) {
+            const float* from = all + (size_t)i * kPart;
+            const float mi = __ldcg(from + 256 * D + row * 2);
+            const float w = mi == -INFINITY ? 0.f : attn::ex2(mi - mm);
+#pragma unroll
+            for (int c = 0; c < 8; ++c) {
+              const float4 v = __ldcg(
+                  reinterpret_cast<const float4*>(from + ((h * 8 + c) * 256 + row) * 4));
+              acc[4 * c] += w * v.x;
+              acc[4 * c + 1] += w * v.y;
+              acc[4 * c + 2] += w * v.z;
+              acc[4 * c + 3] += w * v.w;
+            }
+          }
+          if (cnt > 0) {
+            uint32_t ov[32];
+#pragma unroll
+            for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(acc[c]);
+            stage(h, ov, inv_l);
+          } else if (row < rows) {
+            direct(h, acc, inv_l);
           }
         }
+        if (cnt > 0) copy_out(false);
       }
     }
     tc_fence_before();

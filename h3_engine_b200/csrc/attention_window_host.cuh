@@ -9,6 +9,8 @@ namespace h3b {
 
 constexpr int64_t kMaxKeys = (int64_t)1 << 30;    // positions plus a window stay in 31 bits
 
+static inline int clamp_window(int64_t v) { return (int)std::min<int64_t>(v, kMaxKeys - 1); }
+
 static int tmap_16_rows(CUtensorMap* tm, const void* base, int dtype, int64_t rows, int64_t cols,
                         int64_t stride) {
   auto fn = encode_fn();
@@ -27,7 +29,7 @@ static int tmap_16_rows(CUtensorMap* tm, const void* base, int dtype, int64_t ro
 }
 
 template <int D, typename T>
-static int window_attn_launch(const wattn::Args& a, int items, cudaStream_t st) {
+static int window_attn_launch(const wattn::Args& a, int64_t grid, cudaStream_t st) {
   auto kernel = wattn::k_window_attn<D, T>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   static SmemAttr attr;
@@ -41,17 +43,66 @@ static int window_attn_launch(const wattn::Args& a, int items, cudaStream_t st) 
     regs.store(fa.numRegs, std::memory_order_relaxed);
   }
   if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
-  kernel<<<(unsigned)items, wattn::THREADS, wattn::Smem<D>::BYTES, st>>>(a);
+  kernel<<<(unsigned)grid, wattn::THREADS, wattn::Smem<D>::BYTES, st>>>(a);
   return launched(cudaGetLastError());
 }
+
+// Whole items first, then the last partial wave's items in parts: of `items`
+// CTAs of about equal length on `sms` SMs, items mod sms would run alone, so
+// they are split to fill the SMs (8 heads of 16384 rows, 512 items: 252 us
+// unsplit, see the kernel).  A part should keep four steps or more.
+struct WindowPlan {
+  int whole, parts;
+  WindowPlan(int64_t items, int64_t steps) {
+    const int sms = num_sms();
+    const int rest = (int)(items % sms);
+    whole = (int)items;
+    parts = 1;
+    static const char* ns = getenv("NOSPLIT"); if (rest == 0 || ns) return;
+    const int64_t p = std::min<int64_t>(sms / rest, steps / 4);
+    if (p < 2) return;
+    whole = (int)(items - rest);
+    parts = (int)p;
+  }
+  int64_t split(int64_t items) const { return items - whole; }
+  int64_t grid(int64_t items) const { return whole + split(items) * parts; }
+};
+
+// Key steps of a query-tile pair in a document of n_k keys under a window.
+static int64_t window_steps(int64_t n_k, int64_t left, int64_t right, int64_t sinks) {
+  const int64_t span = std::min<int64_t>(n_k, left + right + 2 * wattn::BQ);
+  return (span + wattn::BK - 1) / wattn::BK + (std::min(sinks, n_k) + wattn::BK - 1) / wattn::BK;
+}
+
+// One launch's documents: up to MAX_DOCS with queries, those with the most keys
+// first (the light items then fill the last wave's gaps), from d0 on.
+struct WindowDocs {
+  int order[wattn::MAX_DOCS];
+  int n = 0, next = 0;
+  int64_t items = 0, steps = 0;
+  WindowDocs(const int32_t* q_len, const int32_t* k_len, int ndocs, int d0, int H, int64_t left,
+             int64_t right, int64_t sinks) {
+    for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0) {
+      if (q_len[d0] == 0) continue;
+      order[n++] = d0;
+      items += ((int64_t)q_len[d0] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
+    }
+    next = d0;
+    std::sort(order, order + n, [&](int a, int b) {
+      return k_len[a] != k_len[b] ? k_len[a] > k_len[b] : a < b;
+    });
+    if (n > 0) steps = window_steps(k_len[order[n - 1]], left, right, sinks);
+  }
+};
+
+static int64_t window_part_bytes(int D) { return ((int64_t)256 * D + 512) * 4; }
+static constexpr int64_t kDoneBytes = 1024;       // a counter per split item (fewer than SMs)
 
 static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, float scale) {
   if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f))
     return H3B_ERR_INVALID_ARG;
   return H3B_OK;
 }
-
-static inline int clamp_window(int64_t v) { return (int)std::min<int64_t>(v, kMaxKeys - 1); }
 
 template <int D, typename T>
 static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st) {
@@ -91,12 +142,30 @@ static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st)
 
 extern "C" {
 
+int64_t h3b_attention_window_ws(const int32_t* q_len, const int32_t* k_len, int ndocs, int H,
+                                int D, int64_t left, int64_t right, int64_t sinks) {
+  if (!q_len || !k_len || ndocs <= 0 || H <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
+  left = clamp_window(left);
+  right = clamp_window(right);
+  int64_t most = 0;
+  for (int d0 = 0; d0 < ndocs;) {
+    const WindowDocs docs(q_len, k_len, ndocs, d0, H, left, right, sinks);
+    d0 = docs.next;
+    const WindowPlan plan(docs.items, docs.steps);
+    const int64_t split = plan.split(docs.items);
+    if (split > 0)
+      most = std::max(most, kDoneBytes + split * plan.parts * window_part_bytes(D));
+  }
+  return most;
+}
+
 int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const void* k,
                          int64_t k_stride, const void* v, int64_t v_stride, int64_t kv_rows,
                          int dtype, int H, int kv_heads, int D, const int32_t* q_start,
                          const int32_t* q_len, const int32_t* k_start, const int32_t* k_len,
                          int ndocs, int64_t left, int64_t right, int64_t sinks, int causal,
-                         float scale, void* out, int64_t ldo, void* stream) {
+                         float scale, void* out, int64_t ldo, void* ws, int64_t ws_bytes,
+                         void* stream) {
   if (!dt_16(dtype) || (D != 64 && D != 128) || H <= 0 || kv_heads <= 0 || H % kv_heads ||
       ndocs < 0 || q_rows < 0 || kv_rows < 0)
     return H3B_ERR_INVALID_ARG;
@@ -142,27 +211,41 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
   a.sinks = clamp_window(sinks);
   a.causal = causal;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
+  const int64_t need =
+      h3b_attention_window_ws(q_len, k_len, ndocs, H, D, left, right, sinks);
+  if (need > 0) {
+    if (!ws || ws_bytes < need) return H3B_ERR_INVALID_ARG;
+    if (reinterpret_cast<uintptr_t>(ws) & 255u) return H3B_ERR_ALIGNMENT;
+    if (cudaMemsetAsync(ws, 0, kDoneBytes, st) != cudaSuccess) return H3B_ERR_CUDA;
+    a.done = static_cast<int*>(ws);
+    a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDoneBytes);
+  }
   for (int d0 = 0; d0 < ndocs;) {               // documents in launches of MAX_DOCS
+    const WindowDocs docs(q_len, k_len, ndocs, d0, H, a.left, a.right, sinks);
+    d0 = docs.next;
+    if (docs.n == 0) break;
+    if (docs.items > INT32_MAX / 2) return H3B_ERR_INVALID_ARG;
     int64_t items = 0;
-    int n = 0;
-    for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0) {
-      if (q_len[d0] == 0) continue;
-      items += ((int64_t)q_len[d0] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
-      if (items > INT32_MAX) return H3B_ERR_INVALID_ARG;
-      a.q_start[n] = q_start[d0];
-      a.q_len[n] = q_len[d0];
-      a.k_start[n] = k_start[d0];
-      a.k_len[n] = k_len[d0];
-      a.item_end[n++] = (int)items;
+    for (int i = 0; i < docs.n; ++i) {
+      const int d = docs.order[i];
+      items += ((int64_t)q_len[d] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
+      a.q_start[i] = q_start[d];
+      a.q_len[i] = q_len[d];
+      a.k_start[i] = k_start[d];
+      a.k_len[i] = k_len[d];
+      a.item_end[i] = (int)items;
     }
-    if (n == 0) break;
-    a.ndocs = n;
+    a.ndocs = docs.n;
+    const WindowPlan plan(items, docs.steps);
+    a.whole = plan.whole;
+    a.parts = plan.parts;
+    const int64_t grid = plan.grid(items);
     if (D == 128)
-      rc = dtype == H3B_DT_F16 ? window_attn_launch<128, __half>(a, (int)items, st)
-                               : window_attn_launch<128, __nv_bfloat16>(a, (int)items, st);
+      rc = dtype == H3B_DT_F16 ? window_attn_launch<128, __half>(a, grid, st)
+                               : window_attn_launch<128, __nv_bfloat16>(a, grid, st);
     else
-      rc = dtype == H3B_DT_F16 ? window_attn_launch<64, __half>(a, (int)items, st)
-                               : window_attn_launch<64, __nv_bfloat16>(a, (int)items, st);
+      rc = dtype == H3B_DT_F16 ? window_attn_launch<64, __half>(a, grid, st)
+                               : window_attn_launch<64, __nv_bfloat16>(a, grid, st);
     if (rc != H3B_OK) return rc;
   }
   return H3B_OK;

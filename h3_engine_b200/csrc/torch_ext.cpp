@@ -420,12 +420,18 @@ struct Packed {
 void window_into(const Call& c, const Packed& p, int64_t heads, int64_t kv_heads, int64_t d,
                  const Rule& r, const Tensor& o) {
   if (p.qd.covered == 0) return;
+  const int docs = (int)p.qd.start.size();
+  const int64_t bytes = h3b_attention_window_ws(p.qd.len.data(), p.kd.len.data(), docs, (int)heads,
+                                                (int)d, r.left, r.right, r.sinks);
+  Tensor ws;
+  if (bytes > 0) ws = at::empty({bytes}, p.q.options().dtype(at::kByte));
   check(h3b_attention_window(p.q.data_ptr(), p.q.size(0), p.q.stride(0), p.k.data_ptr(),
                              p.k.stride(0), p.v.data_ptr(), p.v.stride(0), p.k.size(0),
                              dtype_code(p.q, false, "attention"), (int)heads, (int)kv_heads,
                              (int)d, p.qd.start.data(), p.qd.len.data(), p.kd.start.data(),
-                             p.kd.len.data(), (int)p.qd.start.size(), r.left, r.right, r.sinks,
-                             r.causal, (float)r.scale, o.data_ptr(), o.stride(0), c.stream()),
+                             p.kd.len.data(), docs, r.left, r.right, r.sinks, r.causal,
+                             (float)r.scale, o.data_ptr(), o.stride(0),
+                             bytes > 0 ? ws.data_ptr() : nullptr, bytes, c.stream()),
         "h3b_attention_window");
 }
 

@@ -364,7 +364,12 @@ H3B_API int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride
                                  const int32_t* q_start, const int32_t* q_len,
                                  const int32_t* k_start, const int32_t* k_len, int ndocs,
                                  int64_t left, int64_t right, int64_t sinks, int causal,
-                                 float scale, void* out, int64_t ldo, void* stream);
+                                 float scale, void* out, int64_t ldo, void* ws,
+                                 int64_t ws_bytes, void* stream);
+/* Workspace bytes of that call (256-byte aligned, private to the call until it
+ * has run; 0: none needed) on the current device.                            */
+H3B_API int64_t h3b_attention_window_ws(const int32_t* q_len, const int32_t* k_len, int ndocs,
+                                        int H, int D, int64_t left, int64_t right, int64_t sinks);
 
 /* A few new tokens per sequence against a cache: q [B, n_new, H, D], k and v
  * [B, room, kv_heads, D], each with HOST strides {batch, row, head} in

@@ -81,7 +81,7 @@ def test_host_checks_refuse_without_a_gpu():
         arr = [(ctypes.c_int32 * len(t))(*t) for t in (qs, ql, ks, kl)]
         return lib.h3b_attention_window(q, rows, stride, p, 128, p, 128, rows, dtype, H, kv, D,
                                         *arr, len(qs), left, right, sinks, causal, scale, out,
-                                        256, None)
+                                        256, None, 0, None)
 
     assert packed(D=96) == 1 and packed(dtype=2) == 1 and packed(H=3, kv=2) == 1
     assert packed(H=0) == 1 and packed(scale=0.0) == 1 and packed(scale=float("nan")) == 1
@@ -175,11 +175,20 @@ def test_many_documents_and_large_logits(cuda):
 @pytest.mark.gpu
 def test_equals_full_attention_without_a_window(cuda):
     q, k, v, cq, _ = packed_case([700, 333], [700, 333], 2, 2, 128, BF16)
-    q, k, v = q.to(cuda), k.to(cuda), v.to(cuda)
-    a = ops.attention_window(q, k, v, 2, 128, cq)
-    b = ops.attention_qkv(q, k, v, 2, 128, cq)
-    # one rounding of the result apart at most (their tiles' order agrees)
-    assert ((a.float() - b.float()).abs() <= 2.0 ** -7 * b.float().abs() + 1e-4).all()
+    dev = [t.to(cuda) for t in (q, k, v)]
+    a = ops.attention_window(*dev, 2, 128, cq).cpu().double()
+    b = ops.attention_qkv(*dev, 2, 128, cq).cpu().double()
+    # Both kernels round P to bf16 from exponentials that differ by up to 1.2e-4
+    # (which keys take the polynomial, where the keys are split), so their
+    # results differ by P's rounding steps against sum p |v|, not against |o|:
+    # each is within attend()'s bound of the exact result, so they are within
+    # twice that of each other.
+    for s, e in zip(cq[:-1], cq[1:]):
+        see = torch.ones(e - s, e - s, dtype=torch.bool)
+        for h in (0, 1):
+            c = slice(h * 128, h * 128 + 128)
+            _, off = attend(q[s:e, c], k[s:e, c], v[s:e, c], see, 128 ** -0.5, 2.0 ** -8)
+            assert ((a[s:e, c] - b[s:e, c]).abs() <= 2 * off).all()
 
 
 @pytest.mark.gpu
