@@ -4,7 +4,7 @@
 // (tcgen05.mma kind::mxf4, scale_vec::2X: K = 64 and two scales per row and
 // instruction).
 //
-// Compared with the NVFP4 kernel the scales are half as many: one 128 x 4 tile
+// The scales are half as many as NVFP4's: one 128 x 4 tile
 // of them (512 bytes, one tcgen05.cp of 4 TMEM columns) serves two MMA k-steps,
 // chosen by the scale-factor id of the instruction descriptor (bytes 0-1 or
 // 2-3 of each 32-bit column).  K is any multiple of 32: TMA fills the codes
@@ -26,7 +26,8 @@ constexpr int KB_BYTES = KB_ELEMS / 2;
 constexpr int SF_ATOM = 512;                  // scales of 128 rows x 128 values
 constexpr int KB_ATOMS = KB_ELEMS / 128;
 constexpr int EPI_WARPS = 8;
-constexpr int OUT_WARP_BYTES = 4096;          // 32 rows x 128 bytes, one 128B-swizzled box
+constexpr int OUT_BOX_BYTES = 4096;           // 32 rows x 128 bytes, one 128B-swizzled box
+constexpr int OUT_WARP_BYTES = 2 * OUT_BOX_BYTES;   // both halves of a warp's 128 columns
 constexpr int OUT_COLS = 64;                  // 16-bit columns per TMA store
 constexpr int THREADS = 64 + EPI_WARPS * 32;
 constexpr uint32_t TMEM_COLS = 512;
@@ -42,11 +43,18 @@ __host__ __device__ constexpr uint32_t idesc(uint32_t m, uint32_t n, uint32_t id
          (id << 29);
 }
 
+// Arrive on an mbarrier of a CTA of the cluster without ordering earlier memory
+// operations (the arrival itself is all that the waiter needs).
+__device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote_bar) {
+  asm volatile("mbarrier.arrive.relaxed.cluster.shared::cluster.b64 _, [%0];" ::"r"(remote_bar)
+               : "memory");
+}
+
 enum Epilogue { kOut = 0, kSwigluQuant = 1 };
 
 struct Args {
   CUtensorMap tmap_a;      // u8 [M, K/2], box 128 B x 128 rows, 128B swizzle
-  CUtensorMap tmap_b;      // u8 [N, K/2], box 128 B x 256 rows, 128B swizzle
+  CUtensorMap tmap_b;      // u8 [N, K/2], box 128 B x 128 rows, 128B swizzle
   CUtensorMap tmap_d;      // kOut: 16-bit [M, N] (pitch ldd), box 64 x 32, 128B swizzle
   const uint8_t* sfa;      // blocked scales, M padded to 128 rows
   const uint8_t* sfb;
@@ -59,7 +67,7 @@ struct Args {
   int sf_tiles_k;          // 512-byte scale tiles per 128-row block
   int act;
   int n_tiles;
-  int num_tiles;
+  int early;               // the next launch is of the same chain and may start
 };
 
 __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return bf16x2_to_f2(w); }
@@ -87,11 +95,11 @@ __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc
   const bool row_ok = row < p.M;
   const T* bias = static_cast<const T*>(p.bias);
   const T* residual = static_cast<const T*>(p.residual);
+  if (lane == 0) bulk_wait_read0();                   // the last tile's boxes have been read
+  __syncwarp();
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (n_base + c * OUT_COLS >= p.N) break;          // the box would start past N
-    if (lane == 0) bulk_wait_read0();                 // staging buffer free again
-    __syncwarp();
 #pragma unroll
     for (int j = 0; j < 8; ++j) {
       const int col = n_base + c * OUT_COLS + j * 8;
@@ -122,13 +130,13 @@ __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = mx::pack2(v[e].x, v[e].y, T());
       // 128B swizzle: 16-byte chunk j of row `lane` sits at chunk j ^ (lane % 8)
-      *reinterpret_cast<uint4*>(stage + lane * 128 + ((j ^ (lane & 7)) << 4)) =
+      *reinterpret_cast<uint4*>(stage + c * OUT_BOX_BYTES + lane * 128 + ((j ^ (lane & 7)) << 4)) =
           make_uint4(o[0], o[1], o[2], o[3]);
     }
     fence_proxy_async_smem();
     __syncwarp();
     if (lane == 0) {
-      tma_store_2d(&p.tmap_d, stage_s, n_base + c * OUT_COLS, m0 + qd * 32);
+      tma_store_2d(&p.tmap_d, stage_s + c * OUT_BOX_BYTES, n_base + c * OUT_COLS, m0 + qd * 32);
       bulk_commit();
     }
   }
@@ -179,227 +187,6 @@ __device__ __forceinline__ void epilogue_swiglu_quant(const Args& p, const uint3
       (uint16_t)(s[0] | (s[1] << 8));
 }
 
-// Two MMA k-steps (128 values of K) under one elected lane: the scale tile of
-// A's 128 rows, the tiles of B's two 128-row halves, then one or two MMAs.
-__device__ __forceinline__ void kpair_elect(uint32_t sfa_t, uint64_t sfa_d, uint32_t sfb_t,
-                                            uint64_t sfb_d0, uint64_t sfb_d1, uint32_t d_tmem,
-                                            uint64_t a_desc, uint64_t b_desc, uint32_t accumulate,
-                                            uint32_t second) {
-  asm volatile(
-      "{\n\t.reg .pred p, e, f;\n\t"
-      "setp.ne.b32 p, %9, 0;\n\t"
-      "elect.sync _|e, 0xffffffff;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%0], %1;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%2], %3;\n\t"
-      "@e tcgen05.cp.cta_group::1.32x128b.warpx4 [%4], %5;\n\t"
-      "@e tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
-      " [%6], %7, %8, %10, [%0], [%2], p;\n\t"
-      "setp.ne.and.b32 f, %12, 0, e;\n\t"
-      "setp.eq.u32 p, 0, 0;\n\t"
-      "@f tcgen05.mma.cta_group::1.kind::mxf4.block_scale.scale_vec::2X"
-      " [%6], %13, %14, %11, [%0], [%2], p;\n\t}" ::"r"(sfa_t),
-      "l"(sfa_d), "r"(sfb_t), "l"(sfb_d0), "r"(sfb_t + 4), "l"(sfb_d1), "r"(d_tmem), "l"(a_desc),
-      "l"(b_desc), "r"(accumulate), "r"(idesc(BM, BN, 0)), "r"(idesc(BM, BN, 2)), "r"(second),
-      "l"(a_desc + 2), "l"(b_desc + 2)
-      : "memory");
-}
-
-// ============================================================================
-// Persistent single-CTA kernel, 128 x 256 tiles.  Roles as in the NVFP4
-// kernel: warp 0 TMA producer, warp 1 TMEM allocator and converged MMA issuer,
-// warps 2-9 epilogue (two per TMEM lane quadrant), which pull the accumulator
-// into registers and hand it back before they compute.  Every wait is bounded.
-// ============================================================================
-constexpr int STAGES = 3;
-constexpr int A_BYTES = BM * KB_BYTES;
-constexpr int B_BYTES = BN * KB_BYTES;
-constexpr int SFA_BYTES = KB_ATOMS * SF_ATOM;
-constexpr int SFB_BYTES = 2 * KB_ATOMS * SF_ATOM;
-constexpr int STAGE_BYTES = A_BYTES + B_BYTES + SFA_BYTES + SFB_BYTES;
-constexpr int OUT_OFFSET = STAGES * STAGE_BYTES;
-constexpr int BAR_OFFSET = OUT_OFFSET + EPI_WARPS * OUT_WARP_BYTES;
-constexpr int SMEM_BYTES = BAR_OFFSET + 256 + 1024;
-static_assert(STAGE_BYTES % 1024 == 0 && OUT_OFFSET % 1024 == 0, "swizzle alignment");
-static_assert(SF_COL + STAGES * SF_STAGE_COLS <= TMEM_COLS, "TMEM budget");
-static_assert(SMEM_BYTES <= 232448, "shared memory budget");
-
-template <typename T, int EPI>
-__global__ void __launch_bounds__(THREADS, 1) k_gemm_mxfp4(const __grid_constant__ Args p) {
-  extern __shared__ uint8_t smem_raw[];
-  uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
-                                             ~uintptr_t(1023));
-  uint64_t* bars = reinterpret_cast<uint64_t*>(smem + BAR_OFFSET);
-  uint64_t* full = bars;
-  uint64_t* empty = bars + STAGES;
-  uint64_t* acc_full = bars + 2 * STAGES;
-  uint64_t* acc_empty = bars + 2 * STAGES + 1;
-  uint64_t* drain = bars + 2 * STAGES + 2;
-  uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * STAGES + 3);
-  volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
-
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int num_kb = (p.K + KB_ELEMS - 1) / KB_ELEMS;
-
-  auto sA = [&](int s) { return smem + s * STAGE_BYTES; };
-  auto sB = [&](int s) { return smem + s * STAGE_BYTES + A_BYTES; };
-  auto sSFA = [&](int s) { return smem + s * STAGE_BYTES + A_BYTES + B_BYTES; };
-  auto sSFB = [&](int s) { return smem + s * STAGE_BYTES + A_BYTES + B_BYTES + SFA_BYTES; };
-
-  if (threadIdx.x == 0) {
-    for (int s = 0; s < STAGES; ++s) {
-      mbar_init(smem_u32(&full[s]), 1);
-      mbar_init(smem_u32(&empty[s]), 1);
-    }
-    mbar_init(smem_u32(acc_full), 1);
-    mbar_init(smem_u32(acc_empty), EPI_WARPS);
-    mbar_init(smem_u32(drain), 1);
-    *abort_flag = 0;
-    fence_mbar_init();
-  }
-  if (warp == 1) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
-    tmem_relinquish();
-  }
-  tc_fence_before();
-  __syncthreads();
-  tc_fence_after();
-  const uint32_t tmem = *tmem_slot;
-
-  if (warp == 0) {
-    if (lane == 0) {
-      prefetch_tmap(&p.tmap_a);
-      prefetch_tmap(&p.tmap_b);
-      uint32_t g = 0;
-      bool ok = true;
-      for (int t = blockIdx.x; t < p.num_tiles && ok; t += gridDim.x) {
-        const int m0 = (t / p.n_tiles) * BM, n0 = (t % p.n_tiles) * BN;
-        const bool b_hi = (n0 + 128) < p.N;
-        const size_t sf_row = (size_t)p.sf_tiles_k * SF_ATOM;
-        const uint8_t* sfa_row = p.sfa + (size_t)(m0 / 128) * sf_row;
-        const uint8_t* sfb_row = p.sfb + (size_t)(n0 / 128) * sf_row;
-        for (int kb = 0; kb < num_kb; ++kb, ++g) {
-          const int s = g % STAGES;
-          const uint32_t ph = (g / STAGES) & 1;
-          if (g >= STAGES && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, abort_flag)) {
-            record_error(H3B_ERR_TIMEOUT);
-            *abort_flag = 1;
-            ok = false;
-            break;
-          }
-          // the last k-block may hold one scale tile instead of two
-          const uint32_t sfb_bytes =
-              (uint32_t)min(KB_ATOMS, p.sf_tiles_k - kb * KB_ATOMS) * SF_ATOM;
-          const uint32_t fb = smem_u32(&full[s]);
-          mbar_expect_tx(fb, A_BYTES + B_BYTES + (b_hi ? 3 : 2) * sfb_bytes);
-          tma_load_2d(smem_u32(sA(s)), &p.tmap_a, kb * KB_BYTES, m0, fb);
-          tma_load_2d(smem_u32(sB(s)), &p.tmap_b, kb * KB_BYTES, n0, fb);
-          const size_t off = (size_t)kb * KB_ATOMS * SF_ATOM;
-          bulk_load(smem_u32(sSFA(s)), sfa_row + off, sfb_bytes, fb);
-          bulk_load(smem_u32(sSFB(s)), sfb_row + off, sfb_bytes, fb);
-          if (b_hi)
-            bulk_load(smem_u32(sSFB(s)) + KB_ATOMS * SF_ATOM, sfb_row + sf_row + off, sfb_bytes,
-                      fb);
-        }
-      }
-      if (!ok || *abort_flag) {
-        // Let every copy already in flight land before the CTA can exit.
-        for (uint32_t q = g > (uint32_t)STAGES ? g - STAGES : 0; q < g; ++q)
-          mbar_wait(smem_u32(&full[q % STAGES]), (q / STAGES) & 1, nullptr);
-      }
-    }
-  } else if (warp == 1) {
-    auto wait = [&](uint64_t* bar, uint32_t parity) -> bool {
-      return __all_sync(0xffffffffu, mbar_wait(smem_u32(bar), parity, abort_flag));
-    };
-    const int last_steps = (p.K - (num_kb - 1) * KB_ELEMS + 63) >> 6;   // k-steps of the last block
-    uint32_t g = 0, i = 0;
-    bool ok = true;
-    for (int t = blockIdx.x; t < p.num_tiles && ok; t += gridDim.x, ++i) {
-      if (i > 0 && !wait(acc_empty, (i - 1) & 1)) {
-        ok = false;
-        break;
-      }
-      tc_fence_after();
-      for (int kb = 0; kb < num_kb; ++kb, ++g) {
-        const int s = g % STAGES;
-        const uint32_t ph = (g / STAGES) & 1;
-        if (!wait(&full[s], ph)) {
-          ok = false;
-          break;
-        }
-        tc_fence_after();
-        const int steps = kb == num_kb - 1 ? last_steps : 4;
-        const uint32_t sf_t = tmem + SF_COL + s * SF_STAGE_COLS;
-        const uint64_t sfa_d = desc_sf_atom(smem_u32(sSFA(s)));
-        const uint64_t sfb_d = desc_sf_atom(smem_u32(sSFB(s)));
-        const uint64_t a_d = desc_kmajor_sw128(smem_u32(sA(s)));
-        const uint64_t b_d = desc_kmajor_sw128(smem_u32(sB(s)));
-        // descriptors advance by adding (bytes >> 4): 32 bytes per k-step
-#pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (h * 2 < steps)
-            kpair_elect(sf_t + h * 4, sfa_d + ((h * SF_ATOM) >> 4), sf_t + 8 + h * 8,
-                        sfb_d + ((h * SF_ATOM) >> 4), sfb_d + (((KB_ATOMS + h) * SF_ATOM) >> 4),
-                        tmem + ACC_COL, a_d + h * 4, b_d + h * 4, (kb | h) != 0,
-                        h * 2 + 1 < steps);
-        }
-        tc_commit_elect(smem_u32(&empty[s]));
-      }
-      if (!ok) break;
-      tc_commit_elect(smem_u32(acc_full));
-    }
-    if (!ok) {
-      if (lane == 0 && !*abort_flag) {
-        record_error(H3B_ERR_TIMEOUT);
-        *abort_flag = 1;
-      }
-      tc_commit_elect(smem_u32(drain));
-      mbar_wait(smem_u32(drain), 0, nullptr);
-    }
-  } else {
-    const int ew = warp - 2;
-    const int qd = warp & 3;          // TMEM lane quadrant this warp may access
-    const int half = ew >> 2;         // which 128 of the 256 accumulator columns
-    uint8_t* stage = smem + OUT_OFFSET + ew * OUT_WARP_BYTES;
-    const uint32_t stage_s = smem_u32(stage);
-    uint32_t i = 0;
-    if (EPI == kOut && lane == 0) prefetch_tmap(&p.tmap_d);
-    for (int t = blockIdx.x; t < p.num_tiles; t += gridDim.x, ++i) {
-      const int m0 = (t / p.n_tiles) * BM, n0 = (t % p.n_tiles) * BN;
-      const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(acc_full), i & 1, abort_flag));
-      if (!ready) {
-        if (!*abort_flag) {
-          record_error(H3B_ERR_TIMEOUT);
-          *abort_flag = 1;
-        }
-        break;
-      }
-      tc_fence_after();
-      uint32_t acc[128];
-      const uint32_t taddr = tmem + ACC_COL + ((uint32_t)(qd * 32) << 16) + half * 128;
-      tmem_ld_32x32b_x64(taddr, acc);
-      tmem_ld_32x32b_x64(taddr + 64, acc + 64);
-      tmem_ld_wait();
-      tc_fence_before();
-      __syncwarp();
-      if (lane == 0) mbar_arrive(smem_u32(acc_empty));
-      if (EPI == kOut)
-        epilogue_out<T>(p, acc, m0, n0, half, qd, lane, stage, stage_s);
-      else
-        epilogue_swiglu_quant(p, acc, m0, n0, half, qd, lane);
-    }
-    if (EPI == kOut && lane == 0) bulk_wait0();
-  }
-
-  tc_fence_before();
-  __syncthreads();
-  if (warp == 1) {
-    __syncwarp();
-    tc_fence_after();
-    tmem_dealloc(tmem, TMEM_COLS);
-  }
-}
-
 // ============================================================================
 // CTA-pair kernel (cluster of 2): one 256 x 256 tile per pair, the MMA in its
 // cta_group::2 form.  CTA r loads rows m0 + 128 r .. of A with their scales,
@@ -410,7 +197,13 @@ __global__ void __launch_bounds__(THREADS, 1) k_gemm_mxfp4(const __grid_constant
 // come through tensor maps so that rows and columns outside the operand read
 // as zeros.  Protocol, bounds and teardown as in the NVFP4 pair kernel.
 // ============================================================================
-constexpr int P_STAGES = 5;
+//
+// Between tiles the tensor core waits for the accumulator: commit, the epilogue
+// warps' tcgen05.ld (about 100 cycles), their arrival on the leader's barrier.
+// That arrival is a relaxed one (nothing but registers was produced before it):
+// a release at cluster scope made it wait for the warp's earlier stores, 1900
+// cycles of the 21000 that a tile with K = 7168 took.
+constexpr int P_STAGES = 4;
 constexpr int P_A_BYTES = 128 * KB_BYTES;
 constexpr int P_B_BYTES = 128 * KB_BYTES;
 constexpr int P_SFA_BYTES = KB_ATOMS * SF_ATOM;
@@ -424,7 +217,7 @@ static_assert(SF_COL + P_STAGES * SF_STAGE_COLS <= TMEM_COLS, "TMEM budget");
 static_assert(P_SMEM_BYTES <= 232448, "shared memory budget");
 
 struct PairArgs {
-  Args base;               // tmap_a and tmap_b: box 128 B x 128 rows
+  Args base;
   CUtensorMap tmap_sfa;    // u64 [128-row blocks, scale tiles * 64], box 128 x 1 (one k-block)
   CUtensorMap tmap_sfb;    // the same for B, box 128 x 2
   int m_tiles;             // 256-row tiles
@@ -530,13 +323,35 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       prefetch_tmap(&p.tmap_b);
       prefetch_tmap(&pa.tmap_sfa);
       prefetch_tmap(&pa.tmap_sfb);
+      auto load_b = [&](int s, int kb, int n0) {
+        const uint32_t lb = mapa_shared(smem_u32(&full[s]), 0);
+        if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * P_STAGE_BYTES);
+        tma_load_2d_pair(smem_u32(sB(s)), &p.tmap_b, kb * KB_BYTES, n0 + 128 * (int)rank, lb);
+        tma_load_2d_pair(smem_u32(sSFB(s)), &pa.tmap_sfb, kb * KB_ATOMS * 64, n0 / 128, lb);
+      };
+      auto load_a = [&](int s, int kb, int m0) {
+        const uint32_t lb = mapa_shared(smem_u32(&full[s]), 0);
+        tma_load_2d_pair(smem_u32(sA(s)), &p.tmap_a, kb * KB_BYTES, m0 + 128 * (int)rank, lb);
+        tma_load_2d_pair(smem_u32(sSFA(s)), &pa.tmap_sfa, kb * KB_ATOMS * 64,
+                         m0 / 128 + (int)rank, lb);
+      };
       uint32_t g = 0;
       bool ok = true;
       for (int t = pair_id; t < num_tiles && ok; t += num_pairs) {
         int mt, nt;
         pair_tile(pa, t, mt, nt);
         const int m0 = mt * 256, n0 = nt * BN;
-        for (int kb = 0; kb < num_kb; ++kb, ++g) {
+        int kb = 0;
+        if (t == pair_id) {
+          // the weight's side of the ring fills before the chain's earlier
+          // launch, which produces A, is done
+          kb = min(num_kb, P_STAGES);
+          for (int i = 0; i < kb; ++i) load_b(i, i, n0);
+          mx::grid_wait();
+          for (int i = 0; i < kb; ++i) load_a(i, i, m0);
+          g = kb;
+        }
+        for (; kb < num_kb; ++kb, ++g) {
           const int s = g % P_STAGES;
           const uint32_t ph = (g / P_STAGES) & 1;
           if (g >= P_STAGES && !mbar_wait(smem_u32(&empty[s]), ph ^ 1, abort_flag)) {
@@ -544,13 +359,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
             ok = false;
             break;
           }
-          const uint32_t lb = mapa_shared(smem_u32(&full[s]), 0);
-          if (rank == 0) mbar_expect_tx(smem_u32(&full[s]), 2 * P_STAGE_BYTES);
-          tma_load_2d_pair(smem_u32(sA(s)), &p.tmap_a, kb * KB_BYTES, m0 + 128 * (int)rank, lb);
-          tma_load_2d_pair(smem_u32(sB(s)), &p.tmap_b, kb * KB_BYTES, n0 + 128 * (int)rank, lb);
-          tma_load_2d_pair(smem_u32(sSFA(s)), &pa.tmap_sfa, kb * KB_ATOMS * 64,
-                           m0 / 128 + (int)rank, lb);
-          tma_load_2d_pair(smem_u32(sSFB(s)), &pa.tmap_sfb, kb * KB_ATOMS * 64, n0 / 128, lb);
+          load_b(s, kb, n0);
+          load_a(s, kb, m0);
         }
       }
       // tail: the release of every stage this CTA filled has arrived (the
@@ -617,6 +427,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t stage_s = smem_u32(stage);
     const uint32_t leader_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
     uint32_t i = 0;
+    mx::grid_wait();                     // residual and D follow the chain's earlier launches
+    if (p.early) mx::grid_launch_dependents();
     if (EPI == kOut && lane == 0) prefetch_tmap(&p.tmap_d);
     for (int t = pair_id; t < num_tiles; t += num_pairs, ++i) {
       int mt, nt;
@@ -635,13 +447,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       tmem_ld_wait();
       tc_fence_before();
       __syncwarp();
-      if (lane == 0) mbar_arrive_cluster(leader_acc_empty);
+      if (lane == 0) mbar_arrive_cluster_relaxed(leader_acc_empty);
       if (EPI == kOut)
         epilogue_out<T>(p, acc, m0, n0, half, qd, lane, stage, stage_s);
       else
         epilogue_swiglu_quant(p, acc, m0, n0, half, qd, lane);
     }
-    if (EPI == kOut && lane == 0) bulk_wait0();
+    if (EPI == kOut && lane == 0) bulk_wait_read0();     // shared memory may go
   }
 
   tc_fence_before();
@@ -650,7 +462,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   // accumulator is written by the leader's MMAs, its loads count on the
   // leader's barriers
   if (threadIdx.x == 0) {
-    mbar_arrive_cluster(mapa_shared(smem_u32(bye), rank ^ 1u));
+    mbar_arrive_cluster_relaxed(mapa_shared(smem_u32(bye), rank ^ 1u));
     if (!mbar_wait(smem_u32(bye), 0, nullptr)) record_error(H3B_ERR_TIMEOUT);
   }
   __syncthreads();

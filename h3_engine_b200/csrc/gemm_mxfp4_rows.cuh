@@ -118,9 +118,6 @@ __device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t* r) {
       : "r"(taddr));
 }
 
-__device__ __forceinline__ void grid_wait() {
-  asm volatile("griddepcontrol.wait;" ::: "memory");
-}
 __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
   float4 v;
   asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];"
@@ -217,7 +214,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       };
       const int n = kb1 - kb0, head = min(n, R::STAGES);
       for (int i = 0; i < head; ++i) load_w(kb0 + i, i);
-      if (!FUSED) grid_wait();           // the activation's codes are there from here on
+      if (!FUSED) mx::grid_wait();           // the activation's codes are there from here on
       for (int i = 0; i < head; ++i) load_x(kb0 + i, i);
       int issued = head;
       bool ok = true;
@@ -274,7 +271,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       mbar_wait(smem_u32(drain), 0, nullptr);
     }
   } else {
-    grid_wait();                         // x, bias, residual and out follow earlier work
+    mx::grid_wait();                         // x, bias, residual and out follow earlier work
     if (FUSED) {
       // k-block i of the rows: lane l holds values 8 l .. 8 l + 7 of a row
       for (int i = warp - 2; i < kb1 - kb0; i += 4) {
@@ -347,7 +344,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
   const uint32_t base = smem_u32(smem);
   // (warps 0 and 1 have not waited for the chain's earlier launches: the
   // residual and out are theirs too)
-  grid_wait();
+  mx::grid_wait();
   if (EPI == mxgemm::kOut) {
     // 32 threads cover a row's 128 columns, four each
     const int c = (threadIdx.x & 31) * 4, n = n0 + c;

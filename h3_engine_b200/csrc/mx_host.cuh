@@ -89,12 +89,7 @@ static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64
       static_cast<T*>(out), ldo, (uint32_t)per_row);
 }
 
-// CTA pairs wherever there are two 128-row blocks to share a B tile: 13383 x
-// 5376 x 7168 takes 196 us on them and 212 on single CTAs, 13383 x 28672 x 5376
-// 793 and 1048.
-static bool mx_use_pair(int64_t M, int64_t N) { return M > mxgemm::BM && N > 128; }
-
-// Operands of both MXFP4 GEMM kernels: shapes and alignment.
+// Operands of the CTA-pair kernel: shapes and alignment.
 static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, int64_t M,
                         const void* B, const void* sfB, int64_t N, int64_t K) {
   if (!A || !sfA || !B || !sfB) return H3B_ERR_INVALID_ARG;
@@ -104,12 +99,11 @@ static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, in
   if (rc != H3B_OK) return rc;
   memset(&pa, 0, sizeof(pa));
   mxgemm::Args& a = pa.base;
-  const bool pair = mx_use_pair(M, N);
   rc = make_tmap_u8_sw128(&a.tmap_a, A, (uint64_t)M, (uint64_t)(K / 2), (uint64_t)(K / 2),
                           mxgemm::KB_BYTES, mxgemm::BM);
   if (rc != H3B_OK) return rc;
   rc = make_tmap_u8_sw128(&a.tmap_b, B, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)(K / 2),
-                          mxgemm::KB_BYTES, pair ? 128 : mxgemm::BN);
+                          mxgemm::KB_BYTES, 128);
   if (rc != H3B_OK) return rc;
   a.sfa = static_cast<const uint8_t*>(sfA);
   a.sfb = static_cast<const uint8_t*>(sfB);
@@ -118,47 +112,41 @@ static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, in
   a.K = (int)K;
   a.sf_tiles_k = (int)mx::sf_tiles(K);
   a.n_tiles = (int)((N + mxgemm::BN - 1) / mxgemm::BN);
-  const int64_t tiles = (int64_t)a.n_tiles * ((M + mxgemm::BM - 1) / mxgemm::BM);
-  if (tiles > INT32_MAX) return H3B_ERR_INVALID_ARG;
-  a.num_tiles = (int)tiles;
-  if (pair) {
-    const uint64_t width = (uint64_t)a.sf_tiles_k * (mxgemm::SF_ATOM / 8);
-    rc = make_tmap_u64(&pa.tmap_sfa, sfA, (uint64_t)((M + 127) / 128), width,
-                       mxgemm::KB_ATOMS * 64, 1);
-    if (rc != H3B_OK) return rc;
-    rc = make_tmap_u64(&pa.tmap_sfb, sfB, (uint64_t)((N + 127) / 128), width,
-                       mxgemm::KB_ATOMS * 64, 2);
-    if (rc != H3B_OK) return rc;
-    pa.m_tiles = (int)((M + 255) / 256);
-    // 16 tile rows per raster group: the 74 pairs then work on 16 row and about
-    // 5 column tiles at a time (13383 x 28672 x 5376: 889 us with groups of
-    // one, 843 of 4, 811 of 8, 793 of 16, 784 of 32; shorter N, 193-198)
-    pa.group = 16;
-  }
+  pa.m_tiles = (int)((M + 255) / 256);
+  if ((int64_t)pa.m_tiles * a.n_tiles > INT32_MAX) return H3B_ERR_INVALID_ARG;
+  const uint64_t width = (uint64_t)a.sf_tiles_k * (mxgemm::SF_ATOM / 8);
+  rc = make_tmap_u64(&pa.tmap_sfa, sfA, (uint64_t)((M + 127) / 128), width, mxgemm::KB_ATOMS * 64,
+                     1);
+  if (rc != H3B_OK) return rc;
+  rc = make_tmap_u64(&pa.tmap_sfb, sfB, (uint64_t)((N + 127) / 128), width, mxgemm::KB_ATOMS * 64,
+                     2);
+  if (rc != H3B_OK) return rc;
+  // 16 tile rows per raster group: the 74 pairs then work on 16 row and about
+  // 5 column tiles at a time (13383 x 28672 x 5376: 889 us with groups of one,
+  // 843 of 4, 811 of 8, 793 of 16, 784 of 32; shorter N, 193-198)
+  pa.group = 16;
   return H3B_OK;
 }
 
 template <typename T, int EPI>
-static int mx_gemm_launch(const mxgemm::PairArgs& pa, cudaStream_t st) {
-  const mxgemm::Args& a = pa.base;
-  if (pa.m_tiles > 0) {
-    static SmemAttr attr;
-    const int rc = attr.set(reinterpret_cast<const void*>(&mxgemm::k_gemm_mxfp4_pair<T, EPI>),
-                            mxgemm::P_SMEM_BYTES);
-    if (rc != H3B_OK) return rc;
-    const int64_t tiles = (int64_t)pa.m_tiles * a.n_tiles;
-    const int pairs = (int)std::min<int64_t>(tiles, num_sms() / 2);
-    mxgemm::k_gemm_mxfp4_pair<T, EPI>
-        <<<2 * pairs, mxgemm::THREADS, mxgemm::P_SMEM_BYTES, st>>>(pa);
-    return launched(cudaGetLastError());
-  }
+static int mx_gemm_launch(const mxgemm::PairArgs& pa, bool chained, cudaStream_t st) {
+  auto kernel = mxgemm::k_gemm_mxfp4_pair<T, EPI>;
   static SmemAttr attr;
-  const int rc = attr.set(reinterpret_cast<const void*>(&mxgemm::k_gemm_mxfp4<T, EPI>),
-                          mxgemm::SMEM_BYTES);
+  const int rc = attr.set(reinterpret_cast<const void*>(kernel), mxgemm::P_SMEM_BYTES);
   if (rc != H3B_OK) return rc;
-  const int grid = std::min(a.num_tiles, num_sms());
-  mxgemm::k_gemm_mxfp4<T, EPI><<<grid, mxgemm::THREADS, mxgemm::SMEM_BYTES, st>>>(a);
-  return launched(cudaGetLastError());
+  const int64_t tiles = (int64_t)pa.m_tiles * pa.base.n_tiles;
+  const int pairs = (int)std::min<int64_t>(tiles, num_sms() / 2);
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = dim3((unsigned)(2 * pairs));
+  cfg.blockDim = dim3(mxgemm::THREADS);
+  cfg.dynamicSmemBytes = mxgemm::P_SMEM_BYTES;
+  cfg.stream = st;
+  cudaLaunchAttribute at[1];
+  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+  at[0].val.programmaticStreamSerializationAllowed = 1;
+  cfg.attrs = at;
+  cfg.numAttrs = chained ? 1 : 0;
+  return launched(cudaLaunchKernelEx(&cfg, kernel, pa));
 }
 
 // ---- up to 128 rows: the weight-streaming kernel
@@ -282,8 +270,8 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, c
   a.residual = residual;
   a.ldr = ldr;
   a.act = act;
-  return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(pa, st)
-                             : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(pa, st);
+  return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(pa, chained, st)
+                             : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(pa, chained, st);
 }
 
 // 16-bit rows that a product can quantize itself.
@@ -346,7 +334,7 @@ int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const voi
                        false, st);
   uint8_t* q = static_cast<uint8_t*>(ws);
   uint8_t* sf = q + mx_code_bytes(M, K);
-  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, M <= mxrows::kMaxRows, st);
+  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, true, st);
   if (rc != H3B_OK) return rc;
   return mx_gemm_out(q, sf, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, true, st);
 }
@@ -374,7 +362,7 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   uint8_t* sfh = qh + mx_code_bytes(M, F);
   const bool fused = M <= mxrows::kFusedRows;
   if (!fused) {
-    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, M <= mxrows::kMaxRows, st);
+    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, true, st);
     if (rc != H3B_OK) return rc;
   }
   if (M <= mxrows::kMaxRows) {
@@ -396,7 +384,8 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
     if (rc != H3B_OK) return rc;
     up.base.q_out = qh;
     up.base.sf_out = sfh;
-    rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, st);
+    up.base.early = 1;
+    rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, true, st);
   }
   if (rc != H3B_OK) return rc;
   return mx_gemm_out(qh, sfh, 0, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D,

@@ -127,6 +127,10 @@ __device__ __forceinline__ void grid_launch_dependents() {
   asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
 }
 
+// Waits until the launch before this one is done and its results are visible
+// (at once, where this one was not started early).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 // ---------------------------------------------------------------- quantize
 constexpr int kThreads = 256;
 
