@@ -48,16 +48,41 @@ static inline bool dt_16(int d) { return d == H3B_DT_BF16 || d == H3B_DT_F16; }
 
 constexpr int64_t kMxMaxDim = (int64_t)INT32_MAX - 512;
 
-template <typename T>
+// One unit of work per warp (32768 x 14336 bf16: 207 and 226 us to quantize and
+// unpack with 8 CTAs per SM that loop, 176 and 190 with 32, 177 and 177 with as
+// many as there are units), two loads in flight per lane (one: 186 and 187).
+constexpr int kQuantUnroll = 2;
+static unsigned mx_quant_blocks(int64_t units) {
+  const int64_t blocks = (units + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
+  return (unsigned)std::min<int64_t>(blocks, 1 << 30);
+}
+
+template <typename T, int VPL>
 static void mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
-                               int64_t Mpad, bool early, cudaStream_t st) {
-  constexpr int kUnroll = 4;
-  const int64_t per_row = (mx::sf_tiles(K) * 128 + 256 * kUnroll - 1) / (256 * kUnroll);
-  int64_t blocks = (Mpad * per_row + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
-  blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
-  mx::k_mxfp4_quantize<T, kUnroll><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
-      static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q), static_cast<uint8_t*>(sf),
-      Mpad, (uint32_t)per_row, early);
+                               bool early, cudaStream_t st) {
+  constexpr int kUnit = 32 * VPL * kQuantUnroll;
+  const int64_t Mpad = (M + 127) / 128 * 128;
+  const int64_t per_row = (mx::sf_tiles(K) * 128 + kUnit - 1) / kUnit;
+  mx::k_mxfp4_quantize<T, VPL, kQuantUnroll>
+      <<<mx_quant_blocks(Mpad * per_row), mx::kThreads, 0, st>>>(
+          static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q),
+          static_cast<uint8_t*>(sf), Mpad, (uint32_t)per_row, early);
+}
+
+template <typename T, int VPL>
+static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
+                                 int64_t ldo, cudaStream_t st) {
+  constexpr int kUnit = 32 * VPL * kQuantUnroll;
+  const int64_t per_row = (K + kUnit - 1) / kUnit;
+  mx::k_mxfp4_dequantize<T, VPL, kQuantUnroll>
+      <<<mx_quant_blocks(M * per_row), mx::kThreads, 0, st>>>(
+          static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
+          static_cast<T*>(out), ldo, (uint32_t)per_row);
+}
+
+// 32-byte accesses where base and rows allow them.
+static inline bool wide_rows(const void* p, int64_t ld, int size) {
+  return (reinterpret_cast<uintptr_t>(p) & 31u) == 0 && (ld * size) % 32 == 0;
 }
 
 static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
@@ -67,26 +92,16 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   if (M == 0) return H3B_OK;
   if (!x || !q || !sf) return H3B_ERR_INVALID_ARG;
   if (!aligned16(x) || !aligned16(q) || (ldx * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
-  const int64_t Mpad = (M + 127) / 128 * 128;
-  if (dtype == H3B_DT_BF16)
-    mx_quantize_launch<__nv_bfloat16>(x, M, K, ldx, q, sf, Mpad, early, st);
-  else if (dtype == H3B_DT_F16)
-    mx_quantize_launch<__half>(x, M, K, ldx, q, sf, Mpad, early, st);
-  else
-    mx_quantize_launch<float>(x, M, K, ldx, q, sf, Mpad, early, st);
+  const bool wide = wide_rows(x, ldx, dt_bytes(dtype));
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (wide) mx_quantize_launch<T, 16>(x, M, K, ldx, q, sf, early, st);
+    else mx_quantize_launch<T, 8>(x, M, K, ldx, q, sf, early, st);
+  };
+  if (dtype == H3B_DT_BF16) go(__nv_bfloat16());
+  else if (dtype == H3B_DT_F16) go(__half());
+  else go(float());
   return launched(cudaGetLastError());
-}
-
-template <typename T>
-static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
-                                 int64_t ldo, cudaStream_t st) {
-  constexpr int kUnroll = 4;
-  const int64_t per_row = (K + 256 * kUnroll - 1) / (256 * kUnroll);
-  int64_t blocks = (M * per_row + mx::kThreads / 32 - 1) / (mx::kThreads / 32);
-  blocks = std::min<int64_t>(blocks, (int64_t)num_sms() * 8);
-  mx::k_mxfp4_dequantize<T, kUnroll><<<(unsigned)blocks, mx::kThreads, 0, st>>>(
-      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
-      static_cast<T*>(out), ldo, (uint32_t)per_row);
 }
 
 // Operands of the CTA-pair kernel: shapes and alignment.
@@ -297,9 +312,15 @@ int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, vo
   if (!q || !sf || !out) return H3B_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(out) || (ldo * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (dtype == H3B_DT_BF16) mx_dequantize_launch<__nv_bfloat16>(q, sf, M, K, out, ldo, st);
-  else if (dtype == H3B_DT_F16) mx_dequantize_launch<__half>(q, sf, M, K, out, ldo, st);
-  else mx_dequantize_launch<float>(q, sf, M, K, out, ldo, st);
+  const bool wide = wide_rows(out, ldo, dt_bytes(dtype));
+  auto go = [&](auto t) {
+    using T = decltype(t);
+    if (wide) mx_dequantize_launch<T, 16>(q, sf, M, K, out, ldo, st);
+    else mx_dequantize_launch<T, 8>(q, sf, M, K, out, ldo, st);
+  };
+  if (dtype == H3B_DT_BF16) go(__nv_bfloat16());
+  else if (dtype == H3B_DT_F16) go(__half());
+  else go(float());
   return launched(cudaGetLastError());
 }
 

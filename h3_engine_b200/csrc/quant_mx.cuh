@@ -12,6 +12,8 @@
 
 #include <cuda_fp16.h>
 
+#include <type_traits>
+
 #include "common.cuh"
 #include "quant.cuh"
 
@@ -86,25 +88,6 @@ struct Vec8<__half> {
     }
   }
 };
-template <>
-struct Vec8<float> {
-  uint4 w[2];
-  __device__ __forceinline__ void load(const float* p) {
-    w[0] = ld_nc_v4(p);
-    w[1] = ld_nc_v4(p + 4);
-  }
-  __device__ __forceinline__ void zero() { w[0] = w[1] = make_uint4(0, 0, 0, 0); }
-  __device__ __forceinline__ void get(float (&v)[8]) const {
-#pragma unroll
-    for (int i = 0; i < 2; ++i) {
-      v[4 * i] = __uint_as_float(w[i].x);
-      v[4 * i + 1] = __uint_as_float(w[i].y);
-      v[4 * i + 2] = __uint_as_float(w[i].z);
-      v[4 * i + 3] = __uint_as_float(w[i].w);
-    }
-  }
-};
-
 __device__ __forceinline__ uint32_t pack2(float lo, float hi, __nv_bfloat16) {
   return pack_bf16x2(lo, hi);
 }
@@ -131,128 +114,220 @@ __device__ __forceinline__ void grid_launch_dependents() {
 // (at once, where this one was not started early).
 __device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 
+// ---------------------------------------------------------------- wide accesses
+// 32 bytes per lane in one access (256-bit, 32-byte aligned): a warp moves 1 KiB
+// of one row, whole sectors each.
+__device__ __forceinline__ void ld_nc_v8(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+               : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
+                 "=r"(r[6]), "=r"(r[7])
+               : "l"(p));
+}
+__device__ __forceinline__ void st_v8(void* p, const uint32_t (&r)[8]) {
+  asm volatile("st.global.v8.b32 [%0], {%1,%2,%3,%4,%5,%6,%7,%8};" ::"l"(p), "r"(r[0]), "r"(r[1]),
+               "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7])
+               : "memory");
+}
+
+// VPL values of T per lane: 8 by 16-byte accesses, 16 by 32-byte ones.
+template <typename T, int VPL>
+struct Lane {
+  static constexpr int WORDS = VPL * (int)sizeof(T) / 4;
+  uint32_t w[WORDS];
+  __device__ __forceinline__ void zero() {
+#pragma unroll
+    for (int i = 0; i < WORDS; ++i) w[i] = 0u;
+  }
+  __device__ __forceinline__ void load(const T* p) {
+    const char* c = reinterpret_cast<const char*>(p);
+    if constexpr (VPL == 16) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 8; ++i)
+        ld_nc_v8(c + i * 32, *reinterpret_cast<uint32_t(*)[8]>(w + i * 8));
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i)
+        *reinterpret_cast<uint4*>(w + i * 4) = ld_nc_v4(c + i * 16);
+    }
+  }
+  __device__ __forceinline__ void store(T* p) const {
+    char* c = reinterpret_cast<char*>(p);
+    if constexpr (VPL == 16) {
+#pragma unroll
+      for (int i = 0; i < WORDS / 8; ++i)
+        st_v8(c + i * 32, *reinterpret_cast<const uint32_t(*)[8]>(w + i * 8));
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS / 4; ++i)
+        *reinterpret_cast<uint4*>(c + i * 16) = *reinterpret_cast<const uint4*>(w + i * 4);
+    }
+  }
+  __device__ __forceinline__ float2 get2(int i) const {      // values 2 i and 2 i + 1
+    if constexpr (std::is_same<T, float>::value)
+      return make_float2(__uint_as_float(w[2 * i]), __uint_as_float(w[2 * i + 1]));
+    else if constexpr (std::is_same<T, __half>::value)
+      return __half22float2(*reinterpret_cast<const __half2*>(&w[i]));
+    else
+      return bf16x2_to_f2(w[i]);
+  }
+  __device__ __forceinline__ void set2(int i, float a, float b) {
+    if constexpr (std::is_same<T, float>::value) {
+      w[2 * i] = __float_as_uint(a);
+      w[2 * i + 1] = __float_as_uint(b);
+    } else {
+      w[i] = pack2(a, b, T());
+    }
+  }
+  // max |v| as fp32 bits; 16-bit values compare as their magnitudes' integers,
+  // two at a time (a NaN's are above every number's)
+  __device__ __forceinline__ uint32_t absmax_bits() const {
+    uint32_t m = 0;
+    if constexpr (std::is_same<T, float>::value) {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) m = max(m, w[i] & 0x7FFFFFFFu);
+      return m;
+    } else {
+#pragma unroll
+      for (int i = 0; i < WORDS; ++i) m = __vmaxu2(m, w[i] & 0x7FFF7FFFu);
+      m = max(m & 0xFFFFu, m >> 16);
+      if constexpr (std::is_same<T, __half>::value)
+        return __float_as_uint(__half2float(__ushort_as_half((unsigned short)m)));
+      return m << 16;
+    }
+  }
+};
+
 // ---------------------------------------------------------------- quantize
 constexpr int kThreads = 256;
 
-// A warp's unit of work is UNROLL * 256 consecutive values of a row (units
+// A warp's unit of work is UNROLL * 32 * VPL consecutive values of a row (units
 // grid-stride over rows and pieces alike, so one long row spreads over many
-// warps): four lanes per 32-value block, each lane 8 values per step, UNROLL
-// loads in flight.  Scales of rows in [M, Mpad) and of the columns that pad a
-// row's last tile are written as 0.
-template <typename T, int UNROLL>
+// warps): 32 / VPL lanes per block, UNROLL loads in flight per lane.  The four
+// scales of a 128-value stretch are neighbours in the blocked layout and leave
+// as one word.  Scales of rows in [M, Mpad) and of the columns that pad a row's
+// last tile are written as 0.
+template <typename T, int VPL, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     k_mxfp4_quantize(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
                      uint8_t* __restrict__ q, uint8_t* __restrict__ sf, int64_t Mpad,
                      uint32_t units_per_row, int early) {
   if (early) grid_launch_dependents();
+  constexpr int LPB = BLOCK / VPL;                 // lanes per block
   const int lane = threadIdx.x & 31;
-  const int steps = (int)(K >> 3);                 // 8-value pieces of a row
+  const int k = (int)K;
   const int64_t c4 = sf_tiles(K);
-  const int padded = (int)(c4 * 16);               // pieces up to the padded width
+  const int padded = (int)(c4 * 128);              // values up to the padded width
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
   const int64_t units = Mpad * units_per_row;
-  for (int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < units;
-       w += warps) {
-    const int64_t r = w / units_per_row;
-    const int h0 = (int)(w - r * units_per_row) * (32 * UNROLL);
+  for (int64_t wi = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); wi < units;
+       wi += warps) {
+    const int64_t r = wi / units_per_row;
+    const int v0 = (int)(wi - r * units_per_row) * (32 * VPL * UNROLL) + lane * VPL;
     const bool real = r < M;
     const T* xr = x + r * ldx;
     uint8_t* qr = q + r * (K >> 1);
-    Vec8<T> raw[UNROLL];
+    uint8_t* sr = sf + sf_swizzled_offset(r, 0, c4);
+    Lane<T, VPL> raw[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * 32 + lane;
+      const int v = v0 + u * 32 * VPL;
       raw[u].zero();
-      if (real && h < steps) raw[u].load(xr + (int64_t)h * 8);
+      if (real && v < k) raw[u].load(xr + v);
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * 32 + lane;
-      float v[8];
-      raw[u].get(v);
-      uint32_t m = absmax_bits8(v);
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 1));
-      m = max(m, __shfl_xor_sync(0xffffffffu, m, 2));
+      const int v = v0 + u * 32 * VPL;
+      uint32_t m = raw[u].absmax_bits();
+#pragma unroll
+      for (int o = 1; o < LPB; o *= 2) m = max(m, __shfl_xor_sync(0xffffffffu, m, o));
       const uint32_t s = scale_byte(m);
-      if (real && h < steps)
-        *reinterpret_cast<uint32_t*>(qr + (int64_t)h * 4) = codes8(v, scale_inverse(s));
-      if ((lane & 3) == 0 && h < padded)
-        sf[sf_swizzled_offset(r, h >> 2, c4)] = static_cast<uint8_t>(s);
+      const float inv = scale_inverse(s);
+      uint32_t code[VPL / 8];
+#pragma unroll
+      for (int c = 0; c < VPL / 8; ++c) {
+        code[c] = 0;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          const float2 f = raw[u].get2(c * 4 + i);
+          float a, b;
+          mul_rn_f32x2(f.x, f.y, inv, a, b);
+          code[c] |= f32x2_to_e2m1x2(a, b) << (8 * i);
+        }
+        if (inv == 0.f) code[c] = 0u;              // a NaN block
+      }
+      uint32_t word = s | __shfl_down_sync(0xffffffffu, s, LPB) << 8;
+      word |= __shfl_down_sync(0xffffffffu, word, 2 * LPB) << 16;
+      if (real && v < k) {
+        if constexpr (VPL == 16)
+          *reinterpret_cast<uint2*>(qr + (v >> 1)) = make_uint2(code[0], code[1]);
+        else
+          *reinterpret_cast<uint32_t*>(qr + (v >> 1)) = code[0];
+      }
+      if (lane % (4 * LPB) == 0 && v < padded)
+        *reinterpret_cast<uint32_t*>(sr + (int64_t)(v >> 7) * 512) = word;
     }
   }
 }
 
 // ---------------------------------------------------------------- unpack
-__device__ __forceinline__ void store8(__nv_bfloat16* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) = make_uint4(pack_bf16x2(v[0], v[1]), pack_bf16x2(v[2], v[3]),
-                                            pack_bf16x2(v[4], v[5]), pack_bf16x2(v[6], v[7]));
-}
-__device__ __forceinline__ void store8(__half* p, const float (&v)[8]) {
-  *reinterpret_cast<uint4*>(p) =
-      make_uint4(pack2(v[0], v[1], __half()), pack2(v[2], v[3], __half()),
-                 pack2(v[4], v[5], __half()), pack2(v[6], v[7], __half()));
-}
-__device__ __forceinline__ void store8(float* p, const float (&v)[8]) {
-  *reinterpret_cast<float4*>(p) = make_float4(v[0], v[1], v[2], v[3]);
-  *reinterpret_cast<float4*>(p + 4) = make_float4(v[4], v[5], v[6], v[7]);
-}
-
-// 8 E2M1 codes (4 bytes) times a scale, in fp32 (exact: one significant bit
-// more than the scale's).
-__device__ __forceinline__ void values8(uint32_t codes, float s, float (&v)[8]) {
-  uint32_t hx2[4];
-  asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
-      "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
-      "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
-      : "=r"(hx2[0]), "=r"(hx2[1]), "=r"(hx2[2]), "=r"(hx2[3])
-      : "r"(codes));
-#pragma unroll
-  for (int i = 0; i < 4; ++i) {
-    const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hx2[i]));
-    v[2 * i] = f.x * s;
-    v[2 * i + 1] = f.y * s;
-  }
-}
-
-// Units of UNROLL * 256 values as in the quantizer: lane l takes the 8-value
-// pieces l, l + 32, ... of the unit, all loads in flight.
-template <typename T, int UNROLL>
+// Units as in the quantizer: a lane turns VPL codes into VPL values of T.
+template <typename T, int VPL, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
     k_mxfp4_dequantize(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int64_t M,
                        int64_t K, T* __restrict__ out, int64_t ldo, uint32_t units_per_row) {
   const int lane = threadIdx.x & 31;
-  const int steps = (int)(K >> 3);
+  const int k = (int)K;
   const int64_t c4 = sf_tiles(K);
   const int64_t warps = (int64_t)gridDim.x * (kThreads / 32);
   const int64_t units = M * units_per_row;
-  for (int64_t w = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); w < units;
-       w += warps) {
-    const int64_t r = w / units_per_row;
-    const int h0 = (int)(w - r * units_per_row) * (32 * UNROLL) + lane;
-    const uint32_t* qr = reinterpret_cast<const uint32_t*>(q + r * (K >> 1));
+  for (int64_t wi = (int64_t)blockIdx.x * (kThreads / 32) + (threadIdx.x >> 5); wi < units;
+       wi += warps) {
+    const int64_t r = wi / units_per_row;
+    const int v0 = (int)(wi - r * units_per_row) * (32 * VPL * UNROLL) + lane * VPL;
+    const uint8_t* qr = q + r * (K >> 1);
+    const uint8_t* sr = sf + sf_swizzled_offset(r, 0, c4);
     T* orow = out + r * ldo;
-    uint32_t codes[UNROLL];
+    uint32_t code[UNROLL][VPL / 8];
     uint8_t s[UNROLL];
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * 32;
-      codes[u] = 0;
-      s[u] = 0;
-      if (h < steps) {
-        codes[u] = __ldg(qr + h);
-        s[u] = __ldg(sf + sf_swizzled_offset(r, h >> 2, c4));
+      const int v = v0 + u * 32 * VPL;
+      if (v < k) {
+        if constexpr (VPL == 16) {
+          const uint2 c = __ldg(reinterpret_cast<const uint2*>(qr + (v >> 1)));
+          code[u][0] = c.x;
+          code[u][1] = c.y;
+        } else {
+          code[u][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + (v >> 1)));
+        }
+        s[u] = __ldg(sr + (int64_t)(v >> 7) * 512 + ((v >> 5) & 3));
       }
     }
 #pragma unroll
     for (int u = 0; u < UNROLL; ++u) {
-      const int h = h0 + u * 32;
-      if (h >= steps) break;
-      float v[8];
-      values8(codes[u], scale_value(s[u]), v);
-      store8(orow + (int64_t)h * 8, v);
+      const int v = v0 + u * 32 * VPL;
+      if (v >= k) break;
+      const float sc = scale_value(s[u]);
+      Lane<T, VPL> o;
+#pragma unroll
+      for (int c = 0; c < VPL / 8; ++c) {
+        uint32_t hx2[4];
+        asm("{\n\t.reg .b8 b0, b1, b2, b3;\n\t"
+            "mov.b32 {b0, b1, b2, b3}, %4;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %0, b0;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %1, b1;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %2, b2;\n\t"
+            "cvt.rn.f16x2.e2m1x2 %3, b3;\n\t}"
+            : "=r"(hx2[0]), "=r"(hx2[1]), "=r"(hx2[2]), "=r"(hx2[3])
+            : "r"(code[u][c]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+          // exact in fp32: one significant bit more than the scale's
+          const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&hx2[i]));
+          o.set2(c * 4 + i, f.x * sc, f.y * sc);
+        }
+      }
+      o.store(orow + v);
     }
   }
 }

@@ -153,6 +153,19 @@ def test_quantize_strided_and_batched_inputs(cuda):
         want, s = ref.quantize(r)
         assert torch.equal(ref.values(q, ref.unblock(sf, *r.shape[:1], r.shape[1] // 32)
                                       [:r.shape[0], :r.shape[1] // 32]), want)
+    # rows whose base or stride allows 16-byte accesses but not 32-byte ones
+    for dtype in (BF16, F16, F32):
+        base = rand(7, 24 + 320, seed=3).to(dtype).to(cuda)
+        for view in (base[:, 8:8 + 320], base[:, 24:24 + 288]):
+            q, sf = ops.mxfp4_quantize(view)
+            k = view.shape[1]
+            want, s = ref.quantize(view)
+            assert torch.equal(ref.values(q, ref.unblock(sf, 7, k // 32)[:7, :k // 32]), want)
+            out = torch.full((7, 24 + 320), 3.0, dtype=dtype, device=cuda)
+            back = ops.mxfp4_dequantize(q, sf, 7, k, out=out[:, 8:8 + k])
+            exact = want if dtype == F32 else want.to(dtype).double()
+            assert torch.equal(back.cpu().double(), exact)
+            assert (out[:, :8] == 3).all() and (out[:, 8 + k:] == 3).all()
     q, sf = ops.mxfp4_quantize(wide[:, :0, :64])
     assert q.shape == (0, 32) and sf.numel() == 0
 
