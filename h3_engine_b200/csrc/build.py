@@ -91,7 +91,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
            "-I", str(ROOT / "include"), "-isystem", str(troot / "include"),
            "-isystem", str(cuda / "include"), str(src[0]), "-o", str(tmp),
            "-L", str(PKG), "-lh3b", "-L", str(troot / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
-           "-ltorch", "-Wl,-rpath,$ORIGIN"]
+           "-ltorch_cuda", "-ltorch", "-Wl,-rpath,$ORIGIN"]
     if verbose:
         print(" ".join(cmd), flush=True)
     r = subprocess.run(cmd, capture_output=True, text=True)

@@ -34,7 +34,7 @@ using mxgemm::SF_ATOM;
 constexpr int BN = 128;                       // weight rows per tile
 constexpr int THREADS = 192;                  // producer, MMA, 4 epilogue warps
 constexpr int kMaxRows = 128;
-constexpr int kFusedRows = 16;                // rows that the kernel quantizes itself
+constexpr int kFusedRows = 8;                 // rows that the kernel quantizes itself
 constexpr int kMaxSplit = 8;
 constexpr uint32_t TMEM_COLS = 256;           // two CTAs per SM
 constexpr uint32_t SF_COL = 128;
@@ -124,6 +124,11 @@ __device__ __forceinline__ float4 ld_cluster_f4(uint32_t addr) {
                : "=f"(v.x), "=f"(v.y), "=f"(v.z), "=f"(v.w) : "r"(addr) : "memory");
   return v;
 }
+// Cluster barrier without ordering earlier memory operations.
+__device__ __forceinline__ void cluster_sync_relaxed() {
+  asm volatile("barrier.cluster.arrive.relaxed.aligned;\n\tbarrier.cluster.wait.aligned;" ::
+                   : "memory");
+}
 // Sum over the cluster, in rank order, of the float4 at `addr`; all loads are
 // in flight together.
 __device__ __forceinline__ float4 cluster_sum(uint32_t addr, int ranks) {
@@ -139,7 +144,7 @@ __device__ __forceinline__ float4 cluster_sum(uint32_t addr, int ranks) {
 }
 
 // FUSED: the activation arrives as 16-bit rows and the epilogue warps quantize
-// it into the ring themselves, a k-block per warp in turn (at most 16 rows:
+// it into the ring themselves, a k-block per warp in turn (at most 8 rows:
 // beyond, the CTAs' repeated quantization costs more than a launch of it).
 template <int MT, typename T, int EPI, bool FUSED>
 __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_constant__ Args p) {
@@ -277,9 +282,9 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       for (int i = warp - 2; i < kb1 - kb0; i += 4) {
         const int s = i % R::STAGES, piece = (kb0 + i) * (KB_ELEMS / 8) + lane;
         const bool in_k = piece * 8 < p.K;
-        mx::Vec8<T> raw[MT];
+        mx::Vec8<T> raw[kFusedRows];
 #pragma unroll
-        for (int r = 0; r < MT; ++r) {
+        for (int r = 0; r < kFusedRows; ++r) {
           raw[r].zero();
           if (r < p.M && in_k)
             raw[r].load(static_cast<const T*>(p.x) + (size_t)r * p.ldx + (size_t)piece * 8);
@@ -293,7 +298,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
         uint8_t* xs = sX(s);
         uint8_t* sf = sSFX(s) + (lane >> 4) * SF_ATOM + ((lane >> 2) & 3);
 #pragma unroll
-        for (int r = 0; r < MT; ++r) {
+        for (int r = 0; r < kFusedRows; ++r) {
           if (r < p.M) {
             float v[8];
             raw[r].get(v);
@@ -303,7 +308,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
             const uint32_t sb = mx::scale_byte(m);
             *reinterpret_cast<uint32_t*>(xs + r * 128 + (((lane >> 2) ^ (r & 7)) << 4) +
                                          (lane & 3) * 4) = mx::codes8(v, mx::scale_inverse(sb));
-            if (!(lane & 3)) sf[(r & 31) * 16 + (r >> 5) * 4] = (uint8_t)sb;
+            if (!(lane & 3)) sf[r * 16] = (uint8_t)sb;
           }
         }
         fence_proxy_async_smem();        // the MMA reads them through the async proxy
@@ -340,7 +345,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
     tc_fence_after();
     tmem_dealloc(tmem, TMEM_COLS);
   }
-  cluster_sync_all();                    // every CTA's partial is there
+  if (ranks > 1) cluster_sync_all();     // every CTA's partial is there
   const uint32_t base = smem_u32(smem);
   // (warps 0 and 1 have not waited for the chain's earlier launches: the
   // residual and out are theirs too)
@@ -399,7 +404,9 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       }
     }
   }
-  cluster_sync_all();                    // nobody leaves while its partial is read
+  // nobody leaves while its partial is read; the loads above have returned, and
+  // the results need not be out before the others may go
+  if (ranks > 1) cluster_sync_relaxed();
 }
 
 }  // namespace mxrows

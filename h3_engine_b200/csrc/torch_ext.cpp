@@ -6,6 +6,7 @@
 // its tensors' device.  Only CUDA implementations are registered.  Built as
 // _h3b_torch.so beside libh3b.so, which it links.
 #include <ATen/ATen.h>
+#include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
@@ -70,6 +71,15 @@ Tensor rows2d(const Tensor& t) {
   return r.numel() == 0 || rows_aligned(r) ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 
+// New tensors straight from the caching allocator (no dispatch).
+Tensor new_tensor(at::IntArrayRef shape, at::ScalarType type, const Tensor& like) {
+  return at::detail::empty_cuda(shape, type, like.device(), std::nullopt);
+}
+Tensor scratch(int64_t bytes, const Tensor& like) {
+  return bytes > 0 ? new_tensor({bytes}, at::kByte, like) : Tensor();
+}
+void* ptr(const Tensor& t) { return t.defined() ? t.data_ptr() : nullptr; }
+
 int64_t sf_bytes(int64_t rows, int64_t k) { return (rows + 127) / 128 * ((k + 127) / 128) * 512; }
 
 void check_operand(const Tensor& q, const Tensor& sf, int64_t rows, int64_t k, const char* what) {
@@ -90,7 +100,7 @@ void check_n(int64_t n) {
 Tensor new_out(const Tensor& like, int64_t n, at::ScalarType type) {
   auto shape = like.sizes().vec();
   shape.back() = n;
-  return at::empty(shape, like.options().dtype(type));
+  return new_tensor(shape, type, like);
 }
 
 // The [m, n] view of a caller's output.
@@ -158,8 +168,7 @@ std::tuple<Tensor, Tensor> mxfp4_quantize(const Tensor& x) {
   Call c(x);
   const Tensor x2 = quantize_input(x);
   const int64_t m = x2.size(0), k = x2.size(1);
-  const auto u8 = x.options().dtype(at::kByte);
-  Tensor q = at::empty({m, k / 2}, u8), sf = at::empty({sf_bytes(m, k)}, u8);
+  Tensor q = new_tensor({m, k / 2}, at::kByte, x), sf = new_tensor({sf_bytes(m, k)}, at::kByte, x);
   quantize_into(c, x2, k, q, sf);
   return {q, sf};
 }
@@ -190,7 +199,7 @@ Tensor mxfp4_dequantize(const Tensor& q, const Tensor& sf, int64_t m, int64_t k,
   check_operand(q, sf, m, k, "mxfp4_dequantize");
   TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kHalf || dtype == at::kFloat,
                    "mxfp4_dequantize gives bf16, fp16 or fp32, not ", dtype);
-  Tensor out = at::empty({m, k}, q.options().dtype(dtype));
+  Tensor out = new_tensor({m, k}, dtype, q);
   dequantize_into(c, q, sf, m, k, out);
   return out;
 }
@@ -235,7 +244,7 @@ Tensor mxfp4_gemm(const Tensor& qa, const Tensor& sfa, int64_t m, const Tensor& 
   TORCH_CHECK_TYPE(dtype == at::kBFloat16 || dtype == at::kHalf,
                    "mxfp4_gemm gives bf16 or fp16, not ", dtype);
   const Extras e(bias, residual, m, n, dtype);
-  Tensor out = at::empty({m, n}, qa.options().dtype(dtype));
+  Tensor out = new_tensor({m, n}, dtype, qa);
   gemm_into(c, qa, sfa, m, qb, sfb, n, k, e, act, out);
   return out;
 }
@@ -263,10 +272,10 @@ void linear_into(const Call& c, const Tensor& x2, const Tensor& qb, const Tensor
   const int64_t m = x2.size(0);
   if (m == 0) return;
   const int64_t bytes = h3b_mxfp4_linear_ws(m, n, k);
-  const Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));
+  const Tensor ws = scratch(bytes, x2);
   check(h3b_mxfp4_linear(x2.data_ptr(), dtype_code(x2, false, "mxfp4_linear"), m, x2.stride(0),
                          qb.data_ptr(), sfb.data_ptr(), n, k, e.b, (int)act, e.r, e.ldr,
-                         o.data_ptr(), ldo, ws.data_ptr(), bytes, c.stream()),
+                         o.data_ptr(), ldo, ptr(ws), bytes, c.stream()),
         "h3b_mxfp4_linear");
 }
 
@@ -310,7 +319,7 @@ void ffn_into(const Call& c, const Tensor& x2, const Tensor& qu, const Tensor& s
   const int64_t m = x2.size(0);
   if (m == 0) return;
   const int64_t bytes = h3b_mxfp4_ffn_ws(m, n, f);
-  const Tensor ws = at::empty({bytes}, x2.options().dtype(at::kByte));
+  const Tensor ws = scratch(bytes, x2);
   check(h3b_mxfp4_ffn(x2.data_ptr(), dtype_code(x2, false, "mxfp4_ffn"), m, x2.stride(0),
                       qu.data_ptr(), sfu.data_ptr(), qd.data_ptr(), sfd.data_ptr(), n, f, e.r,
                       e.ldr, o.data_ptr(), ldo, ws.data_ptr(), bytes, c.stream()),
@@ -423,15 +432,14 @@ void window_into(const Call& c, const Packed& p, int64_t heads, int64_t kv_heads
   const int docs = (int)p.qd.start.size();
   const int64_t bytes = h3b_attention_window_ws(p.qd.len.data(), p.kd.len.data(), docs, (int)heads,
                                                 (int)d, r.left, r.right, r.sinks);
-  Tensor ws;
-  if (bytes > 0) ws = at::empty({bytes}, p.q.options().dtype(at::kByte));
+  const Tensor ws = scratch(bytes, p.q);
   check(h3b_attention_window(p.q.data_ptr(), p.q.size(0), p.q.stride(0), p.k.data_ptr(),
                              p.k.stride(0), p.v.data_ptr(), p.v.stride(0), p.k.size(0),
                              dtype_code(p.q, false, "attention"), (int)heads, (int)kv_heads,
                              (int)d, p.qd.start.data(), p.qd.len.data(), p.kd.start.data(),
                              p.kd.len.data(), docs, r.left, r.right, r.sinks, r.causal,
                              (float)r.scale, o.data_ptr(), o.stride(0),
-                             bytes > 0 ? ws.data_ptr() : nullptr, bytes, c.stream()),
+                             ptr(ws), bytes, c.stream()),
         "h3b_attention_window");
 }
 
@@ -443,7 +451,7 @@ Tensor attention_window(const Tensor& q, const Tensor& k, const Tensor& v, int64
   const Rule r{left, right, sinks, causal, scale};
   const Packed p(c, q, k, v, heads, kv_heads, d, cu, cu_k, r);
   // rows of no document read as zeros
-  Tensor out = p.qd.covered == p.q.size(0) ? at::empty({p.q.size(0), heads * d}, q.options())
+  Tensor out = p.qd.covered == p.q.size(0) ? new_tensor({p.q.size(0), heads * d}, q.scalar_type(), q)
                                            : at::zeros({p.q.size(0), heads * d}, q.options());
   window_into(c, p, heads, kv_heads, d, r, out);
   return out;
@@ -503,7 +511,7 @@ Tensor attention_window_decode(const Tensor& q, const Tensor& k, const Tensor& v
                                const Tensor& len, int64_t left, int64_t right, int64_t sinks,
                                bool causal, double scale) {
   Call c(q);
-  Tensor out = at::empty(q.sizes(), q.options());
+  Tensor out = new_tensor(q.sizes(), q.scalar_type(), q);
   decode_into(c, q, k, v, len, Rule{left, right, sinks, causal, scale}, out);
   return out;
 }

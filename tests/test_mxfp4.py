@@ -41,16 +41,19 @@ def test_host_checks_refuse_without_a_gpu():
     assert g(p, p, 4, p, p, 16, 64, odd, 0, None, 0, p, 0, 16, None) == 2
     assert g(p, p, 0, p, p, 16, 64, None, 0, None, 0, p, 0, 16, None) == 0
     lin = lib.h3b_mxfp4_linear
-    need = lib.h3b_mxfp4_linear_ws(4, 16, 64)
-    assert need == 256 + 512                              # codes to 256 bytes, one scale tile
-    assert lin(p, 0, 4, 64, p, p, 16, 64, None, 0, None, 0, p, 16, p, need - 1, None) == 1
-    assert lin(p, 0, 4, 64, p, p, 16, 64, None, 0, None, 0, p, 16, odd, need, None) == 2
+    assert lib.h3b_mxfp4_linear_ws(4, 16, 64) == 0        # few rows need none
+    need = lib.h3b_mxfp4_linear_ws(20, 16, 64)
+    assert need == 768 + 512                              # codes to 256 bytes, one scale tile
+    assert lin(p, 0, 20, 64, p, p, 16, 64, None, 0, None, 0, p, 16, p, need - 1, None) == 1
+    assert lin(p, 0, 20, 64, p, p, 16, 64, None, 0, None, 0, p, 16, odd, need, None) == 2
+    assert lin(p, 0, 20, 32, p, p, 16, 64, None, 0, None, 0, p, 16, p, need, None) == 1   # ldx < K
     f = lib.h3b_mxfp4_ffn
     need = lib.h3b_mxfp4_ffn_ws(4, 64, 128)
     assert need == 2 * (256 + 512)
     assert f(p, 0, 4, 64, p, p, p, p, 64, 192, None, 0, p, 64, p, 1 << 30, None) == 1   # F % 128
     assert f(p, 0, 4, 64, p, p, p, p, 48, 128, None, 0, p, 48, p, 1 << 30, None) == 1   # N % 32
     assert f(p, 0, 4, 64, p, p, p, p, 64, 128, None, 0, p, 64, p, need - 1, None) == 1
+    assert f(odd, 0, 4, 64, p, p, p, p, 64, 128, None, 0, p, 64, p, need, None) == 2
 
 
 def test_cpu_tensors_are_refused():
@@ -172,7 +175,7 @@ def test_quantize_strided_and_batched_inputs(cuda):
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
-@pytest.mark.parametrize("m,n,k", [(1, 8, 32), (2, 264, 96), (16, 128, 256), (17, 520, 160),
+@pytest.mark.parametrize("m,n,k", [(1, 8, 32), (2, 264, 96), (8, 128, 2720), (9, 136, 64), (16, 128, 256), (17, 520, 160),
                                    (33, 128, 2720), (64, 72, 512), (128, 1000, 1088),
                                    (129, 256, 64), (200, 392, 352), (513, 1032, 416)])
 def test_linear_against_64_bits(cuda, dtype, m, n, k):
