@@ -31,9 +31,14 @@ struct Smem {
   static constexpr int STAGE = 2 * TILE;
   static constexpr int WARP = kStages * STAGE;
   static constexpr int RING = kWarps * WARP;
-  // after the pass: per warp and then per CTA 16 x D fp32 plus 16 (max, sum)
-  static constexpr int PART = kRows * D * 4 + kRows * 8;
-  static constexpr int BYTES = RING > kWarps * PART ? RING : kWarps * PART;
+  // after the pass: per warp 16 rows of D (+ 8, which keeps a warp's stores off
+  // one bank) fp32 and 16 (max, sum)
+  static constexpr int PITCH = D + 8;
+  static constexpr int PART = kRows * PITCH * 4 + kRows * 8;
+  // received from the cluster, per rank: its share's elements (float4s) and
+  // every row's (max, sum)
+  static constexpr int RECV = RING > kWarps * PART ? RING : kWarps * PART;
+  static constexpr int BYTES = RECV + kRows * D * 4 + kMaxCluster * 16 + kMaxCluster * kRows * 8;
 };
 
 struct Args {
@@ -78,11 +83,25 @@ __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], 
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
 }
-__device__ __forceinline__ float2 ld_cluster_f2(uint32_t addr) {
-  float2 v;
-  asm volatile("ld.shared::cluster.v2.f32 {%0, %1}, [%2];"
-               : "=f"(v.x), "=f"(v.y) : "r"(addr) : "memory");
-  return v;
+// Asynchronous stores to a CTA of the cluster (addresses from mapa_shared),
+// their bytes counted on that CTA's mbarrier.
+__device__ __forceinline__ void st_async_f4(uint32_t addr, float4 v, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v4.f32 [%0], {%1, %2, %3, %4}, [%5];" ::
+          "r"(addr), "f"(v.x), "f"(v.y), "f"(v.z), "f"(v.w), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void st_async_f2(uint32_t addr, float2 v, uint32_t bar) {
+  asm volatile(
+      "st.async.shared::cluster.mbarrier::complete_tx::bytes.v2.f32 [%0], {%1, %2}, [%3];" ::
+          "r"(addr), "f"(v.x), "f"(v.y), "r"(bar)
+      : "memory");
+}
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
+__device__ __forceinline__ void cluster_wait() {
+  asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory");
 }
 __device__ __forceinline__ uint32_t cluster_nctarank() {
   uint32_t r;
@@ -101,7 +120,7 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   using L = Smem<D>;
   constexpr int CH = D / 8;                       // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t smem[];
-  __shared__ float2 total_ml[kRows];
+  __shared__ __align__(8) uint64_t recv_bar;
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int rank = (int)cluster_ctarank(), ranks = (int)cluster_nctarank();
   const int rows_all = p.n_new * p.group;
@@ -110,6 +129,18 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   const int row0 = (blockIdx.y % row_tiles) * kRows;
   const int rows = min(kRows, rows_all - row0);
   const int b = blockIdx.z;
+  // the cluster's receive barriers exist before anything is sent (waited for
+  // after the pass)
+  const int f4s = rows * (D / 4);                 // the result's float4s; rank r adds up
+  const int share = (f4s + ranks - 1) / ranks;    // [r * share, (r + 1) * share)
+  const int mine = max(0, min(share, f4s - rank * share));
+  if (threadIdx.x == 0) {
+    mbar_init(smem_u32(&recv_bar), 1);
+    fence_mbar_init();
+    mbar_expect_tx(smem_u32(&recv_bar), (uint32_t)(ranks * (mine * 16 + rows * 8)));
+  }
+  __syncthreads();
+  cluster_arrive();
   const int n = min(max(__ldg(p.len + b), 0), p.room);
 
   // keys that any of this tile's rows sees: [0, sink_end) and [lo, end), visited
@@ -159,18 +190,37 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   const uint32_t ring = smem_u32(smem) + warp * L::WARP;
   const int first = rank * kWarps + warp, stride = ranks * kWarps;
 
-  // copy tile i into stage s; keys behind the last are filled with zeros
+  // copy tile i into stage s: a lane's chunk of every 32 / CH-th row; a tile
+  // inside one region advances one pointer per matrix, one that straddles the
+  // sinks' end or the last key (zeros behind it) asks for each row
+  const int ch0 = lane % CH, r0 = lane / CH;
+  constexpr int RPP = 32 / CH;                    // rows per pass
   auto fetch = [&](int i, int s) {
     if (i < tiles) {
+      const int u0 = i * kKeys;
+      const uint32_t st = ring + s * L::STAGE;
+      if (u0 + kKeys <= total && (u0 >= sink_end || u0 + kKeys <= sink_end)) {
+        const long long key = (u0 < sink_end ? u0 : lo + (u0 - sink_end)) + r0;
+        const T* kp = kb + key * p.k_s + ch0 * 8;
+        const T* vp = vb + key * p.v_s + ch0 * 8;
 #pragma unroll
-      for (int c = lane; c < kKeys * CH; c += 32) {
-        const int r = c / CH, ch = c % CH;
-        const int u = i * kKeys + r;
-        const bool ok = u < total;
-        const long long key = !ok ? 0 : u < sink_end ? u : lo + (u - sink_end);
-        const uint32_t dst = ring + s * L::STAGE + r * (D * 2) + ((ch ^ (r & 7)) << 4);
-        cp_async16(dst, kb + key * p.k_s + ch * 8, ok ? 16 : 0);
-        cp_async16(dst + L::TILE, vb + key * p.v_s + ch * 8, ok ? 16 : 0);
+        for (int r = 0; r < kKeys; r += RPP) {
+          const uint32_t dst = st + (r + r0) * (D * 2) + ((ch0 ^ ((r + r0) & 7)) << 4);
+          cp_async16(dst, kp, 16);
+          cp_async16(dst + L::TILE, vp, 16);
+          kp += RPP * p.k_s;
+          vp += RPP * p.v_s;
+        }
+      } else {
+#pragma unroll 1
+        for (int r = r0; r < kKeys; r += RPP) {
+          const int u = u0 + r;
+          const bool ok = u < total;
+          const long long key = !ok ? 0 : u < sink_end ? u : lo + (u - sink_end);
+          const uint32_t dst = st + r * (D * 2) + ((ch0 ^ (r & 7)) << 4);
+          cp_async16(dst, kb + key * p.k_s + ch0 * 8, ok ? 16 : 0);
+          cp_async16(dst + L::TILE, vb + key * p.v_s + ch0 * 8, ok ? 16 : 0);
+        }
       }
     }
     cp_commit();
@@ -186,19 +236,25 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
     cp_wait<L::kStages - 1>();
     __syncwarp();
     const uint32_t ks = ring + s * L::STAGE, vs = ks + L::TILE;
-    float sc[2][4];                               // S of keys 0-7 and 8-15
+    // S of keys 0-7 and 8-15, even and odd k-steps apart: four chains of MMAs
+    float sc[2][4], sd[2][4];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
-      for (int c = 0; c < 4; ++c) sc[j][c] = 0.f;
+      for (int c = 0; c < 4; ++c) sc[j][c] = sd[j][c] = 0.f;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
       // matrices: keys 0-7 dims 0-7, dims 8-15, keys 8-15 dims 0-7, dims 8-15
       const int r = lr + (lm >> 1) * 8, ch = kk * 2 + (lm & 1);
       uint32_t f[4];
       ldsm4(ks + r * (D * 2) + ((ch ^ (r & 7)) << 4), f);
-      mma16816<T>(sc[0], qf[kk], f[0], f[1]);
-      mma16816<T>(sc[1], qf[kk], f[2], f[3]);
+      if (kk & 1) {
+        mma16816<T>(sd[0], qf[kk], f[0], f[1]);
+        mma16816<T>(sd[1], qf[kk], f[2], f[3]);
+      } else {
+        mma16816<T>(sc[0], qf[kk], f[0], f[1]);
+        mma16816<T>(sc[1], qf[kk], f[2], f[3]);
+      }
     }
     // visibility and scaling (log2 units)
     const int u0 = i * kKeys + (lane & 3) * 2;
@@ -212,7 +268,7 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
         const int ps = pos[c >> 1];
         const bool near = key >= ps - p.left && key <= ps + p.right;
         const bool seen = u < total && (near || key < p.sinks) && (!p.causal || key <= ps);
-        sc[j][c] = seen ? sc[j][c] * p.scale_log2 : -INFINITY;
+        sc[j][c] = seen ? (sc[j][c] + sd[j][c]) * p.scale_log2 : -INFINITY;
         mx[c >> 1] = fmaxf(mx[c >> 1], sc[j][c]);
       }
     float al[2], mb[2];
@@ -265,10 +321,10 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   }
   __syncthreads();                                // every warp is done with its ring
 
-  // partials: part w at w * PART: O [16][D] fp32, then 16 (m, l)
+  // partials: part w at w * PART: O [16][PITCH] fp32, then 16 (m, l)
   auto part_o = [&](int w) { return reinterpret_cast<float*>(smem + w * L::PART); };
   auto part_ml = [&](int w) {
-    return reinterpret_cast<float2*>(smem + w * L::PART + kRows * D * 4);
+    return reinterpret_cast<float2*>(smem + w * L::PART + kRows * L::PITCH * 4);
   };
   {
     float* po = part_o(warp);
@@ -276,7 +332,7 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
     for (int d = 0; d < D / 8; ++d)
 #pragma unroll
       for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(po + ((lane >> 2) + 8 * h) * D + d * 8 + (lane & 3) * 2) =
+        *reinterpret_cast<float2*>(po + ((lane >> 2) + 8 * h) * L::PITCH + d * 8 + (lane & 3) * 2) =
             make_float2(o[d][2 * h], o[d][2 * h + 1]);
     if ((lane & 3) == 0) {
 #pragma unroll
@@ -284,10 +340,13 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
         part_ml(warp)[(lane >> 2) + 8 * h] = make_float2(m[h], l[h]);
     }
   }
+  cluster_wait();                                 // the receivers are ready
   __syncthreads();
-  // the CTA's own total, over part 0: each warp's weight per row once, in the
-  // place of its maximum, then the elements
-  if (threadIdx.x < kRows) {
+  // the CTA's own total: each warp's weight per row once, in the place of its
+  // maximum; the row's (max, sum) goes to every rank
+  const uint32_t recv = smem_u32(smem) + L::RECV, bar = smem_u32(&recv_bar);
+  const uint32_t recv_ml = recv + share * ranks * 16;
+  if (threadIdx.x < rows) {
     const int r = threadIdx.x;
     float2 ml[kWarps];
     float mm = -INFINITY, ll = 0.f;
@@ -302,52 +361,50 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
       ll += f * ml[w].y;
       part_ml(w)[r].x = f;
     }
-    total_ml[r] = make_float2(mm, ll);
+    for (int c = 0; c < ranks; ++c)
+      st_async_f2(mapa_shared(recv_ml + (rank * kRows + r) * 8, c), make_float2(mm, ll),
+                  mapa_shared(bar, c));
   }
   __syncthreads();
-  for (int e = threadIdx.x * 4; e < rows * D; e += kThreads * 4) {
+  for (int e = threadIdx.x; e < f4s; e += kThreads) {
+    const int r = e / (D / 4), c4 = e % (D / 4);
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
-      const float f = part_ml(w)[e / D].x;
-      const float4 v = *reinterpret_cast<const float4*>(part_o(w) + e);
+      const float f = part_ml(w)[r].x;
+      const float4 v = *reinterpret_cast<const float4*>(part_o(w) + r * L::PITCH + c4 * 4);
       acc = make_float4(acc.x + f * v.x, acc.y + f * v.y, acc.z + f * v.z, acc.w + f * v.w);
     }
-    *reinterpret_cast<float4*>(part_o(0) + e) = acc;
+    const int to = e / share;
+    st_async_f4(mapa_shared(recv + (rank * share + e - to * share) * 16, to), acc,
+                mapa_shared(bar, to));
   }
-  // the cluster's total: this CTA's share of the rows' elements, every rank's
-  // part in flight at once
-  cluster_sync_all();
-  const uint32_t base = smem_u32(smem), mls = smem_u32(total_ml);
-  for (int e = rank * kThreads + threadIdx.x; e < rows * (D / 2); e += ranks * kThreads) {
-    const int r = e / (D / 2), d = (e % (D / 2)) * 2;
-    float2 ml[kMaxCluster], po[kMaxCluster];
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {
-      ml[c] = make_float2(-INFINITY, 0.f);
-      po[c] = make_float2(0.f, 0.f);
-      if (c < ranks) {
-        ml[c] = ld_cluster_f2(mapa_shared(mls + r * 8, c));
-        po[c] = ld_cluster_f2(mapa_shared(base + (r * D + d) * 4, c));
-      }
-    }
-    float mm = -INFINITY, ll = 0.f, a0 = 0.f, a1 = 0.f;
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) mm = fmaxf(mm, ml[c].x);
-#pragma unroll
-    for (int c = 0; c < kMaxCluster; ++c) {
-      const float f = weight(ml[c].x, mm);
-      ll += f * ml[c].y;
-      a0 += f * po[c].x;
-      a1 += f * po[c].y;
+  // the cluster's total of this rank's share, in rank order
+  if (!mbar_wait(bar, 0, nullptr)) {
+    record_error(H3B_ERR_TIMEOUT);
+    return;
+  }
+  const float4* ro = reinterpret_cast<const float4*>(smem + L::RECV);
+  const float2* rml = reinterpret_cast<const float2*>(smem + L::RECV + share * ranks * 16);
+  for (int i = threadIdx.x; i < mine; i += kThreads) {
+    const int e = rank * share + i, r = e / (D / 4), d = (e % (D / 4)) * 4;
+    float mm = -INFINITY, ll = 0.f;
+    for (int c = 0; c < ranks; ++c) mm = fmaxf(mm, rml[c * kRows + r].x);
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int c = 0; c < ranks; ++c) {
+      const float f = weight(rml[c * kRows + r].x, mm);
+      const float4 v = ro[c * share + i];
+      ll += f * rml[c * kRows + r].y;
+      acc = make_float4(acc.x + f * v.x, acc.y + f * v.y, acc.z + f * v.z, acc.w + f * v.w);
     }
     const int t = (row0 + r) / p.group, g = (row0 + r) % p.group;
     const size_t at = (((size_t)b * p.n_new + t) * p.H + kvh * p.group + g) * D + d;
     const float inv = 1.0f / ll;
-    *reinterpret_cast<uint32_t*>(static_cast<T*>(p.out) + at) =
-        ll != 0.f ? wattn::pack16<T>(a0 * inv, a1 * inv) : 0u;
+    *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) =
+        ll != 0.f ? make_uint2(wattn::pack16<T>(acc.x * inv, acc.y * inv),
+                               wattn::pack16<T>(acc.z * inv, acc.w * inv))
+                  : make_uint2(0u, 0u);
   }
-  cluster_sync_all();                             // nobody leaves while its memory is read
 }
 
 }  // namespace wdec
