@@ -50,12 +50,12 @@ __device__ __forceinline__ void mbar_arrive_cluster_relaxed(uint32_t remote_bar)
                : "memory");
 }
 
-enum Epilogue { kOut = 0, kSwigluQuant = 1 };
+enum Epilogue { kOut = 0, kSwigluQuant = 1, kOutGelu = 2 };
 
 struct Args {
   CUtensorMap tmap_a;      // u8 [M, K/2], box 128 B x 128 rows, 128B swizzle
   CUtensorMap tmap_b;      // u8 [N, K/2], box 128 B x 128 rows, 128B swizzle
-  CUtensorMap tmap_d;      // kOut: 16-bit [M, N] (pitch ldd), box 64 x 32, 128B swizzle
+  CUtensorMap tmap_d;      // kOut(Gelu): 16-bit [M, N] (pitch ldd), box 64 x 32, 128B swizzle
   const uint8_t* sfa;      // blocked scales, M padded to 128 rows
   const uint8_t* sfb;
   const void* bias;        // [N], type of D
@@ -65,7 +65,6 @@ struct Args {
   long long ldr;
   int M, N, K;
   int sf_tiles_k;          // 512-byte scale tiles per 128-row block
-  int act;
   int n_tiles;
   int early;               // the next launch is of the same chain and may start
 };
@@ -75,17 +74,17 @@ __device__ __forceinline__ float2 unpack2(uint32_t w, __half) {
   return __half22float2(*reinterpret_cast<const __half2*>(&w));
 }
 
-// One lane's 8 columns of the plain epilogue: bias, activation, residual.
-// GELU's tanh is tanhf here, not the approximate instruction: fp16 outputs
-// have 11 significant bits.
+// GELU (tanh form) as v * sigmoid(2 u), u = sqrt(2 / pi) (v + 0.044715 v^3):
+// (1 + tanh u) / 2 is sigmoid(2 u), so nothing cancels, and the exponential's
+// relative error (2 + 1.2 |2 u| steps of 2^-23) is all there is.
 __device__ __forceinline__ float gelu_tanh_f32(float v) {
-  const float u = 0.7978845608028654f * fmaf(0.044715f * v, v * v, v);
-  return 0.5f * v * (1.0f + tanhf(u));
+  const float u2 = 1.5957691216057308f * fmaf(0.044715f * v, v * v, v);
+  return __fdividef(v, 1.0f + __expf(-u2));
 }
 
 // Epilogue of one warp's 32 rows x 128 accumulator columns: columns
 // n0 + 128 * half .. of a tile whose rows start at m0.
-template <typename T>
+template <typename T, bool GELU>
 __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc)[128], int m0,
                                              int n0, int half, int qd, int lane, uint8_t* stage,
                                              uint32_t stage_s) {
@@ -115,7 +114,7 @@ __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = add2(v[e], unpack2(bw[e], T()));
       }
-      if (p.act == H3B_ACT_GELU_TANH) {
+      if (GELU) {
 #pragma unroll
         for (int e = 0; e < 4; ++e)
           v[e] = make_float2(gelu_tanh_f32(v[e].x), gelu_tanh_f32(v[e].y));
@@ -429,7 +428,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint32_t i = 0;
     mx::grid_wait();                     // residual and D follow the chain's earlier launches
     if (p.early) mx::grid_launch_dependents();
-    if (EPI == kOut && lane == 0) prefetch_tmap(&p.tmap_d);
+    if (EPI != kSwigluQuant && lane == 0) prefetch_tmap(&p.tmap_d);
     for (int t = pair_id; t < num_tiles; t += num_pairs, ++i) {
       int mt, nt;
       pair_tile(pa, t, mt, nt);
@@ -448,12 +447,12 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
       tc_fence_before();
       __syncwarp();
       if (lane == 0) mbar_arrive_cluster_relaxed(leader_acc_empty);
-      if (EPI == kOut)
-        epilogue_out<T>(p, acc, m0, n0, half, qd, lane, stage, stage_s);
-      else
+      if (EPI == kSwigluQuant)
         epilogue_swiglu_quant(p, acc, m0, n0, half, qd, lane);
+      else
+        epilogue_out<T, EPI == kOutGelu>(p, acc, m0, n0, half, qd, lane, stage, stage_s);
     }
-    if (EPI == kOut && lane == 0) bulk_wait_read0();     // shared memory may go
+    if (EPI != kSwigluQuant && lane == 0) bulk_wait_read0();     // shared memory may go
   }
 
   tc_fence_before();

@@ -289,7 +289,10 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, c
   a.bias = bias;
   a.residual = residual;
   a.ldr = ldr;
-  a.act = act;
+  if (act == H3B_ACT_GELU_TANH)
+    return dtype == H3B_DT_F16
+               ? mx_gemm_launch<__half, mxgemm::kOutGelu>(pa, chained, st)
+               : mx_gemm_launch<__nv_bfloat16, mxgemm::kOutGelu>(pa, chained, st);
   return dtype == H3B_DT_F16 ? mx_gemm_launch<__half, mxgemm::kOut>(pa, chained, st)
                              : mx_gemm_launch<__nv_bfloat16, mxgemm::kOut>(pa, chained, st);
 }

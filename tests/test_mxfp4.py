@@ -196,6 +196,32 @@ def test_linear_against_64_bits(cuda, dtype, m, n, k):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 140])
+def test_activations_saturate(cuda, m):
+    """GELU and the gate far out on both sides: v or 0, never NaN."""
+    k, big = 64, 500.0
+    x = torch.zeros(m, k, dtype=BF16)
+    x[:, 0] = 1
+    rows = torch.tensor([big, -big, 30.0, -30.0, 0.0, 6.0, -6.0, 1.0])   # products, exact
+    w = torch.zeros(8, k)
+    w[:, 0] = rows
+    wv, _ = ref.quantize(w)
+    got = mxfp4.mxfp4_linear(mxfp4.MXFP4Weight(w.to(BF16).to(cuda)), x.to(cuda), act="gelu")
+    want = ref.gelu(wv[:, 0]).expand(m, 8)
+    assert ((got.cpu().double() - want).abs() <= 2.0 ** -8 * want.abs() + 1e-6).all()
+    f, d = 128, 64
+    up = torch.zeros(2 * f, k)
+    up[:f, 0], up[f:, 0] = 1.0, rows.repeat(16)
+    down = torch.eye(d, f)
+    h, dh = ref.swiglu_bounded(torch.ones(1, f).double(), torch.zeros(1, f).double(),
+                               ref.quantize(up[f:])[0][:, 0][None], torch.zeros(1, f).double())
+    hq, far = ref.quantize_bounded(h, dh)
+    got = mxfp4.gated_ffn(mxfp4.gated_up_weight(up.to(BF16).to(cuda)),
+                          mxfp4.MXFP4Weight(down.to(BF16).to(cuda)), x.to(cuda)).cpu().double()
+    assert ((got - hq[:, :d]).abs() <= far[:, :d] + 2.0 ** -8 * hq[:, :d].abs() + 1e-6).all()
+
+
+@pytest.mark.gpu
 def test_gemm_takes_quantized_operands(cuda):
     m, n, k = 150, 136, 224
     x = rand(m, k).to(BF16).to(cuda)
