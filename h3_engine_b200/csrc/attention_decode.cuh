@@ -3,14 +3,19 @@
 // rule of attention_window.cuh for queries at positions len - n_new ... len - 1.
 //
 // Bound by reading the visible keys and values once.  The rows that share a key
-// head, n_new tokens times the group's query heads, form the 16 rows of one
-// mma.sync m16n8k16 tile; a warp's work is a 16-row flash pass over key tiles
-// of kKeys, K and V copied by cp.async into its own ring of stages (no barrier
-// among warps).  A cluster of CTAs along the keys shares a (sequence, key
-// head): tile i belongs to warp i mod (cluster warps), and the partial results
-// (maximum, sum, unnormalised output, all fp32) are joined first in a CTA's
-// shared memory, then across the cluster through distributed shared memory,
-// always in the same order.
+// head, n_new tokens times the group's query heads, are the 8 (or twice 8)
+// columns of mma.sync m16n8k16 products with the keys on the other side:
+// S^T = K Q^T and O^T = V^T P^T, which for up to 8 rows takes half the
+// instructions of the form with 16 rows of queries.  A warp's work is a flash
+// pass over key tiles of 16, K and V copied by cp.async into its own ring of
+// stages (no barrier among warps); all fragments of K, and of V, are asked for
+// before the arithmetic that uses them.  A cluster of CTAs along the keys shares
+// a (sequence, key head): tile i belongs to warp i mod (cluster warps), and the
+// partial results (maximum, sum, unnormalised output, all fp32) are joined first
+// in a CTA's shared memory, then across the cluster: every CTA sends each rank
+// the share of the rows' elements which that rank adds up (st.async, counted on
+// the receiver's mbarrier; a cluster barrier at this place cost about 2000
+// cycles, and another one before the exit), always in the same order.
 #pragma once
 
 #include "attention_window.cuh"
@@ -20,20 +25,22 @@ namespace wdec {
 
 constexpr int kWarps = 4;            // 96 KiB of rings (D = 128): two CTAs per SM
 constexpr int kThreads = kWarps * 32;
-constexpr int kRows = 16;
 constexpr int kKeys = 16;           // keys per tile
 constexpr int kMaxCluster = 8;
 
-template <int D>
+// Rings of three stages: 96 KiB (D = 128), two CTAs per SM.  NT: 8-row columns
+// of the products.
+template <int D, int NT>
 struct Smem {
+  static constexpr int kRows = 8 * NT;
   static constexpr int kStages = 3;
   static constexpr int TILE = kKeys * D * 2;                  // K or V of one stage
   static constexpr int STAGE = 2 * TILE;
   static constexpr int WARP = kStages * STAGE;
   static constexpr int RING = kWarps * WARP;
-  // after the pass: per warp 16 rows of D (+ 8, which keeps a warp's stores off
-  // one bank) fp32 and 16 (max, sum)
-  static constexpr int PITCH = D + 8;
+  // after the pass: per warp the rows of D (+ 4, which spreads a warp's stores
+  // over the banks) fp32 and their (max, sum)
+  static constexpr int PITCH = D + 4;
   static constexpr int PART = kRows * PITCH * 4 + kRows * 8;
   // received from the cluster, per rank: its share's elements (float4s) and
   // every row's (max, sum)
@@ -65,6 +72,12 @@ __device__ __forceinline__ void ldsm4(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
 }
+// Transpose of an 8 x 8 matrix of 16-bit values held two per lane.
+__device__ __forceinline__ uint32_t movm(uint32_t a) {
+  uint32_t d;
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(d) : "r"(a));
+  return d;
+}
 __device__ __forceinline__ void ldsm4_t(uint32_t a, uint32_t (&r)[4]) {
   asm volatile("ldmatrix.sync.aligned.m8n8.x4.trans.shared.b16 {%0,%1,%2,%3}, [%4];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]) : "r"(a) : "memory");
@@ -73,12 +86,12 @@ template <typename T>
 __device__ __forceinline__ void mma16816(float (&d)[4], const uint32_t (&a)[4], uint32_t b0,
                                          uint32_t b1) {
   if constexpr (std::is_same<T, __half>::value)
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0,%1,%2,%3}, "
                  "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
   else
-    asm volatile("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, "
+    asm("mma.sync.aligned.m16n8k16.row.col.f32.bf16.bf16.f32 {%0,%1,%2,%3}, "
                  "{%4,%5,%6,%7}, {%8,%9}, {%0,%1,%2,%3};"
                  : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
                  : "r"(a[0]), "r"(a[1]), "r"(a[2]), "r"(a[3]), "r"(b0), "r"(b1));
@@ -115,9 +128,10 @@ __device__ __forceinline__ float weight(float m, float top) {
   return m == -INFINITY ? 0.f : attn::ex2(m - top);
 }
 
-template <int D, typename T>
+template <int D, typename T, int NT>
 __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constant__ Args p) {
-  using L = Smem<D>;
+  using L = Smem<D, NT>;
+  constexpr int kRows = L::kRows;
   constexpr int CH = D / 8;                       // 16-byte chunks of a row
   extern __shared__ __align__(128) uint8_t smem[];
   __shared__ __align__(8) uint64_t recv_bar;
@@ -159,31 +173,41 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   const int total = sink_end + max(0, end - lo);
   const int tiles = (total + kKeys - 1) / kKeys;
 
-  // Q as A fragments: rows lane / 4 and + 8, dims (lane % 4) * 2 + {0, 1} and + 8
-  uint32_t qf[D / 16][4];
-  int pos[2];                                     // key position of this lane's two rows
+  // Q^T as B fragments: row lane / 4 of each 8, dims (lane % 4) * 2 + {0, 1} and + 8
+  uint32_t qf[D / 16][NT][2];
 #pragma unroll
-  for (int i = 0; i < 2; ++i) {
-    const int r = (lane >> 2) + 8 * i;
+  for (int j = 0; j < NT; ++j) {
+    const int r = j * 8 + (lane >> 2);
     const bool ok = r < rows;
     const int t = (row0 + min(r, rows - 1)) / p.group;
     const int g = (row0 + min(r, rows - 1)) % p.group;
-    pos[i] = n - p.n_new + t;
     const T* q = static_cast<const T*>(p.q) + b * p.q_b + t * p.q_t +
                  (long long)(kvh * p.group + g) * p.q_h + (lane & 3) * 2;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-      qf[kk][i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
-      qf[kk][2 + i] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16 + 8)) : 0u;
+      qf[kk][j][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
+      qf[kk][j][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16 + 8)) : 0u;
     }
   }
-
-  float o[D / 8][4];
+  // this lane's rows in the products: j * 8 + (lane % 4) * 2 + {0, 1}
+  int pos[NT][2];                                 // their key positions
+  float m[NT][2], l[NT][2];
 #pragma unroll
-  for (int i = 0; i < D / 8; ++i)
+  for (int j = 0; j < NT; ++j)
 #pragma unroll
-    for (int c = 0; c < 4; ++c) o[i][c] = 0.f;
-  float m[2] = {-INFINITY, -INFINITY}, l[2] = {0.f, 0.f};
+    for (int h = 0; h < 2; ++h) {
+      const int r = min(j * 8 + (lane & 3) * 2 + h, rows - 1);
+      pos[j][h] = n - p.n_new + (row0 + r) / p.group;
+      m[j][h] = -INFINITY;
+      l[j][h] = 0.f;
+    }
+  float o[D / 16][NT][4];                         // O^T: dims 16 d + lane / 4 and + 8
+#pragma unroll
+  for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
+#pragma unroll
+      for (int c = 0; c < 4; ++c) o[d][j][c] = 0.f;
 
   const T* kb = static_cast<const T*>(p.k) + b * p.k_b + kvh * p.k_h;
   const T* vb = static_cast<const T*>(p.v) + b * p.v_b + kvh * p.v_h;
@@ -232,96 +256,96 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   for (int s = 0; s < L::kStages - 1; ++s) fetch(first + s * stride, s);
   int s = 0;
   for (int i = first; i < tiles; i += stride) {
-    fetch(i + (L::kStages - 1) * stride, (s + L::kStages - 1) % L::kStages);
-    cp_wait<L::kStages - 1>();
+    cp_wait<L::kStages - 2>();
     __syncwarp();
     const uint32_t ks = ring + s * L::STAGE, vs = ks + L::TILE;
-    // S of keys 0-7 and 8-15, even and odd k-steps apart: four chains of MMAs
-    float sc[2][4], sd[2][4];
+    uint32_t f[D / 16][4];
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+    for (int kk = 0; kk < D / 16; ++kk) {
+      // K as A: keys 0-7 and 8-15 of dims 0-7, then of dims 8-15
+      const int r = lr + (lm & 1) * 8, ch = kk * 2 + (lm >> 1);
+      ldsm4(ks + r * (D * 2) + ((ch ^ (r & 7)) << 4), f[kk]);
+    }
+    // into the stage of the last tile, which every lane read before the
+    // __syncwarp above
+    fetch(i + (L::kStages - 1) * stride, (s + L::kStages - 1) % L::kStages);
+    // S^T, even and odd k-steps apart: shorter chains of MMAs
+    float sc[NT][4], sd[NT][4];
+#pragma unroll
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
       for (int c = 0; c < 4; ++c) sc[j][c] = sd[j][c] = 0.f;
 #pragma unroll
-    for (int kk = 0; kk < D / 16; ++kk) {
-      // matrices: keys 0-7 dims 0-7, dims 8-15, keys 8-15 dims 0-7, dims 8-15
-      const int r = lr + (lm >> 1) * 8, ch = kk * 2 + (lm & 1);
-      uint32_t f[4];
-      ldsm4(ks + r * (D * 2) + ((ch ^ (r & 7)) << 4), f);
-      if (kk & 1) {
-        mma16816<T>(sd[0], qf[kk], f[0], f[1]);
-        mma16816<T>(sd[1], qf[kk], f[2], f[3]);
-      } else {
-        mma16816<T>(sc[0], qf[kk], f[0], f[1]);
-        mma16816<T>(sc[1], qf[kk], f[2], f[3]);
-      }
-    }
-    // visibility and scaling (log2 units)
-    const int u0 = i * kKeys + (lane & 3) * 2;
-    float mx[2] = {-INFINITY, -INFINITY};
+    for (int kk = 0; kk < D / 16; ++kk)
 #pragma unroll
-    for (int j = 0; j < 2; ++j)
+      for (int j = 0; j < NT; ++j)
+        mma16816<T>(kk & 1 ? sd[j] : sc[j], f[kk], qf[kk][j][0], qf[kk][j][1]);
+    uint32_t g[D / 16][4];
+#pragma unroll
+    for (int dd = 0; dd < D / 16; ++dd) {
+      // V^T as A: dims 0-7 and 8-15 of keys 0-7, then of keys 8-15
+      const int r = lr + (lm >> 1) * 8, ch = dd * 2 + (lm & 1);
+      ldsm4_t(vs + r * (D * 2) + ((ch ^ (r & 7)) << 4), g[dd]);
+    }
+    // visibility and scaling (log2 units): this lane's keys lane / 4 and + 8
+    const int u0 = i * kKeys + (lane >> 2);
+    uint32_t pf[NT][2];
+    float al[NT][2];
+    bool moved = false;
+#pragma unroll
+    for (int j = 0; j < NT; ++j) {
+      float mx[2] = {-INFINITY, -INFINITY};
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
-        const int u = u0 + j * 8 + (c & 1);
+        const int u = u0 + (c >> 1) * 8;
         const int key = u < sink_end ? u : lo + (u - sink_end);
-        const int ps = pos[c >> 1];
+        const int ps = pos[j][c & 1];
         const bool near = key >= ps - p.left && key <= ps + p.right;
         const bool seen = u < total && (near || key < p.sinks) && (!p.causal || key <= ps);
         sc[j][c] = seen ? (sc[j][c] + sd[j][c]) * p.scale_log2 : -INFINITY;
-        mx[c >> 1] = fmaxf(mx[c >> 1], sc[j][c]);
+        mx[c & 1] = fmaxf(mx[c & 1], sc[j][c]);
       }
-    float al[2], mb[2];
 #pragma unroll
-    for (int h = 0; h < 2; ++h) {
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 1));
-      mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], 2));
-      const float mn = fmaxf(m[h], mx[h]);
-      mb[h] = mn == -INFINITY ? 0.f : mn;
-      al[h] = attn::ex2(m[h] - mb[h]);            // 0 while nothing was seen
-      m[h] = mn;
-    }
-    uint32_t pf[4];
-    float sum[2] = {0.f, 0.f};
+      for (int h = 0; h < 2; ++h) {
 #pragma unroll
-    for (int j = 0; j < 2; ++j) {
-#pragma unroll
-      for (int c = 0; c < 4; ++c) {
-        sc[j][c] = attn::ex2(sc[j][c] - mb[c >> 1]);
-        sum[c >> 1] += sc[j][c];
+        for (int x = 4; x < 32; x *= 2) mx[h] = fmaxf(mx[h], __shfl_xor_sync(0xffffffffu, mx[h], x));
+        const float mn = fmaxf(m[j][h], mx[h]);
+        const float mb = mn == -INFINITY ? 0.f : mn;
+        al[j][h] = attn::ex2(m[j][h] - mb);       // 0 while nothing was seen
+        m[j][h] = mn;
+        moved |= al[j][h] != 1.f;
+        sc[j][h] = attn::ex2(sc[j][h] - mb);
+        sc[j][h + 2] = attn::ex2(sc[j][h + 2] - mb);
+        l[j][h] = l[j][h] * al[j][h] + (sc[j][h] + sc[j][h + 2]);
       }
-      pf[j * 2] = wattn::pack16<T>(sc[j][0], sc[j][1]);
-      pf[j * 2 + 1] = wattn::pack16<T>(sc[j][2], sc[j][3]);
+      // P^T as B: the 8 x 8 halves transposed
+      pf[j][0] = movm(wattn::pack16<T>(sc[j][0], sc[j][1]));
+      pf[j][1] = movm(wattn::pack16<T>(sc[j][2], sc[j][3]));
+    }
+    if (__any_sync(0xffffffffu, moved)) {
+#pragma unroll
+      for (int d = 0; d < D / 16; ++d)
+#pragma unroll
+        for (int j = 0; j < NT; ++j)
+#pragma unroll
+          for (int c = 0; c < 4; ++c) o[d][j][c] *= al[j][c & 1];
     }
 #pragma unroll
-    for (int h = 0; h < 2; ++h) l[h] = l[h] * al[h] + sum[h];
-    if (__any_sync(0xffffffffu, al[0] != 1.f || al[1] != 1.f)) {
+    for (int dd = 0; dd < D / 16; ++dd)
 #pragma unroll
-      for (int d = 0; d < D / 8; ++d)
-#pragma unroll
-        for (int c = 0; c < 4; ++c) o[d][c] *= al[c >> 1];
-    }
-#pragma unroll
-    for (int dd = 0; dd < D / 16; ++dd) {
-      // transposed matrices: keys 0-7 dims 0-7, keys 8-15 dims 0-7, then dims 8-15
-      const int r = lr + (lm & 1) * 8, ch = dd * 2 + (lm >> 1);
-      uint32_t f[4];
-      ldsm4_t(vs + r * (D * 2) + ((ch ^ (r & 7)) << 4), f);
-      mma16816<T>(o[2 * dd], pf, f[0], f[1]);
-      mma16816<T>(o[2 * dd + 1], pf, f[2], f[3]);
-    }
-    __syncwarp();
+      for (int j = 0; j < NT; ++j) mma16816<T>(o[dd][j], g[dd], pf[j][0], pf[j][1]);
     s = (s + 1) % L::kStages;
   }
   cp_wait<0>();
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 1);
-    l[h] += __shfl_xor_sync(0xffffffffu, l[h], 2);
-  }
+  for (int j = 0; j < NT; ++j)
+#pragma unroll
+    for (int h = 0; h < 2; ++h)
+#pragma unroll
+      for (int x = 4; x < 32; x *= 2) l[j][h] += __shfl_xor_sync(0xffffffffu, l[j][h], x);
   __syncthreads();                                // every warp is done with its ring
 
-  // partials: part w at w * PART: O [16][PITCH] fp32, then 16 (m, l)
+  // partials: part w at w * PART: O [rows][PITCH] fp32, then (m, l) per row
   auto part_o = [&](int w) { return reinterpret_cast<float*>(smem + w * L::PART); };
   auto part_ml = [&](int w) {
     return reinterpret_cast<float2*>(smem + w * L::PART + kRows * L::PITCH * 4);
@@ -329,16 +353,17 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   {
     float* po = part_o(warp);
 #pragma unroll
-    for (int d = 0; d < D / 8; ++d)
+    for (int j = 0; j < NT; ++j)
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        *reinterpret_cast<float2*>(po + ((lane >> 2) + 8 * h) * L::PITCH + d * 8 + (lane & 3) * 2) =
-            make_float2(o[d][2 * h], o[d][2 * h + 1]);
-    if ((lane & 3) == 0) {
+      for (int h = 0; h < 2; ++h) {
+        const int r = j * 8 + (lane & 3) * 2 + h;
 #pragma unroll
-      for (int h = 0; h < 2; ++h)
-        part_ml(warp)[(lane >> 2) + 8 * h] = make_float2(m[h], l[h]);
-    }
+        for (int d = 0; d < D / 16; ++d) {
+          po[r * L::PITCH + d * 16 + (lane >> 2)] = o[d][j][h];
+          po[r * L::PITCH + d * 16 + (lane >> 2) + 8] = o[d][j][h + 2];
+        }
+        if (lane < 4) part_ml(warp)[r] = make_float2(m[j][h], l[j][h]);
+      }
   }
   cluster_wait();                                 // the receivers are ready
   __syncthreads();

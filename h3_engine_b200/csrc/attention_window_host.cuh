@@ -104,13 +104,14 @@ static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, f
   return H3B_OK;
 }
 
-template <int D, typename T>
-static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st) {
-  auto kernel = wdec::k_window_decode<D, T>;
+template <int D, typename T, int NT>
+static int window_decode_rows(const wdec::Args& a, int64_t B, cudaStream_t st) {
+  auto kernel = wdec::k_window_decode<D, T, NT>;
+  constexpr int kBytes = wdec::Smem<D, NT>::BYTES;
   static SmemAttr attr;
-  int rc = attr.set(reinterpret_cast<const void*>(kernel), wdec::Smem<D>::BYTES);
+  int rc = attr.set(reinterpret_cast<const void*>(kernel), kBytes);
   if (rc != H3B_OK) return rc;
-  const int64_t row_tiles = ((int64_t)a.n_new * a.group + wdec::kRows - 1) / wdec::kRows;
+  const int64_t row_tiles = ((int64_t)a.n_new * a.group + 8 * NT - 1) / (8 * NT);
   const int64_t groups = row_tiles * a.kv_heads;
   if (groups > 65535 || B > 65535) return H3B_ERR_INVALID_ARG;
   // CTAs along the keys: until there are two per SM, which run at a time (32
@@ -126,7 +127,7 @@ static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st)
   cudaLaunchConfig_t cfg = {};
   cfg.gridDim = dim3((unsigned)split, (unsigned)groups, (unsigned)B);
   cfg.blockDim = dim3(wdec::kThreads);
-  cfg.dynamicSmemBytes = wdec::Smem<D>::BYTES;
+  cfg.dynamicSmemBytes = kBytes;
   cfg.stream = st;
   cudaLaunchAttribute at[1];
   at[0].id = cudaLaunchAttributeClusterDimension;
@@ -136,6 +137,13 @@ static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st)
   cfg.attrs = at;
   cfg.numAttrs = 1;
   return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+}
+
+// Rows that share a key head: 8 of them in one product's columns, more in two.
+template <int D, typename T>
+static int window_decode_launch(const wdec::Args& a, int64_t B, cudaStream_t st) {
+  return (int64_t)a.n_new * a.group <= 8 ? window_decode_rows<D, T, 1>(a, B, st)
+                                         : window_decode_rows<D, T, 2>(a, B, st);
 }
 
 }  // namespace h3b
