@@ -10,11 +10,11 @@
 // One CTA = two 128-row query tiles (A, B) of one head of one document, the
 // roles, TMEM layout and MMA order of attention.cuh.  Of the document's keys it
 // visits only those that some query of the pair sees: the sink keys
-// [0, sink_end) and the window [lo, hi], each in steps of 128 keys that start
+// [0, sink_end) and the window [lo, hi], each in steps of 128 (64) keys that start
 // at 0 and at lo (TMA rows need no alignment, so the first step of the window
 // starts at its first key); the two are one range where they touch.  A step that no query of tile A (or B) sees is skipped for that tile:
 // neither its MMAs nor its softmax run, which is what the window's triangular
-// ends cost least with.  Within a step a row's 128 keys are four words of 32, of
+// ends cost least with.  Within a step a row's keys are words of 32, of
 // which only those that some row of the warp does not see whole are masked.
 //
 // The grid is a number of full waves of items, one CTA per SM, and a last
@@ -38,27 +38,39 @@
 namespace h3b {
 namespace wattn {
 
-constexpr int BQ = 128, BK = 128;
-constexpr int THREADS = 384;
-constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
-static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= THREADS * kLaunchRegs, "register split");
-constexpr uint32_t TMEM_COLS = 512;
+constexpr int BQ = 128;
 constexpr int MAX_DOCS = 64;          // documents per launch
 constexpr int kPrefetchTiles = 4;
 
+// head_dim 128: steps of 128 keys, all of tensor memory, one CTA per SM whose
+// softmax warpgroups get the registers that the control warps give back.
+// head_dim 64: the products are half as long while the softmax is not, and two
+// softmax warps per scheduler leave it idle half the time; steps of 64 keys
+// need half the registers and tensor memory, so two CTAs share an SM.
 template <int D>
-struct Smem {
-  static constexpr int BOX_BYTES = 128 * 128;              // 128 rows x 64 columns
-  static constexpr int TILE_BYTES = (D / 64) * BOX_BYTES;
-  static constexpr int Q_OFF = 0;
-  static constexpr int K_OFF = 2 * TILE_BYTES;
-  static constexpr int V_OFF = K_OFF + 2 * TILE_BYTES;
-  static constexpr int BAR_OFF = V_OFF + 2 * TILE_BYTES;
+struct Cfg {
+  static constexpr int BK = D;                             // keys per step
+  static constexpr int CTAS = D == 128 ? 1 : 2;            // per SM
+  static constexpr int THREADS = D == 128 ? 384 : 320;
+  static constexpr int HALVES = BK / 64;                   // P reaches the MMA 64 keys at a time
+  static constexpr uint32_t TMEM_COLS = 512 / CTAS;
+  static constexpr int Q_BOX = 128 * 128;                  // 128 rows x 64 columns
+  static constexpr int Q_BYTES = (D / 64) * Q_BOX;
+  static constexpr int KV_BOX = BK * 128;
+  static constexpr int KV_BYTES = (D / 64) * KV_BOX;
+  static constexpr int K_OFF = 2 * Q_BYTES;
+  static constexpr int V_OFF = K_OFF + 2 * KV_BYTES;
+  static constexpr int BAR_OFF = V_OFF + 2 * KV_BYTES;
   static constexpr int BYTES = BAR_OFF + 256 + 1024;
+  static __device__ constexpr uint32_t s_col(int t) { return (uint32_t)(t * BK); }   // P over S
+  static __device__ constexpr uint32_t o_col(int t) { return (uint32_t)(2 * BK + t * D); }
 };
+constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
+static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= Cfg<128>::THREADS * kLaunchRegs,
+              "register split");
 
 struct Args {
-  CUtensorMap tmap_q, tmap_k, tmap_v;      // 16-bit [rows, heads * D], box 64 x 128, 128B swizzle
+  CUtensorMap tmap_q, tmap_k, tmap_v;      // 16-bit [rows, heads * D], 64 columns, 128B swizzle
   void* out;                               // [q rows, ldo]; head h at columns h * D
   long long ldo;
   int H, group;                            // query heads; query heads per key head
@@ -86,6 +98,7 @@ struct Range {
 };
 
 // The key steps of a CTA.
+template <int BK>
 struct Steps {
   int n_sink, n, lo, end, sink_end;        // window steps start at lo, end one past the last key
   int first = 0;                           // of this CTA's part; n counts its own
@@ -153,24 +166,45 @@ __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   }
 }
 
-// P = 2^(S * scale - m) of one row's 128 keys, stored as 16-bit pairs over 64
+// Warp-collective load and store of 16 consecutive 32-bit TMEM columns per lane.
+__device__ __forceinline__ void tmem_ld_x16(uint32_t taddr, uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.ld.sync.aligned.32x32b.x16.b32 "
+      "{%0,%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15}, [%16];"
+      : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]), "=r"(r[6]),
+        "=r"(r[7]), "=r"(r[8]), "=r"(r[9]), "=r"(r[10]), "=r"(r[11]), "=r"(r[12]), "=r"(r[13]),
+        "=r"(r[14]), "=r"(r[15])
+      : "r"(taddr));
+}
+__device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[16]) {
+  asm volatile(
+      "tcgen05.st.sync.aligned.32x32b.x16.b32 [%0], "
+      "{%1,%2,%3,%4,%5,%6,%7,%8,%9,%10,%11,%12,%13,%14,%15,%16};" ::"r"(taddr),
+      "r"(r[0]), "r"(r[1]), "r"(r[2]), "r"(r[3]), "r"(r[4]), "r"(r[5]), "r"(r[6]), "r"(r[7]),
+      "r"(r[8]), "r"(r[9]), "r"(r[10]), "r"(r[11]), "r"(r[12]), "r"(r[13]), "r"(r[14]),
+      "r"(r[15])
+      : "memory");
+}
+
+// P = 2^(S * scale - m) of one row's BK keys, stored as 16-bit pairs over BK / 2
 // columns of tensor memory; returns the row sum.  P is rounded to 16 bits
 // because the tensor core reads it so; the sum is of the unrounded fp32 values.
 // 3 of 8 pairs go to the polynomial; a masked key (S = -inf) that falls there
 // gives 2^-120 instead of 0, which no sum of 2^0 or more notices (a row's sum
 // holds its maximum's 2^0, and a row that sees nothing is told by its range).
-template <typename T>
-__device__ __forceinline__ float softmax_store(uint32_t (&sv)[128], float scale_log2, float m,
+template <typename T, int BK>
+__device__ __forceinline__ float softmax_store(uint32_t (&sv)[BK], float scale_log2, float m,
                                                uint32_t p_addr, uint32_t half_bar) {
   const float2 sc = make_float2(scale_log2, scale_log2);
   const float2 nm = make_float2(-m, -m);
   float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
+  constexpr int G = BK == 64 ? 16 : 32;            // pairs packed before a store
 #pragma unroll
-  for (int h = 0; h < 2; ++h) {
-    uint32_t pk[32];
+  for (int h = 0; h < BK / (2 * G); ++h) {
+    uint32_t pk[G];
 #pragma unroll
-    for (int c = 0; c < 32; ++c) {
-      const int k = h * 64 + 2 * c;
+    for (int c = 0; c < G; ++c) {
+      const int k = h * 2 * G + 2 * c;
       const float2 x = fma2(make_float2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc, nm);
       float2 e;
       if ((attn::kPolyPairs >> (c & 7)) & 1u) e = ex2_poly2(x);
@@ -179,8 +213,9 @@ __device__ __forceinline__ float softmax_store(uint32_t (&sv)[128], float scale_
       else acc0 = add2(acc0, e);
       pk[c] = pack16<T>(e.x, e.y);
     }
-    tmem_st_32x32b_x32(p_addr + h * 32, pk);
-    if (h == 0) {
+    if constexpr (G == 16) tmem_st_x16(p_addr + h * G, pk);
+    else tmem_st_32x32b_x32(p_addr + h * G, pk);
+    if (h == 0 && BK > 64) {
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -199,8 +234,10 @@ __device__ __forceinline__ uint32_t span_word(int a, int b, int w) {
 }
 
 template <int D, typename T>
-__global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constant__ Args p) {
-  using L = Smem<D>;
+__global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
+    k_window_attn(const __grid_constant__ Args p) {
+  using L = Cfg<D>;
+  constexpr int BK = L::BK;
   // kind::f16: D fp32 (bit 4), A and B bf16 (bits 7, 10) or fp16 (0)
   constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t IDESC_QK =
@@ -208,11 +245,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   // P V: B = V is MN-major (head dim contiguous): bit 16
   constexpr uint32_t IDESC_PV =
       (1u << 4) | kType | (1u << 16) | ((uint32_t)(D >> 3) << 17) | ((uint32_t)(BQ >> 4) << 24);
-
-  // head_dim 64 leaves 128 columns of tensor memory, which hold P apart from S:
-  // S(j + 1) is then computed under the exponentials of step j.
-  constexpr bool SEP = D == 64;
-  auto p_col = [](int t) { return SEP ? 320u + (uint32_t)t * 128u : attn::s_col(t); };
 
   extern __shared__ uint8_t smem_raw[];
   uint8_t* smem = reinterpret_cast<uint8_t*>((reinterpret_cast<uintptr_t>(smem_raw) + 1023) &
@@ -226,10 +258,9 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   uint64_t* kv_empty = bars + 3;     // 2
   uint64_t* s_full = bars + 5;       // 2 (tile A, B)
   uint64_t* p_full = bars + 7;       // 2
-  uint64_t* pv_done = bars + 9;      // 2: the last PV of a tile (SEP: every PV)
+  uint64_t* pv_done = bars + 9;      // 2: the last PV of a tile
   uint64_t* drain = bars + 11;       // 1
-  uint64_t* p_half = bars + 12;      // 2
-  uint64_t* s_free = bars + 14;      // 2 (SEP): S has been read
+  uint64_t* p_half = bars + 12;      // 2: P of the first 64 keys of 128
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -251,7 +282,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   const int k_row = p.k_start[doc];
   const int pos0 = qp * 2 * BQ + n_k - n_q;               // position of tile A's first row
   const int rows = min(2 * BQ, n_q - qp * 2 * BQ);        // queries of this pair
-  Steps st(Range(p, n_k, pos0, pos0 + rows - 1));
+  Steps<BK> st(Range(p, n_k, pos0, pos0 + rows - 1));
   if (!whole) st.take(part, p.parts);
   // what each tile sees; a tile without queries sees nothing
   auto tile_range = [&](int t) {
@@ -266,10 +297,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   };
 
   const int qx = head * D, kx = (head / p.group) * D;
-  auto load = [&](uint8_t* dst, const CUtensorMap* map, int x, int y, uint32_t bar) {
+  auto load = [&](uint8_t* dst, int box, const CUtensorMap* map, int x, int y, uint32_t bar) {
 #pragma unroll
     for (int b = 0; b < D / 64; ++b)
-      tma_load_2d(smem_u32(dst + b * L::BOX_BYTES), map, x + b * 64, y, bar);
+      tma_load_2d(smem_u32(dst + b * box), map, x + b * 64, y, bar);
   };
   if (warp == 8 && lane == 0) {
     mbar_init(smem_u32(q_full), 1);
@@ -280,7 +311,6 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       mbar_init(smem_u32(&p_full[i]), 4);
       mbar_init(smem_u32(&p_half[i]), 4);
       mbar_init(smem_u32(&pv_done[i]), 1);
-      mbar_init(smem_u32(&s_free[i]), 4);
     }
     mbar_init(smem_u32(drain), 1);
     *abort_flag = 0;
@@ -288,14 +318,14 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
     if (st.n > 0) {
       // the first loads run while tensor memory is allocated
       const uint32_t qb = smem_u32(q_full);
-      mbar_expect_tx(qb, 3 * L::TILE_BYTES);
-      load(smem + L::Q_OFF, &p.tmap_q, qx, q_row, qb);
-      load(smem + L::K_OFF, &p.tmap_k, kx, k_row + st.base(0), qb);
-      load(smem + L::Q_OFF + L::TILE_BYTES, &p.tmap_q, qx, q_row + BQ, qb);
+      mbar_expect_tx(qb, 2 * L::Q_BYTES + L::KV_BYTES);
+      load(smem, L::Q_BOX, &p.tmap_q, qx, q_row, qb);
+      load(smem + L::K_OFF, L::KV_BOX, &p.tmap_k, kx, k_row + st.base(0), qb);
+      load(smem + L::Q_BYTES, L::Q_BOX, &p.tmap_q, qx, q_row + BQ, qb);
     }
   }
   if (warp == 9) {
-    tmem_alloc(smem_u32(tmem_slot), TMEM_COLS);
+    tmem_alloc(smem_u32(tmem_slot), L::TMEM_COLS);
     tmem_relinquish();
   }
   tc_fence_before();
@@ -313,7 +343,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
   // Each warpgroup changes its register limit inside its own branch and leaves
   // through its own copy of the teardown barrier.
   if (warp >= 8) {
-    asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
     if (warp == 8) {
       if (lane == 0 && st.n > 0) {
         auto prefetch = [&](int j) {
@@ -343,10 +373,11 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
           }
           const bool more = j + 1 < st.n;
           const uint32_t b = smem_u32(&kv_full[j & 1]);
-          mbar_expect_tx(b, more ? 2 * L::TILE_BYTES : L::TILE_BYTES);
-          load(smem + L::V_OFF + (j & 1) * L::TILE_BYTES, &p.tmap_v, kx, k_row + st.base(j), b);
+          mbar_expect_tx(b, more ? 2 * L::KV_BYTES : L::KV_BYTES);
+          load(smem + L::V_OFF + (j & 1) * L::KV_BYTES, L::KV_BOX, &p.tmap_v, kx,
+               k_row + st.base(j), b);
           if (more)
-            load(smem + L::K_OFF + ((j + 1) & 1) * L::TILE_BYTES, &p.tmap_k, kx,
+            load(smem + L::K_OFF + ((j + 1) & 1) * L::KV_BYTES, L::KV_BOX, &p.tmap_k, kx,
                  k_row + st.base(j + 1), b);
           ++issued;
         }
@@ -370,33 +401,33 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       }
       auto need = [&](int t, int j) { return st.needed(t ? rb : ra, j); };
       auto issue_qk = [&](int t, int j) {
-        const uint64_t qd = desc_kmajor_sw128(smem_u32(smem + L::Q_OFF + t * L::TILE_BYTES));
-        const uint64_t kd = desc_kmajor_sw128(smem_u32(smem + L::K_OFF + (j & 1) * L::TILE_BYTES));
+        const uint64_t qd = desc_kmajor_sw128(smem_u32(smem + t * L::Q_BYTES));
+        const uint64_t kd = desc_kmajor_sw128(smem_u32(smem + L::K_OFF + (j & 1) * L::KV_BYTES));
 #pragma unroll
-        for (int kk = 0; kk < D / 16; ++kk) {
-          const uint32_t off = ((kk >> 2) * L::BOX_BYTES + (kk & 3) * 32) >> 4;   // 16 head dims
-          tc_mma_bf16_ss_elect(tmem + attn::s_col(t), qd + off, kd + off, IDESC_QK, kk != 0);
-        }
+        for (int kk = 0; kk < D / 16; ++kk)                // 16 head dims each
+          tc_mma_bf16_ss_elect(tmem + L::s_col(t), qd + (((kk >> 2) * L::Q_BOX + (kk & 3) * 32) >> 4),
+                               kd + (((kk >> 2) * L::KV_BOX + (kk & 3) * 32) >> 4), IDESC_QK,
+                               kk != 0);
         tc_commit_elect(smem_u32(&s_full[t]));
       };
       int cnt[2] = {0, 0};                                 // needed steps done per tile
       auto pv_tile = [&](int t, int j) -> bool {
         // 16 keys per MMA: P columns kk * 8.. (pairs), V rows kk * 16.. (MN-major:
-        // 64-dim chunks 16 KiB apart, 8-row groups 1 KiB)
-        const uint64_t vd = smem_desc(smem_u32(smem + L::V_OFF + (j & 1) * L::TILE_BYTES),
-                                      L::BOX_BYTES, 1024, 2);
+        // 64-dim chunks a box apart, 8-row groups 1 KiB)
+        const uint64_t vd = smem_desc(smem_u32(smem + L::V_OFF + (j & 1) * L::KV_BYTES),
+                                      L::KV_BOX, 1024, 2);
 #pragma unroll
-        for (int h = 0; h < 2; ++h) {
-          if (!wait(h ? &p_full[t] : &p_half[t], cnt[t] & 1)) return false;
+        for (int h = 0; h < L::HALVES; ++h) {
+          if (!wait(h == L::HALVES - 1 ? &p_full[t] : &p_half[t], cnt[t] & 1)) return false;
           tc_fence_after();
 #pragma unroll
           for (int i = 0; i < 4; ++i) {
             const int kk = h * 4 + i;
-            tc_mma_bf16_ts_elect(tmem + attn::o_col(t), tmem + p_col(t) + kk * 8,
+            tc_mma_bf16_ts_elect(tmem + L::o_col(t), tmem + L::s_col(t) + kk * 8,
                                  vd + kk * (2048 >> 4), IDESC_PV, (cnt[t] | kk) != 0);
           }
         }
-        if (SEP || j == last[t]) tc_commit_elect(smem_u32(&pv_done[t]));
+        if (j == last[t]) tc_commit_elect(smem_u32(&pv_done[t]));
         ++cnt[t];
         return true;
       };
@@ -416,37 +447,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
         const int valid = st.valid(j);
         if (valid < BK) {
           // V rows that no query sees: 8 chunks of 16 bytes per row and box
-          uint8_t* v = smem + L::V_OFF + (j & 1) * L::TILE_BYTES;
+          uint8_t* v = smem + L::V_OFF + (j & 1) * L::KV_BYTES;
           for (int c = lane + valid * 8; c < BK * 8; c += 32) {
 #pragma unroll
             for (int b = 0; b < D / 64; ++b)
-              *reinterpret_cast<uint4*>(v + b * L::BOX_BYTES + c * 16) = make_uint4(0, 0, 0, 0);
+              *reinterpret_cast<uint4*>(v + b * L::KV_BOX + c * 16) = make_uint4(0, 0, 0, 0);
           }
           fence_proxy_async_smem();
           __syncwarp();
         }
-        if (SEP) {
-#pragma unroll
-          for (int t = 0; t < 2; ++t) {
-            if (!(more && need(t, j + 1))) continue;
-            // S of the tile's latest step has been read (none yet: nothing to wait for)
-            const int read = cnt[t] + (need(t, j) ? 1 : 0);
-            if (read > 0 && !wait(&s_free[t], (read - 1) & 1)) {
-              ok = false;
-              break;
-            }
-            tc_fence_after();
-            issue_qk(t, j + 1);
-          }
-        }
 #pragma unroll
         for (int t = 0; t < 2; ++t) {
-          if (!ok) break;
           if (need(t, j) && !pv_tile(t, j)) {
             ok = false;
             break;
           }
-          if (!SEP && more && need(t, j + 1)) issue_qk(t, j + 1);
+          if (more && need(t, j + 1)) issue_qk(t, j + 1);
         }
         if (ok) tc_commit_elect(smem_u32(&kv_empty[j & 1]));
       }
@@ -457,22 +473,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       }
     }
     tc_fence_before();
-    named_barrier_sync(1, THREADS);
+    named_barrier_sync(1, L::THREADS);
     if (warp == 9) {
       __syncwarp();
       tc_fence_after();
-      tmem_dealloc(tmem, TMEM_COLS);
+      tmem_dealloc(tmem, L::TMEM_COLS);
     }
   } else {
-    asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
+    if constexpr (D == 128)
+      asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // softmax of tile t: thread = query row (TMEM lane quadrant warp % 4)
     const int t = warp >> 2;
     const int qd = warp & 3;
     const int r = qd * 32 + lane;
     const uint32_t lane_addr = (uint32_t)(qd * 32) << 16;
-    const uint32_t s_t = tmem + lane_addr + attn::s_col(t);
-    const uint32_t o_t = tmem + lane_addr + attn::o_col(t);
-    const uint32_t p_t = tmem + lane_addr + p_col(t);
+    const uint32_t s_t = tmem + lane_addr + L::s_col(t);
+    const uint32_t o_t = tmem + lane_addr + L::o_col(t);
     const Range rt = tile_range(t);
     const int pos = pos0 + t * BQ + r;                    // this row's key position
     const int w_first = pos0 + t * BQ + qd * 32;          // first and last position of the warp
@@ -487,15 +503,10 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&s_full[t]), cnt & 1, abort_flag));
       if (!ok) break;
       tc_fence_after();
-      uint32_t sv[128];
-      tmem_ld_32x32b_x64(s_t, sv);
-      tmem_ld_32x32b_x64(s_t + 64, sv + 64);
+      uint32_t sv[BK];
+#pragma unroll
+      for (int h = 0; h < BK / 64; ++h) tmem_ld_32x32b_x64(s_t + h * 64, sv + h * 64);
       tmem_ld_wait();
-      if (SEP) {
-        tc_fence_before();
-        __syncwarp();
-        if (lane == 0) mbar_arrive(smem_u32(&s_free[t]));
-      }
       const int base = st.base(j), valid = st.valid(j);
       const bool all_seen =                               // warp-uniform
           valid == BK && base + BK - 1 <= w_top &&
@@ -505,7 +516,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
         const int b = min(min(pos + p.right, top) - base, valid - 1);
         const int s = min(min(p.sinks - 1, top) - base, valid - 1);
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
+        for (int w = 0; w < BK / 32; ++w) {
           const uint32_t seen = span_word(a, b, w) | span_word(0, s, w);
           if (!__all_sync(0xffffffffu, seen == 0xffffffffu)) {
 #pragma unroll
@@ -517,7 +528,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       // row max of the scaled logits (scale > 0 commutes with max)
       float m4[4] = {-INFINITY, -INFINITY, -INFINITY, -INFINITY};
 #pragma unroll
-      for (int c = 0; c < 128; c += 8) {
+      for (int c = 0; c < BK; c += 8) {
 #pragma unroll
         for (int u = 0; u < 4; ++u)
           m4[u] = attn::max3(m4[u], __uint_as_float(sv[c + 2 * u]), __uint_as_float(sv[c + 2 * u + 1]));
@@ -531,28 +542,22 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
         alpha = m_new == -INFINITY ? 1.f : attn::ex2(m_used - m_new);
         m_used = m_new;
       }
-      if (SEP && cnt > 0) {
-        // the previous PV has read its P and written O
-        ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), (cnt - 1) & 1, abort_flag));
-        if (!ok) break;
-        tc_fence_after();
-      }
       if (rescale && cnt > 0) {
-        // O is final up to the previous needed step (without SEP: s_full of this
-        // one was committed after its PV)
+        // O is final up to the previous needed step: s_full of this one was
+        // committed after its PV
 #pragma unroll
-        for (int h = 0; h < D / 32; ++h) {
-          uint32_t ov[32];
-          tmem_ld_32x32b_x32(o_t + h * 32, ov);
+        for (int h = 0; h < D / 16; ++h) {                 // 16 at a time: S is in registers
+          uint32_t ov[16];
+          tmem_ld_x16(o_t + h * 16, ov);
           tmem_ld_wait();
 #pragma unroll
-          for (int c = 0; c < 32; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-          tmem_st_32x32b_x32(o_t + h * 32, ov);
+          for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+          tmem_st_x16(o_t + h * 16, ov);
         }
       }
       const uint32_t hb = smem_u32(&p_half[t]);
       const float m = m_used == -INFINITY ? 0.f : m_used;   // -inf - (-inf) is no exponent
-      l = l * alpha + softmax_store<T>(sv, p.scale_log2, m, p_t, hb);
+      l = l * alpha + softmax_store<T, BK>(sv, p.scale_log2, m, s_t, hb);
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();
@@ -560,8 +565,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       ++cnt;
     }
     if (ok && cnt > 0)
-      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), SEP ? (cnt - 1) & 1 : 0,
-                                             abort_flag));
+      ok = __all_sync(0xffffffffu, mbar_wait(smem_u32(&pv_done[t]), 0, abort_flag));
     if (!ok) fail();
     tc_fence_after();
     const int row = t * BQ + r;                            // of the pair's 256
@@ -572,7 +576,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
     // warp's 32 rows at a time: written a row per lane, 16-byte chunk c of row r
     // at chunk c ^ (r % 8), and copied out whole rows at a time.
     constexpr int CH = D / 8;                              // 16-byte chunks of a row
-    uint4* const ostage = reinterpret_cast<uint4*>(smem + L::Q_OFF + t * L::TILE_BYTES) + qd * 32 * CH;
+    uint4* const ostage = reinterpret_cast<uint4*>(smem + t * L::Q_BYTES) + qd * 32 * CH;
     auto stage = [&](int h, const uint32_t (&ov)[32], float inv_l) {
 #pragma unroll
       for (int c = 0; c < 4; ++c) {
@@ -690,7 +694,7 @@ __global__ void __launch_bounds__(THREADS, 1) k_window_attn(const __grid_constan
       }
     }
     tc_fence_before();
-    named_barrier_sync(1, THREADS);
+    named_barrier_sync(1, L::THREADS);
   }
 }
 

@@ -12,12 +12,12 @@ constexpr int64_t kMaxKeys = (int64_t)1 << 30;    // positions plus a window sta
 static inline int clamp_window(int64_t v) { return (int)std::min<int64_t>(v, kMaxKeys - 1); }
 
 static int tmap_16_rows(CUtensorMap* tm, const void* base, int dtype, int64_t rows, int64_t cols,
-                        int64_t stride) {
+                        int64_t stride, uint32_t box_rows) {
   auto fn = encode_fn();
   if (!fn) return H3B_ERR_UNSUPPORTED;
   cuuint64_t dims[2] = {(cuuint64_t)cols, (cuuint64_t)rows};
   cuuint64_t strides[1] = {(cuuint64_t)stride * 2};
-  cuuint32_t box[2] = {64, wattn::BK};
+  cuuint32_t box[2] = {64, box_rows};
   cuuint32_t estr[2] = {1, 1};
   return fn(tm, dtype == H3B_DT_F16 ? CU_TENSOR_MAP_DATA_TYPE_FLOAT16
                                     : CU_TENSOR_MAP_DATA_TYPE_BFLOAT16,
@@ -33,33 +33,35 @@ static int window_attn_launch(const wattn::Args& a, int64_t grid, cudaStream_t s
   auto kernel = wattn::k_window_attn<D, T>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   static SmemAttr attr;
-  int rc = attr.set(fn, wattn::Smem<D>::BYTES);
+  int rc = attr.set(fn, wattn::Cfg<D>::BYTES);
   if (rc != H3B_OK) return rc;
-  // the kernel's setmaxnreg split draws on this many launch registers
-  static std::atomic<int> regs{0};
-  if (!regs.load(std::memory_order_relaxed)) {
-    cudaFuncAttributes fa;
-    if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) return H3B_ERR_CUDA;
-    regs.store(fa.numRegs, std::memory_order_relaxed);
+  if (D == 128) {
+    // the kernel's setmaxnreg split draws on this many launch registers
+    static std::atomic<int> regs{0};
+    if (!regs.load(std::memory_order_relaxed)) {
+      cudaFuncAttributes fa;
+      if (cudaFuncGetAttributes(&fa, fn) != cudaSuccess) return H3B_ERR_CUDA;
+      regs.store(fa.numRegs, std::memory_order_relaxed);
+    }
+    if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
   }
-  if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
-  kernel<<<(unsigned)grid, wattn::THREADS, wattn::Smem<D>::BYTES, st>>>(a);
+  kernel<<<(unsigned)grid, wattn::Cfg<D>::THREADS, wattn::Cfg<D>::BYTES, st>>>(a);
   return launched(cudaGetLastError());
 }
 
 // Whole items first, then the last partial wave's items in parts: of `items`
-// CTAs of about equal length on `sms` SMs, items mod sms would run alone, so
-// they are split to fill the SMs (8 heads of 16384 rows, 512 items: 252 us
-// unsplit, see the kernel).  A part should keep four steps or more.
+// CTAs of about equal length in `slots` places, items mod slots would run alone,
+// so they are split to fill the places (8 heads of 16384 rows, 512 items on 148
+// SMs: 221 us, unsplit 235).  A part should keep 512 keys or more.
 struct WindowPlan {
   int whole, parts;
-  WindowPlan(int64_t items, int64_t steps) {
-    const int sms = num_sms();
-    const int rest = (int)(items % sms);
+  WindowPlan(int64_t items, int64_t keys, int D) {
+    const int slots = num_sms() * (D == 128 ? wattn::Cfg<128>::CTAS : wattn::Cfg<64>::CTAS);
+    const int rest = (int)(items % slots);
     whole = (int)items;
     parts = 1;
-    static const char* ns = getenv("NOSPLIT"); if (rest == 0 || ns) return;
-    const int64_t p = std::min<int64_t>(sms / rest, steps / 4);
+    if (rest == 0) return;
+    const int64_t p = std::min<int64_t>(slots / rest, keys / 512);
     if (p < 2) return;
     whole = (int)(items - rest);
     parts = (int)p;
@@ -68,10 +70,9 @@ struct WindowPlan {
   int64_t grid(int64_t items) const { return whole + split(items) * parts; }
 };
 
-// Key steps of a query-tile pair in a document of n_k keys under a window.
-static int64_t window_steps(int64_t n_k, int64_t left, int64_t right, int64_t sinks) {
-  const int64_t span = std::min<int64_t>(n_k, left + right + 2 * wattn::BQ);
-  return (span + wattn::BK - 1) / wattn::BK + (std::min(sinks, n_k) + wattn::BK - 1) / wattn::BK;
+// Keys that a query-tile pair of a document of n_k keys visits under a window.
+static int64_t window_keys(int64_t n_k, int64_t left, int64_t right, int64_t sinks) {
+  return std::min<int64_t>(n_k, left + right + 2 * wattn::BQ + sinks);
 }
 
 // One launch's documents: up to MAX_DOCS with queries, those with the most keys
@@ -79,7 +80,7 @@ static int64_t window_steps(int64_t n_k, int64_t left, int64_t right, int64_t si
 struct WindowDocs {
   int order[wattn::MAX_DOCS];
   int n = 0, next = 0;
-  int64_t items = 0, steps = 0;
+  int64_t items = 0, keys = 0;              // keys: of the lightest document's pairs
   WindowDocs(const int32_t* q_len, const int32_t* k_len, int ndocs, int d0, int H, int64_t left,
              int64_t right, int64_t sinks) {
     for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0) {
@@ -91,12 +92,12 @@ struct WindowDocs {
     std::sort(order, order + n, [&](int a, int b) {
       return k_len[a] != k_len[b] ? k_len[a] > k_len[b] : a < b;
     });
-    if (n > 0) steps = window_steps(k_len[order[n - 1]], left, right, sinks);
+    if (n > 0) keys = window_keys(k_len[order[n - 1]], left, right, sinks);
   }
 };
 
 static int64_t window_part_bytes(int D) { return ((int64_t)256 * D + 512) * 4; }
-static constexpr int64_t kDoneBytes = 1024;       // a counter per split item (fewer than SMs)
+static constexpr int64_t kDoneBytes = 2048;       // a counter per split item (fewer than slots)
 
 static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, float scale) {
   if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f))
@@ -159,7 +160,7 @@ int64_t h3b_attention_window_ws(const int32_t* q_len, const int32_t* k_len, int 
   for (int d0 = 0; d0 < ndocs;) {
     const WindowDocs docs(q_len, k_len, ndocs, d0, H, left, right, sinks);
     d0 = docs.next;
-    const WindowPlan plan(docs.items, docs.steps);
+    const WindowPlan plan(docs.items, docs.keys, D);
     const int64_t split = plan.split(docs.items);
     if (split > 0)
       most = std::max(most, kDoneBytes + split * plan.parts * window_part_bytes(D));
@@ -201,12 +202,12 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
 
   wattn::Args a;
   memset(&a, 0, sizeof(a));
-  rc = tmap_16_rows(&a.tmap_q, q, dtype, q_rows, hd, q_stride);
+  rc = tmap_16_rows(&a.tmap_q, q, dtype, q_rows, hd, q_stride, wattn::BQ);
   if (rc != H3B_OK) return rc;
   if (keys > 0) {
-    rc = tmap_16_rows(&a.tmap_k, k, dtype, kv_rows, kd, k_stride);
+    rc = tmap_16_rows(&a.tmap_k, k, dtype, kv_rows, kd, k_stride, (uint32_t)D);
     if (rc != H3B_OK) return rc;
-    rc = tmap_16_rows(&a.tmap_v, v, dtype, kv_rows, kd, v_stride);
+    rc = tmap_16_rows(&a.tmap_v, v, dtype, kv_rows, kd, v_stride, (uint32_t)D);
     if (rc != H3B_OK) return rc;
   }
   a.out = out;
@@ -244,7 +245,7 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
       a.item_end[i] = (int)items;
     }
     a.ndocs = docs.n;
-    const WindowPlan plan(items, docs.steps);
+    const WindowPlan plan(items, docs.keys, D);
     a.whole = plan.whole;
     a.parts = plan.parts;
     const int64_t grid = plan.grid(items);
