@@ -16,7 +16,9 @@ residual (h3_inference/transformer/model.py:81-106,191-198).  With a
 ``SequenceShard`` the block runs on this rank's token rows: the projection
 writes Q locally and K|V straight into this rank's rows of the full-sequence
 K|V buffer, one in-place NCCL all-gather completes it, and attention reads
-local queries against all keys.
+local queries against all keys.  With a ``window`` (and ``sinks``) each token
+attends to its neighbourhood and the document's first tokens only
+(``ops.attention_window``).
 
 ``DiTBlock`` -- attention then FFN with the six adaLN-zero tables (shift /
 scale / gate per half), gathered per token by ``mod_idx``.
@@ -148,6 +150,21 @@ class FFNBlock(_GemmTimer):
         return y.reshape(shape)
 
 
+def window_pairs(n: int, window: tuple | None, sinks: int = 0, causal: bool = False) -> int:
+    """(query, key) pairs that attention over a document of n tokens computes."""
+    if window is None:
+        return n * n
+    left, right = (n if v is None else min(int(v), n) for v in window)
+    if causal:
+        right = 0
+    i = torch.arange(n)
+    lo, hi = (i - left).clamp(min=0), (i + right).clamp(max=n - 1)
+    seen = hi - lo + 1
+    first = torch.minimum(lo, torch.full_like(lo, min(sinks, n)))     # sinks left of the window
+    past = (min(sinks, n) - 1 - hi).clamp(min=0)                      # and right of it
+    return int((seen + first + (0 if causal else past)).sum())
+
+
 @dataclass
 class SequenceShard:
     """This rank's slice ``[row0, row0 + rows)`` of a token-sharded sequence of
@@ -180,7 +197,11 @@ class AttnBlock(_GemmTimer):
     def __init__(self, wq: torch.Tensor, wk: torch.Tensor, wv: torch.Tensor, wo: torch.Tensor,
                  gamma: torch.Tensor, norm_q: torch.Tensor | None, norm_k: torch.Tensor | None,
                  heads: int, eps: float = 1e-6, qk_eps: float = 1e-6,
-                 bo: torch.Tensor | None = None, workspace: dict | None = None):
+                 bo: torch.Tensor | None = None, workspace: dict | None = None,
+                 window: tuple | None = None, sinks: int = 0, causal: bool = False):
+        if window is None and (sinks or causal):
+            raise ValueError("sinks and causal belong to a windowed block")
+        self.window, self.sinks, self.causal = window, sinks, causal
         ws = [NVFP4Weight(w) for w in (wq, wk, wv)]
         self.heads = heads
         self.inner = ws[0].out_features
@@ -202,7 +223,8 @@ class AttnBlock(_GemmTimer):
     def flops(self, tokens: int, cu_seqlens) -> dict:
         hd, d = self.inner, self.hidden
         cu = list(cu_seqlens)
-        attn = sum(4 * hd * (b - a) ** 2 for a, b in zip(cu[:-1], cu[1:]))
+        attn = sum(4 * hd * window_pairs(b - a, self.window, self.sinks, self.causal)
+                   for a, b in zip(cu[:-1], cu[1:]))
         return {"nvfp4": 2 * tokens * d * 3 * hd + 2 * tokens * hd * d, "attention": attn}
 
     def _sf_rows(self, r0: int, r1: int) -> torch.Tensor:
@@ -301,6 +323,8 @@ class AttnBlock(_GemmTimer):
         HD, H, D = self.inner, self.heads, self.head_dim
         dev = x.device
         split = shard is not None and shard.all_gather is not None
+        if split and self.window is not None:
+            raise NotImplementedError("windowed attention runs on whole sequences, not on shards")
         ws = self._ws.setdefault(("attn", T, self.hidden, self.inner, dev, split), {"norm": {}})
         cos, sin = rope if rope is not None else (None, None)
         hook = None if shard is None else shard.reduce_max
@@ -315,8 +339,12 @@ class AttnBlock(_GemmTimer):
             ops.qk_norm_rope(qkv, H, D, q_off=0, k_off=HD, wq=self.norm_q, wk=self.norm_k,
                              eps=self.qk_eps, cos=cos, sin=sin)
             ev = self._event(sink=self.attn_events)
-            o = ops.attention_varlen(qkv, H, D, cu_seqlens, q_off=0, k_off=HD, v_off=2 * HD,
-                                     out=_buf(ws, "o", (T, HD), torch.bfloat16, dev))
+            o = _buf(ws, "o", (T, HD), torch.bfloat16, dev)
+            if self.window is None:
+                ops.attention_varlen(qkv, H, D, cu_seqlens, q_off=0, k_off=HD, v_off=2 * HD, out=o)
+            else:
+                ops.attention_window(*qkv.split(HD, 1), H, D, cu_seqlens, window=self.window,
+                                     sinks=self.sinks, causal=self.causal, out=o)
             self._event(ev, sink=self.attn_events)
         else:
             if shard.rows != T:

@@ -6,6 +6,7 @@
 // its tensors' device.  Only CUDA implementations are registered.  Built as
 // _h3b_torch.so beside libh3b.so, which it links.
 #include <ATen/ATen.h>
+#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -103,6 +104,18 @@ Tensor new_out(const Tensor& like, int64_t n, at::ScalarType type) {
   return new_tensor(shape, type, like);
 }
 
+// An output may be one of its inputs where every element is read before it is
+// written by the same thread (exact), and shares no memory with the others.
+void apart(const Tensor& out, const Tensor& in, bool exact_ok, const char* what) {
+  const auto s = at::get_overlap_status(out, in);
+  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Partial &&
+                        (exact_ok || s != at::MemOverlapStatus::Full),
+                    "out shares memory with ", what);
+}
+void apart(const Tensor& out, const optional<Tensor>& in, bool exact_ok, const char* what) {
+  if (in) apart(out, *in, exact_ok, what);
+}
+
 // The [m, n] view of a caller's output.
 Tensor out_rows(const Tensor& out, at::IntArrayRef lead, int64_t m, int64_t n,
                 at::ScalarType type) {
@@ -179,6 +192,9 @@ void mxfp4_quantize_out(const Tensor& x, Tensor q, Tensor sf) {
   c.same(sf);
   const Tensor x2 = quantize_input(x);
   check_operand(q, sf, x2.size(0), x2.size(1), "mxfp4_quantize");
+  apart(q, x, false, "x");
+  apart(sf, x, false, "x");
+  apart(sf, q, false, "the codes");
   q.unsafeGetTensorImpl()->bump_version();
   sf.unsafeGetTensorImpl()->bump_version();
   quantize_into(c, x2, x2.size(1), q, sf);
@@ -209,6 +225,8 @@ void mxfp4_dequantize_out(const Tensor& q, const Tensor& sf, int64_t m, int64_t 
   c.same(sf);
   c.same(out);
   check_operand(q, sf, m, k, "mxfp4_dequantize");
+  apart(out, q, false, "the codes");
+  apart(out, sf, false, "the scales");
   dequantize_into(c, q, sf, m, k, out_rows(out, {m}, m, k, out.scalar_type()));
 }
 
@@ -256,6 +274,9 @@ void mxfp4_gemm_out(const Tensor& qa, const Tensor& sfa, int64_t m, const Tensor
   gemm_checks(c, sfa, qa, m, qb, sfb, n, k, bias, act, residual);
   c.same(out);
   dtype_code(out, false, "mxfp4_gemm");
+  apart(out, qa, false, "A");
+  apart(out, residual, true, "the residual");
+  apart(out, bias, false, "the bias");
   const Extras e(bias, residual, m, n, out.scalar_type());
   gemm_into(c, qa, sfa, m, qb, sfb, n, k, e, act, out_rows(out, {m}, m, n, out.scalar_type()));
 }
@@ -307,6 +328,9 @@ void mxfp4_linear_out(const Tensor& x, const Tensor& qb, const Tensor& sfb, int6
   Call c(x);
   linear_checks(c, qb, sfb, n, k, bias, act, residual);
   c.same(out);
+  apart(out, x, false, "x");
+  apart(out, residual, true, "the residual");
+  apart(out, bias, false, "the bias");
   const Tensor x2 = product_input(x, k);
   const Extras e(bias, residual, x2.size(0), n, x.scalar_type());
   const Tensor o = out_rows(out, x.sizes().slice(0, x.dim() - 1), x2.size(0), n, x.scalar_type());
@@ -356,6 +380,8 @@ void mxfp4_ffn_out(const Tensor& x, const Tensor& qu, const Tensor& sfu, const T
   Call c(x);
   ffn_checks(c, qu, sfu, qd, sfd, n, f, residual);
   c.same(out);
+  apart(out, x, true, "x");
+  apart(out, residual, true, "the residual");
   const Tensor x2 = product_input(x, n);
   const Extras e(std::nullopt, residual, x2.size(0), n, x.scalar_type());
   const Tensor o = out_rows(out, x.sizes().slice(0, x.dim() - 1), x2.size(0), n, x.scalar_type());
@@ -466,6 +492,9 @@ void attention_window_out(const Tensor& q, const Tensor& k, const Tensor& v, int
   const Rule r{left, right, sinks, causal, scale};
   const Packed p(c, q, k, v, heads, kv_heads, d, cu, cu_k, r);
   const int64_t rows = p.q.size(0);
+  apart(out, q, true, "q");
+  apart(out, k, false, "k");
+  apart(out, v, false, "v");
   window_into(c, p, heads, kv_heads, d, r,
               out_rows(out, {rows}, rows, heads * d, q.scalar_type()));
 }
@@ -521,6 +550,9 @@ void attention_window_decode_out(const Tensor& q, const Tensor& k, const Tensor&
                                  bool causal, double scale, Tensor out) {
   Call c(q);
   c.same(out);
+  apart(out, q, true, "q");
+  apart(out, k, false, "k");
+  apart(out, v, false, "v");
   decode_into(c, q, k, v, len, Rule{left, right, sinks, causal, scale}, out);
   out.unsafeGetTensorImpl()->bump_version();
 }

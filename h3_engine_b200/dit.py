@@ -27,7 +27,7 @@ import torch
 import torch.distributed as dist
 
 from . import ops
-from .blocks import AttnBlock, DiTBlock, FFNBlock
+from .blocks import AttnBlock, DiTBlock, FFNBlock, window_pairs
 from .nvfp4 import NVFP4Weight
 from .parallel import ParallelLayout
 from .rope import packed_positions, rope_tables
@@ -47,6 +47,8 @@ class DiTConfig:
     video_grid: tuple[int, int, int] = (21, 30, 52)
     audio_tokens: int = 1024
     guidance: float = 5.0
+    window: tuple | None = None      # (left, right) tokens that attention sees; None: all
+    sinks: int = 0                   # first tokens of a document that every token sees
 
     @property
     def tokens(self) -> int:
@@ -61,7 +63,8 @@ class DiTConfig:
         """FLOPs of one model evaluation of one CFG branch."""
         T, d, f, hd = self.tokens, self.hidden, self.ffn, self.heads * self.head_dim
         cu = self.cu_seqlens()
-        attn = sum(4 * hd * (b - a) ** 2 for a, b in zip(cu[:-1], cu[1:]))
+        attn = sum(4 * hd * window_pairs(b - a, self.window, self.sinks)
+                   for a, b in zip(cu[:-1], cu[1:]))
         gemm = 2 * T * d * (3 * hd) + 2 * T * hd * d + 4 * T * d * f
         return {"nvfp4": self.blocks * gemm, "attention": self.blocks * attn}
 
@@ -116,7 +119,8 @@ class RandomDiT:
         for _ in range(cfg.blocks):
             attn = AttnBlock(w(HD, d), w(HD, d), w(HD, d), w(d, HD), vec(d, 1.0, 0.1),
                              vec(cfg.head_dim, 1.0, 0.1), vec(cfg.head_dim, 1.0, 0.1), cfg.heads,
-                             eps=cfg.eps, qk_eps=cfg.eps, workspace=self.workspace)
+                             eps=cfg.eps, qk_eps=cfg.eps, workspace=self.workspace,
+                             window=cfg.window, sinks=cfg.sinks)
             ffn = FFNBlock(w(f, d), vec(f), w(d, f), vec(d), vec(d, 1.0, 0.1), eps=cfg.eps,
                            workspace=self.workspace)
             self.blocks.append(DiTBlock(attn, ffn))

@@ -15,7 +15,9 @@ Same functions, signatures and env flags as the reference:
 "Quantized" means the linears carry an NVFP4 weight: this library's
 ``nvfp4._QuantLinear`` (``quantize_blocks`` / ``load_quantized``) or the
 reference's own quantized linear (same packed format, read with global
-scale 1); other linears take the reference's stock path.
+scale 1); or an MXFP4 one, ``mxfp4.MXFP4Linear`` (``mxfp4.quantize_blocks``),
+whose feed-forward never holds its hidden activation in 16 bits.  Other linears
+take the reference's stock path.
 """
 from __future__ import annotations
 
@@ -26,15 +28,19 @@ from h3_engine_b200.kernels._dispatch import MISS, enabled, note_miss
 
 
 def qkv_kernel(to_q, to_k, to_v, x: torch.Tensor):
-    from h3_engine_b200 import nvfp4
+    from h3_engine_b200 import mxfp4, nvfp4
     if not x.is_cuda:
         return MISS
     out = nvfp4.shared_qkv(to_q, to_k, to_v, x)
+    if out is None:
+        out = mxfp4.shared_qkv(to_q, to_k, to_v, x)
     return MISS if out is None else out
 
 
 def out_kernel(to_out, x: torch.Tensor):
-    from h3_engine_b200 import nvfp4
+    from h3_engine_b200 import mxfp4, nvfp4
+    if x.is_cuda and isinstance(to_out, mxfp4.MXFP4Linear) and x.dtype in mxfp4.DTYPES:
+        return to_out(x)
     if not (x.is_cuda and nvfp4._is_quant_linear(to_out)):
         return MISS
     if isinstance(to_out, nvfp4._QuantLinear):
@@ -62,17 +68,23 @@ def _swiglu_weight(lin):
 
 
 def ffn_kernel(ff: nn.Module, x: torch.Tensor):
-    """``net.2(value * silu(gate))`` with ``value | gate = net.0.proj(x)`` in NVFP4, or MISS."""
-    from h3_engine_b200 import nvfp4, ops
+    """``net.2(value * silu(gate))`` with ``value | gate = net.0.proj(x)`` in NVFP4 or MXFP4,
+    or MISS."""
+    from h3_engine_b200 import mxfp4, nvfp4, ops
     net = getattr(ff, "net", None)
-    if net is None or len(net) != 3 or not x.is_cuda or x.dtype != torch.bfloat16:
+    if net is None or len(net) != 3 or not x.is_cuda:
         return MISS
     gate_mod, down = net[0], net[2]
     up = getattr(gate_mod, "proj", None)
     act_fn = getattr(gate_mod, "activation", None)
-    if not (nvfp4._is_quant_linear(up) and nvfp4._is_quant_linear(down)):
-        return MISS
     if act_fn is not None and not isinstance(act_fn, nn.SiLU):
+        return MISS
+    if isinstance(up, mxfp4.MXFP4Linear) and isinstance(down, mxfp4.MXFP4Linear):
+        out = mxfp4.linear_ffn(up, down, x)
+        return MISS if out is None else out
+    if x.dtype != torch.bfloat16:
+        return MISS
+    if not (nvfp4._is_quant_linear(up) and nvfp4._is_quant_linear(down)):
         return MISS
     f = up.out_features // 2
     # the GEMMs take K in whole 256-element k-blocks; the SwiGLU epilogue

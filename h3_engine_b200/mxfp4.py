@@ -13,9 +13,10 @@ import torch
 from torch import nn
 
 from . import ops
-from .nvfp4 import _block_linears, _set_child
+from .nvfp4 import _block_linears, _set_child, _swizzle, _unswizzle
 
 MXFP4_BLOCK = ops.MX_BLOCK
+DTYPES = (torch.bfloat16, torch.float16)      # of activations and results
 
 _ACTS = {None: ops.ACT_NONE, "gelu": ops.ACT_GELU_TANH}
 
@@ -90,9 +91,47 @@ class MXFP4Linear(nn.Module):
         self.in_features, self.out_features = linear.in_features, linear.out_features
         self.bias = None if linear.bias is None else nn.Parameter(linear.bias.data,
                                                                   requires_grad=False)
+        self._fused = self._gated = None      # laid out once: shared_qkv, linear_ffn
 
     def forward(self, x: torch.Tensor) -> torch.Tensor:
         return mxfp4_linear(self.weight_mxfp4, x, bias=self.bias)
+
+
+def shared_qkv(to_q, to_k, to_v, x: torch.Tensor):
+    """q, k and v projections from one quantization of ``x`` as one product over
+    the weights concatenated along N (kept on ``to_q``): None unless all three
+    are ``MXFP4Linear`` of one input width, without bias, with output widths in
+    whole 128-row scale tiles, and ``x`` is of a type they take."""
+    mods = (to_q, to_k, to_v)
+    if not all(isinstance(m, MXFP4Linear) and m.bias is None and m.out_features % 128 == 0
+               and m.in_features == to_q.in_features for m in mods) or x.dtype not in DTYPES:
+        return None
+    ws = tuple(m.weight_mxfp4 for m in mods)
+    cached = to_q._fused
+    if cached is None or any(a is not b for a, b in zip(cached[0], ws)):
+        w = MXFP4Weight.from_packed(torch.cat([w.qdata for w in ws]),
+                                    torch.cat([w.scale for w in ws]),
+                                    sum(w.out_features for w in ws), to_q.in_features)
+        cached = to_q._fused = (ws, w)
+    return mxfp4_linear(cached[1], x).split([w.out_features for w in ws], -1)
+
+
+def linear_ffn(up: "MXFP4Linear", down: "MXFP4Linear", x: torch.Tensor):
+    """``gated_ffn`` of a feed-forward's two linears, ``up`` the fused
+    [value | gate] projection in the reference's chunk order (its rows are
+    reordered once and kept on ``up``): None if ``gated_ffn`` does not take them."""
+    f = down.in_features
+    if (up.bias is not None or down.bias is not None or f % 128 or up.out_features != 2 * f
+            or down.out_features != up.in_features or x.dtype not in DTYPES):
+        return None
+    w = up.weight_mxfp4
+    if up._gated is None or up._gated[0] is not w:
+        perm = ops.swiglu_rows(f).to(w.qdata.device)
+        sf = _unswizzle(w.scale, 2 * f, w.in_features // MXFP4_BLOCK)[perm]
+        up._gated = (w, MXFP4Weight.from_packed(w.qdata[perm].contiguous(),
+                                                _swizzle(sf.contiguous()).view(torch.uint8),
+                                                2 * f, w.in_features))
+    return gated_ffn(up._gated[1], down.weight_mxfp4, x)
 
 
 @torch.no_grad()
