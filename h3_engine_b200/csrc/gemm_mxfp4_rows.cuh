@@ -1,5 +1,6 @@
-// MXFP4 product for up to 128 rows of activations (single tokens, text and
-// conditioning rows), where reading the weight once is the bound.
+// MXFP4 product for few rows of activations (single tokens, text and
+// conditioning rows), where reading the weight once is the bound: up to 128, or a
+// few tiles of 128.
 //
 // The operands change places: the weight's 128-row tiles are the MMA's M side
 // and the MT (16 ... 128) activation rows its N side, so every byte that
@@ -33,7 +34,7 @@ using mxgemm::SF_ATOM;
 
 constexpr int BN = 128;                       // weight rows per tile
 constexpr int THREADS = 192;                  // producer, MMA, 4 epilogue warps
-constexpr int kMaxRows = 128;
+constexpr int kMaxRows = 128;                 // of one tile
 constexpr int kFusedRows = 8;                 // rows that the kernel quantizes itself
 constexpr int kMaxSplit = 8;
 constexpr uint32_t TMEM_COLS = 256;           // two CTAs per SM
@@ -163,6 +164,8 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const int ranks = (int)gridDim.x, rank = (int)blockIdx.x;   // the cluster spans grid x
   const int n0 = (int)blockIdx.y * BN;
+  const int m0 = (int)blockIdx.z * MT;         // first row of this tile of activations
+  const int rows = min(MT, p.M - m0);
   const int num_kb = (p.K + KB_ELEMS - 1) / KB_ELEMS;
   const int kb0 = (int)((long long)num_kb * rank / ranks);
   const int kb1 = (int)((long long)num_kb * (rank + 1) / ranks);
@@ -205,6 +208,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
         return (uint32_t)min(KB_ATOMS, p.sf_tiles_k - kb * KB_ATOMS) * SF_ATOM;
       };
       const uint8_t* sfw = p.sfw + (size_t)blockIdx.y * p.sf_tiles_k * SF_ATOM;
+      const uint8_t* sfx = p.sfx + (size_t)blockIdx.z * p.sf_tiles_k * SF_ATOM;   // z > 0: MT 128
       auto load_w = [&](int kb, int s) {
         const uint32_t fb = smem_u32(&full[s]);
         mbar_expect_tx(fb, R::W_BYTES + sf_bytes(kb) + (FUSED ? 0 : R::X_BYTES + sf_bytes(kb)));
@@ -214,8 +218,8 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       auto load_x = [&](int kb, int s) {
         if (FUSED) return;
         const uint32_t fb = smem_u32(&full[s]);
-        tma_load_2d(smem_u32(sX(s)), &p.tmap_x, kb * KB_BYTES, 0, fb);
-        bulk_load(smem_u32(sSFX(s)), p.sfx + (size_t)kb * KB_ATOMS * SF_ATOM, sf_bytes(kb), fb);
+        tma_load_2d(smem_u32(sX(s)), &p.tmap_x, kb * KB_BYTES, m0, fb);
+        bulk_load(smem_u32(sSFX(s)), sfx + (size_t)kb * KB_ATOMS * SF_ATOM, sf_bytes(kb), fb);
       };
       const int n = kb1 - kb0, head = min(n, R::STAGES);
       for (int i = 0; i < head; ++i) load_w(kb0 + i, i);
@@ -326,13 +330,13 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       tc_fence_after();
 #pragma unroll
       for (int c = 0; c < MT; c += 16) {
-        if (c < p.M) {
+        if (c < rows) {
           uint32_t acc[16];
           tmem_ld_x16(tmem + ((uint32_t)(qd * 32) << 16) + c, acc);
           tmem_ld_wait();
 #pragma unroll
           for (int i = 0; i < 16; ++i)
-            if (c + i < p.M) part[(c + i) * BN + qd * 32 + lane] = __uint_as_float(acc[i]);
+            if (c + i < rows) part[(c + i) * BN + qd * 32 + lane] = __uint_as_float(acc[i]);
         }
       }
     } else {
@@ -357,17 +361,17 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
     if (n < p.N) {                       // N % 8 == 0: all four or none
       float4 b = make_float4(0.f, 0.f, 0.f, 0.f);
       if (p.bias) b = load4(static_cast<const T*>(p.bias) + n);
-      for (int m = rank * (THREADS / 32) + warp; m < p.M; m += ranks * (THREADS / 32)) {
+      for (int m = rank * (THREADS / 32) + warp; m < rows; m += ranks * (THREADS / 32)) {
         float4 v = cluster_sum(base + (m * BN + c) * 4, ranks);
         v = make_float4(v.x + b.x, v.y + b.y, v.z + b.z, v.w + b.w);
         if (p.act == H3B_ACT_GELU_TANH)
           v = make_float4(mxgemm::gelu_tanh_f32(v.x), mxgemm::gelu_tanh_f32(v.y),
                           mxgemm::gelu_tanh_f32(v.z), mxgemm::gelu_tanh_f32(v.w));
         if (residual) {
-          const float4 r = load4(residual + (size_t)m * p.ldr + n);
+          const float4 r = load4(residual + (size_t)(m0 + m) * p.ldr + n);
           v = make_float4(v.x + r.x, v.y + r.y, v.z + r.z, v.w + r.w);
         }
-        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)m * p.ldd + n) =
+        *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + (size_t)(m0 + m) * p.ldd + n) =
             make_uint2(mx::pack2(v.x, v.y, T()), mx::pack2(v.z, v.w, T()));
       }
     }
@@ -376,11 +380,11 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
     // cover a row's 64 hidden columns, eight of them one 32-value block
     const int c = (threadIdx.x & 15) * 4;
     const int F = p.N >> 1, f = (n0 >> 1) + c;
-    const int rows = THREADS / 16;       // per pass; all lanes of a warp stay in the loop
-    for (int m0 = rank * rows; m0 < p.M; m0 += ranks * rows) {
-      const int m = m0 + (int)(threadIdx.x >> 4);
+    const int pass = THREADS / 16;       // rows; all lanes of a warp stay in the loop
+    for (int i = rank * pass; i < rows; i += ranks * pass) {
+      const int m = i + (int)(threadIdx.x >> 4);
       float h[4] = {0.f, 0.f, 0.f, 0.f};
-      if (m < p.M) {
+      if (m < rows) {
         const float4 v = cluster_sum(base + (m * BN + c) * 4, ranks);
         const float4 g = cluster_sum(base + (m * BN + 64 + c) * 4, ranks);
         h[0] = mxgemm::swiglu_f32(v.x, g.x);
@@ -397,10 +401,10 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       const float inv = mx::scale_inverse(s);
       const uint32_t code = f32x2_to_e2m1x2(h[0] * inv, h[1] * inv) |
                             f32x2_to_e2m1x2(h[2] * inv, h[3] * inv) << 8;
-      if (m < p.M) {
-        *reinterpret_cast<uint16_t*>(p.q_out + (size_t)m * (F >> 1) + (f >> 1)) =
+      if (m < rows) {
+        *reinterpret_cast<uint16_t*>(p.q_out + (size_t)(m0 + m) * (F >> 1) + (f >> 1)) =
             (uint16_t)(inv != 0.f ? code : 0u);
-        if (!(threadIdx.x & 7)) p.sf_out[sf_swizzled_offset(m, f >> 5, F >> 7)] = (uint8_t)s;
+        if (!(threadIdx.x & 7)) p.sf_out[sf_swizzled_offset(m0 + m, f >> 5, F >> 7)] = (uint8_t)s;
       }
     }
   }

@@ -187,11 +187,12 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
   // each (1 x 7168 x 5376: 10.2 us on one, 8.4 on two, 8.0 on four; 77 x 4136 x
   // 2720: 12.6, 10.6, 9.6 and, with one k-block each on eight, 10.8)
   int split = 1;
-  while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles <= 2 * num_sms() &&
+  const int m_tiles = (a.M + MT - 1) / MT;      // more than one only for MT = 128
+  while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles * m_tiles <= 2 * num_sms() &&
          num_kb >= split * 4)
     split *= 2;
   cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split, (unsigned)tiles, 1);
+  cfg.gridDim = dim3((unsigned)split, (unsigned)tiles, (unsigned)m_tiles);
   cfg.blockDim = dim3(mxrows::THREADS);
   cfg.dynamicSmemBytes = mxrows::Ring<MT>::BYTES;
   cfg.stream = st;
@@ -258,6 +259,17 @@ static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* 
   return H3B_OK;
 }
 
+// Which kernel: the rows kernel up to 128 rows, and beyond them in tiles of 128
+// where the pair kernel would leave most SMs idle over a long K: where three
+// CTAs along K find room for each of its tiles (144 x 2048 x 5376: 12.0 us
+// against 15.0, 512 x 2048 x 5376: 13.4 and 15.2, 256 x 5376 x 14336: 22.8 and
+// 28.7; past that 512 x 5376 x 14336: 35.0 and 30.0; with K = 2048 the pair
+// kernel is ahead, 256 x 5376: 12.3 and 10.7).
+static bool mx_by_rows(int64_t M, int64_t N, int64_t K) {
+  return M <= mxrows::kMaxRows ||
+         (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms());
+}
+
 // D = act(A B^T + bias) + residual.  sfA NULL (M <= kFusedRows): A is 16-bit
 // rows of stride ldx.  chained: the launch before is of the same entry point.
 static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, const void* B,
@@ -265,7 +277,7 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, c
                        const void* residual, int64_t ldr, void* D, int dtype, int64_t ldd,
                        bool chained, cudaStream_t st) {
   ldr = residual ? ldr : 0;
-  if (M <= mxrows::kMaxRows) {
+  if (mx_by_rows(M, N, K)) {
     mxrows::Args a;
     memset(&a, 0, sizeof(a));
     a.bias = bias;
@@ -395,7 +407,7 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
     rc = mx_quantize(x, dtype, M, N, ldx, q, sf, true, st);
     if (rc != H3B_OK) return rc;
   }
-  if (M <= mxrows::kMaxRows) {
+  if (mx_by_rows(M, 2 * F, N)) {
     mxrows::Args a;
     memset(&a, 0, sizeof(a));
     a.q_out = qh;

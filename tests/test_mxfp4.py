@@ -177,7 +177,8 @@ def test_quantize_strided_and_batched_inputs(cuda):
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("m,n,k", [(1, 8, 32), (2, 264, 96), (8, 128, 2720), (9, 136, 64), (16, 128, 256), (17, 520, 160),
                                    (33, 128, 2720), (64, 72, 512), (128, 1000, 1088),
-                                   (129, 256, 64), (200, 392, 352), (513, 1032, 416)])
+                                   (129, 256, 64), (200, 392, 352), (513, 1032, 416),
+                                   (257, 136, 4128), (384, 264, 4352)])
 def test_linear_against_64_bits(cuda, dtype, m, n, k):
     x = rand(m, k, seed=m).to(dtype)
     w, wv = mx_weight(n, k, cuda)
@@ -256,7 +257,8 @@ def test_linear_views_outputs_and_nan_rows(cuda, m):
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16])
 @pytest.mark.parametrize("m,d,f", [(1, 32, 128), (3, 288, 384), (16, 256, 256), (40, 160, 512),
-                                   (129, 544, 256), (260, 96, 640)])
+                                   (129, 544, 256), (260, 96, 640), (150, 4128, 128),
+                                   (200, 64, 4224)])
 def test_gated_ffn_against_64_bits(cuda, dtype, m, d, f):
     x, r = rand(m, d, seed=m).to(dtype), rand(m, d, seed=2).to(dtype)
     wu = rand(2 * f, d, seed=11, scale=d ** -0.5).to(BF16)
