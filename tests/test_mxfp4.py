@@ -279,8 +279,10 @@ def test_gated_ffn_against_64_bits(cuda, dtype, m, d, f):
         assert got.dtype == dtype
         assert ((got.cpu().double() - want).abs()
                 <= off + ref.half_step(dtype) * (want.abs() + off) + 1e-7).all()
-    # the bound is not vacuous: most hidden values are away from every boundary
-    assert (far == 0).double().mean() > 0.9
+    # the bound is not vacuous: most hidden values are away from every boundary.
+    # It covers d steps of 2^-23 of sum |x w|, about d^1.5 2^-23 of a typical
+    # value: 3 % of it, a sixteenth of an E2M1 step on each side, at d = 4128.
+    assert (far == 0).double().mean() > (0.9 if d < 1024 else 0.5)
 
 
 @pytest.mark.gpu
