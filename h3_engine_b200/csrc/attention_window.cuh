@@ -7,19 +7,20 @@
 //     (p - left <= j <= p + right  or  j < sinks)  and  (not causal or j <= p).
 // A query that sees no key gets zeros.
 //
-// One CTA = two 128-row query tiles (A, B) of one head of one document, the
-// roles, TMEM layout and MMA order of attention.cuh.  Of the document's keys it
-// visits only those that some query of the pair sees: the sink keys
-// [0, sink_end) and the window [lo, hi], each in steps of 128 (64) keys that start
-// at 0 and at lo (TMA rows need no alignment, so the first step of the window
-// starts at its first key); the two are one range where they touch.  A step that no query of tile A (or B) sees is skipped for that tile:
+// One CTA = an item: two 128-row query tiles (A, B), or tile A alone, of one
+// head of one document, in the roles and MMA order of attention.cuh.  Of the
+// document's keys it visits only those that some query of the item sees: the
+// sink keys [0, sink_end) and the window [lo, hi], each in steps of 128 or 64
+// keys that start at 0 and at lo (TMA rows need no alignment, so the first step
+// of the window starts at its first key); the two are one range where they
+// touch.  A step that no query of tile A (or B) sees is skipped for that tile:
 // neither its MMAs nor its softmax run, which is what the window's triangular
 // ends cost least with.  Within a step a row's keys are words of 32, of
 // which only those that some row of the warp does not see whole are masked.
 //
-// The grid is a number of full waves of items, one CTA per SM, and a last
-// partial wave whose items are split along their keys so that it fills the SMs
-// too: the parts leave their unnormalised O, row maximum and sum (fp32) in a
+// The grid is a number of full waves of items, one or two CTAs per SM, and a
+// last partial wave whose items are split along their keys so that it fills
+// the SMs too: the parts leave their unnormalised O, row maximum and sum (fp32) in a
 // workspace, and the part that finishes last adds them up, in part order, so
 // the result does not depend on which one that is.
 //
@@ -42,16 +43,18 @@ constexpr int BQ = 128;
 constexpr int MAX_DOCS = 64;          // documents per launch
 constexpr int kPrefetchTiles = 4;
 
-// head_dim 128: steps of 128 keys, all of tensor memory, one CTA per SM whose
-// softmax warpgroups get the registers that the control warps give back.
-// head_dim 64: the products are half as long while the softmax is not, and two
-// softmax warps per scheduler leave it idle half the time; steps of 64 keys
-// need half the registers and tensor memory, so two CTAs share an SM.
-template <int D>
+// Steps of 128 keys: all of tensor memory, one CTA per SM whose softmax
+// warpgroups get the registers that the control warps give back.  With head_dim
+// 64 the products are half as long while the softmax is not, and two softmax
+// warps per scheduler leave it idle half the time; steps of 64 keys need half
+// the registers and tensor memory, so two CTAs share an SM, where there are
+// more CTAs than SMs (148 of them: 19 us in steps of 128, 22 in steps of 64;
+// 240: 35 and 30).
+template <int D, int KEYS>
 struct Cfg {
-  static constexpr int BK = D;                             // keys per step
-  static constexpr int CTAS = D == 128 ? 1 : 2;            // per SM
-  static constexpr int THREADS = D == 128 ? 384 : 320;
+  static constexpr int BK = KEYS;                          // keys per step
+  static constexpr int CTAS = BK == 128 ? 1 : 2;           // per SM
+  static constexpr int THREADS = BK == 128 ? 384 : 320;
   static constexpr int HALVES = BK / 64;                   // P reaches the MMA 64 keys at a time
   static constexpr uint32_t TMEM_COLS = 512 / CTAS;
   static constexpr int Q_BOX = 128 * 128;                  // 128 rows x 64 columns
@@ -66,7 +69,7 @@ struct Cfg {
   static __device__ constexpr uint32_t o_col(int t) { return (uint32_t)(2 * BK + t * D); }
 };
 constexpr int kLaunchRegs = 168, kCtrlRegs = 72, kSoftmaxRegs = 216;
-static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= Cfg<128>::THREADS * kLaunchRegs,
+static_assert(128 * kCtrlRegs + 256 * kSoftmaxRegs <= Cfg<128, 128>::THREADS * kLaunchRegs,
               "register split");
 
 struct Args {
@@ -76,6 +79,7 @@ struct Args {
   int H, group;                            // query heads; query heads per key head
   float scale_log2;                        // softmax scale * log2(e)
   int left, right, sinks, causal;          // left, right < 2^30
+  int item_rows;                           // queries per item: 256, or 128 (tile A only)
   int whole, parts;                        // items [0, whole) are whole, the others in `parts`
   float* partial;                          // [split item][part]: O [D/4][256][4], then (m, l) [256]
   int* done;                               // [split item]: parts finished (0 between launches)
@@ -233,11 +237,10 @@ __device__ __forceinline__ uint32_t span_word(int a, int b, int w) {
   return (0xffffffffu << lo) & (0xffffffffu >> (31 - hi));
 }
 
-template <int D, typename T>
-__global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
+template <int D, int BK, typename T>
+__global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
     k_window_attn(const __grid_constant__ Args p) {
-  using L = Cfg<D>;
-  constexpr int BK = L::BK;
+  using L = Cfg<D, BK>;
   // kind::f16: D fp32 (bit 4), A and B bf16 (bits 7, 10) or fp16 (0)
   constexpr uint32_t kType = std::is_same<T, __half>::value ? 0u : (1u << 7) | (1u << 10);
   constexpr uint32_t IDESC_QK =
@@ -275,13 +278,13 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   while (doc + 1 < p.ndocs && idx >= p.item_end[doc]) ++doc;
   const int item = idx - (doc > 0 ? p.item_end[doc - 1] : 0);
   const int n_q = p.q_len[doc], n_k = p.k_len[doc];
-  const int pairs = (n_q + 2 * BQ - 1) / (2 * BQ);
+  const int pairs = (n_q + p.item_rows - 1) / p.item_rows;
   const int head = item / pairs;
-  const int qp = item - head * pairs;
-  const int q_row = p.q_start[doc] + qp * 2 * BQ;
+  const int q0 = (item - head * pairs) * p.item_rows;     // first query in the document
+  const int q_row = p.q_start[doc] + q0;
   const int k_row = p.k_start[doc];
-  const int pos0 = qp * 2 * BQ + n_k - n_q;               // position of tile A's first row
-  const int rows = min(2 * BQ, n_q - qp * 2 * BQ);        // queries of this pair
+  const int pos0 = q0 + n_k - n_q;                        // position of tile A's first row
+  const int rows = min(p.item_rows, n_q - q0);            // queries of this item
   Steps<BK> st(Range(p, n_k, pos0, pos0 + rows - 1));
   if (!whole) st.take(part, p.parts);
   // what each tile sees; a tile without queries sees nothing
@@ -343,7 +346,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
   // Each warpgroup changes its register limit inside its own branch and leaves
   // through its own copy of the teardown barrier.
   if (warp >= 8) {
-    if constexpr (D == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
+    if constexpr (BK == 128) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kCtrlRegs));
     if (warp == 8) {
       if (lane == 0 && st.n > 0) {
         auto prefetch = [&](int j) {
@@ -480,7 +483,7 @@ __global__ void __launch_bounds__(Cfg<D>::THREADS, Cfg<D>::CTAS)
       tmem_dealloc(tmem, L::TMEM_COLS);
     }
   } else {
-    if constexpr (D == 128)
+    if constexpr (BK == 128)
       asm volatile("setmaxnreg.inc.sync.aligned.u32 %0;" ::"n"(kSoftmaxRegs));
     // softmax of tile t: thread = query row (TMEM lane quadrant warp % 4)
     const int t = warp >> 2;

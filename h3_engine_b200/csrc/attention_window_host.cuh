@@ -1,6 +1,8 @@
 // Host side of the windowed-attention entry points (declared in include/h3b.h).
 #pragma once
 
+#include <cmath>
+
 #include "attention_decode.cuh"
 #include "attention_window.cuh"
 #include "mx_host.cuh"
@@ -28,14 +30,15 @@ static int tmap_16_rows(CUtensorMap* tm, const void* base, int dtype, int64_t ro
              : H3B_ERR_INVALID_ARG;
 }
 
-template <int D, typename T>
+template <int D, int BK, typename T>
 static int window_attn_launch(const wattn::Args& a, int64_t grid, cudaStream_t st) {
-  auto kernel = wattn::k_window_attn<D, T>;
+  auto kernel = wattn::k_window_attn<D, BK, T>;
+  using L = wattn::Cfg<D, BK>;
   const void* fn = reinterpret_cast<const void*>(kernel);
   static SmemAttr attr;
-  int rc = attr.set(fn, wattn::Cfg<D>::BYTES);
+  int rc = attr.set(fn, L::BYTES);
   if (rc != H3B_OK) return rc;
-  if (D == 128) {
+  if (BK == 128) {
     // the kernel's setmaxnreg split draws on this many launch registers
     static std::atomic<int> regs{0};
     if (!regs.load(std::memory_order_relaxed)) {
@@ -45,62 +48,74 @@ static int window_attn_launch(const wattn::Args& a, int64_t grid, cudaStream_t s
     }
     if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
   }
-  kernel<<<(unsigned)grid, wattn::Cfg<D>::THREADS, wattn::Cfg<D>::BYTES, st>>>(a);
+  kernel<<<(unsigned)grid, L::THREADS, L::BYTES, st>>>(a);
   return launched(cudaGetLastError());
 }
 
-// Whole items first, then the last partial wave's items in parts: of `items`
-// CTAs of about equal length in `slots` places, items mod slots would run alone,
-// so they are split to fill the places (8 heads of 16384 rows, 512 items on 148
-// SMs: 221 us, unsplit 235).  A part should keep 512 keys or more.
-struct WindowPlan {
-  int whole, parts;
-  WindowPlan(int64_t items, int64_t keys, int D) {
-    const int slots = num_sms() * (D == 128 ? wattn::Cfg<128>::CTAS : wattn::Cfg<64>::CTAS);
-    const int rest = (int)(items % slots);
-    whole = (int)items;
-    parts = 1;
-    if (rest == 0) return;
-    const int64_t p = std::min<int64_t>(slots / rest, keys / 512);
-    if (p < 2) return;
-    whole = (int)(items - rest);
-    parts = (int)p;
-  }
-  int64_t split(int64_t items) const { return items - whole; }
-  int64_t grid(int64_t items) const { return whole + split(items) * parts; }
-};
-
-// Keys that a query-tile pair of a document of n_k keys visits under a window.
+// Keys that an item of a document of n_k keys visits under a window.
 static int64_t window_keys(int64_t n_k, int64_t left, int64_t right, int64_t sinks) {
   return std::min<int64_t>(n_k, left + right + 2 * wattn::BQ + sinks);
 }
 
-// One launch's documents: up to MAX_DOCS with queries, those with the most keys
-// first (the light items then fill the last wave's gaps), from d0 on.
-struct WindowDocs {
+// One launch: up to MAX_DOCS documents with queries from d0 on, those with the
+// most keys first (the light items then fill the last wave's gaps), and how
+// their work is cut.
+//   Items of 256 queries, or of 128 where those all have a place at once (1000
+// rows, 8 heads: 19.0 us, in items of 256 21.0; 16384 rows, where they have
+// not: 341 us, in items of 256 221), unless items of 256 can be cut into 3/2 as
+// many parts.  The ratio lies between the cases measured: with as many parts
+// items of 128 win as above, with twice as many items of 256 do (2000 rows:
+// 32.8 us, in items of 128 33.8; head_dim 64 26.7 and 29.2).
+//   Whole items first, then the last partial wave's in parts: items mod places
+// would run alone, so they are split to fill the places (8 heads of 16384 rows,
+// 512 items on 148 SMs: 221 us, unsplit 230).  A part keeps kPartKeys keys.
+struct WindowPlan {
+  static constexpr int64_t kPartKeys = 512;
   int order[wattn::MAX_DOCS];
   int n = 0, next = 0;
-  int64_t items = 0, keys = 0;              // keys: of the lightest document's pairs
-  WindowDocs(const int32_t* q_len, const int32_t* k_len, int ndocs, int d0, int H, int64_t left,
-             int64_t right, int64_t sinks) {
-    for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0) {
-      if (q_len[d0] == 0) continue;
-      order[n++] = d0;
-      items += ((int64_t)q_len[d0] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
-    }
+  int item_rows = 2 * wattn::BQ, step = 128, whole = 0, parts = 1;
+  int64_t items = 0;
+  WindowPlan(const int32_t* q_len, const int32_t* k_len, int ndocs, int d0, int H, int D,
+             int64_t left, int64_t right, int64_t sinks) {
+    for (; d0 < ndocs && n < wattn::MAX_DOCS; ++d0)
+      if (q_len[d0] > 0) order[n++] = d0;
     next = d0;
+    if (n == 0) return;
     std::sort(order, order + n, [&](int a, int b) {
       return k_len[a] != k_len[b] ? k_len[a] > k_len[b] : a < b;
     });
-    if (n > 0) keys = window_keys(k_len[order[n - 1]], left, right, sinks);
+    auto count = [&](int rows) {
+      int64_t c = 0;
+      for (int i = 0; i < n; ++i) c += ((int64_t)q_len[order[i]] + rows - 1) / rows * H;
+      return c;
+    };
+    const int sms = num_sms();
+    const int64_t keys = window_keys(k_len[order[n - 1]], left, right, sinks);
+    auto cut = [&](int64_t rest, int places) {
+      return rest ? std::max<int64_t>(1, std::min<int64_t>(places / rest, keys / kPartKeys)) : 1;
+    };
+    items = count(item_rows);
+    if (const int64_t c = count(wattn::BQ);
+        c <= sms && 2 * cut(items % sms, sms) < 3 * cut(c % sms, sms)) {
+      item_rows = wattn::BQ;
+      items = c;
+    }
+    if (D == 64 && items > sms) step = 64;
+    const int places = step == 64 ? 2 * sms : sms;
+    const int64_t rest = items % places;
+    parts = (int)cut(rest, places);
+    whole = (int)std::min<int64_t>(parts > 1 ? items - rest : items, INT32_MAX);
   }
+  int64_t split() const { return items - whole; }
+  int64_t grid() const { return whole + split() * parts; }
 };
 
 static int64_t window_part_bytes(int D) { return ((int64_t)256 * D + 512) * 4; }
 static constexpr int64_t kDoneBytes = 2048;       // a counter per split item (fewer than slots)
 
 static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, float scale) {
-  if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f))
+  if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f) ||
+      !std::isfinite(scale))
     return H3B_ERR_INVALID_ARG;
   return H3B_OK;
 }
@@ -156,14 +171,13 @@ int64_t h3b_attention_window_ws(const int32_t* q_len, const int32_t* k_len, int 
   if (!q_len || !k_len || ndocs <= 0 || H <= 0 || left < 0 || right < 0 || sinks < 0) return 0;
   left = clamp_window(left);
   right = clamp_window(right);
+  sinks = clamp_window(sinks);
   int64_t most = 0;
   for (int d0 = 0; d0 < ndocs;) {
-    const WindowDocs docs(q_len, k_len, ndocs, d0, H, left, right, sinks);
-    d0 = docs.next;
-    const WindowPlan plan(docs.items, docs.keys, D);
-    const int64_t split = plan.split(docs.items);
-    if (split > 0)
-      most = std::max(most, kDoneBytes + split * plan.parts * window_part_bytes(D));
+    const WindowPlan plan(q_len, k_len, ndocs, d0, H, D, left, right, sinks);
+    d0 = plan.next;
+    if (plan.n > 0 && plan.split() > 0)
+      most = std::max(most, kDoneBytes + plan.split() * plan.parts * window_part_bytes(D));
   }
   return most;
 }
@@ -204,12 +218,6 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
   memset(&a, 0, sizeof(a));
   rc = tmap_16_rows(&a.tmap_q, q, dtype, q_rows, hd, q_stride, wattn::BQ);
   if (rc != H3B_OK) return rc;
-  if (keys > 0) {
-    rc = tmap_16_rows(&a.tmap_k, k, dtype, kv_rows, kd, k_stride, (uint32_t)D);
-    if (rc != H3B_OK) return rc;
-    rc = tmap_16_rows(&a.tmap_v, v, dtype, kv_rows, kd, v_stride, (uint32_t)D);
-    if (rc != H3B_OK) return rc;
-  }
   a.out = out;
   a.ldo = ldo;
   a.H = H;
@@ -230,31 +238,38 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
     a.partial = reinterpret_cast<float*>(static_cast<uint8_t*>(ws) + kDoneBytes);
   }
   for (int d0 = 0; d0 < ndocs;) {               // documents in launches of MAX_DOCS
-    const WindowDocs docs(q_len, k_len, ndocs, d0, H, a.left, a.right, sinks);
-    d0 = docs.next;
-    if (docs.n == 0) break;
-    if (docs.items > INT32_MAX / 2) return H3B_ERR_INVALID_ARG;
+    const WindowPlan plan(q_len, k_len, ndocs, d0, H, D, a.left, a.right, a.sinks);
+    d0 = plan.next;
+    if (plan.n == 0) break;
+    if (plan.items > INT32_MAX / 2) return H3B_ERR_INVALID_ARG;
     int64_t items = 0;
-    for (int i = 0; i < docs.n; ++i) {
-      const int d = docs.order[i];
-      items += ((int64_t)q_len[d] + 2 * wattn::BQ - 1) / (2 * wattn::BQ) * H;
+    for (int i = 0; i < plan.n; ++i) {
+      const int d = plan.order[i];
+      items += ((int64_t)q_len[d] + plan.item_rows - 1) / plan.item_rows * H;
       a.q_start[i] = q_start[d];
       a.q_len[i] = q_len[d];
       a.k_start[i] = k_start[d];
       a.k_len[i] = k_len[d];
       a.item_end[i] = (int)items;
     }
-    a.ndocs = docs.n;
-    const WindowPlan plan(items, docs.keys, D);
+    a.ndocs = plan.n;
+    a.item_rows = plan.item_rows;
     a.whole = plan.whole;
     a.parts = plan.parts;
-    const int64_t grid = plan.grid(items);
-    if (D == 128)
-      rc = dtype == H3B_DT_F16 ? window_attn_launch<128, __half>(a, grid, st)
-                               : window_attn_launch<128, __nv_bfloat16>(a, grid, st);
-    else
-      rc = dtype == H3B_DT_F16 ? window_attn_launch<64, __half>(a, grid, st)
-                               : window_attn_launch<64, __nv_bfloat16>(a, grid, st);
+    // a step's keys are a box of the key and value maps
+    if (keys > 0) {
+      rc = tmap_16_rows(&a.tmap_k, k, dtype, kv_rows, kd, k_stride, (uint32_t)plan.step);
+      if (rc != H3B_OK) return rc;
+      rc = tmap_16_rows(&a.tmap_v, v, dtype, kv_rows, kd, v_stride, (uint32_t)plan.step);
+      if (rc != H3B_OK) return rc;
+    }
+    auto go = [&](auto t) {
+      using T = decltype(t);
+      if (D == 128) return window_attn_launch<128, 128, T>(a, plan.grid(), st);
+      if (plan.step == 128) return window_attn_launch<64, 128, T>(a, plan.grid(), st);
+      return window_attn_launch<64, 64, T>(a, plan.grid(), st);
+    };
+    rc = dtype == H3B_DT_F16 ? go(__half()) : go(__nv_bfloat16());
     if (rc != H3B_OK) return rc;
   }
   return H3B_OK;

@@ -12,6 +12,7 @@
 #include <c10/cuda/CUDAStream.h>
 #include <torch/library.h>
 
+#include <cmath>
 #include <vector>
 
 #include "h3b.h"
@@ -401,7 +402,7 @@ void check_rule(const Rule& r, int64_t heads, int64_t kv_heads, int64_t d) {
                     " query heads are not a multiple of ", kv_heads, " key heads");
   TORCH_CHECK_VALUE(r.left >= 0 && r.right >= 0 && r.sinks >= 0,
                     "window sides and sinks must not be negative");
-  TORCH_CHECK_VALUE(r.scale > 0, "scale must be positive");
+  TORCH_CHECK_VALUE(r.scale > 0 && std::isfinite(r.scale), "scale must be positive and finite");
 }
 
 // Row ranges of the documents that boundaries give.

@@ -105,6 +105,19 @@ def test_host_checks_refuse_without_a_gpu():
     assert decode(B=0) == 0 and decode(n=0) == 0
 
 
+def test_scale_must_be_finite_and_workspace_sizes_hold_for_huge_rules():
+    lib = _lib.lib()
+    p = ctypes.c_void_p(1 << 20)
+    one, zero, huge = (ctypes.c_int32 * 1)(4), (ctypes.c_int32 * 1)(0), (1 << 63) - 1
+    assert lib.h3b_attention_window(p, 4, 128, p, 128, p, 128, 4, 0, 1, 1, 128, zero, one, zero,
+                                    one, 1, 0, 0, 0, 0, float("inf"), p, 128, None, 0, None) == 1
+    long = (ctypes.c_int32 * 1)(4000)
+    need = lib.h3b_attention_window_ws(long, long, 1, 2, 128, 4000, 4000, 0)
+    assert need > 0
+    for left, right, sinks in ((huge, huge, huge), (huge, 0, 0), (0, 0, huge)):
+        assert lib.h3b_attention_window_ws(long, long, 1, 2, 128, left, right, sinks) == need
+
+
 def test_cpu_tensors_are_refused():
     x = torch.zeros(4, 128, dtype=BF16)
     with pytest.raises(ValueError):
@@ -159,6 +172,35 @@ def test_queries_and_keys_of_different_lengths(cuda, rule, d, dtype):
     got = ops.attention_window(q.to(cuda), k.to(cuda), v.to(cuda), 4, d, cq, kv_heads=2,
                                cu_seqlens_k=ck, window=rule[:2], sinks=rule[2], causal=rule[3])
     check_packed(got.cpu(), q, k, v, cq, ck, 4, 2, d, rule)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("tokens,heads,kv,d", [
+    (1500, 2, 1, 128),      # items of 128 queries, their keys in parts
+    (2200, 2, 2, 64),       # the same, head_dim 64
+    (2100, 8, 4, 128),      # items of 256 in parts
+    (2100, 8, 8, 64),       # the same in steps of 128 keys
+    (1300, 52, 13, 64),     # whole waves of steps of 64 keys, the rest in parts
+])
+@pytest.mark.parametrize("rule", [(None, None, 0, False), (700, 500, 70, True)])
+def test_items_and_parts(cuda, tokens, heads, kv, d, rule):
+    q, k, v, cq, ck = packed_case([tokens], [tokens], heads, kv, d, BF16, seed=5)
+    got = ops.attention_window(q.to(cuda), k.to(cuda), v.to(cuda), heads, d, cq, kv_heads=kv,
+                               window=rule[:2], sinks=rule[2], causal=rule[3])
+    check_packed(got.cpu(), q, k, v, cq, ck, heads, kv, d, rule)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_launches_that_share_their_counters(cuda, d):
+    """More documents than one launch takes, each launch with keys in parts."""
+    lq = [3 + i % 4 for i in range(70)]
+    lk = [1100 + 3 * i for i in range(70)]
+    q, k, v, cq, ck = packed_case(lq, lk, 1, 1, d, F16, seed=6)
+    for rule in ((None, None, 0, True), (900, 0, 40, True)):
+        got = ops.attention_window(q.to(cuda), k.to(cuda), v.to(cuda), 1, d, cq, cu_seqlens_k=ck,
+                                   window=rule[:2], sinks=rule[2], causal=rule[3])
+        check_packed(got.cpu(), q, k, v, cq, ck, 1, 1, d, rule)
 
 
 @pytest.mark.gpu
