@@ -91,7 +91,8 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
   if (M == 0) return H3B_OK;
   if (!x || !q || !sf) return H3B_ERR_INVALID_ARG;
-  if (!aligned16(x) || !aligned16(q) || (ldx * dt_bytes(dtype)) % 16) return H3B_ERR_ALIGNMENT;
+  if (!aligned16(x) || !aligned16(q) || !aligned16(sf) || (ldx * dt_bytes(dtype)) % 16)
+    return H3B_ERR_ALIGNMENT;
   const bool wide = wide_rows(x, ldx, dt_bytes(dtype));
   auto go = [&](auto t) {
     using T = decltype(t);

@@ -93,6 +93,8 @@ void check_operand(const Tensor& q, const Tensor& sf, int64_t rows, int64_t k, c
                     ": codes and scales must be contiguous");
   TORCH_CHECK_VALUE(q.numel() >= rows * (k / 2) && sf.numel() >= sf_bytes(rows, k), what,
                     ": codes or scales too small for ", rows, " x ", k, " values");
+  TORCH_CHECK_VALUE(aligned(q.data_ptr()) && aligned(sf.data_ptr()), what,
+                    ": codes and scales must be 16-byte aligned");
 }
 
 void check_n(int64_t n) {

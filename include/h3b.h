@@ -304,7 +304,7 @@ H3B_API int h3b_amax_exchange(float* amax, const void* slot_table, int rank, int
  *           pad128(rows) / 128 * ceil(K / 128) * 512 bytes.
  *
  * Quantize: x [M, K] of `dtype` (bf16, fp16 or fp32), row stride ldx elements;
- * x, q and ldx * size are 16-byte aligned.  The scales of the padding rows are
+ * x, q, sf and ldx * size are 16-byte aligned.  The scales of the padding rows are
  * written as zero; codes are written for the M rows only.                    */
 H3B_API int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx,
                                void* q, void* sf, void* stream);

@@ -98,6 +98,14 @@ def mx_weight(n, k, cuda, seed=3):
     return w, ref.values(w.qdata, s)
 
 
+def test_scales_must_be_aligned():
+    lib = _lib.lib()
+    p, odd = ctypes.c_void_p(1 << 20), ctypes.c_void_p((1 << 20) + 1)
+    assert lib.h3b_mxfp4_quantize(p, 0, 4, 64, 64, p, odd, None) == 2
+    assert lib.h3b_mxfp4_gemm(p, odd, 4, p, p, 16, 64, None, 0, None, 0, p, 0, 16, None) == 2
+    assert lib.h3b_mxfp4_gemm(p, p, 4, p, odd, 16, 64, None, 0, None, 0, p, 0, 16, None) == 2
+
+
 @pytest.mark.gpu
 @pytest.mark.parametrize("dtype", [BF16, F16, F32])
 @pytest.mark.parametrize("rows,k", [(1, 32), (3, 64), (127, 96), (129, 160), (33, 1056),
