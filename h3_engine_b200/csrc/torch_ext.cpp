@@ -6,7 +6,6 @@
 // its tensors' device.  Only CUDA implementations are registered.  Built as
 // _h3b_torch.so beside libh3b.so, which it links.
 #include <ATen/ATen.h>
-#include <ATen/MemoryOverlap.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -107,13 +106,51 @@ Tensor new_out(const Tensor& like, int64_t n, at::ScalarType type) {
   return new_tensor(shape, type, like);
 }
 
+// A tensor's bytes: from `at`, up to `end`, and, where its leading dimensions
+// are evenly spaced, as `rows` rows of `width` bytes every `pitch`.
+struct Bytes {
+  uintptr_t at, end;
+  int64_t rows = 1, width, pitch = 0;
+  bool even;
+  explicit Bytes(const Tensor& t) : at(reinterpret_cast<uintptr_t>(t.data_ptr())) {
+    const int64_t size = t.element_size();
+    int64_t last = 0;
+    for (int64_t i = 0; i < t.dim(); ++i) last += (t.size(i) - 1) * t.stride(i);
+    end = at + (last + 1) * size;
+    const int64_t cols = t.dim() ? t.size(-1) : 1;
+    width = cols * size;
+    even = t.dim() == 0 || cols == 1 || t.stride(-1) == 1;
+    for (int64_t i = t.dim() - 2; i >= 0; --i) {
+      if (t.size(i) == 1) continue;
+      if (rows == 1) pitch = t.stride(i) * size;
+      else even = even && t.stride(i) * size == pitch * rows;
+      rows *= t.size(i);
+    }
+    if (rows > 1 && pitch == width) {              // no gaps: one row
+      width *= rows;
+      rows = 1;
+    }
+  }
+};
+
 // An output may be one of its inputs where every element is read before it is
-// written by the same thread (exact), and shares no memory with the others.
+// written by the same thread (exact_ok), and shares no memory with the others;
+// columns side by side in the same rows share none.
 void apart(const Tensor& out, const Tensor& in, bool exact_ok, const char* what) {
-  const auto s = at::get_overlap_status(out, in);
-  TORCH_CHECK_VALUE(s != at::MemOverlapStatus::Partial &&
-                        (exact_ok || s != at::MemOverlapStatus::Full),
-                    "out shares memory with ", what);
+  if (out.numel() == 0 || in.numel() == 0) return;
+  const Bytes a(out), b(in);
+  if (a.end <= b.at || b.end <= a.at) return;
+  bool ok = false;
+  if (a.even && b.even) {
+    if (a.at == b.at && a.rows == b.rows && a.width == b.width && a.pitch == b.pitch) {
+      ok = exact_ok;
+    } else if (a.rows > 1 && b.rows > 1 && a.pitch == b.pitch && a.pitch > 0) {
+      const Bytes &lo = a.at < b.at ? a : b, &hi = a.at < b.at ? b : a;
+      const int64_t d = (int64_t)(hi.at - lo.at) % a.pitch;
+      ok = d >= lo.width && d + hi.width <= a.pitch;
+    }
+  }
+  TORCH_CHECK_VALUE(ok, "out shares memory with ", what);
 }
 void apart(const Tensor& out, const optional<Tensor>& in, bool exact_ok, const char* what) {
   if (in) apart(out, *in, exact_ok, what);

@@ -289,6 +289,37 @@ def test_outputs_must_stand_apart(cuda):
 
 
 @pytest.mark.gpu
+def test_outputs_in_rows_that_hold_other_columns(cuda):
+    """Columns beside the inputs' in the same rows are free; columns that reach
+    into an input's are refused, whatever the layout."""
+    d = 64
+    buf = rand(40, 6 * d).to(BF16).to(cuda)
+    q, k, v = buf[:, :d], buf[:, d:2 * d], buf[:, 2 * d:3 * d]
+    args = (1, d, [0, 40])
+    want = ops.attention_window(q, k, v, *args, window=(3, 3))
+    got = ops.attention_window(q, k, v, *args, window=(3, 3), out=buf[:, 3 * d:4 * d])
+    assert torch.equal(got, want)
+    for bad in (buf[:, d:2 * d], buf[:, d // 2:d // 2 + d], buf[:, 2 * d + 8:3 * d + 8]):
+        with pytest.raises(ValueError):
+            ops.attention_window(q, k, v, *args, out=bad)
+    assert torch.equal(ops.attention_window(q, k, v, *args, window=(3, 3), out=q), want)
+
+    w = mxfp4.MXFP4Weight(rand(d, 2 * d, seed=1, scale=0.1).to(BF16).to(cuda))
+    x = buf[:, 4 * d:]
+    r3 = buf[:, :d].unflatten(0, (4, 10))            # the same rows, one more dimension
+    want = mxfp4.mxfp4_linear(w, x, residual=r3)
+    assert torch.equal(mxfp4.mxfp4_linear(w, x, residual=r3, out=buf[:, 3 * d:4 * d]), want)
+    with pytest.raises(ValueError):
+        mxfp4.mxfp4_linear(w, x, out=buf[:, 5 * d:])
+    with pytest.raises(ValueError):
+        mxfp4.mxfp4_linear(w, x, residual=r3, out=buf[:, 8:8 + d])
+    rows = buf[:20, :d]
+    with pytest.raises(ValueError):                  # the same columns, two rows on
+        mxfp4.mxfp4_linear(w, x[:20], residual=rows, out=buf[2:22, :d])
+    assert torch.equal(mxfp4.mxfp4_linear(w, x, residual=r3, out=buf[:, :d]), want)
+
+
+@pytest.mark.gpu
 def test_compiled_callers_keep_the_operators(cuda):
     w = mxfp4.MXFP4Weight(rand(64, 128, scale=0.1).to(BF16).to(cuda))
     x = rand(20, 128).to(BF16).to(cuda)
