@@ -638,3 +638,14 @@ TORCH_LIBRARY_IMPL(h3b, CUDA, m) {
   m.impl("attention_window_decode", &attention_window_decode);
   m.impl("attention_window_decode_out", &attention_window_decode_out);
 }
+
+// Inference only, as the package's other operators: results carry no gradient
+// (without this, backward() would run and leave the inputs' gradients out).
+TORCH_LIBRARY_IMPL(h3b, Autograd, m) {
+  for (const char* name :
+       {"mxfp4_quantize", "mxfp4_quantize_out", "mxfp4_dequantize", "mxfp4_dequantize_out",
+        "mxfp4_gemm", "mxfp4_gemm_out", "mxfp4_linear", "mxfp4_linear_out", "mxfp4_ffn",
+        "mxfp4_ffn_out", "attention_window", "attention_window_out", "attention_window_decode",
+        "attention_window_decode_out"})
+    m.impl(name, torch::CppFunction::makeFallthrough());
+}

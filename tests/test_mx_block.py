@@ -320,6 +320,20 @@ def test_outputs_in_rows_that_hold_other_columns(cuda):
 
 
 @pytest.mark.gpu
+def test_results_carry_no_gradient(cuda):
+    x = rand(20, 128).to(BF16).to(cuda).requires_grad_()
+    w = mxfp4.MXFP4Weight(rand(64, 128, scale=0.1).to(BF16).to(cuda))
+    y = mxfp4.mxfp4_linear(w, x)
+    a = ops.attention_window(x, x, x, 1, 128, [0, 20])
+    c = x.view(1, 20, 1, 128)
+    d = ops.attention_window_decode(c[:, -1:], c, c, torch.tensor([20], dtype=torch.int32).to(cuda))
+    for t in (y, a, d):
+        assert not t.requires_grad and t.grad_fn is None
+    with pytest.raises(RuntimeError):
+        (y.float().sum() + a.float().sum()).backward()
+
+
+@pytest.mark.gpu
 def test_compiled_callers_keep_the_operators(cuda):
     w = mxfp4.MXFP4Weight(rand(64, 128, scale=0.1).to(BF16).to(cuda))
     x = rand(20, 128).to(BF16).to(cuda)
