@@ -122,8 +122,8 @@ struct Steps {
     }
   }
   __device__ __forceinline__ void take(int part, int parts) {
-    first = n * part / parts;
-    n = n * (part + 1) / parts - first;
+    first = (int)((long long)n * part / parts);
+    n = (int)((long long)n * (part + 1) / parts) - first;
   }
   __device__ __forceinline__ int base(int j) const {
     j += first;

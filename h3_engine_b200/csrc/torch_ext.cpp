@@ -69,7 +69,7 @@ bool rows_aligned(const Tensor& t) {
 Tensor rows2d(const Tensor& t) {
   TORCH_CHECK_VALUE(t.dim() >= 1, "a tensor of rows is expected");
   Tensor r = t.dim() == 2 ? t : t.reshape({-1, t.size(-1)});
-  return r.numel() == 0 || rows_aligned(r) ? r : r.clone(at::MemoryFormat::Contiguous);
+  return rows_aligned(r) ? r : r.clone(at::MemoryFormat::Contiguous);
 }
 
 // New tensors straight from the caching allocator (no dispatch).
@@ -568,8 +568,11 @@ void decode_into(const Call& c, const Tensor& q_in, const Tensor& k, const Tenso
                     "caches need a contiguous head_dim and 16-byte aligned rows");
   if (out.numel() == 0) return;
   const Tensor q = decode_strides(q_in) ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
+  static const int64_t none[4] = {0, 0, 0, 0};       // an empty cache's strides mean nothing
+  const bool empty = k.numel() == 0;
   check(h3b_attention_window_decode(q.data_ptr(), q.strides().data(), k.data_ptr(),
-                                    k.strides().data(), v.data_ptr(), v.strides().data(),
+                                    empty ? none : k.strides().data(), v.data_ptr(),
+                                    empty ? none : v.strides().data(),
                                     len.const_data_ptr<int32_t>(), B, k.size(1), n, dt, (int)heads,
                                     (int)k.size(2), (int)d, r.left, r.right, r.sinks, r.causal,
                                     (float)r.scale, out.data_ptr(), c.stream()),

@@ -256,6 +256,24 @@ def test_rows_nobody_sees_do_not_matter(cuda, d):
 
 
 @pytest.mark.gpu
+def test_no_rows_and_no_keys_at_odd_strides(cuda):
+    """Empty views keep the strides of what they were cut from."""
+    d = 64
+    buf = torch.randn(8, d + 3, generator=torch.Generator().manual_seed(7)).to(BF16).to(cuda)
+    q = buf[:, :d].contiguous()
+    none = buf[:0, 1:1 + d]
+    got = ops.attention_window(q, none, none, 1, d, [0, 8], cu_seqlens_k=[0, 0])
+    assert got.shape == (8, d) and (got == 0).all()
+    assert ops.attention_window(none, q, q, 1, d, [0, 0], cu_seqlens_k=[0, 8]).shape == (0, d)
+    assert ops.attention_window(none, none, none, 1, d, [0]).shape == (0, d)
+    n = torch.zeros(2, dtype=torch.int32, device=cuda)
+    qd = q.view(2, 4, 1, d)
+    empty = torch.empty(2, 0, 1, d + 3, dtype=BF16, device=cuda)[..., 1:1 + d]
+    got = ops.attention_window_decode(qd, empty, empty, n)
+    assert got.shape == qd.shape and (got == 0).all()
+
+
+@pytest.mark.gpu
 def test_strided_views_and_outputs(cuda):
     d, rows = 64, 150
     qkv = torch.randn(rows, 4 * d, generator=torch.Generator().manual_seed(4)).to(BF16).to(cuda)
