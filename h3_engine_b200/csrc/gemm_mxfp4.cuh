@@ -59,10 +59,10 @@ struct Args {
   const uint8_t* sfa;      // blocked scales, M padded to 128 rows
   const uint8_t* sfb;
   const void* bias;        // [N], type of D
-  const void* residual;    // [M, N], type of D
+  CUtensorMap tmap_r;      // the residual (pitch ldr), as tmap_d
+  int residual;            // there is one
   uint8_t* q_out;          // kSwigluQuant: codes u8 [M, N/4]
   uint8_t* sf_out;         // and their blocked scales
-  long long ldr;
   int M, N, K;
   int sf_tiles_k;          // 512-byte scale tiles per 128-row block
   int n_tiles;
@@ -82,20 +82,39 @@ __device__ __forceinline__ float gelu_tanh_f32(float v) {
   return __fdividef(v, 1.0f + __expf(-u2));
 }
 
+// The residual of a warp's 32 rows x 128 columns into its staging boxes, under
+// the MMAs of the tile; false where the warp has none.
+__device__ __forceinline__ bool residual_load(const Args& p, int m0, int n0, int half, int qd,
+                                              int lane, uint32_t stage_s, uint32_t bar) {
+  const int n_base = n0 + half * 128, row = m0 + qd * 32;
+  if (!p.residual || n_base >= p.N || row >= p.M) return false;
+  if (lane == 0) {
+    bulk_wait_read0();                                // the last tile's boxes have been read
+    const int boxes = n_base + OUT_COLS < p.N ? 2 : 1;
+    mbar_expect_tx(bar, (uint32_t)boxes * OUT_BOX_BYTES);
+    for (int c = 0; c < boxes; ++c)
+      tma_load_2d(stage_s + c * OUT_BOX_BYTES, &p.tmap_r, n_base + c * OUT_COLS, row, bar);
+  }
+  __syncwarp();
+  return true;
+}
+
 // Epilogue of one warp's 32 rows x 128 accumulator columns: columns
-// n0 + 128 * half .. of a tile whose rows start at m0.
+// n0 + 128 * half .. of a tile whose rows start at m0.  With a residual the
+// boxes hold it, and each 16 bytes are replaced by the result (13383 x 5376 x
+// 7168: 200 us, 204 with the residual read from global memory here, a row per
+// lane; K = 2048: 84 and 146, 1025 x 2016 x 5504: 14.1 and 17.8).
 template <typename T, bool GELU>
 __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc)[128], int m0,
                                              int n0, int half, int qd, int lane, uint8_t* stage,
                                              uint32_t stage_s) {
   const int n_base = n0 + half * 128;
   if (n_base >= p.N || m0 + qd * 32 >= p.M) return;   // warp-uniform
-  const int row = m0 + qd * 32 + lane;
-  const bool row_ok = row < p.M;
   const T* bias = static_cast<const T*>(p.bias);
-  const T* residual = static_cast<const T*>(p.residual);
-  if (lane == 0) bulk_wait_read0();                   // the last tile's boxes have been read
-  __syncwarp();
+  if (!p.residual) {
+    if (lane == 0) bulk_wait_read0();                 // the last tile's boxes have been read
+    __syncwarp();
+  }
 #pragma unroll
   for (int c = 0; c < 2; ++c) {
     if (n_base + c * OUT_COLS >= p.N) break;          // the box would start past N
@@ -119,8 +138,11 @@ __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc
         for (int e = 0; e < 4; ++e)
           v[e] = make_float2(gelu_tanh_f32(v[e].x), gelu_tanh_f32(v[e].y));
       }
-      if (residual && row_ok && col_ok) {
-        const uint4 b = __ldg(reinterpret_cast<const uint4*>(residual + (size_t)row * p.ldr + col));
+      // 128B swizzle: 16-byte chunk j of row `lane` sits at chunk j ^ (lane % 8)
+      uint4* const at = reinterpret_cast<uint4*>(stage + c * OUT_BOX_BYTES + lane * 128 +
+                                                 ((j ^ (lane & 7)) << 4));
+      if (p.residual) {
+        const uint4 b = *at;
         const uint32_t bw[4] = {b.x, b.y, b.z, b.w};
 #pragma unroll
         for (int e = 0; e < 4; ++e) v[e] = add2(v[e], unpack2(bw[e], T()));
@@ -128,9 +150,7 @@ __device__ __forceinline__ void epilogue_out(const Args& p, const uint32_t (&acc
       uint32_t o[4];
 #pragma unroll
       for (int e = 0; e < 4; ++e) o[e] = mx::pack2(v[e].x, v[e].y, T());
-      // 128B swizzle: 16-byte chunk j of row `lane` sits at chunk j ^ (lane % 8)
-      *reinterpret_cast<uint4*>(stage + c * OUT_BOX_BYTES + lane * 128 + ((j ^ (lane & 7)) << 4)) =
-          make_uint4(o[0], o[1], o[2], o[3]);
+      *at = make_uint4(o[0], o[1], o[2], o[3]);
     }
     fence_proxy_async_smem();
     __syncwarp();
@@ -272,6 +292,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
   uint64_t* bye = bars + 2 * P_STAGES + 3;     // both: the peer is done
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 2 * P_STAGES + 4);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
+  uint64_t* res_full = bars + 16;              // per epilogue warp: the residual's boxes
 
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
   const uint32_t rank = cluster_ctarank();
@@ -296,6 +317,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     mbar_init(smem_u32(acc_empty), 2 * EPI_WARPS);
     mbar_init(smem_u32(drain), 1);
     mbar_init(smem_u32(bye), 1);
+    for (int i = 0; i < EPI_WARPS; ++i) mbar_init(smem_u32(&res_full[i]), 1);
     *abort_flag = 0;
     fence_mbar_init();
   }
@@ -425,15 +447,23 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     uint8_t* stage = smem + P_OUT_OFFSET + ew * OUT_WARP_BYTES;
     const uint32_t stage_s = smem_u32(stage);
     const uint32_t leader_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
-    uint32_t i = 0;
+    const uint32_t rbar = smem_u32(&res_full[ew]);
+    uint32_t i = 0, loads = 0;
     mx::grid_wait();                     // residual and D follow the chain's earlier launches
     if (p.early) mx::grid_launch_dependents();
-    if (EPI != kSwigluQuant && lane == 0) prefetch_tmap(&p.tmap_d);
+    if (EPI != kSwigluQuant && lane == 0) {
+      prefetch_tmap(&p.tmap_d);
+      if (p.residual) prefetch_tmap(&p.tmap_r);
+    }
     for (int t = pair_id; t < num_tiles; t += num_pairs, ++i) {
       int mt, nt;
       pair_tile(pa, t, mt, nt);
       const int m0 = mt * 256 + 128 * (int)rank, n0 = nt * BN;
-      const bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(acc_full), i & 1, abort_flag));
+      const bool res = EPI != kSwigluQuant &&
+                       residual_load(p, m0, n0, half, qd, lane, stage_s, rbar);
+      bool ready = __all_sync(0xffffffffu, mbar_wait(smem_u32(acc_full), i & 1, abort_flag));
+      // (bounded, but not cut short: no copy may still be landing at the exit)
+      if (res) ready = __all_sync(0xffffffffu, mbar_wait(rbar, loads++ & 1, nullptr)) && ready;
       if (!ready) {
         fail();
         break;

@@ -300,8 +300,12 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, c
                           mxgemm::OUT_COLS, 32);
   if (rc != H3B_OK) return rc;
   a.bias = bias;
-  a.residual = residual;
-  a.ldr = ldr;
+  if (residual) {
+    rc = make_tmap_16_sw128(&a.tmap_r, residual, dtype, (uint64_t)M, (uint64_t)N, (uint64_t)ldr,
+                            mxgemm::OUT_COLS, 32);
+    if (rc != H3B_OK) return rc;
+    a.residual = 1;
+  }
   if (act == H3B_ACT_GELU_TANH)
     return dtype == H3B_DT_F16
                ? mx_gemm_launch<__half, mxgemm::kOutGelu>(pa, chained, st)
