@@ -155,7 +155,9 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
   }
   __syncthreads();
   cluster_arrive();
-  const int n = min(max(__ldg(p.len + b), 0), p.room);
+  grid_wait();
+  grid_launch_dependents();
+  const int n = min(max(p.len[b], 0), p.room);
 
   // keys that any of this tile's rows sees: [0, sink_end) and [lo, end), visited
   // as one list of `total` keys
@@ -185,8 +187,8 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
                  (long long)(kvh * p.group + g) * p.q_h + (lane & 3) * 2;
 #pragma unroll
     for (int kk = 0; kk < D / 16; ++kk) {
-      qf[kk][j][0] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16)) : 0u;
-      qf[kk][j][1] = ok ? __ldg(reinterpret_cast<const uint32_t*>(q + kk * 16 + 8)) : 0u;
+      qf[kk][j][0] = ok ? *reinterpret_cast<const uint32_t*>(q + kk * 16) : 0u;
+      qf[kk][j][1] = ok ? *reinterpret_cast<const uint32_t*>(q + kk * 16 + 8) : 0u;
     }
   }
   // this lane's rows in the products: j * 8 + (lane % 4) * 2 + {0, 1}

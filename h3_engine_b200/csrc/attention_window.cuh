@@ -319,6 +319,7 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
     *abort_flag = 0;
     fence_mbar_init();
     if (st.n > 0) {
+      grid_wait();
       // the first loads run while tensor memory is allocated
       const uint32_t qb = smem_u32(q_full);
       mbar_expect_tx(qb, 2 * L::Q_BYTES + L::KV_BYTES);
@@ -331,10 +332,12 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
     tmem_alloc(smem_u32(tmem_slot), L::TMEM_COLS);
     tmem_relinquish();
   }
+  grid_wait();
   tc_fence_before();
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
+  grid_launch_dependents();
 
   auto fail = [&]() {
     if (!*abort_flag) {

@@ -48,8 +48,7 @@ static int window_attn_launch(const wattn::Args& a, int64_t grid, cudaStream_t s
     }
     if (regs.load(std::memory_order_relaxed) != wattn::kLaunchRegs) return H3B_ERR_UNSUPPORTED;
   }
-  kernel<<<(unsigned)grid, L::THREADS, L::BYTES, st>>>(a);
-  return launched(cudaGetLastError());
+  return launch(true, kernel, dim3((unsigned)grid), L::THREADS, L::BYTES, 0, st, a);
 }
 
 // Keys that an item of a document of n_k keys visits under a window.
@@ -140,19 +139,8 @@ static int window_decode_rows(const wdec::Args& a, int64_t B, cudaStream_t st) {
   while (split < wdec::kMaxCluster && groups * B * split < 2 * (int64_t)num_sms() &&
          most > (int64_t)split * wdec::kWarps * wdec::kKeys * 2)
     split *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split, (unsigned)groups, (unsigned)B);
-  cfg.blockDim = dim3(wdec::kThreads);
-  cfg.dynamicSmemBytes = kBytes;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)split;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = 1;
-  return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+  return launch(true, kernel, dim3((unsigned)split, (unsigned)groups, (unsigned)B), wdec::kThreads,
+                      kBytes, split, st, a);
 }
 
 // Rows that share a key head: 8 of them in one product's columns, more in two.

@@ -490,4 +490,21 @@ __device__ __forceinline__ uint64_t desc_sf_atom(uint32_t saddr) {
   return smem_desc(saddr, 0, 128, 0);
 }
 
+// Launches that start early (programmatic stream serialization): a kernel comes
+// up under the end of the one before it, and
+//   - waits for that one before it touches memory which that one, or one before
+//     it, may read or write (grid_wait: all of it is done and visible);
+//   - lets the next one come up only after its own wait, so that a kernel which
+//     runs at all knows that everything up to two launches back is done.
+// The second rule is what lets a later launch of a call read its weight before
+// its wait: the call's first launch has waited for whatever wrote the weight.
+// A kernel of any other origin in between neither starts nor is started early.
+__device__ __forceinline__ void grid_launch_dependents() {
+  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
+}
+
+// Waits until the launch before this one is done and its results are visible
+// (at once, where this one was not started early).
+__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
 }  // namespace h3b

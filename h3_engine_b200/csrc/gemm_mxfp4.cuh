@@ -66,7 +66,7 @@ struct Args {
   int M, N, K;
   int sf_tiles_k;          // 512-byte scale tiles per 128-row block
   int n_tiles;
-  int early;               // the next launch is of the same chain and may start
+  int early;               // the next launch may come up under this one
 };
 
 __device__ __forceinline__ float2 unpack2(uint32_t w, __nv_bfloat16) { return bf16x2_to_f2(w); }
@@ -368,7 +368,7 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
           // launch, which produces A, is done
           kb = min(num_kb, P_STAGES);
           for (int i = 0; i < kb; ++i) load_b(i, i, n0);
-          mx::grid_wait();
+          grid_wait();
           for (int i = 0; i < kb; ++i) load_a(i, i, m0);
           g = kb;
         }
@@ -449,8 +449,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(THREADS, 1)
     const uint32_t leader_acc_empty = mapa_shared(smem_u32(acc_empty), 0);
     const uint32_t rbar = smem_u32(&res_full[ew]);
     uint32_t i = 0, loads = 0;
-    mx::grid_wait();                     // residual and D follow the chain's earlier launches
-    if (p.early) mx::grid_launch_dependents();
+    grid_wait();                     // residual and D follow the chain's earlier launches
+    if (p.early) grid_launch_dependents();
     if (EPI != kSwigluQuant && lane == 0) {
       prefetch_tmap(&p.tmap_d);
       if (p.residual) prefetch_tmap(&p.tmap_r);

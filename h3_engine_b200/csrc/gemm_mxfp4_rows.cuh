@@ -16,10 +16,8 @@
 //
 // Inside one entry point's chain of launches (quantize, product, or quantize,
 // up, down) the weight's loads do not depend on the launch before, which only
-// produces the activation's codes: there the kernel is launched with
-// programmatic stream serialization and fills its ring before it waits for that
-// launch.  The first launch of a chain is an ordinary one, so whatever the
-// stream did before the call, a weight's own quantization included, is done.
+// produces the activation's codes: there the kernel fills its ring before it
+// waits for that launch.
 #pragma once
 
 #include "gemm_mxfp4.cuh"
@@ -72,13 +70,13 @@ struct Args {
   int M, N, K;
   int sf_tiles_k;
   int act;
-  int early;               // the next launch is of the same chain and may start
+  int first;               // of a call: the weight, too, follows the launches before
 };
 
 // Four consecutive 16-bit values.
 template <typename T>
 __device__ __forceinline__ float4 load4(const T* p) {
-  const uint2 w = __ldg(reinterpret_cast<const uint2*>(p));
+  const uint2 w = *reinterpret_cast<const uint2*>(p);
   const float2 a = mxgemm::unpack2(w.x, T()), b = mxgemm::unpack2(w.y, T());
   return make_float4(a.x, a.y, b.x, b.y);
 }
@@ -221,9 +219,10 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
         tma_load_2d(smem_u32(sX(s)), &p.tmap_x, kb * KB_BYTES, m0, fb);
         bulk_load(smem_u32(sSFX(s)), sfx + (size_t)kb * KB_ATOMS * SF_ATOM, sf_bytes(kb), fb);
       };
+      if (p.first) grid_wait();
       const int n = kb1 - kb0, head = min(n, R::STAGES);
       for (int i = 0; i < head; ++i) load_w(kb0 + i, i);
-      if (!FUSED) mx::grid_wait();           // the activation's codes are there from here on
+      if (!FUSED) grid_wait();           // the activation's codes are there from here on
       for (int i = 0; i < head; ++i) load_x(kb0 + i, i);
       int issued = head;
       bool ok = true;
@@ -280,7 +279,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
       mbar_wait(smem_u32(drain), 0, nullptr);
     }
   } else {
-    mx::grid_wait();                         // x, bias, residual and out follow earlier work
+    grid_wait();                         // x, bias, residual and out follow earlier work
     if (FUSED) {
       // k-block i of the rows: lane l holds values 8 l .. 8 l + 7 of a row
       for (int i = warp - 2; i < kb1 - kb0; i += 4) {
@@ -320,7 +319,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
         if (lane == 0) mbar_arrive(smem_u32(&full[s]));
       }
     }
-    if (p.early) mx::grid_launch_dependents();
+    grid_launch_dependents();
     // partial D^T of this CTA, row-major [MT][128], over the ring (every load
     // has landed and been read when the accumulator is complete)
     float* part = reinterpret_cast<float*>(smem);
@@ -353,7 +352,7 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
   const uint32_t base = smem_u32(smem);
   // (warps 0 and 1 have not waited for the chain's earlier launches: the
   // residual and out are theirs too)
-  mx::grid_wait();
+  grid_wait();
   if (EPI == mxgemm::kOut) {
     // 32 threads cover a row's 128 columns, four each
     const int c = (threadIdx.x & 31) * 4, n = n0 + c;

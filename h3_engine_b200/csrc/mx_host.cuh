@@ -24,6 +24,33 @@ struct SmemAttr {
   }
 };
 
+// One launch, as clusters of `cluster` CTAs along x.  early: it may come up
+// under the end of the launch before it in the stream (common.cuh has the rules;
+// one token against a cache of 4100 keys in a row of such calls: 7.8 us, 10.3 as
+// an ordinary launch).
+template <typename... P, typename... A>
+static int launch(bool early, void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster,
+                  cudaStream_t st, const A&... args) {
+  cudaLaunchConfig_t cfg = {};
+  cfg.gridDim = grid;
+  cfg.blockDim = dim3((unsigned)threads);
+  cfg.dynamicSmemBytes = (size_t)smem;
+  cfg.stream = st;
+  cudaLaunchAttribute at[2];
+  cfg.attrs = at;
+  if (early) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    at[cfg.numAttrs++].val.programmaticStreamSerializationAllowed = 1;
+  }
+  if (cluster > 0) {
+    at[cfg.numAttrs].id = cudaLaunchAttributeClusterDimension;
+    at[cfg.numAttrs].val.clusterDim.x = (unsigned)cluster;
+    at[cfg.numAttrs].val.clusterDim.y = 1;
+    at[cfg.numAttrs++].val.clusterDim.z = 1;
+  }
+  return launched(cudaLaunchKernelEx(&cfg, kernel, args...));
+}
+
 // 2-D tensor of 16-bit values, box box_cols x box_rows, 128-byte swizzle.
 static int make_tmap_16_sw128(CUtensorMap* map, const void* base, int dtype, uint64_t rows,
                               uint64_t cols, uint64_t pitch_elems, uint32_t box_cols,
@@ -58,26 +85,26 @@ static unsigned mx_quant_blocks(int64_t units) {
 }
 
 template <typename T, int VPL>
-static void mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
-                               bool early, cudaStream_t st) {
+static int mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
+                              cudaStream_t st) {
   constexpr int kUnit = 32 * VPL * kQuantUnroll;
   const int64_t Mpad = (M + 127) / 128 * 128;
   const int64_t per_row = (mx::sf_tiles(K) * 128 + kUnit - 1) / kUnit;
-  mx::k_mxfp4_quantize<T, VPL, kQuantUnroll>
-      <<<mx_quant_blocks(Mpad * per_row), mx::kThreads, 0, st>>>(
-          static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q),
-          static_cast<uint8_t*>(sf), Mpad, (uint32_t)per_row, early);
+  return launch(true, mx::k_mxfp4_quantize<T, VPL, kQuantUnroll>,
+                      dim3(mx_quant_blocks(Mpad * per_row)), mx::kThreads, 0, 0, st,
+                      static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q),
+                      static_cast<uint8_t*>(sf), Mpad, (uint32_t)per_row);
 }
 
 template <typename T, int VPL>
-static void mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
-                                 int64_t ldo, cudaStream_t st) {
+static int mx_dequantize_launch(const void* q, const void* sf, int64_t M, int64_t K, void* out,
+                                int64_t ldo, cudaStream_t st) {
   constexpr int kUnit = 32 * VPL * kQuantUnroll;
   const int64_t per_row = (K + kUnit - 1) / kUnit;
-  mx::k_mxfp4_dequantize<T, VPL, kQuantUnroll>
-      <<<mx_quant_blocks(M * per_row), mx::kThreads, 0, st>>>(
-          static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
-          static_cast<T*>(out), ldo, (uint32_t)per_row);
+  return launch(true, mx::k_mxfp4_dequantize<T, VPL, kQuantUnroll>,
+                      dim3(mx_quant_blocks(M * per_row)), mx::kThreads, 0, 0, st,
+                      static_cast<const uint8_t*>(q), static_cast<const uint8_t*>(sf), M, K,
+                      static_cast<T*>(out), ldo, (uint32_t)per_row);
 }
 
 // 32-byte accesses where base and rows allow them.
@@ -86,7 +113,7 @@ static inline bool wide_rows(const void* p, int64_t ld, int size) {
 }
 
 static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
-                       void* sf, bool early, cudaStream_t st) {
+                       void* sf, cudaStream_t st) {
   if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldx < K) return H3B_ERR_INVALID_ARG;
   if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
   if (M == 0) return H3B_OK;
@@ -96,13 +123,12 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   const bool wide = wide_rows(x, ldx, dt_bytes(dtype));
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (wide) mx_quantize_launch<T, 16>(x, M, K, ldx, q, sf, early, st);
-    else mx_quantize_launch<T, 8>(x, M, K, ldx, q, sf, early, st);
+    return wide ? mx_quantize_launch<T, 16>(x, M, K, ldx, q, sf, st)
+                : mx_quantize_launch<T, 8>(x, M, K, ldx, q, sf, st);
   };
-  if (dtype == H3B_DT_BF16) go(__nv_bfloat16());
-  else if (dtype == H3B_DT_F16) go(__half());
-  else go(float());
-  return launched(cudaGetLastError());
+  if (dtype == H3B_DT_BF16) return go(__nv_bfloat16());
+  if (dtype == H3B_DT_F16) return go(__half());
+  return go(float());
 }
 
 // Operands of the CTA-pair kernel: shapes and alignment.
@@ -144,31 +170,30 @@ static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, in
   return H3B_OK;
 }
 
+// chained: the launch before is of the same call, and the weight does not wait
+// for it (a product alone is an ordinary launch).  The next launch comes up under
+// a product in a chain (the feed-forward's up projection), and under one of a
+// single wave of tiles (1025 rows through 2016 x 5504 and back: 31.1 us, else
+// 33.0); under a longer one it costs more than the launch (13383 x 5376 x 7168
+// with its quantization: 237 us, else 231).
 template <typename T, int EPI>
-static int mx_gemm_launch(const mxgemm::PairArgs& pa, bool chained, cudaStream_t st) {
+static int mx_gemm_launch(mxgemm::PairArgs& pa, bool chained, cudaStream_t st) {
   auto kernel = mxgemm::k_gemm_mxfp4_pair<T, EPI>;
   static SmemAttr attr;
   const int rc = attr.set(reinterpret_cast<const void*>(kernel), mxgemm::P_SMEM_BYTES);
   if (rc != H3B_OK) return rc;
   const int64_t tiles = (int64_t)pa.m_tiles * pa.base.n_tiles;
   const int pairs = (int)std::min<int64_t>(tiles, num_sms() / 2);
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)(2 * pairs));
-  cfg.blockDim = dim3(mxgemm::THREADS);
-  cfg.dynamicSmemBytes = mxgemm::P_SMEM_BYTES;
-  cfg.stream = st;
-  cudaLaunchAttribute at[1];
-  at[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[0].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = chained ? 1 : 0;
-  return launched(cudaLaunchKernelEx(&cfg, kernel, pa));
+  pa.base.early = EPI == mxgemm::kSwigluQuant || tiles <= pairs;
+  return launch(chained, kernel, dim3((unsigned)(2 * pairs)), mxgemm::THREADS,
+                mxgemm::P_SMEM_BYTES, 0, st, pa);
 }
 
 // ---- up to 128 rows: the weight-streaming kernel
 template <int MT, typename T, int EPI, bool FUSED>
 static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool chained,
                           cudaStream_t st) {
+  a.first = !chained;
   int rc = make_tmap_u8_sw128(&a.tmap_w, B, (uint64_t)a.N, (uint64_t)(a.K / 2),
                               (uint64_t)(a.K / 2), mxrows::KB_BYTES, mxrows::BN);
   if (rc != H3B_OK) return rc;
@@ -192,21 +217,8 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
   while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles * m_tiles <= 2 * num_sms() &&
          num_kb >= split * 4)
     split *= 2;
-  cudaLaunchConfig_t cfg = {};
-  cfg.gridDim = dim3((unsigned)split, (unsigned)tiles, (unsigned)m_tiles);
-  cfg.blockDim = dim3(mxrows::THREADS);
-  cfg.dynamicSmemBytes = mxrows::Ring<MT>::BYTES;
-  cfg.stream = st;
-  cudaLaunchAttribute at[2];
-  at[0].id = cudaLaunchAttributeClusterDimension;
-  at[0].val.clusterDim.x = (unsigned)split;
-  at[0].val.clusterDim.y = 1;
-  at[0].val.clusterDim.z = 1;
-  at[1].id = cudaLaunchAttributeProgrammaticStreamSerialization;
-  at[1].val.programmaticStreamSerializationAllowed = 1;
-  cfg.attrs = at;
-  cfg.numAttrs = chained ? 2 : 1;
-  return launched(cudaLaunchKernelEx(&cfg, kernel, a));
+  return launch(true, kernel, dim3((unsigned)split, (unsigned)tiles, (unsigned)m_tiles),
+                      mxrows::THREADS, mxrows::Ring<MT>::BYTES, split, st, a);
 }
 
 // Operands of the rows kernel: A as codes and scales, or (sfA NULL) as 16-bit
@@ -326,7 +338,7 @@ extern "C" {
 
 int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
                        void* sf, void* stream) {
-  return mx_quantize(x, dtype, M, K, ldx, q, sf, false, static_cast<cudaStream_t>(stream));
+  return mx_quantize(x, dtype, M, K, ldx, q, sf, static_cast<cudaStream_t>(stream));
 }
 
 int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, void* out, int dtype,
@@ -340,13 +352,12 @@ int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, vo
   const bool wide = wide_rows(out, ldo, dt_bytes(dtype));
   auto go = [&](auto t) {
     using T = decltype(t);
-    if (wide) mx_dequantize_launch<T, 16>(q, sf, M, K, out, ldo, st);
-    else mx_dequantize_launch<T, 8>(q, sf, M, K, out, ldo, st);
+    return wide ? mx_dequantize_launch<T, 16>(q, sf, M, K, out, ldo, st)
+                : mx_dequantize_launch<T, 8>(q, sf, M, K, out, ldo, st);
   };
-  if (dtype == H3B_DT_BF16) go(__nv_bfloat16());
-  else if (dtype == H3B_DT_F16) go(__half());
-  else go(float());
-  return launched(cudaGetLastError());
+  if (dtype == H3B_DT_BF16) return go(__nv_bfloat16());
+  if (dtype == H3B_DT_F16) return go(__half());
+  return go(float());
 }
 
 int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, const void* sfB,
@@ -381,7 +392,7 @@ int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const voi
                        false, st);
   uint8_t* q = static_cast<uint8_t*>(ws);
   uint8_t* sf = q + mx_code_bytes(M, K);
-  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, true, st);
+  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, st);
   if (rc != H3B_OK) return rc;
   return mx_gemm_out(q, sf, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, true, st);
 }
@@ -409,7 +420,7 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   uint8_t* sfh = qh + mx_code_bytes(M, F);
   const bool fused = M <= mxrows::kFusedRows;
   if (!fused) {
-    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, true, st);
+    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, st);
     if (rc != H3B_OK) return rc;
   }
   if (mx_by_rows(M, 2 * F, N)) {
@@ -417,7 +428,6 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
     memset(&a, 0, sizeof(a));
     a.q_out = qh;
     a.sf_out = sfh;
-    a.early = 1;
     const void* A = fused ? x : q;
     const void* sfA = fused ? nullptr : sf;
     rc = dtype == H3B_DT_F16
@@ -431,7 +441,6 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
     if (rc != H3B_OK) return rc;
     up.base.q_out = qh;
     up.base.sf_out = sfh;
-    up.base.early = 1;
     rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, true, st);
   }
   if (rc != H3B_OK) return rc;

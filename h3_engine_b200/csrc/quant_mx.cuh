@@ -56,13 +56,22 @@ __device__ __forceinline__ uint32_t codes8(const float (&v)[8], float inv) {
   return inv != 0.f ? packed : 0u;
 }
 
+// Loads of what an earlier launch may still be writing while this one starts:
+// ordinary ones (the read-only path wants data that never changes under it).
+__device__ __forceinline__ uint4 ld_v4(const void* p) {
+  uint4 r;
+  asm volatile("ld.global.L1::no_allocate.v4.u32 {%0,%1,%2,%3}, [%4];"
+               : "=r"(r.x), "=r"(r.y), "=r"(r.z), "=r"(r.w) : "l"(p));
+  return r;
+}
+
 // ---------------------------------------------------------------- typed 8-value loads / stores
 template <typename T>
 struct Vec8;                       // 8 values of T as 16-byte words
 template <>
 struct Vec8<__nv_bfloat16> {
   uint4 w;
-  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = ld_nc_v4(p); }
+  __device__ __forceinline__ void load(const __nv_bfloat16* p) { w = ld_v4(p); }
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -76,7 +85,7 @@ struct Vec8<__nv_bfloat16> {
 template <>
 struct Vec8<__half> {
   uint4 w;
-  __device__ __forceinline__ void load(const __half* p) { w = ld_nc_v4(p); }
+  __device__ __forceinline__ void load(const __half* p) { w = ld_v4(p); }
   __device__ __forceinline__ void zero() { w = make_uint4(0, 0, 0, 0); }
   __device__ __forceinline__ void get(float (&v)[8]) const {
     const uint32_t u[4] = {w.x, w.y, w.z, w.w};
@@ -104,21 +113,11 @@ __device__ __forceinline__ uint32_t absmax_bits8(const float (&v)[8]) {
   return m;
 }
 
-// Lets the next launch of the stream start before this one is done, where that
-// launch waits for this one before it reads its results.
-__device__ __forceinline__ void grid_launch_dependents() {
-  asm volatile("griddepcontrol.launch_dependents;" ::: "memory");
-}
-
-// Waits until the launch before this one is done and its results are visible
-// (at once, where this one was not started early).
-__device__ __forceinline__ void grid_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
-
 // ---------------------------------------------------------------- wide accesses
 // 32 bytes per lane in one access (256-bit, 32-byte aligned): a warp moves 1 KiB
 // of one row, whole sectors each.
-__device__ __forceinline__ void ld_nc_v8(const void* p, uint32_t (&r)[8]) {
-  asm volatile("ld.global.nc.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
+__device__ __forceinline__ void ld_v8(const void* p, uint32_t (&r)[8]) {
+  asm volatile("ld.global.L1::no_allocate.v8.b32 {%0,%1,%2,%3,%4,%5,%6,%7}, [%8];"
                : "=r"(r[0]), "=r"(r[1]), "=r"(r[2]), "=r"(r[3]), "=r"(r[4]), "=r"(r[5]),
                  "=r"(r[6]), "=r"(r[7])
                : "l"(p));
@@ -143,11 +142,11 @@ struct Lane {
     if constexpr (VPL == 16) {
 #pragma unroll
       for (int i = 0; i < WORDS / 8; ++i)
-        ld_nc_v8(c + i * 32, *reinterpret_cast<uint32_t(*)[8]>(w + i * 8));
+        ld_v8(c + i * 32, *reinterpret_cast<uint32_t(*)[8]>(w + i * 8));
     } else {
 #pragma unroll
       for (int i = 0; i < WORDS / 4; ++i)
-        *reinterpret_cast<uint4*>(w + i * 4) = ld_nc_v4(c + i * 16);
+        *reinterpret_cast<uint4*>(w + i * 4) = ld_v4(c + i * 16);
     }
   }
   __device__ __forceinline__ void store(T* p) const {
@@ -208,10 +207,10 @@ constexpr int kThreads = 256;
 // last tile are written as 0.
 template <typename T, int VPL, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
-    k_mxfp4_quantize(const T* __restrict__ x, int64_t M, int64_t K, int64_t ldx,
-                     uint8_t* __restrict__ q, uint8_t* __restrict__ sf, int64_t Mpad,
-                     uint32_t units_per_row, int early) {
-  if (early) grid_launch_dependents();
+    k_mxfp4_quantize(const T* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, uint8_t* sf,
+                     int64_t Mpad, uint32_t units_per_row) {
+  grid_wait();
+  grid_launch_dependents();
   constexpr int LPB = BLOCK / VPL;                 // lanes per block
   const int lane = threadIdx.x & 31;
   const int k = (int)K;
@@ -273,8 +272,10 @@ __global__ void __launch_bounds__(kThreads)
 // Units as in the quantizer: a lane turns VPL codes into VPL values of T.
 template <typename T, int VPL, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
-    k_mxfp4_dequantize(const uint8_t* __restrict__ q, const uint8_t* __restrict__ sf, int64_t M,
-                       int64_t K, T* __restrict__ out, int64_t ldo, uint32_t units_per_row) {
+    k_mxfp4_dequantize(const uint8_t* q, const uint8_t* sf, int64_t M, int64_t K, T* out,
+                       int64_t ldo, uint32_t units_per_row) {
+  grid_wait();
+  grid_launch_dependents();
   const int lane = threadIdx.x & 31;
   const int k = (int)K;
   const int64_t c4 = sf_tiles(K);
@@ -294,13 +295,13 @@ __global__ void __launch_bounds__(kThreads)
       const int v = v0 + u * 32 * VPL;
       if (v < k) {
         if constexpr (VPL == 16) {
-          const uint2 c = __ldg(reinterpret_cast<const uint2*>(qr + (v >> 1)));
+          const uint2 c = *reinterpret_cast<const uint2*>(qr + (v >> 1));
           code[u][0] = c.x;
           code[u][1] = c.y;
         } else {
-          code[u][0] = __ldg(reinterpret_cast<const uint32_t*>(qr + (v >> 1)));
+          code[u][0] = *reinterpret_cast<const uint32_t*>(qr + (v >> 1));
         }
-        s[u] = __ldg(sr + (int64_t)(v >> 7) * 512 + ((v >> 5) & 3));
+        s[u] = sr[(int64_t)(v >> 7) * 512 + ((v >> 5) & 3)];
       }
     }
 #pragma unroll

@@ -262,6 +262,73 @@ def test_weights_and_inputs_written_just_before(cuda, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [1, 5, 12, 100, 300])
+def test_calls_in_a_row_follow_each_other(cuda, m):
+    """Kernels come up under the end of the one before: in a row without a pause,
+    eager and captured, calls that reuse one another's buffers give what they
+    give with a synchronisation after each."""
+    d, f = 256, 512
+    w = mxfp4.MXFP4Weight(rand(d, d, scale=0.1).to(BF16).to(cuda))
+    up = mxfp4.gated_up_weight(rand(2 * f, d, seed=1, scale=0.1).to(BF16).to(cuda))
+    down = mxfp4.MXFP4Weight(rand(d, f, seed=2, scale=0.1).to(BF16).to(cuda))
+    x0 = rand(m, d, seed=3).to(BF16).to(cuda)
+    cache = rand(2, 600, 2, 128, seed=4).to(BF16).to(cuda)
+    n = torch.tensor([m + 300, 7], dtype=torch.int32, device=cuda)
+    a, b, o = (torch.empty_like(x0) for _ in range(3))
+    q, sf = ops.mxfp4_quantize(x0)
+    x, dec = x0.clone(), torch.empty(2, 1, 2, 128, dtype=BF16, device=cuda)
+
+    def step(pause):
+        mxfp4.mxfp4_linear(w, x, residual=x0, out=a)
+        pause()
+        ops.attention_window(a, x, x0, 2, 128, [0, m], window=(40, 40), sinks=2, out=o)
+        pause()
+        cache[0, :1].copy_(o.view(m, 2, 128)[:1])
+        pause()
+        ops.attention_window_decode(o[-1:].view(1, 1, 2, 128).expand(2, 1, 2, 128), cache, cache, n,
+                                    out=dec)
+        pause()
+        o[:1] += dec[0].view(1, d)
+        pause()
+        mxfp4.gated_ffn(up, down, o, residual=a, out=b)
+        pause()
+        ops.mxfp4_quantize(b, q_out=q, sf_out=sf)
+        pause()
+        ops.mxfp4_dequantize(q, sf, m, d, out=x)
+        pause()
+        ops.mxfp4_gemm(q, sf, m, w.qdata, w.scale, d, d, residual=x, out=x)
+        pause()
+        torch.clamp_(x, -4, 4)
+        pause()
+
+    def reset():
+        x.copy_(x0)
+        cache[0, :1].zero_()
+
+    reset()
+    for _ in range(6):
+        step(torch.cuda.synchronize)
+    want = x.clone(), dec.clone()
+    for _ in range(10):
+        reset()
+        for _ in range(6):
+            step(lambda: None)
+        assert torch.equal(x, want[0]) and torch.equal(dec, want[1])
+    side = torch.cuda.Stream()
+    side.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(side):
+        with torch.cuda.graph(graph, stream=side):
+            for _ in range(6):
+                step(lambda: None)
+    torch.cuda.current_stream().wait_stream(side)
+    for _ in range(10):
+        reset()
+        graph.replay()
+        assert torch.equal(x, want[0]) and torch.equal(dec, want[1])
+
+
+@pytest.mark.gpu
 def test_outputs_must_stand_apart(cuda):
     w = mxfp4.MXFP4Weight(rand(64, 64).to(BF16).to(cuda))
     buf = rand(9, 64).to(BF16).to(cuda)
