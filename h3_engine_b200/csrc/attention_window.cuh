@@ -24,6 +24,14 @@
 // workspace, and the part that finishes last adds them up, in part order, so
 // the result does not depend on which one that is.
 //
+// What bounds it: a tile's own cycle, softmax (1920 clocks per 128 x 128 step, of
+// which the exponentials take at least 1024), P V (512) and Q K^T (512), which P
+// over S makes take turns; the other tile's products run under the softmax.  8
+// heads of 16384 rows that see 3200 keys each: 212 us, 962 TFLOP/s.  Measured and
+// not taken: two S buffers per tile with steps of 64 keys (252 us: a product of
+// 64 keys is bound by reading shared memory), two warpgroups per tile (232), a
+// polynomial for part of the exponentials (222).
+//
 // Rows of V behind the last visible key of a step (the document's end, the
 // next document, the gap behind the sinks) are cleared in shared memory before
 // the MMA reads them: their P is 0, and 0 times what lies there must be 0.
@@ -48,14 +56,18 @@ constexpr int kPrefetchTiles = 4;
 // 64 the products are half as long while the softmax is not, and two softmax
 // warps per scheduler leave it idle half the time; steps of 64 keys need half
 // the registers and tensor memory, so two CTAs share an SM, where there are
-// more CTAs than SMs (148 of them: 19 us in steps of 128, 22 in steps of 64;
-// 240: 35 and 30).
+// more CTAs than SMs (148 of them: 18.4 us in steps of 128, 20.5 in steps of
+// 64; 240: 35.8 and 27.9).
 template <int D, int KEYS>
 struct Cfg {
   static constexpr int BK = KEYS;                          // keys per step
   static constexpr int CTAS = BK == 128 ? 1 : 2;           // per SM
   static constexpr int THREADS = BK == 128 ? 384 : 320;
-  static constexpr int HALVES = BK / 64;                   // P reaches the MMA 64 keys at a time
+  // P reaches the MMA in two pieces: the first 96 keys' products run under the
+  // exponentials of the last 32 (in halves of 64 the second half's were waited
+  // for: 16384 rows, 8 heads 218 us, 214 so)
+  static constexpr int HALVES = BK / 64;
+  static constexpr int P_FIRST = BK == 128 ? 96 : BK;
   static constexpr uint32_t TMEM_COLS = 512 / CTAS;
   static constexpr int Q_BOX = 128 * 128;                  // 128 rows x 64 columns
   static constexpr int Q_BYTES = (D / 64) * Q_BOX;
@@ -139,27 +151,6 @@ struct Steps {
   }
 };
 
-// 2^x for two lanes on the FMA pipe, as attention.cuh's ex2_poly2 but keeping
-// NaN logits NaN (or at least not finite).
-__device__ __forceinline__ float max_nan(float a, float b) {
-  float d;
-  asm("max.NaN.f32 %0, %1, %2;" : "=f"(d) : "f"(a), "f"(b));
-  return d;
-}
-__device__ __forceinline__ float2 ex2_poly2(float2 x) {
-  x.x = max_nan(x.x, -120.0f);
-  x.y = max_nan(x.y, -120.0f);
-  const float2 magic = make_float2(12582912.0f, 12582912.0f);
-  const float2 t = add2(x, magic);
-  const float2 f = sub2(x, sub2(t, magic));
-  float2 q = fma2(f, make_float2(0.05459282547235489f, 0.05459282547235489f),
-                  make_float2(0.24221783876419067f, 0.24221783876419067f));
-  q = fma2(f, q, make_float2(0.6933686137199402f, 0.6933686137199402f));
-  q = fma2(f, q, make_float2(1.0f, 1.0f));
-  return make_float2(__int_as_float(__float_as_int(q.x) + (__float_as_int(t.x) << 23)),
-                     __int_as_float(__float_as_int(q.y) + (__float_as_int(t.y) << 23)));
-}
-
 template <typename T>
 __device__ __forceinline__ uint32_t pack16(float lo, float hi) {
   if constexpr (std::is_same<T, __half>::value) {
@@ -190,44 +181,28 @@ __device__ __forceinline__ void tmem_st_x16(uint32_t taddr, const uint32_t (&r)[
       : "memory");
 }
 
-// P = 2^(S * scale - m) of one row's BK keys, stored as 16-bit pairs over BK / 2
-// columns of tensor memory; returns the row sum.  P is rounded to 16 bits
-// because the tensor core reads it so; the sum is of the unrounded fp32 values.
-// 3 of 8 pairs go to the polynomial; a masked key (S = -inf) that falls there
-// gives 2^-120 instead of 0, which no sum of 2^0 or more notices (a row's sum
-// holds its maximum's 2^0, and a row that sees nothing is told by its range).
-template <typename T, int BK>
-__device__ __forceinline__ float softmax_store(uint32_t (&sv)[BK], float scale_log2, float m,
-                                               uint32_t p_addr, uint32_t half_bar) {
+// P = 2^(S * scale - m) of keys [K0, K0 + N) of a row, stored as 16-bit pairs over
+// tensor memory from p_addr; adds them to acc.  P is rounded to 16 bits because
+// the tensor core reads it so; the sum is of the unrounded fp32 values.  A masked
+// key's S is -inf and its P 0.
+template <typename T, int K0, int N, int BK>
+__device__ __forceinline__ void softmax_store(const uint32_t (&sv)[BK], float scale_log2, float m,
+                                              uint32_t p_addr, float2 (&acc)[2]) {
   const float2 sc = make_float2(scale_log2, scale_log2);
   const float2 nm = make_float2(-m, -m);
-  float2 acc0 = make_float2(0.f, 0.f), acc1 = make_float2(0.f, 0.f);
-  constexpr int G = BK == 64 ? 16 : 32;            // pairs packed before a store
 #pragma unroll
-  for (int h = 0; h < BK / (2 * G); ++h) {
-    uint32_t pk[G];
+  for (int g = 0; g < N / 32; ++g) {
+    uint32_t pk[16];
 #pragma unroll
-    for (int c = 0; c < G; ++c) {
-      const int k = h * 2 * G + 2 * c;
+    for (int c = 0; c < 16; ++c) {
+      const int k = K0 + g * 32 + 2 * c;
       const float2 x = fma2(make_float2(__uint_as_float(sv[k]), __uint_as_float(sv[k + 1])), sc, nm);
-      float2 e;
-      if ((attn::kPolyPairs >> (c & 7)) & 1u) e = ex2_poly2(x);
-      else e = make_float2(attn::ex2(x.x), attn::ex2(x.y));
-      if (c & 1) acc1 = add2(acc1, e);
-      else acc0 = add2(acc0, e);
+      const float2 e = make_float2(attn::ex2(x.x), attn::ex2(x.y));
+      acc[c & 1] = add2(acc[c & 1], e);
       pk[c] = pack16<T>(e.x, e.y);
     }
-    if constexpr (G == 16) tmem_st_x16(p_addr + h * G, pk);
-    else tmem_st_32x32b_x32(p_addr + h * G, pk);
-    if (h == 0 && BK > 64) {
-      tmem_st_wait();
-      tc_fence_before();
-      __syncwarp();
-      if ((threadIdx.x & 31) == 0) mbar_arrive(half_bar);
-    }
+    tmem_st_x16(p_addr + K0 / 2 + g * 16, pk);
   }
-  const float2 s = add2(acc0, acc1);
-  return s.x + s.y;
 }
 
 // Bits [a, b] of 32-bit word w of a 128-bit mask (a, b any ints).
@@ -263,7 +238,7 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
   uint64_t* p_full = bars + 7;       // 2
   uint64_t* pv_done = bars + 9;      // 2: the last PV of a tile
   uint64_t* drain = bars + 11;       // 1
-  uint64_t* p_half = bars + 12;      // 2: P of the first 64 keys of 128
+  uint64_t* p_half = bars + 12;      // 2: P of the first 96 keys of 128
   uint32_t* tmem_slot = reinterpret_cast<uint32_t*>(bars + 16);
   volatile int* abort_flag = reinterpret_cast<volatile int*>(tmem_slot + 1);
 
@@ -427,8 +402,8 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
           if (!wait(h == L::HALVES - 1 ? &p_full[t] : &p_half[t], cnt[t] & 1)) return false;
           tc_fence_after();
 #pragma unroll
-          for (int i = 0; i < 4; ++i) {
-            const int kk = h * 4 + i;
+          for (int kk = h * (L::P_FIRST / 16); kk < (h + 1 == L::HALVES ? BK : L::P_FIRST) / 16;
+               ++kk) {
             tc_mma_bf16_ts_elect(tmem + L::o_col(t), tmem + L::s_col(t) + kk * 8,
                                  vd + kk * (2048 >> 4), IDESC_PV, (cnt[t] | kk) != 0);
           }
@@ -541,29 +516,37 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
       }
       const float mx = fmaxf(fmaxf(m4[0], m4[1]), fmaxf(m4[2], m4[3])) * p.scale_log2;
       const float m_new = fmaxf(m_used, mx);
-      const bool rescale = __any_sync(0xffffffffu, m_new > m_used + attn::kRescaleLog2);
-      float alpha = 1.f;
-      if (rescale) {
+      if (__any_sync(0xffffffffu, m_new > m_used + attn::kRescaleLog2)) {
         // a row that has seen nothing yet stays at -inf (its l and O are 0)
-        alpha = m_new == -INFINITY ? 1.f : attn::ex2(m_used - m_new);
+        const float alpha = m_new == -INFINITY ? 1.f : attn::ex2(m_used - m_new);
         m_used = m_new;
-      }
-      if (rescale && cnt > 0) {
-        // O is final up to the previous needed step: s_full of this one was
-        // committed after its PV
+        l *= alpha;
+        if (cnt > 0) {
+          // O is final up to the previous needed step: s_full of this one was
+          // committed after its PV
+#pragma unroll 1
+          for (int h = 0; h < D / 16; ++h) {               // 16 at a time: S is in registers
+            uint32_t ov[16];
+            tmem_ld_x16(o_t + h * 16, ov);
+            tmem_ld_wait();
 #pragma unroll
-        for (int h = 0; h < D / 16; ++h) {                 // 16 at a time: S is in registers
-          uint32_t ov[16];
-          tmem_ld_x16(o_t + h * 16, ov);
-          tmem_ld_wait();
-#pragma unroll
-          for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
-          tmem_st_x16(o_t + h * 16, ov);
+            for (int c = 0; c < 16; ++c) ov[c] = __float_as_uint(__uint_as_float(ov[c]) * alpha);
+            tmem_st_x16(o_t + h * 16, ov);
+          }
         }
       }
-      const uint32_t hb = smem_u32(&p_half[t]);
       const float m = m_used == -INFINITY ? 0.f : m_used;   // -inf - (-inf) is no exponent
-      l = l * alpha + softmax_store<T, BK>(sv, p.scale_log2, m, s_t, hb);
+      float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
+      softmax_store<T, 0, L::P_FIRST>(sv, p.scale_log2, m, s_t, acc);
+      if constexpr (L::HALVES == 2) {
+        tmem_st_wait();
+        tc_fence_before();
+        __syncwarp();
+        if (lane == 0) mbar_arrive(smem_u32(&p_half[t]));
+        softmax_store<T, L::P_FIRST, BK - L::P_FIRST>(sv, p.scale_log2, m, s_t, acc);
+      }
+      acc[0] = add2(acc[0], acc[1]);
+      l += acc[0].x + acc[0].y;
       tmem_st_wait();
       tc_fence_before();
       __syncwarp();

@@ -60,14 +60,14 @@ static int64_t window_keys(int64_t n_k, int64_t left, int64_t right, int64_t sin
 // most keys first (the light items then fill the last wave's gaps), and how
 // their work is cut.
 //   Items of 256 queries, or of 128 where those all have a place at once (1000
-// rows, 8 heads: 19.0 us, in items of 256 21.0; 16384 rows, where they have
-// not: 341 us, in items of 256 221), unless items of 256 can be cut into 3/2 as
+// rows, 8 heads: 17.9 us, in items of 256 19.5; 16384 rows, where they have
+// not: 334 us, in items of 256 212), unless items of 256 can be cut into 3/2 as
 // many parts.  The ratio lies between the cases measured: with as many parts
-// items of 128 win as above, with twice as many items of 256 do (2000 rows:
-// 32.8 us, in items of 128 33.8; head_dim 64 26.7 and 29.2).
+// items of 128 win as above, with twice as many items of 256 do (4000 rows, 2
+// heads: 32.9 us, in items of 128 40.5).
 //   Whole items first, then the last partial wave's in parts: items mod places
 // would run alone, so they are split to fill the places (8 heads of 16384 rows,
-// 512 items on 148 SMs: 221 us, unsplit 230).  A part keeps kPartKeys keys.
+// 512 items on 148 SMs: 212 us, unsplit 220).  A part keeps kPartKeys keys.
 struct WindowPlan {
   static constexpr int64_t kPartKeys = 512;
   int order[wattn::MAX_DOCS];
