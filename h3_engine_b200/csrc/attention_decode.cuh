@@ -2,8 +2,9 @@
 // read on the device (so a captured launch serves every step): the visibility
 // rule of attention_window.cuh for queries at positions len - n_new ... len - 1.
 //
-// Bound by reading the visible keys and values once.  The rows that share a key
-// head, n_new tokens times the group's query heads, are the 8 (or twice 8)
+// Bound by reading the visible keys and values once: 32 uneven sequences (503 MB)
+// in 75.7 us, 6.6 TB/s; one sequence of 4100 keys (16.8 MB) in 7.6 us, where
+// latencies are half of it.  The rows that share a key head, n_new tokens times the group's query heads, are the 8 (or twice 8)
 // columns of mma.sync m16n8k16 products with the keys on the other side:
 // S^T = K Q^T and O^T = V^T P^T, which for up to 8 rows takes half the
 // instructions of the form with 16 rows of queries.  A warp's work is a flash

@@ -130,8 +130,8 @@ static int window_decode_rows(const wdec::Args& a, int64_t B, cudaStream_t st) {
   const int64_t groups = row_tiles * a.kv_heads;
   if (groups > 65535 || B > 65535) return H3B_ERR_INVALID_ARG;
   // CTAs along the keys: until there are two per SM, which run at a time (32
-  // uneven sequences of 8 key heads: 135 us without a split, 84 with 512 CTAs,
-  // 89 with 1024, 106 with 2048), but no more than give every warp two tiles
+  // uneven sequences of 8 key heads: 91 us without a split, 76 with 512 CTAs,
+  // 77 with 1024, 93 with 2048), but no more than give every warp two tiles
   // of a full window
   const int64_t most =
       std::min<int64_t>(a.room, (int64_t)a.left + a.right + a.n_new + (int64_t)a.sinks);

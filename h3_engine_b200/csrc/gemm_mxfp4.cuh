@@ -4,12 +4,16 @@
 // (tcgen05.mma kind::mxf4, scale_vec::2X: K = 64 and two scales per row and
 // instruction).
 //
-// The scales are half as many as NVFP4's: one 128 x 4 tile
-// of them (512 bytes, one tcgen05.cp of 4 TMEM columns) serves two MMA k-steps,
-// chosen by the scale-factor id of the instruction descriptor (bytes 0-1 or
-// 2-3 of each 32-bit column).  K is any multiple of 32: TMA fills the codes
-// past K with zeros, the last k-block issues only the k-steps that hold values,
-// and the scale bytes past K/32 are zeros (2^-127) by the format.
+// The scales are half as many as NVFP4's: one 128 x 4 tile of them (512 bytes,
+// one tcgen05.cp of 4 TMEM columns) serves two MMA k-steps, chosen by the
+// scale-factor id of the instruction descriptor (bytes 0-1 or 2-3 of each 32-bit
+// column).  K is any multiple of 32: TMA fills the codes past K with zeros, the
+// last k-block issues only the k-steps that hold values, and the scale bytes
+// past K/32 are zeros (2^-127) by the format.
+//
+// Bound by the tensor core's pipe: 256 values of K of a 256 x 256 tile take about
+// 650 clocks, 512 of them the MMAs and the rest the copies of the scales, which
+// share the pipe.  13383 x 28672 x 5376: 735 us, 5.6 PFLOP/s.
 #pragma once
 
 #include "common.cuh"

@@ -13,6 +13,8 @@
 // the CTAs then each add up a share of the rows over distributed shared memory,
 // always in rank order, and run the epilogue.  Two CTAs fit an SM, and a CTA's
 // share of K usually fits its ring, so the whole weight is in flight at once.
+// 1 x 7168 x 5376 (20.5 MB): 6.9 us, 3 TB/s, the rest of it the launch, the first
+// loads' latency and the cluster's two barriers.
 //
 // Inside one entry point's chain of launches (quantize, product, or quantize,
 // up, down) the weight's loads do not depend on the launch before, which only

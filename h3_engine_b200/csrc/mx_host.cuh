@@ -26,8 +26,8 @@ struct SmemAttr {
 
 // One launch, as clusters of `cluster` CTAs along x.  early: it may come up
 // under the end of the launch before it in the stream (common.cuh has the rules;
-// one token against a cache of 4100 keys in a row of such calls: 7.8 us, 10.3 as
-// an ordinary launch).
+// one token against a cache of 4100 keys, calls in a row: 8.4 us, 10.4 as an
+// ordinary launch).
 template <typename... P, typename... A>
 static int launch(bool early, void (*kernel)(P...), dim3 grid, int threads, int smem, int cluster,
                   cudaStream_t st, const A&... args) {
@@ -210,8 +210,8 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
   const int num_kb = (a.K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS;
   // CTAs along K, a power of two of them (clusters of odd sizes do not all find
   // room at once): while two per SM hold them all and two k-blocks are left to
-  // each (1 x 7168 x 5376: 10.2 us on one, 8.4 on two, 8.0 on four; 77 x 4136 x
-  // 2720: 12.6, 10.6, 9.6 and, with one k-block each on eight, 10.8)
+  // each (1 x 7168 x 5376: 9.1 us on one, 7.3 on two, 6.9 on four; 77 x 4136 x
+  // 2720: 11.5, 9.5, 8.5 and, with one k-block each on eight, 9.6)
   int split = 1;
   const int m_tiles = (a.M + MT - 1) / MT;      // more than one only for MT = 128
   while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles * m_tiles <= 2 * num_sms() &&
@@ -274,10 +274,10 @@ static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* 
 
 // Which kernel: the rows kernel up to 128 rows, and beyond them in tiles of 128
 // where the pair kernel would leave most SMs idle over a long K: where three
-// CTAs along K find room for each of its tiles (144 x 2048 x 5376: 12.0 us
-// against 15.0, 512 x 2048 x 5376: 13.4 and 15.2, 256 x 5376 x 14336: 22.8 and
-// 28.7; past that 512 x 5376 x 14336: 35.0 and 30.0; with K = 2048 the pair
-// kernel is ahead, 256 x 5376: 12.3 and 10.7).
+// CTAs along K find room for each of its tiles (144 x 2048 x 5376: 11.1 us
+// against 13.5, 512 x 2048 x 5376: 12.8 and 13.4, 256 x 5376 x 14336: 22.3 and
+// 26.9; past that 512 x 5376 x 14336: 34.1 and 28.7; with K = 2048 the pair
+// kernel is ahead, 256 x 5376: 11.2 and 9.5).
 static bool mx_by_rows(int64_t M, int64_t N, int64_t K) {
   return M <= mxrows::kMaxRows ||
          (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms());
