@@ -535,15 +535,26 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
           }
         }
       }
-      const float m = m_used == -INFINITY ? 0.f : m_used;   // -inf - (-inf) is no exponent
+      float m = m_used == -INFINITY ? 0.f : m_used;         // -inf - (-inf) is no exponent
+      float sc = p.scale_log2;
+      // S * scale - m is one rounding of the exact product against a maximum that
+      // was rounded before: the same for all keys of the row, so it cancels, but
+      // from 2^27 on it reaches 2^3 and P its type's limit.  Then both are rounded.
+      if (__any_sync(0xffffffffu, fabsf(m) > 16777216.f)) {
+#pragma unroll
+        for (int c = 0; c < BK; ++c)
+          sv[c] = __float_as_uint(__fsub_rn(__fmul_rn(__uint_as_float(sv[c]), sc), m));
+        m = 0.f;
+        sc = 1.f;
+      }
       float2 acc[2] = {make_float2(0.f, 0.f), make_float2(0.f, 0.f)};
-      softmax_store<T, 0, L::P_FIRST>(sv, p.scale_log2, m, s_t, acc);
+      softmax_store<T, 0, L::P_FIRST>(sv, sc, m, s_t, acc);
       if constexpr (L::HALVES == 2) {
         tmem_st_wait();
         tc_fence_before();
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&p_half[t]));
-        softmax_store<T, L::P_FIRST, BK - L::P_FIRST>(sv, p.scale_log2, m, s_t, acc);
+        softmax_store<T, L::P_FIRST, BK - L::P_FIRST>(sv, sc, m, s_t, acc);
       }
       acc[0] = add2(acc[0], acc[1]);
       l += acc[0].x + acc[0].y;

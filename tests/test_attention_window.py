@@ -214,6 +214,45 @@ def test_many_documents_and_large_logits(cuda):
     check_packed(got.cpu(), q, k, v, cq, ck, 1, 1, 64, rule)
 
 
+def one_hot_rows(q, k, see, scale):
+    """The key each query picks, and which queries pick one for certain: where the
+    second logit is further below than the kernel's error on both and the
+    exponent that rounds to 0, every weight but one is exactly 0."""
+    q, k = q.double(), k.double()
+    z = (q @ k.T * scale).masked_fill(~see, -1e300)
+    dz = (q.abs() @ k.abs().T).amax(-1) * scale * (q.shape[1] + 2) * 2.0 ** -23
+    top = z.topk(2, -1).values
+    return z.argmax(-1), top[:, 0] - top[:, 1] > 2 * dz + 200
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("size", [2.0 ** 10, 2.0 ** 14, 2.0 ** 30])
+@pytest.mark.parametrize("d", [64, 128])
+def test_huge_logits_pick_one_key(cuda, size, d):
+    """Logits of 10^7 ... 10^18: one weight is 1 and the others 0."""
+    n, rule = 300, (200, 50, 3, False)
+    q, k, v, cq, _ = packed_case([n], [n], 2, 1, d, BF16, seed=8)
+    q, k = q * size, k * size
+    dev = [t.to(cuda) for t in (q, k, v)]
+    got = ops.attention_window(*dev, 2, d, cq, kv_heads=1, window=rule[:2], sinks=rule[2]).cpu()
+    one = ops.attention_window_decode(
+        dev[0].view(1, n, 2, d), dev[1].view(1, n, 1, d), dev[2].view(1, n, 1, d),
+        torch.tensor([n], dtype=torch.int32, device=cuda), window=rule[:2], sinks=rule[2],
+        causal=False).cpu().view(n, 2 * d)
+    see = seen_mask(n, n, *rule)
+    for h in range(2):
+        c = slice(h * d, h * d + d)
+        pick, sure = one_hot_rows(q[:, c], k, see, d ** -0.5)
+        assert sure.float().mean() > 0.5
+        # out = round16(round16(P) v / P): P is 2^(z - m) for a maximum m so far, no
+        # power of two, so its rounding shows beside the output's: half a step each
+        # (their product and the division's 2^-22 are in the 1 %)
+        for o in (got, one):
+            assert ((o[sure, c].double() - v[pick[sure]].double()).abs()
+                    <= 2.01 * 2.0 ** -8 * v[pick[sure]].double().abs()).all()
+        assert torch.isfinite(got[:, c]).all()
+
+
 @pytest.mark.gpu
 def test_equals_full_attention_without_a_window(cuda):
     q, k, v, cq, _ = packed_case([700, 333], [700, 333], 2, 2, 128, BF16)
