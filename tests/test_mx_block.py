@@ -329,6 +329,65 @@ def test_calls_in_a_row_follow_each_other(cuda, m):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [3, 40, 700])
+def test_streams_that_fork_and_join(cuda, m):
+    """A kernel with two predecessors, on its own stream and on another, eager
+    and captured: it follows both, and what they read is not written before."""
+    d, f = 256, 512
+    w = mxfp4.MXFP4Weight(rand(d, d, scale=0.1).to(BF16).to(cuda))
+    up = mxfp4.gated_up_weight(rand(2 * f, d, seed=1, scale=0.1).to(BF16).to(cuda))
+    down = mxfp4.MXFP4Weight(rand(d, f, seed=2, scale=0.1).to(BF16).to(cuda))
+    x0 = rand(m, d, seed=3).to(BF16).to(cuda)
+    x, a, b, h, o = (torch.empty_like(x0) for _ in range(5))
+    side = torch.cuda.Stream()
+
+    def step():
+        main = torch.cuda.current_stream()
+        side.wait_stream(main)
+        with torch.cuda.stream(side):
+            mxfp4.gated_ffn(up, down, x, out=h)
+            mxfp4.mxfp4_linear(w, h, residual=x, out=b)
+        mxfp4.mxfp4_linear(w, x, act="gelu", out=a)
+        main.wait_stream(side)
+        ops.attention_window(a, b, x, 2, 128, [0, m], window=(600, 5), sinks=1, out=o)
+        mxfp4.mxfp4_linear(w, o, residual=b, out=x)
+
+    def alone():
+        mxfp4.gated_ffn(up, down, x, out=h)
+        torch.cuda.synchronize()
+        mxfp4.mxfp4_linear(w, h, residual=x, out=b)
+        torch.cuda.synchronize()
+        mxfp4.mxfp4_linear(w, x, act="gelu", out=a)
+        torch.cuda.synchronize()
+        ops.attention_window(a, b, x, 2, 128, [0, m], window=(600, 5), sinks=1, out=o)
+        torch.cuda.synchronize()
+        mxfp4.mxfp4_linear(w, o, residual=b, out=x)
+        torch.cuda.synchronize()
+
+    x.copy_(x0)
+    for _ in range(4):
+        alone()
+    want = x.view(torch.int16).clone()       # bits: the values grow from step to step
+    for _ in range(10):
+        x.copy_(x0)
+        for _ in range(4):
+            step()
+        assert torch.equal(x.view(torch.int16), want)
+    capture = torch.cuda.Stream()
+    capture.wait_stream(torch.cuda.current_stream())
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.stream(capture):
+        with torch.cuda.graph(graph, stream=capture):
+            for _ in range(4):
+                step()
+    torch.cuda.current_stream().wait_stream(capture)
+    for _ in range(10):
+        x.copy_(x0)
+        graph.replay()
+        assert torch.equal(x.view(torch.int16), want)
+
+
+@pytest.mark.gpu
 def test_outputs_must_stand_apart(cuda):
     w = mxfp4.MXFP4Weight(rand(64, 64).to(BF16).to(cuda))
     buf = rand(9, 64).to(BF16).to(cuda)
