@@ -428,8 +428,12 @@ __global__ void __launch_bounds__(kThreads) k_window_decode(const __grid_constan
     const int t = (row0 + r) / p.group, g = (row0 + r) % p.group;
     const size_t at = (((size_t)b * p.n_new + t) * p.H + kvh * p.group + g) * D + d;
     const float inv = 1.0f / ll;
+    // does the row see any key at all (one that does, and only logits of -inf, is NaN)
+    const int ps = n - p.n_new + t;
+    const int top_r = p.causal ? min(ps, n - 1) : n - 1;
+    const bool some = min(p.sinks, top_r + 1) > 0 || min(ps + p.right, top_r) >= max(0, ps - p.left);
     *reinterpret_cast<uint2*>(static_cast<T*>(p.out) + at) =
-        ll != 0.f ? make_uint2(wattn::pack16<T>(acc.x * inv, acc.y * inv),
+        some ? make_uint2(wattn::pack16<T>(acc.x * inv, acc.y * inv),
                                wattn::pack16<T>(acc.z * inv, acc.w * inv))
                   : make_uint2(0u, 0u);
   }

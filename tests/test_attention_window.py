@@ -254,6 +254,36 @@ def test_huge_logits_pick_one_key(cuda, size, d):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("d", [64, 128])
+def test_infinite_logits(cuda, d):
+    """A visible key whose logit is -inf weighs nothing; a row that sees only such
+    keys, or one whose logit is +inf or NaN, is NaN; a row that sees none is 0."""
+    n = 40
+    q, k, v, cq, _ = packed_case([n], [n], 1, 1, d, BF16, seed=9)
+    q = q.abs() + 0.1
+    inf = float("inf")
+    k[5], k[20:24], k[30], k[35, 0] = -inf, -inf, inf, float("nan")
+    left, right = 2, 0
+    z = (q.double() @ k.double().T) * d ** -0.5
+    see = seen_mask(n, n, left, right, 0, False)
+    want = torch.softmax(z.masked_fill(~see, -inf), -1)
+    dead = want.isnan().any(-1)
+    assert dead.tolist() == [i in (22, 23, 30, 31, 32, 35, 36, 37) for i in range(n)]
+    dev = [t.to(cuda) for t in (q, k, v)]
+    got = ops.attention_window(*dev, 1, d, cq, window=(left, right)).cpu()
+    one = ops.attention_window_decode(
+        dev[0].view(1, n, 1, d), *(t.view(1, n, 1, d) for t in dev[1:]),
+        torch.tensor([n], dtype=torch.int32, device=cuda), window=(left, right)).cpu().view(n, d)
+    # attend()'s terms against max |v|: twice P's half step and the logits' 4e-4
+    # (64 or 128 products of at most 40 in sum, 1.3e-4), then the output's half step
+    tol = (2 * (2.0 ** -8 + 4e-4) + 1.02 * 2.0 ** -8) * v.double().abs().amax()
+    ref = (want.nan_to_num() @ v.double())[~dead]
+    for o in (got, one):
+        assert torch.isnan(o[dead]).all()
+        assert ((o[~dead].double() - ref).abs() <= tol).all()
+
+
+@pytest.mark.gpu
 def test_equals_full_attention_without_a_window(cuda):
     q, k, v, cq, _ = packed_case([700, 333], [700, 333], 2, 2, 128, BF16)
     dev = [t.to(cuda) for t in (q, k, v)]
