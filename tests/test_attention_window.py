@@ -275,7 +275,8 @@ def test_infinite_logits(cuda, d):
         dev[0].view(1, n, 1, d), *(t.view(1, n, 1, d) for t in dev[1:]),
         torch.tensor([n], dtype=torch.int32, device=cuda), window=(left, right)).cpu().view(n, d)
     # attend()'s terms against max |v|: twice P's half step and the logits' 4e-4
-    # (64 or 128 products of at most 40 in sum, 1.3e-4), then the output's half step
+    # (scaled sums |q k| of at most 16.1, times D 2^-23: 2.5e-4; exponentials 1.3e-4),
+    # then the output's half step
     tol = (2 * (2.0 ** -8 + 4e-4) + 1.02 * 2.0 ** -8) * v.double().abs().amax()
     ref = (want.nan_to_num() @ v.double())[~dead]
     for o in (got, one):
