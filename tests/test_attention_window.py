@@ -446,6 +446,27 @@ def test_decode_graph_follows_device_lengths(cuda):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda):
+    """The last keys of 2^31 and more elements, in a cache and in packed rows."""
+    room, kv, d, m = 1 << 21, 4, 128, 300
+    g = torch.Generator().manual_seed(10)
+    tail = torch.randn(m, kv, d, generator=g).to(BF16)
+    cache = torch.zeros(2, room + 8, kv, d, dtype=BF16, device=cuda)
+    cache[1, room + 8 - m:] = tail.to(cuda)
+    q = torch.randn(2, 1, 2 * kv, d, generator=g).to(BF16)
+    lens = torch.tensor([1, room + 8], dtype=torch.int32, device=cuda)
+    got = ops.attention_window_decode(q.to(cuda), cache, cache, lens, window=(m - 1, 0)).cpu()
+    check_decode(got[1:], q[1:], tail[None], tail[None], [m], (m - 1, 0, 0, True))
+    rows = cache.view(-1, kv * d)
+    end = rows.shape[0]
+    qp = torch.randn(70, 2 * kv * d, generator=g).to(BF16)
+    got = ops.attention_window(qp.to(cuda), rows, rows, 2 * kv, d, [0, 70], kv_heads=kv,
+                               cu_seqlens_k=[end - m, end], window=(100, 0)).cpu()
+    t = tail.view(m, kv * d)
+    check_packed(got, qp, t, t, [0, 70], [0, m], 2 * kv, kv, d, (100, 0, 0, False))
+
+
+@pytest.mark.gpu
 def test_gpu_refusals(cuda):
     x = torch.zeros(8, 256, dtype=BF16, device=cuda)
     for bad in (dict(heads=2, head_dim=96), dict(heads=3, head_dim=128, kv_heads=2),

@@ -294,6 +294,28 @@ def test_gated_ffn_against_64_bits(cuda, dtype, m, d, f):
 
 
 @pytest.mark.gpu
+def test_offsets_beyond_32_bits(cuda):
+    """The last rows of more than 2^31 values, there and back, and as a product."""
+    m, k, last = 65600, 32832, 40
+    x = torch.zeros(m, k, dtype=BF16, device=cuda)
+    tail = rand(last, k, seed=11).to(BF16)
+    x[m - last:] = tail.to(cuda)
+    q, sf = ops.mxfp4_quantize(x)
+    qt, st = ops.mxfp4_quantize(tail.to(cuda))
+    assert torch.equal(q[m - last:], qt) and not q[:m - last].any()
+    back = ops.mxfp4_dequantize(q, sf, m, k, out=x)
+    assert torch.equal(back[m - last:], ops.mxfp4_dequantize(qt, st, last, k))
+    w = mxfp4.MXFP4Weight(rand(8, k, seed=12).to(BF16).to(cuda))
+    got = ops.mxfp4_gemm(q, sf, m, w.qdata, w.scale, 8, k)
+    want = back[m - last:].double() @ w.dequantize(torch.float32).double().T
+    # exact products summed in fp32: k 2^-23 of the sum of their magnitudes, then bf16
+    size = back[m - last:].double().abs() @ w.dequantize(torch.float32).double().abs().T
+    assert ((got[m - last:].double() - want).abs()
+            <= k * 2.0 ** -23 * size + 2.0 ** -8 * want.abs()).all()
+    assert not got[:m - last].any()
+
+
+@pytest.mark.gpu
 def test_gpu_refusals(cuda):
     w, _ = mx_weight(64, 64, cuda)
     x = torch.zeros(4, 64, dtype=BF16, device=cuda)
