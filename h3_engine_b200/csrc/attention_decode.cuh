@@ -4,11 +4,12 @@
 //
 // Bound by reading the visible keys and values once: 32 uneven sequences (503 MB)
 // in 75.7 us, 6.6 TB/s; one sequence of 4100 keys (16.8 MB) in 7.6 us, where
-// latencies are half of it.  The rows that share a key head, n_new tokens times the group's query heads, are the 8 (or twice 8)
-// columns of mma.sync m16n8k16 products with the keys on the other side:
-// S^T = K Q^T and O^T = V^T P^T, which for up to 8 rows takes half the
-// instructions of the form with 16 rows of queries.  A warp's work is a flash
-// pass over key tiles of 16, K and V copied by cp.async into its own ring of
+// latencies are half of it.  The rows that share a key head, n_new tokens times
+// the group's query heads, are the 8 (or twice 8) columns of mma.sync m16n8k16
+// products with the keys on the other side: S^T = K Q^T and O^T = V^T P^T, which
+// for up to 8 rows takes half the instructions of the form with 16 rows of
+// queries.  A warp's work is one pass, with a running maximum and sum, over key
+// tiles of 16, K and V copied by cp.async into its own ring of
 // stages (no barrier among warps); all fragments of K, and of V, are asked for
 // before the arithmetic that uses them.  A cluster of CTAs along the keys shares
 // a (sequence, key head): tile i belongs to warp i mod (cluster warps), and the
