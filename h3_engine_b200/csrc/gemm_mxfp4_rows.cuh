@@ -35,7 +35,8 @@ using mxgemm::SF_ATOM;
 constexpr int BN = 128;                       // weight rows per tile
 constexpr int THREADS = 192;                  // producer, MMA, 4 epilogue warps
 constexpr int kMaxRows = 128;                 // of one tile
-constexpr int kFusedRows = 8;                 // rows that the kernel quantizes itself
+constexpr int kFusedRows = 32;                // rows that the kernel can quantize itself,
+constexpr int kUnitRows = 8;                  // in units of 8 rows of a k-block
 constexpr int kMaxSplit = 8;
 constexpr uint32_t TMEM_COLS = 256;           // two CTAs per SM
 constexpr uint32_t SF_COL = 128;
@@ -145,9 +146,9 @@ __device__ __forceinline__ float4 cluster_sum(uint32_t addr, int ranks) {
 }
 
 // FUSED: the activation arrives as 16-bit rows and the epilogue warps quantize
-// it into the ring themselves, a k-block per warp in turn (at most 8 rows:
-// beyond, the CTAs' repeated quantization costs more than a launch of it).
-template <int MT, typename T, int EPI, bool FUSED>
+// it into the ring themselves, units of 8 rows of a k-block in turn (1: there are
+// 8 rows at most).
+template <int MT, typename T, int EPI, int FUSED>
 __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_constant__ Args p) {
   using R = Ring<MT>;
   extern __shared__ uint8_t smem_raw[];
@@ -175,9 +176,11 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
   auto sSFW = [&](int s) { return smem + s * R::STAGE + R::W_BYTES + R::X_BYTES; };
   auto sSFX = [&](int s) { return sSFW(s) + R::SF_BYTES; };
 
+  const int groups = FUSED == 1 ? 1 : (rows + kUnitRows - 1) / kUnitRows;
+
   if (threadIdx.x == 0) {
     for (int s = 0; s < R::STAGES; ++s) {
-      mbar_init(smem_u32(&full[s]), FUSED ? 2 : 1);   // the loads; the quantized rows
+      mbar_init(smem_u32(&full[s]), FUSED ? 1 + groups : 1);   // the loads; the quantized rows
       mbar_init(smem_u32(&empty[s]), 1);
     }
     mbar_init(smem_u32(acc_full), 1);
@@ -283,16 +286,19 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
   } else {
     grid_wait();                         // x, bias, residual and out follow earlier work
     if (FUSED) {
-      // k-block i of the rows: lane l holds values 8 l .. 8 l + 7 of a row
-      for (int i = warp - 2; i < kb1 - kb0; i += 4) {
+      // rows r0 .. r0 + 7 of k-block i: lane l holds values 8 l .. 8 l + 7 of a row
+      for (int i = FUSED == 1 ? warp - 2 : 0, g = FUSED == 1 ? 0 : warp - 2;;) {
+        for (; g >= groups; g -= groups) ++i;
+        if (i >= kb1 - kb0) break;
+        const int r0 = FUSED == 1 ? 0 : g * kUnitRows;
         const int s = i % R::STAGES, piece = (kb0 + i) * (KB_ELEMS / 8) + lane;
         const bool in_k = piece * 8 < p.K;
-        mx::Vec8<T> raw[kFusedRows];
+        const T* x = static_cast<const T*>(p.x) + (size_t)r0 * p.ldx + (size_t)piece * 8;
+        mx::Vec8<T> raw[kUnitRows];
 #pragma unroll
-        for (int r = 0; r < kFusedRows; ++r) {
+        for (int r = 0; r < kUnitRows; ++r) {
           raw[r].zero();
-          if (r < p.M && in_k)
-            raw[r].load(static_cast<const T*>(p.x) + (size_t)r * p.ldx + (size_t)piece * 8);
+          if (r0 + r < p.M && in_k) raw[r].load(x + (size_t)r * p.ldx);
         }
         if (i >= R::STAGES &&
             !__all_sync(0xffffffffu, mbar_wait(smem_u32(&empty[s]), ((i / R::STAGES) & 1) ^ 1,
@@ -300,11 +306,11 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
           fail();
           break;
         }
-        uint8_t* xs = sX(s);
-        uint8_t* sf = sSFX(s) + (lane >> 4) * SF_ATOM + ((lane >> 2) & 3);
+        uint8_t* xs = sX(s) + r0 * 128;
+        uint8_t* sf = sSFX(s) + (lane >> 4) * SF_ATOM + ((lane >> 2) & 3) + r0 * 16;
 #pragma unroll
-        for (int r = 0; r < kFusedRows; ++r) {
-          if (r < p.M) {
+        for (int r = 0; r < kUnitRows; ++r) {
+          if (r0 + r < p.M) {
             float v[8];
             raw[r].get(v);
             uint32_t m = mx::absmax_bits8(v);
@@ -319,6 +325,8 @@ __global__ void __launch_bounds__(THREADS) k_gemm_mxfp4_rows(const __grid_consta
         fence_proxy_async_smem();        // the MMA reads them through the async proxy
         __syncwarp();
         if (lane == 0) mbar_arrive(smem_u32(&full[s]));
+        if (FUSED == 1) i += 4;
+        else g += 4;
       }
     }
     grid_launch_dependents();

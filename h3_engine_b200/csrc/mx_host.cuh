@@ -190,7 +190,33 @@ static int mx_gemm_launch(mxgemm::PairArgs& pa, bool chained, cudaStream_t st) {
 }
 
 // ---- up to 128 rows: the weight-streaming kernel
-template <int MT, typename T, int EPI, bool FUSED>
+// CTAs along K, a power of two of them (clusters of odd sizes do not all find
+// room at once): while two per SM hold them all and two k-blocks are left to
+// each (1 x 7168 x 5376: 9.1 us on one, 7.3 on two, 6.9 on four; 77 x 4136 x
+// 2720: 11.5, 9.5, 8.5 and, with one k-block each on eight, 9.6)
+static int mx_rows_split(int64_t tiles, int64_t K) {
+  const int64_t num_kb = (K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS;
+  int split = 1;
+  while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles <= 2 * num_sms() &&
+         num_kb >= split * 4)
+    split *= 2;
+  return split;
+}
+
+// Does the product quantize its rows itself: up to 8, and up to 32 where that is
+// at most two units of 8 rows and a k-block for each of a CTA's four warps (16 x
+// 2048 x 2048, one unit: 4.5 us on the device, 5.1 with a launch of its own; 32 x
+// 2048 x 2048, two: 5.8 and 5.5, but calls in a row are bound by their launches,
+// 7.6 and 10.4; past that 16 x 7168 x 5376: 10.6 and 8.8).
+static bool mx_fused(int64_t M, int64_t N, int64_t K) {
+  if (M <= mxrows::kUnitRows) return true;
+  if (M > mxrows::kFusedRows) return false;
+  const int split = mx_rows_split((N + mxrows::BN - 1) / mxrows::BN, K);
+  const int64_t kbs = ((K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS + split - 1) / split;
+  return kbs * ((M + mxrows::kUnitRows - 1) / mxrows::kUnitRows) <= 8;
+}
+
+template <int MT, typename T, int EPI, int FUSED>
 static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool chained,
                           cudaStream_t st) {
   a.first = !chained;
@@ -207,16 +233,8 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
   rc = attr.set(reinterpret_cast<const void*>(kernel), mxrows::Ring<MT>::BYTES);
   if (rc != H3B_OK) return rc;
   const int tiles = (a.N + mxrows::BN - 1) / mxrows::BN;
-  const int num_kb = (a.K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS;
-  // CTAs along K, a power of two of them (clusters of odd sizes do not all find
-  // room at once): while two per SM hold them all and two k-blocks are left to
-  // each (1 x 7168 x 5376: 9.1 us on one, 7.3 on two, 6.9 on four; 77 x 4136 x
-  // 2720: 11.5, 9.5, 8.5 and, with one k-block each on eight, 9.6)
-  int split = 1;
   const int m_tiles = (a.M + MT - 1) / MT;      // more than one only for MT = 128
-  while (split * 2 <= mxrows::kMaxSplit && split * 2 * tiles * m_tiles <= 2 * num_sms() &&
-         num_kb >= split * 4)
-    split *= 2;
+  const int split = mx_rows_split((int64_t)tiles * m_tiles, a.K);
   return launch(true, kernel, dim3((unsigned)split, (unsigned)tiles, (unsigned)m_tiles),
                       mxrows::THREADS, mxrows::Ring<MT>::BYTES, split, st, a);
 }
@@ -241,11 +259,14 @@ static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t
   a.N = (int)N;
   a.K = (int)K;
   a.sf_tiles_k = (int)mx::sf_tiles(K);
-  if (!sfA) return mx_rows_launch<16, T, EPI, true>(a, A, B, chained, st);
-  if (M <= 16) return mx_rows_launch<16, T, EPI, false>(a, A, B, chained, st);
-  if (M <= 32) return mx_rows_launch<32, T, EPI, false>(a, A, B, chained, st);
-  if (M <= 64) return mx_rows_launch<64, T, EPI, false>(a, A, B, chained, st);
-  return mx_rows_launch<128, T, EPI, false>(a, A, B, chained, st);
+  if (!sfA)
+    return M <= mxrows::kUnitRows ? mx_rows_launch<16, T, EPI, 1>(a, A, B, chained, st)
+           : M <= 16              ? mx_rows_launch<16, T, EPI, 2>(a, A, B, chained, st)
+                                  : mx_rows_launch<32, T, EPI, 2>(a, A, B, chained, st);
+  if (M <= 16) return mx_rows_launch<16, T, EPI, 0>(a, A, B, chained, st);
+  if (M <= 32) return mx_rows_launch<32, T, EPI, 0>(a, A, B, chained, st);
+  if (M <= 64) return mx_rows_launch<64, T, EPI, 0>(a, A, B, chained, st);
+  return mx_rows_launch<128, T, EPI, 0>(a, A, B, chained, st);
 }
 
 // Bytes of an activation's codes and blocked scales in a workspace, each part
@@ -283,7 +304,7 @@ static bool mx_by_rows(int64_t M, int64_t N, int64_t K) {
          (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms());
 }
 
-// D = act(A B^T + bias) + residual.  sfA NULL (M <= kFusedRows): A is 16-bit
+// D = act(A B^T + bias) + residual.  sfA NULL (mx_fused): A is 16-bit
 // rows of stride ldx.  chained: the launch before is of the same entry point.
 static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, const void* B,
                        const void* sfB, int64_t N, int64_t K, const void* bias, int act,
@@ -371,7 +392,7 @@ int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, con
 }
 
 int64_t h3b_mxfp4_linear_ws(int64_t M, int64_t N, int64_t K) {
-  if (M <= mxrows::kFusedRows || N <= 0 || K <= 0 || M > kMxMaxDim || K > kMxMaxDim) return 0;
+  if (M <= mxrows::kUnitRows || N <= 0 || K <= 0 || M > kMxMaxDim || K > kMxMaxDim) return 0;
   return mx_operand_bytes(M, K);
 }
 
@@ -387,7 +408,7 @@ int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const voi
   rc = mx_input_check(x, ldx, K);
   if (rc != H3B_OK) return rc;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
-  if (M <= mxrows::kFusedRows)
+  if (mx_fused(M, N, K))
     return mx_gemm_out(x, nullptr, ldx, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd,
                        false, st);
   uint8_t* q = static_cast<uint8_t*>(ws);
@@ -418,7 +439,7 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   uint8_t* sf = q + mx_code_bytes(M, N);
   uint8_t* qh = q + mx_operand_bytes(M, N);
   uint8_t* sfh = qh + mx_code_bytes(M, F);
-  const bool fused = M <= mxrows::kFusedRows;
+  const bool fused = mx_fused(M, 2 * F, N);
   if (!fused) {
     rc = mx_quantize(x, dtype, M, N, ldx, q, sf, st);
     if (rc != H3B_OK) return rc;

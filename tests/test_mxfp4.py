@@ -294,6 +294,27 @@ def test_gated_ffn_against_64_bits(cuda, dtype, m, d, f):
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("m", [8, 9, 16, 17, 24, 25, 32, 33])
+@pytest.mark.parametrize("n,k", [(136, 512), (520, 416), (264, 4128), (1024, 32)])
+def test_rows_quantized_in_the_product_or_before(cuda, m, n, k):
+    """The linear gives the bits of a quantization and a product, whichever kernel
+    quantizes the rows (few rows of short K: the product's own)."""
+    w = mxfp4.MXFP4Weight(rand(n, k, seed=13, scale=0.2).to(BF16).to(cuda))
+    buf = rand(m, k + 16, seed=14).to(BF16).to(cuda)
+    x, bias = buf[:, 8:8 + k], rand(n, seed=15).to(BF16).to(cuda)
+    got = mxfp4.mxfp4_linear(w, x, bias=bias, act="gelu")
+    q, sf = ops.mxfp4_quantize(x)
+    want = ops.mxfp4_gemm(q, sf, m, w.qdata, w.scale, n, k, bias=bias, act=ops.ACT_GELU_TANH)
+    assert torch.equal(got, want)
+    if n % 128 == 0 and k % 32 == 0:
+        up = mxfp4.gated_up_weight(rand(2 * n, k, seed=16, scale=0.2).to(BF16).to(cuda))
+        down = mxfp4.MXFP4Weight(rand(k, n, seed=17, scale=0.2).to(BF16).to(cuda))
+        one = mxfp4.gated_ffn(up, down, x)
+        rows = torch.cat([mxfp4.gated_ffn(up, down, x[i:i + 1]) for i in range(m)])
+        assert torch.equal(one, rows)
+
+
+@pytest.mark.gpu
 def test_offsets_beyond_32_bits(cuda):
     """The last rows of more than 2^31 values, there and back, and as a product."""
     m, k, last = 65600, 32832, 40
