@@ -12,12 +12,13 @@ from __future__ import annotations
 import torch
 from torch import nn
 
-from . import ops
+from . import ops, torch_ops
 from .nvfp4 import _block_linears, _set_child, _swizzle, _unswizzle
 
 MXFP4_BLOCK = ops.MX_BLOCK
 DTYPES = (torch.bfloat16, torch.float16)      # of activations and results
 
+_LINEAR = torch_ops.ext_op("mxfp4_linear")
 _ACTS = {None: ops.ACT_NONE, "gelu": ops.ACT_GELU_TANH}
 
 
@@ -58,6 +59,9 @@ def mxfp4_linear(w: MXFP4Weight, x: torch.Tensor, *, bias: torch.Tensor | None =
     ``act`` is None or "gelu" (tanh form)."""
     if act not in _ACTS:
         raise ValueError(f"unknown activation {act!r}")
+    if out is None and x.is_cuda:         # single tokens: no call in between
+        return _LINEAR(x, w.qdata, w.scale, w.out_features, w.in_features, bias, _ACTS[act],
+                       residual)
     return ops.mxfp4_linear(x, w.qdata, w.scale, w.out_features, w.in_features, bias=bias,
                             act=_ACTS[act], residual=residual, out=out)
 
