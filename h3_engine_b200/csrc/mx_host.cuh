@@ -85,14 +85,14 @@ static unsigned mx_quant_blocks(int64_t units) {
 }
 
 template <typename T, int VPL>
-static int mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q, void* sf,
-                              cudaStream_t st) {
+static int mx_quantize_launch(const void* x, int64_t M, int64_t K, int64_t ldx, void* q,
+                              int64_t ldq, void* sf, cudaStream_t st) {
   constexpr int kUnit = 32 * VPL * kQuantUnroll;
   const int64_t Mpad = (M + 127) / 128 * 128;
   const int64_t per_row = (mx::sf_tiles(K) * 128 + kUnit - 1) / kUnit;
   return launch(true, mx::k_mxfp4_quantize<T, VPL, kQuantUnroll>,
                       dim3(mx_quant_blocks(Mpad * per_row)), mx::kThreads, 0, 0, st,
-                      static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q),
+                      static_cast<const T*>(x), M, K, ldx, static_cast<uint8_t*>(q), ldq,
                       static_cast<uint8_t*>(sf), Mpad, (uint32_t)per_row);
 }
 
@@ -113,7 +113,7 @@ static inline bool wide_rows(const void* p, int64_t ld, int size) {
 }
 
 static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
-                       void* sf, cudaStream_t st) {
+                       int64_t ldq, void* sf, cudaStream_t st) {
   if (!dt_any(dtype) || M < 0 || K <= 0 || K % mx::BLOCK || ldx < K) return H3B_ERR_INVALID_ARG;
   if (M > kMxMaxDim || K > kMxMaxDim) return H3B_ERR_INVALID_ARG;
   if (M == 0) return H3B_OK;
@@ -123,8 +123,8 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
   const bool wide = wide_rows(x, ldx, dt_bytes(dtype));
   auto go = [&](auto t) {
     using T = decltype(t);
-    return wide ? mx_quantize_launch<T, 16>(x, M, K, ldx, q, sf, st)
-                : mx_quantize_launch<T, 8>(x, M, K, ldx, q, sf, st);
+    return wide ? mx_quantize_launch<T, 16>(x, M, K, ldx, q, ldq, sf, st)
+                : mx_quantize_launch<T, 8>(x, M, K, ldx, q, ldq, sf, st);
   };
   if (dtype == H3B_DT_BF16) return go(__nv_bfloat16());
   if (dtype == H3B_DT_F16) return go(__half());
@@ -132,8 +132,8 @@ static int mx_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t l
 }
 
 // Operands of the CTA-pair kernel: shapes and alignment.
-static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, int64_t M,
-                        const void* B, const void* sfB, int64_t N, int64_t K) {
+static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, int64_t lda, const void* sfA,
+                        int64_t M, const void* B, const void* sfB, int64_t N, int64_t K) {
   if (!A || !sfA || !B || !sfB) return H3B_ERR_INVALID_ARG;
   if (!aligned16(A) || !aligned16(sfA) || !aligned16(B) || !aligned16(sfB))
     return H3B_ERR_ALIGNMENT;
@@ -141,7 +141,7 @@ static int mx_gemm_args(mxgemm::PairArgs& pa, const void* A, const void* sfA, in
   if (rc != H3B_OK) return rc;
   memset(&pa, 0, sizeof(pa));
   mxgemm::Args& a = pa.base;
-  rc = make_tmap_u8_sw128(&a.tmap_a, A, (uint64_t)M, (uint64_t)(K / 2), (uint64_t)(K / 2),
+  rc = make_tmap_u8_sw128(&a.tmap_a, A, (uint64_t)M, (uint64_t)(K / 2), (uint64_t)lda,
                           mxgemm::KB_BYTES, mxgemm::BM);
   if (rc != H3B_OK) return rc;
   rc = make_tmap_u8_sw128(&a.tmap_b, B, (uint64_t)N, (uint64_t)(K / 2), (uint64_t)(K / 2),
@@ -224,8 +224,8 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
                               (uint64_t)(a.K / 2), mxrows::KB_BYTES, mxrows::BN);
   if (rc != H3B_OK) return rc;
   if (!FUSED) {
-    rc = make_tmap_u8_sw128(&a.tmap_x, A, (uint64_t)a.M, (uint64_t)(a.K / 2),
-                            (uint64_t)(a.K / 2), mxrows::KB_BYTES, MT);
+    rc = make_tmap_u8_sw128(&a.tmap_x, A, (uint64_t)a.M, (uint64_t)(a.K / 2), (uint64_t)a.ldx,
+                            mxrows::KB_BYTES, MT);
     if (rc != H3B_OK) return rc;
   }
   auto kernel = mxrows::k_gemm_mxfp4_rows<MT, T, EPI, FUSED>;
@@ -239,8 +239,8 @@ static int mx_rows_launch(mxrows::Args& a, const void* A, const void* B, bool ch
                       mxrows::THREADS, mxrows::Ring<MT>::BYTES, split, st, a);
 }
 
-// Operands of the rows kernel: A as codes and scales, or (sfA NULL) as 16-bit
-// rows of stride ldx that the kernel quantizes itself.
+// Operands of the rows kernel: A as codes (ldx bytes a row) and scales, or (sfA
+// NULL) as 16-bit rows of ldx elements that the kernel quantizes itself.
 template <typename T, int EPI>
 static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t ldx, int64_t M,
                         const void* B, const void* sfB, int64_t N, int64_t K, bool chained,
@@ -271,8 +271,13 @@ static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t
 
 // Bytes of an activation's codes and blocked scales in a workspace, each part
 // rounded up to 256 bytes.
+// An activation's codes are ours to lay out: rows start at whole sectors (32
+// bytes), so that a TMA box's rows take no sector more than they fill (13383 x
+// 4096 x 4064 with its quantization: 114 us, 122 with rows of K / 2 bytes; 1025 x
+// 11008 x 2016: 19.0 and 20.3).
+static inline int64_t mx_code_pitch(int64_t k) { return (k / 2 + 31) / 32 * 32; }
 static inline int64_t mx_code_bytes(int64_t rows, int64_t k) {
-  return (rows * (k / 2) + 255) / 256 * 256;
+  return (rows * mx_code_pitch(k) + 255) / 256 * 256;
 }
 static inline int64_t mx_operand_bytes(int64_t rows, int64_t k) {
   return mx_code_bytes(rows, k) + (rows + 127) / 128 * mx::sf_tiles(k) * mxgemm::SF_ATOM;
@@ -304,8 +309,8 @@ static bool mx_by_rows(int64_t M, int64_t N, int64_t K) {
          (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms());
 }
 
-// D = act(A B^T + bias) + residual.  sfA NULL (mx_fused): A is 16-bit
-// rows of stride ldx.  chained: the launch before is of the same entry point.
+// D = act(A B^T + bias) + residual.  A is codes, ldx bytes a row, or (sfA NULL,
+// mx_fused) 16-bit rows of ldx elements.  chained: the launch before is of the same entry point.
 static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, const void* B,
                        const void* sfB, int64_t N, int64_t K, const void* bias, int act,
                        const void* residual, int64_t ldr, void* D, int dtype, int64_t ldd,
@@ -326,7 +331,7 @@ static int mx_gemm_out(const void* A, const void* sfA, int64_t ldx, int64_t M, c
                                                            chained, st);
   }
   mxgemm::PairArgs pa;
-  int rc = mx_gemm_args(pa, A, sfA, M, B, sfB, N, K);
+  int rc = mx_gemm_args(pa, A, ldx, sfA, M, B, sfB, N, K);
   if (rc != H3B_OK) return rc;
   mxgemm::Args& a = pa.base;
   rc = make_tmap_16_sw128(&a.tmap_d, D, dtype, (uint64_t)M, (uint64_t)N, (uint64_t)ldd,
@@ -359,7 +364,7 @@ extern "C" {
 
 int h3b_mxfp4_quantize(const void* x, int dtype, int64_t M, int64_t K, int64_t ldx, void* q,
                        void* sf, void* stream) {
-  return mx_quantize(x, dtype, M, K, ldx, q, sf, static_cast<cudaStream_t>(stream));
+  return mx_quantize(x, dtype, M, K, ldx, q, K / 2, sf, static_cast<cudaStream_t>(stream));
 }
 
 int h3b_mxfp4_dequantize(const void* q, const void* sf, int64_t M, int64_t K, void* out, int dtype,
@@ -387,7 +392,7 @@ int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, con
   const int rc = mx_out_check(dtype, M, N, K, bias, act, residual, ldr, D, ldd);
   if (rc != H3B_OK || M == 0) return rc;
   if (!sfA) return H3B_ERR_INVALID_ARG;
-  return mx_gemm_out(A, sfA, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, false,
+  return mx_gemm_out(A, sfA, K / 2, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, false,
                      static_cast<cudaStream_t>(stream));
 }
 
@@ -413,9 +418,10 @@ int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const voi
                        false, st);
   uint8_t* q = static_cast<uint8_t*>(ws);
   uint8_t* sf = q + mx_code_bytes(M, K);
-  rc = mx_quantize(x, dtype, M, K, ldx, q, sf, st);
+  const int64_t pitch = mx_code_pitch(K);
+  rc = mx_quantize(x, dtype, M, K, ldx, q, pitch, sf, st);
   if (rc != H3B_OK) return rc;
-  return mx_gemm_out(q, sf, 0, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, true, st);
+  return mx_gemm_out(q, sf, pitch, M, B, sfB, N, K, bias, act, residual, ldr, D, dtype, ldd, true, st);
 }
 
 int64_t h3b_mxfp4_ffn_ws(int64_t M, int64_t N, int64_t F) {
@@ -440,8 +446,9 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
   uint8_t* qh = q + mx_operand_bytes(M, N);
   uint8_t* sfh = qh + mx_code_bytes(M, F);
   const bool fused = mx_fused(M, 2 * F, N);
+  const int64_t pitch = mx_code_pitch(N);
   if (!fused) {
-    rc = mx_quantize(x, dtype, M, N, ldx, q, sf, st);
+    rc = mx_quantize(x, dtype, M, N, ldx, q, pitch, sf, st);
     if (rc != H3B_OK) return rc;
   }
   if (mx_by_rows(M, 2 * F, N)) {
@@ -451,21 +458,22 @@ int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, const void* 
     a.sf_out = sfh;
     const void* A = fused ? x : q;
     const void* sfA = fused ? nullptr : sf;
+    const int64_t lda = fused ? ldx : pitch;
     rc = dtype == H3B_DT_F16
-             ? mx_rows_gemm<__half, mxgemm::kSwigluQuant>(a, A, sfA, ldx, M, Bu, sfBu, 2 * F, N,
+             ? mx_rows_gemm<__half, mxgemm::kSwigluQuant>(a, A, sfA, lda, M, Bu, sfBu, 2 * F, N,
                                                           !fused, st)
-             : mx_rows_gemm<__nv_bfloat16, mxgemm::kSwigluQuant>(a, A, sfA, ldx, M, Bu, sfBu,
+             : mx_rows_gemm<__nv_bfloat16, mxgemm::kSwigluQuant>(a, A, sfA, lda, M, Bu, sfBu,
                                                                  2 * F, N, !fused, st);
   } else {
     mxgemm::PairArgs up;
-    rc = mx_gemm_args(up, q, sf, M, Bu, sfBu, 2 * F, N);
+    rc = mx_gemm_args(up, q, pitch, sf, M, Bu, sfBu, 2 * F, N);
     if (rc != H3B_OK) return rc;
     up.base.q_out = qh;
     up.base.sf_out = sfh;
     rc = mx_gemm_launch<__nv_bfloat16, mxgemm::kSwigluQuant>(up, true, st);
   }
   if (rc != H3B_OK) return rc;
-  return mx_gemm_out(qh, sfh, 0, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D,
+  return mx_gemm_out(qh, sfh, F / 2, M, Bd, sfBd, N, F, nullptr, H3B_ACT_NONE, residual, ldr, D,
                      dtype, ldd, true, st);
 }
 

@@ -208,8 +208,8 @@ constexpr int kThreads = 256;
 // last tile are written as 0.
 template <typename T, int VPL, int UNROLL>
 __global__ void __launch_bounds__(kThreads)
-    k_mxfp4_quantize(const T* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, uint8_t* sf,
-                     int64_t Mpad, uint32_t units_per_row) {
+    k_mxfp4_quantize(const T* x, int64_t M, int64_t K, int64_t ldx, uint8_t* q, int64_t ldq,
+                     uint8_t* sf, int64_t Mpad, uint32_t units_per_row) {
   grid_wait();
   grid_launch_dependents();
   constexpr int LPB = BLOCK / VPL;                 // lanes per block
@@ -225,7 +225,7 @@ __global__ void __launch_bounds__(kThreads)
     const int v0 = (int)(wi - r * units_per_row) * (32 * VPL * UNROLL) + lane * VPL;
     const bool real = r < M;
     const T* xr = x + r * ldx;
-    uint8_t* qr = q + r * (K >> 1);
+    uint8_t* qr = q + r * ldq;
     uint8_t* sr = sf + sf_swizzled_offset(r, 0, c4);
     Lane<T, VPL> raw[UNROLL];
 #pragma unroll
