@@ -33,7 +33,9 @@ class MXFP4Weight:
         self.out_features, self.in_features = weight.shape
         if self.out_features % 8:
             raise ValueError(f"out_features = {self.out_features} must be a multiple of 8")
-        self.qdata, self.scale = ops.mxfp4_quantize(weight.detach())
+        # normal tensors in every mode: those of inference mode count no versions (_laid_out)
+        with torch.inference_mode(False):
+            self.qdata, self.scale = ops.mxfp4_quantize(weight.detach())
 
     @classmethod
     def from_packed(cls, qdata: torch.Tensor, scale: torch.Tensor, out_features: int,
@@ -101,41 +103,91 @@ class MXFP4Linear(nn.Module):
         return mxfp4_linear(self.weight_mxfp4, x, bias=self.bias)
 
 
+def _laid_out(module: nn.Module, slot: str, ws: tuple, lay_out) -> MXFP4Weight:
+    """``lay_out()``, a weight made of the weights ``ws``, kept in ``module.slot``
+    until one of them has another tensor or, as the tensor's version tells, other
+    contents.  (Writes that no version counts, through ``.data`` or by a graph's
+    replay, are not seen.)
+
+    A change is written into the kept tensors, which live as long as the module:
+    a captured call goes on reading them, and follows at the next call that is not
+    captured.  The device is waited for around that, and after the first layout,
+    because calls on every stream read them.  Not kept is what would only be there
+    after a replay or inside a compiled call, and what is made of tensors without
+    versions (those of inference mode)."""
+    if torch.compiler.is_compiling():
+        return lay_out()
+    kept = getattr(module, slot)
+    if kept is not None and len(kept[0]) == len(ws):
+        for w, (q, q_version, sf, sf_version, n, k) in zip(ws, kept[0]):
+            if (w.qdata is not q or q._version != q_version or w.scale is not sf
+                    or sf._version != sf_version or w.out_features != n or w.in_features != k):
+                break
+        else:
+            return kept[1]
+    sources = [t for w in ws for t in (w.qdata, w.scale)]
+    if any(t.is_inference() for t in sources):
+        return lay_out()
+    made_of = [(w.qdata, w.qdata._version, w.scale, w.scale._version, w.out_features,
+                w.in_features) for w in ws]
+    on_gpu = sources[0].is_cuda
+    with torch.inference_mode(False):
+        w = lay_out()
+        if on_gpu and torch.cuda.is_current_stream_capturing():
+            return w
+        if kept is not None:
+            if on_gpu:
+                torch.cuda.synchronize(sources[0].device)
+            if all(a.shape == b.shape and a.device == b.device for a, b in
+                   ((kept[1].qdata, w.qdata), (kept[1].scale, w.scale))):
+                w.qdata, w.scale = kept[1].qdata.copy_(w.qdata), kept[1].scale.copy_(w.scale)
+    if on_gpu:
+        torch.cuda.current_stream(sources[0].device).synchronize()
+    setattr(module, slot, (made_of, w))
+    return w
+
+
 def shared_qkv(to_q, to_k, to_v, x: torch.Tensor):
     """q, k and v projections from one quantization of ``x`` as one product over
-    the weights concatenated along N (kept on ``to_q``): None unless all three
-    are ``MXFP4Linear`` of one input width, without bias, with output widths in
-    whole 128-row scale tiles, and ``x`` is of a type they take."""
+    the weights concatenated along N (a second copy of them, kept on ``to_q`` and
+    following them): None unless all three are ``MXFP4Linear`` of one input width,
+    without bias, with output widths in whole 128-row scale tiles, and ``x`` is of
+    a type they take."""
     mods = (to_q, to_k, to_v)
-    if not all(isinstance(m, MXFP4Linear) and m.bias is None and m.out_features % 128 == 0
-               and m.in_features == to_q.in_features for m in mods) or x.dtype not in DTYPES:
+    if x.dtype not in DTYPES or not all(isinstance(m, MXFP4Linear) and m.bias is None
+                                        for m in mods):
         return None
     ws = tuple(m.weight_mxfp4 for m in mods)
-    cached = to_q._fused
-    if cached is None or any(a is not b for a, b in zip(cached[0], ws)):
-        w = MXFP4Weight.from_packed(torch.cat([w.qdata for w in ws]),
-                                    torch.cat([w.scale for w in ws]),
-                                    sum(w.out_features for w in ws), to_q.in_features)
-        cached = to_q._fused = (ws, w)
-    return mxfp4_linear(cached[1], x).split([w.out_features for w in ws], -1)
+    k = ws[0].in_features
+    if any(w.out_features % 128 or w.in_features != k for w in ws):
+        return None
+    fused = _laid_out(to_q, "_fused", ws, lambda: MXFP4Weight.from_packed(
+        torch.cat([w.qdata for w in ws]), torch.cat([w.scale for w in ws]),
+        sum(w.out_features for w in ws), k))
+    return mxfp4_linear(fused, x).split([w.out_features for w in ws], -1)
 
 
 def linear_ffn(up: "MXFP4Linear", down: "MXFP4Linear", x: torch.Tensor):
     """``gated_ffn`` of a feed-forward's two linears, ``up`` the fused
-    [value | gate] projection in the reference's chunk order (its rows are
-    reordered once and kept on ``up``): None if ``gated_ffn`` does not take them."""
-    f = down.in_features
-    if (up.bias is not None or down.bias is not None or f % 128 or up.out_features != 2 * f
-            or down.out_features != up.in_features or x.dtype not in DTYPES):
+    [value | gate] projection in the reference's chunk order (a copy with its rows
+    reordered is kept on ``up`` and follows it): None if ``gated_ffn`` does not
+    take them."""
+    w, wd = up.weight_mxfp4, down.weight_mxfp4
+    f = wd.in_features
+    if (up.bias is not None or down.bias is not None or f % 128 or w.out_features != 2 * f
+            or wd.out_features != w.in_features or x.dtype not in DTYPES):
         return None
-    w = up.weight_mxfp4
-    if up._gated is None or up._gated[0] is not w:
-        perm = ops.swiglu_rows(f).to(w.qdata.device)
-        sf = _unswizzle(w.scale, 2 * f, w.in_features // MXFP4_BLOCK)[perm]
-        up._gated = (w, MXFP4Weight.from_packed(w.qdata[perm].contiguous(),
-                                                _swizzle(sf.contiguous()).view(torch.uint8),
-                                                2 * f, w.in_features))
-    return gated_ffn(up._gated[1], down.weight_mxfp4, x)
+
+    def in_groups(t):        # rows in swiglu_rows order: groups of 64 values and 64 gates
+        return t.view(2, f // 64, 64, -1).transpose(0, 1).reshape(2 * f, -1)
+
+    def reordered():
+        sf = _unswizzle(w.scale, 2 * f, w.in_features // MXFP4_BLOCK)
+        return MXFP4Weight.from_packed(in_groups(w.qdata),
+                                       _swizzle(in_groups(sf)).view(torch.uint8),
+                                       2 * f, w.in_features)
+
+    return gated_ffn(_laid_out(up, "_gated", (w,), reordered), wd, x)
 
 
 @torch.no_grad()
