@@ -78,16 +78,21 @@ def build(force: bool = False, verbose: bool = False, ptxas_v: bool = False) -> 
 
 
 def build_ext(force: bool = False, verbose: bool = False) -> Path:
-    """_h3b_torch.so from torch_ext.cpp, against the installed torch and LIB."""
+    """_h3b_torch.so from torch_ext.cpp, against the installed torch and LIB.  A
+    file beside it says which torch that was: another one needs another build."""
     import torch
     src = [HERE / "torch_ext.cpp", ROOT / "include" / "h3b.h"]
-    if not force and EXT.exists() and all(p.stat().st_mtime <= EXT.stat().st_mtime for p in src):
+    abi = int(torch._C._GLIBCXX_USE_CXX11_ABI)
+    built_for = f"torch {torch.__version__}, C++11 ABI {abi}\n"
+    stamp = EXT.with_suffix(".so.torch")
+    if (not force and EXT.exists() and stamp.exists() and stamp.read_text() == built_for
+            and all(p.stat().st_mtime <= EXT.stat().st_mtime for p in src)):
         return EXT
     troot = Path(torch.__file__).resolve().parent
     cuda = Path(nvcc()).resolve().parent.parent
     tmp = EXT.with_suffix(".so.tmp")
     cmd = [cxx(), "-O2", "-std=c++17", "-fPIC", "-shared",
-           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={int(torch._C._GLIBCXX_USE_CXX11_ABI)}",
+           "-fvisibility=hidden", f"-D_GLIBCXX_USE_CXX11_ABI={abi}",
            "-I", str(ROOT / "include"), "-isystem", str(troot / "include"),
            "-isystem", str(cuda / "include"), str(src[0]), "-o", str(tmp),
            "-L", str(PKG), "-lh3b", "-L", str(troot / "lib"), "-lc10", "-lc10_cuda", "-ltorch_cpu",
@@ -99,6 +104,7 @@ def build_ext(force: bool = False, verbose: bool = False) -> Path:
         sys.stderr.write(r.stdout + r.stderr)
         raise RuntimeError(f"{cmd[0]} failed with exit code {r.returncode}")
     os.replace(tmp, EXT)
+    stamp.write_text(built_for)
     return EXT
 
 

@@ -219,26 +219,32 @@ _FAKES = {
 }
 
 
-def _load_ext() -> bool:
-    if not EXT_PATH.exists():
-        return False
-    torch.ops.load_library(str(EXT_PATH))
-    for name, fake in _FAKES.items():
-        torch.library.register_fake(f"h3b::{name}", fake)
-        torch.library.register_fake(f"h3b::{name}_out", _no_output)
-    return True
+def _load_ext(path=EXT_PATH) -> str | None:
+    """None once the operators are there, else why they are not.  What does not
+    load (it may be built against another torch) leaves the rest of the package
+    usable, as a missing file does."""
+    if not path.exists():
+        return f"{path} is missing"
+    try:
+        torch.ops.load_library(str(path))
+        for name, fake in _FAKES.items():
+            torch.library.register_fake(f"h3b::{name}", fake)
+            torch.library.register_fake(f"h3b::{name}_out", _no_output)
+    except (OSError, RuntimeError) as exc:
+        return f"{path} does not load ({exc})"
+    return None
 
 
-_EXT_LOADED = _load_ext()
+_EXT_ERROR = _load_ext()
 
 
 def ext_op(name: str):
     """The C++ operator ``h3b::name``; without the built extension a callable
     that raises (there is no other path)."""
-    if _EXT_LOADED:
+    if _EXT_ERROR is None:
         return getattr(torch.ops.h3b, name).default
 
     def missing(*_args, **_kwargs):
-        raise RuntimeError(f"{EXT_PATH} is missing: build it with "
+        raise RuntimeError(f"{_EXT_ERROR}: build it with "
                            "`python -m h3_engine_b200.csrc.build`")
     return missing
