@@ -190,6 +190,8 @@ static int mx_gemm_launch(mxgemm::PairArgs& pa, bool chained, cudaStream_t st) {
 }
 
 // ---- up to 128 rows: the weight-streaming kernel
+constexpr int64_t kRowsMaxN = (int64_t)65535 * mxrows::BN;    // weight tiles are its grid's y
+
 // CTAs along K, a power of two of them (clusters of odd sizes do not all find
 // room at once): while two per SM hold them all and two k-blocks are left to
 // each (1 x 7168 x 5376: 9.1 us on one, 7.3 on two, 6.9 on four; 77 x 4136 x
@@ -209,8 +211,8 @@ static int mx_rows_split(int64_t tiles, int64_t K) {
 // 2048 x 2048, two: 5.8 and 5.5, but calls in a row are bound by their launches,
 // 7.6 and 10.4; past that 16 x 7168 x 5376: 10.6 and 8.8).
 static bool mx_fused(int64_t M, int64_t N, int64_t K) {
+  if (M > mxrows::kFusedRows || N > kRowsMaxN) return false;
   if (M <= mxrows::kUnitRows) return true;
-  if (M > mxrows::kFusedRows) return false;
   const int split = mx_rows_split((N + mxrows::BN - 1) / mxrows::BN, K);
   const int64_t kbs = ((K + mxrows::KB_ELEMS - 1) / mxrows::KB_ELEMS + split - 1) / split;
   return kbs * ((M + mxrows::kUnitRows - 1) / mxrows::kUnitRows) <= 8;
@@ -248,7 +250,6 @@ static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t
   if (!A || !B || !sfB) return H3B_ERR_INVALID_ARG;
   if (!aligned16(A) || !aligned16(sfA) || !aligned16(B) || !aligned16(sfB))
     return H3B_ERR_ALIGNMENT;
-  if ((N + mxrows::BN - 1) / mxrows::BN > 65535) return H3B_ERR_INVALID_ARG;
   const int rc = check_sm100();
   if (rc != H3B_OK) return rc;
   a.sfw = static_cast<const uint8_t*>(sfB);
@@ -298,15 +299,17 @@ static int mx_out_check(int dtype, int64_t M, int64_t N, int64_t K, const void* 
   return H3B_OK;
 }
 
-// Which kernel: the rows kernel up to 128 rows, and beyond them in tiles of 128
+// Which kernel: the rows kernel (whose grid takes N up to kRowsMaxN) up to 128
+// rows, and beyond them in tiles of 128
 // where the pair kernel would leave most SMs idle over a long K: where three
 // CTAs along K find room for each of its tiles (144 x 2048 x 5376: 11.1 us
 // against 13.5, 512 x 2048 x 5376: 12.8 and 13.4, 256 x 5376 x 14336: 22.3 and
 // 26.9; past that 512 x 5376 x 14336: 34.1 and 28.7; with K = 2048 the pair
 // kernel is ahead, 256 x 5376: 11.2 and 9.5).
 static bool mx_by_rows(int64_t M, int64_t N, int64_t K) {
-  return M <= mxrows::kMaxRows ||
-         (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms());
+  return N <= kRowsMaxN &&
+         (M <= mxrows::kMaxRows ||
+          (K >= 4096 && ((M + 127) / 128) * ((N + 127) / 128) * 3 <= 2 * num_sms()));
 }
 
 // D = act(A B^T + bias) + residual.  A is codes, ldx bytes a row, or (sfA NULL,
@@ -397,7 +400,8 @@ int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void* B, con
 }
 
 int64_t h3b_mxfp4_linear_ws(int64_t M, int64_t N, int64_t K) {
-  if (M <= mxrows::kUnitRows || N <= 0 || K <= 0 || M > kMxMaxDim || K > kMxMaxDim) return 0;
+  if (M <= 0 || N <= 0 || K <= 0 || M > kMxMaxDim || K > kMxMaxDim) return 0;
+  if (M <= mxrows::kUnitRows && N <= kRowsMaxN) return 0;
   return mx_operand_bytes(M, K);
 }
 

@@ -324,7 +324,8 @@ H3B_API int h3b_mxfp4_gemm(const void* A, const void* sfA, int64_t M, const void
 
 /* h3b_mxfp4_linear: the same with A = x [M, K] of D's type (row stride ldx),
  * quantized on the way.  `ws`: h3b_mxfp4_linear_ws(M, N, K) bytes of scratch (0
- * up to 8 rows), 256-byte aligned, private to this call until it has run.   */
+ * up to 8 rows and 8388480 columns), 256-byte aligned, private to this call
+ * until it has run.                                                         */
 H3B_API int64_t h3b_mxfp4_linear_ws(int64_t M, int64_t N, int64_t K);
 H3B_API int h3b_mxfp4_linear(const void* x, int dtype, int64_t M, int64_t ldx, const void* B,
                              const void* sfB, int64_t N, int64_t K, const void* bias, int act,
