@@ -92,13 +92,15 @@ struct Args {
   float scale_log2;                        // softmax scale * log2(e)
   int left, right, sinks, causal;          // left, right < 2^30
   int item_rows;                           // queries per item: 256, or 128 (tile A only)
-  int whole, parts;                        // items [0, whole) are whole, the others in `parts`
+  int whole, parts;                        // items [0, whole) are whole, the others in parts,
+                                           // each with places for `parts` of them
   float* partial;                          // [split item][part]: O [D/4][256][4], then (m, l) [256]
   int* done;                               // [split item]: parts finished (0 between launches)
   int ndocs;
   int q_start[MAX_DOCS], q_len[MAX_DOCS];
   int k_start[MAX_DOCS], k_len[MAX_DOCS];
-  int item_end[MAX_DOCS];                  // cumulative CTA counts
+  int item_end[MAX_DOCS];                  // cumulative item counts
+  int parts_of[MAX_DOCS];                  // of a split item of the document, at most `parts`
 };
 
 // What queries at positions [p0, p1] of a document of n_k keys see: sink keys
@@ -252,6 +254,8 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
   int doc = 0;
   while (doc + 1 < p.ndocs && idx >= p.item_end[doc]) ++doc;
   const int item = idx - (doc > 0 ? p.item_end[doc - 1] : 0);
+  const int parts = p.parts_of[doc];                      // of this item, where it is split
+  if (!whole && part >= parts) return;                    // (part 0 of every item stays)
   const int n_q = p.q_len[doc], n_k = p.k_len[doc];
   const int pairs = (n_q + p.item_rows - 1) / p.item_rows;
   const int head = item / pairs;
@@ -261,7 +265,7 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
   const int pos0 = q0 + n_k - n_q;                        // position of tile A's first row
   const int rows = min(p.item_rows, n_q - q0);            // queries of this item
   Steps<BK> st(Range(p, n_k, pos0, pos0 + rows - 1));
-  if (!whole) st.take(part, p.parts);
+  if (!whole) st.take(part, parts);
   // what each tile sees; a tile without queries sees nothing
   auto tile_range = [&](int t) {
     const int n = min(BQ, rows - t * BQ);
@@ -645,7 +649,7 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
       named_barrier_sync(2, 256);
       volatile int* last = reinterpret_cast<volatile int*>(tmem_slot + 2);
       if (threadIdx.x == 0) {
-        const bool is_last = atomicAdd(p.done + split, 1) == p.parts - 1;
+        const bool is_last = atomicAdd(p.done + split, 1) == parts - 1;
         if (is_last) p.done[split] = 0;                    // for the next launch
         *last = is_last;
       }
@@ -654,9 +658,9 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
         __threadfence();
         const float* all = p.partial + (size_t)split * p.parts * kPart;
         float mm = -INFINITY, ll = 0.f;
-        for (int i = 0; i < p.parts; ++i)
+        for (int i = 0; i < parts; ++i)
           mm = fmaxf(mm, __ldcg(all + (size_t)i * kPart + 256 * D + row * 2));
-        for (int i = 0; i < p.parts; ++i) {
+        for (int i = 0; i < parts; ++i) {
           const float* ml = all + (size_t)i * kPart + 256 * D + row * 2;
           const float mi = __ldcg(ml);
           ll += mi == -INFINITY ? 0.f : attn::ex2(mi - mm) * __ldcg(ml + 1);
@@ -667,7 +671,7 @@ __global__ void __launch_bounds__(Cfg<D, BK>::THREADS, Cfg<D, BK>::CTAS)
           float acc[32];
 #pragma unroll
           for (int c = 0; c < 32; ++c) acc[c] = 0.f;
-          for (int i = 0; i < p.parts; ++i) {
+          for (int i = 0; i < parts; ++i) {
             const float* from = all + (size_t)i * kPart;
             const float mi = __ldcg(from + 256 * D + row * 2);
             const float w = mi == -INFINITY ? 0.f : attn::ex2(mi - mm);

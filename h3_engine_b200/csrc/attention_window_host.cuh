@@ -67,10 +67,14 @@ static int64_t window_keys(int64_t n_k, int64_t left, int64_t right, int64_t sin
 // heads: 32.9 us, in items of 128 40.5).
 //   Whole items first, then the last partial wave's in parts: items mod places
 // would run alone, so they are split to fill the places (8 heads of 16384 rows,
-// 512 items on 148 SMs: 212 us, unsplit 220).  A part keeps kPartKeys keys.
+// 512 items on 148 SMs: 212 us, unsplit 220).  A part keeps kPartKeys keys: the
+// first split item, whose document has the most, says how many parts there are
+// places for, and an item of fewer keys takes the first of them only (16 queries
+// against 16000 keys beside a document of one key, one head: 64 us, 202 with as
+// many parts for all as the fewest keys give).
 struct WindowPlan {
   static constexpr int64_t kPartKeys = 512;
-  int order[wattn::MAX_DOCS];
+  int order[wattn::MAX_DOCS], doc_parts[wattn::MAX_DOCS];
   int n = 0, next = 0;
   int item_rows = 2 * wattn::BQ, step = 128, whole = 0, parts = 1;
   int64_t items = 0;
@@ -89,21 +93,30 @@ struct WindowPlan {
       return c;
     };
     const int sms = num_sms();
-    const int64_t keys = window_keys(k_len[order[n - 1]], left, right, sinks);
-    auto cut = [&](int64_t rest, int places) {
-      return rest ? std::max<int64_t>(1, std::min<int64_t>(places / rest, keys / kPartKeys)) : 1;
+    auto doc_cut = [&](int i) {        // parts that a document's keys are enough for
+      return std::max<int64_t>(1, window_keys(k_len[order[i]], left, right, sinks) / kPartKeys);
+    };
+    auto cut = [&](int64_t all, int rows, int places) {
+      const int64_t rest = all % places;
+      if (rest == 0) return (int64_t)1;
+      int i = 0;                       // the document of the first split item
+      for (int64_t end = 0;; ++i) {
+        end += ((int64_t)q_len[order[i]] + rows - 1) / rows * H;
+        if (end > all - rest) break;
+      }
+      return std::min<int64_t>(places / rest, doc_cut(i));
     };
     items = count(item_rows);
     if (const int64_t c = count(wattn::BQ);
-        c <= sms && 2 * cut(items % sms, sms) < 3 * cut(c % sms, sms)) {
+        c <= sms && 2 * cut(items, item_rows, sms) < 3 * cut(c, wattn::BQ, sms)) {
       item_rows = wattn::BQ;
       items = c;
     }
     if (D == 64 && items > sms) step = 64;
     const int places = step == 64 ? 2 * sms : sms;
-    const int64_t rest = items % places;
-    parts = (int)cut(rest, places);
-    whole = (int)std::min<int64_t>(parts > 1 ? items - rest : items, INT32_MAX);
+    parts = (int)cut(items, item_rows, places);
+    whole = (int)std::min<int64_t>(parts > 1 ? items - items % places : items, INT32_MAX);
+    for (int i = 0; i < n; ++i) doc_parts[i] = (int)std::min<int64_t>(parts, doc_cut(i));
   }
   int64_t split() const { return items - whole; }
   int64_t grid() const { return whole + split() * parts; }
@@ -239,6 +252,7 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
       a.k_start[i] = k_start[d];
       a.k_len[i] = k_len[d];
       a.item_end[i] = (int)items;
+      a.parts_of[i] = plan.doc_parts[i];
     }
     a.ndocs = plan.n;
     a.item_rows = plan.item_rows;

@@ -148,3 +148,38 @@ def test_calls_in_a_row(cuda, d):
     for _ in range(6):
         graph.replay()
         assert torch.equal(x, want)
+
+
+# ---------------------------------------------------------------- documents of uneven lengths
+def test_a_short_document_leaves_the_others_their_parts():
+    """The workspace of one long history is not lost to a short document beside it."""
+    rule = (None, None, 0, True)
+    alone = workspace([16], [16000], 1, 128, rule)
+    assert alone > 0
+    for lq, lk in (([16, 1], [16000, 1]), ([1, 16], [1, 16000]), ([16, 5], [16000, 0]),
+                   ([16, 0], [16000, 0]), ([16, 3, 8], [16000, 700, 8])):
+        assert workspace(lq, lk, 1, 128, rule) >= alone
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("heads,kv", [(1, 1), (4, 2)])
+@pytest.mark.parametrize("d,dtype", [(64, F16), (128, BF16)])
+@pytest.mark.parametrize("rule", [(None, None, 0, True), (None, None, 0, False), (3000, 0, 5, True),
+                                  (40, 30, 300, False)])
+def test_parts_of_uneven_documents(cuda, heads, kv, d, dtype, rule):
+    """One long history beside documents that fill some of its parts, one or none."""
+    lq = [16, 1, 5, 300, 7, 130, 0, 40]
+    lk = [9000, 1, 0, 700, 3000, 60, 50, 1100]
+    q, k, v, cq, ck = packed_case(lq, lk, heads, kv, d, dtype, seed=30)
+    if rule[0] != 40:
+        assert workspace(lq, lk, heads, d, rule) > 0
+    args = [t.to(cuda) for t in (q, k, v)]
+
+    def call():
+        return ops.attention_window(*args, heads, d, cq, kv_heads=kv, cu_seqlens_k=ck,
+                                    window=rule[:2], sinks=rule[2], causal=rule[3])
+
+    got = call()
+    check_packed(got.cpu(), q, k, v, cq, ck, heads, kv, d, rule)
+    for _ in range(5):                   # whichever part is last, and counters left at 0
+        assert torch.equal(call(), got)
