@@ -125,9 +125,11 @@ struct WindowPlan {
 static int64_t window_part_bytes(int D) { return ((int64_t)256 * D + 512) * 4; }
 static constexpr int64_t kDoneBytes = 2048;       // a counter per split item (fewer than slots)
 
+constexpr float kLog2e = 1.4426950408889634f;      // the kernels' exponents are of 2
+
 static int window_rule(int64_t left, int64_t right, int64_t sinks, int causal, float scale) {
   if (left < 0 || right < 0 || sinks < 0 || (causal != 0 && causal != 1) || !(scale > 0.f) ||
-      !std::isfinite(scale))
+      !std::isfinite(scale * kLog2e))
     return H3B_ERR_INVALID_ARG;
   return H3B_OK;
 }
@@ -223,7 +225,7 @@ int h3b_attention_window(const void* q, int64_t q_rows, int64_t q_stride, const 
   a.ldo = ldo;
   a.H = H;
   a.group = H / kv_heads;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2e;
   a.left = clamp_window(left);
   a.right = clamp_window(right);
   a.sinks = clamp_window(sinks);
@@ -318,7 +320,7 @@ int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const v
   a.right = clamp_window(right);
   a.sinks = clamp_window(sinks);
   a.causal = causal;
-  a.scale_log2 = scale * 1.4426950408889634f;
+  a.scale_log2 = scale * kLog2e;
   cudaStream_t st = static_cast<cudaStream_t>(stream);
   if (D == 128)
     return dtype == H3B_DT_F16 ? window_decode_launch<128, __half>(a, B, st)

@@ -441,7 +441,9 @@ void check_rule(const Rule& r, int64_t heads, int64_t kv_heads, int64_t d) {
                     " query heads are not a multiple of ", kv_heads, " key heads");
   TORCH_CHECK_VALUE(r.left >= 0 && r.right >= 0 && r.sinks >= 0,
                     "window sides and sinks must not be negative");
-  TORCH_CHECK_VALUE(r.scale > 0 && std::isfinite(r.scale), "scale must be positive and finite");
+  const float scale = (float)r.scale;              // the kernels', times log2(e)
+  TORCH_CHECK_VALUE(scale > 0 && std::isfinite(scale * 1.4426950408889634f),
+                    "scale must be positive, and scale * log2(e) finite in fp32");
 }
 
 // Row ranges of the documents that boundaries give.

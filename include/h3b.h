@@ -350,7 +350,8 @@ H3B_API int h3b_mxfp4_ffn(const void* x, int dtype, int64_t M, int64_t ldx, cons
  *   (p - left <= j <= p + right  or  j < sinks)  and  (not causal or j <= p);
  * softmax(scale * q k^T) v over the keys it sees, zeros where it sees none.
  * bf16 or fp16, D 64 or 128, H query heads over kv_heads key heads (H a
- * multiple; query head h reads key head h / (H / kv_heads)).
+ * multiple; query head h reads key head h / (H / kv_heads)); scale positive,
+ * scale * log2(e) finite.
  * A value row that some query sees must be finite to leave the other queries
  * of the same 256-row tile finite; what lies in rows that no query of the
  * tile sees (past a document's end, outside every window) does not matter.
