@@ -10,6 +10,7 @@
 namespace h3b {
 
 constexpr int64_t kMaxKeys = (int64_t)1 << 30;    // positions plus a window stay in 31 bits
+constexpr int64_t kMaxGrid = 65535;               // along y and z
 
 static inline int clamp_window(int64_t v) { return (int)std::min<int64_t>(v, kMaxKeys - 1); }
 
@@ -143,7 +144,6 @@ static int window_decode_rows(const wdec::Args& a, int64_t B, cudaStream_t st) {
   if (rc != H3B_OK) return rc;
   const int64_t row_tiles = ((int64_t)a.n_new * a.group + 8 * NT - 1) / (8 * NT);
   const int64_t groups = row_tiles * a.kv_heads;
-  if (groups > 65535 || B > 65535) return H3B_ERR_INVALID_ARG;
   // CTAs along the keys: until there are two per SM, which run at a time (32
   // uneven sequences of 8 key heads: 91 us without a split, 76 with 512 CTAs,
   // 77 with 1024, 93 with 2048), but no more than give every warp two tiles
@@ -285,7 +285,7 @@ int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const v
                                 int dtype, int H, int kv_heads, int D, int64_t left, int64_t right,
                                 int64_t sinks, int causal, float scale, void* out, void* stream) {
   if (!dt_16(dtype) || (D != 64 && D != 128) || H <= 0 || kv_heads <= 0 || H % kv_heads || B < 0 ||
-      room < 0 || n_new < 0 || room > kMaxKeys || n_new > 65535 || !q_strides || !k_strides ||
+      room < 0 || n_new < 0 || room > kMaxKeys || n_new > kMaxGrid || !q_strides || !k_strides ||
       !v_strides)
     return H3B_ERR_INVALID_ARG;
   int rc = window_rule(left, right, sinks, causal, scale);
@@ -296,6 +296,9 @@ int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const v
   }
   if (B == 0 || n_new == 0) return H3B_OK;
   if (!q || !len || !out || (room > 0 && (!k || !v))) return H3B_ERR_INVALID_ARG;
+  // the grid's y and z
+  if (B > kMaxGrid || (n_new * (H / kv_heads) + 15) / 16 * kv_heads > kMaxGrid)
+    return H3B_ERR_INVALID_ARG;
   if (!aligned16(q) || !aligned16(k) || !aligned16(v) || !aligned16(out) ||
       (reinterpret_cast<uintptr_t>(len) & 3u))
     return H3B_ERR_ALIGNMENT;

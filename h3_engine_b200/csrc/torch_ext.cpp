@@ -569,6 +569,10 @@ void decode_into(const Call& c, const Tensor& q_in, const Tensor& k, const Tenso
   TORCH_CHECK_VALUE(k.numel() == 0 || (decode_strides(k) && decode_strides(v)),
                     "caches need a contiguous head_dim and 16-byte aligned rows");
   if (out.numel() == 0) return;
+  TORCH_CHECK_VALUE(B <= 65535 && n <= 65535 &&
+                        (n * (heads / k.size(2)) + 15) / 16 * k.size(2) <= 65535,
+                    "at most 65535 sequences, and 65535 blocks of 16 rows that share a key head, "
+                    "not ", B, " and ", n, " new tokens of ", heads, " heads");
   const Tensor q = decode_strides(q_in) ? q_in : q_in.clone(at::MemoryFormat::Contiguous);
   static const int64_t none[4] = {0, 0, 0, 0};       // an empty cache's strides mean nothing
   const bool empty = k.numel() == 0;

@@ -516,7 +516,9 @@ def attention_window_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     aligned; caches are never copied), ``kv_len`` int32 [B] on the device: the
     keys in use, the new tokens' own included, so token t stands at position
     ``kv_len - n_new + t``.  Lengths are read when the kernel runs (a captured
-    call follows them) and clamped to [0, room].  Returns [B, n_new, heads, D]."""
+    call follows them) and clamped to [0, room].  Returns [B, n_new, heads, D].
+    At most 65535 sequences, and as many blocks of 16 rows (new tokens times query
+    heads) that share a key head."""
     _cuda_only(q)
     left, right = window
     left = _ALL_KEYS if left is None else left

@@ -378,7 +378,8 @@ H3B_API int64_t h3b_attention_window_ws(const int32_t* q_len, const int32_t* k_l
  * elements (multiples of 8; the last dimension contiguous), out [B, n_new, H,
  * D] contiguous.  len: DEVICE int32 [B], the keys in use per sequence with the
  * new tokens' own (read when the kernel runs, clamped to [0, room]), so that
- * token t stands at position len - n_new + t.                               */
+ * token t stands at position len - n_new + t.  B, n_new and
+ * ceil(n_new * H / kv_heads / 16) * kv_heads are at most 65535.              */
 H3B_API int h3b_attention_window_decode(const void* q, const int64_t* q_strides, const void* k,
                                         const int64_t* k_strides, const void* v,
                                         const int64_t* v_strides, const int32_t* len, int64_t B,

@@ -44,3 +44,31 @@ def test_the_largest_scale(cuda):
     n = torch.tensor([8], dtype=torch.int32, device=cuda)
     assert (ops.attention_window(x, x, v, 1, 128, [0, 8], scale=LARGE / 1.45) == 3.5).all()
     assert (ops.attention_window_decode(c[:, :1], c, cv, n, scale=LARGE / 1.45) == 3.5).all()
+
+
+def decode(B, n_new, H, kv):
+    p = ctypes.c_void_p(1 << 20)
+    st = (ctypes.c_int64 * 3)(128, 128, 128)
+    return _lib.lib().h3b_attention_window_decode(p, st, p, st, p, st, p, B, 4, n_new, 0, H, kv, 128,
+                                                  0, 0, 0, 1, 0.1, p, None)
+
+
+def test_decode_sizes_beyond_the_grid_are_refused_before_a_launch():
+    for args in ((65536, 1, 1, 1), (1, 65536, 1, 1), (1, 16384, 128, 128), (1, 1, 65536, 65536)):
+        assert decode(*args) == 1, args
+
+
+@pytest.mark.gpu
+def test_decode_sizes(cuda):
+    """The largest batch and the largest number of rows, and one more of each."""
+    def call(B, n, H, kv, d=64):
+        q = torch.ones(1, 1, 1, 1, dtype=BF16, device=cuda).expand(B, n, H, d)
+        k = torch.ones(B, 1, kv, d, dtype=BF16, device=cuda)
+        length = torch.ones(B, dtype=torch.int32, device=cuda)
+        return ops.attention_window_decode(q.contiguous(), k, k, length, causal=False)
+
+    for args in ((65535, 1, 1, 1), (1, 65535, 16, 1), (1, 1, 65535, 65535)):
+        assert (call(*args) == 1).all()
+    for args in ((65536, 1, 1, 1), (1, 65536, 1, 1), (1, 65535, 17, 1), (1, 1, 65536, 65536)):
+        with pytest.raises(ValueError):
+            call(*args)
