@@ -499,7 +499,7 @@ def attention_window(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, heads: i
     args = (q, k, v, heads, heads if kv_heads is None else kv_heads, head_dim,
             _host_ints(cu_seqlens), _host_ints(cu_seqlens_k),
             _ALL_KEYS if left is None else left, _ALL_KEYS if right is None else right, sinks,
-            causal, head_dim ** -0.5 if scale is None else scale)
+            causal, max(head_dim, 1) ** -0.5 if scale is None else scale)
     if out is None:
         return _WINDOW(*args)
     _WINDOW_OUT(*args, out)
@@ -523,7 +523,7 @@ def attention_window_decode(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor,
     left, right = window
     left = _ALL_KEYS if left is None else left
     right = _ALL_KEYS if right is None else right
-    scale = q.shape[-1] ** -0.5 if scale is None else scale
+    scale = max(q.shape[-1], 1) ** -0.5 if scale is None else scale
     if out is None:
         return _DECODE(q, k, v, kv_len, left, right, sinks, causal, scale)
     _DECODE_OUT(q, k, v, kv_len, left, right, sinks, causal, scale, out)

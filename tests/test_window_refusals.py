@@ -72,3 +72,14 @@ def test_decode_sizes(cuda):
     for args in ((65536, 1, 1, 1), (1, 65536, 1, 1), (1, 65535, 17, 1), (1, 1, 65536, 65536)):
         with pytest.raises(ValueError):
             call(*args)
+
+
+@pytest.mark.gpu
+def test_head_dims_without_a_scale_of_their_own(cuda):
+    x = torch.zeros(8, 128, dtype=BF16, device=cuda)
+    for d in (0, -2, -64):
+        with pytest.raises(ValueError):
+            ops.attention_window(x, x, x, 1, d, [0, 8])
+    c = torch.zeros(1, 8, 1, 0, dtype=BF16, device=cuda)
+    with pytest.raises(ValueError):
+        ops.attention_window_decode(c[:, :1], c, c, torch.ones(1, dtype=torch.int32, device=cuda))
