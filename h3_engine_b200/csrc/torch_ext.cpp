@@ -6,6 +6,7 @@
 // its tensors' device.  Only CUDA implementations are registered.  Built as
 // _h3b_torch.so beside libh3b.so, which it links.
 #include <ATen/ATen.h>
+#include <ATen/TensorUtils.h>
 #include <ATen/cuda/EmptyTensor.h>
 #include <c10/cuda/CUDAGuard.h>
 #include <c10/cuda/CUDAStream.h>
@@ -163,6 +164,9 @@ Tensor out_rows(const Tensor& out, at::IntArrayRef lead, int64_t m, int64_t n,
   shape.push_back(n);
   TORCH_CHECK_VALUE(out.scalar_type() == type && out.sizes() == at::IntArrayRef(shape),
                     "out must be ", type, " ", at::IntArrayRef(shape));
+  TORCH_CHECK_VALUE(out.dim() == 2 ||
+                        at::detail::computeStride(out.sizes(), out.strides(), at::DimVector{m, n}),
+                    "out must be a view of rows at one stride");
   Tensor o = out.dim() == 2 ? out : out.view({m, n});
   TORCH_CHECK_VALUE(m == 0 || rows_aligned(o), "out must have contiguous, 16-byte aligned rows");
   out.unsafeGetTensorImpl()->bump_version();
