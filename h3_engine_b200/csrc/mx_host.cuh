@@ -270,13 +270,12 @@ static int mx_rows_gemm(mxrows::Args& a, const void* A, const void* sfA, int64_t
   return mx_rows_launch<128, T, EPI, 0>(a, A, B, chained, st);
 }
 
-// Bytes of an activation's codes and blocked scales in a workspace, each part
-// rounded up to 256 bytes.
 // An activation's codes are ours to lay out: rows start at whole sectors (32
 // bytes), so that a TMA box's rows take no sector more than they fill (13383 x
 // 4096 x 4064 with its quantization: 114 us, 122 with rows of K / 2 bytes; 1025 x
 // 11008 x 2016: 19.0 and 20.3).
 static inline int64_t mx_code_pitch(int64_t k) { return (k / 2 + 31) / 32 * 32; }
+// Bytes of them in a workspace, rounded up to 256, and with their blocked scales.
 static inline int64_t mx_code_bytes(int64_t rows, int64_t k) {
   return (rows * mx_code_pitch(k) + 255) / 256 * 256;
 }
